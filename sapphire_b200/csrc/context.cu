@@ -574,8 +574,9 @@ void sapphire_on_tensor_release(uint64_t uid) {
 // -------------------------------------------------------------- streams ---
 extern "C" SAPPHIRE_API int kernel_ctx_synchronize(kernel_context_t *ctx) {
     if (!ctx) return -1;
-    if (!ctx->stream) return 0;
+    if (!ctx->initialized) return 0;
     DeviceGuard g(ctx->device);
+    // A NULL stream is the legacy default stream of an external caller.
     CUDA_TRY(ctx, cudaStreamSynchronize(ctx->stream));
     // Errors of asynchronous calls (kernel_gemv_device and the like) surface
     // here: a kernel whose bounded wait expired set the error word.
