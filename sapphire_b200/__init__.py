@@ -79,6 +79,10 @@ class Context:
     def device(self) -> int:
         return lib.kernel_ctx_get_device(self.handle)
 
+    def set_stream(self, stream: int) -> None:
+        """Use an external cudaStream_t (0: the legacy default stream)."""
+        self.check(lib.kernel_ctx_set_stream(self.handle, stream), "kernel_ctx_set_stream")
+
     def synchronize(self) -> None:
         self.check(lib.kernel_ctx_synchronize(self.handle), "kernel_ctx_synchronize")
 

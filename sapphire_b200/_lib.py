@@ -120,6 +120,15 @@ _SIGNATURES = {
     "sapphire_decoder_launches_per_token": (i32, [vp]),
     "sapphire_decoder_launches_per_prompt_token": (i32, [vp]),
     "sapphire_decoder_destroy": (None, [vp]),
+    # include/sapphire_attention.h
+    "sapphire_rope_create": (vp, [vp, vp]),
+    "sapphire_rope_destroy": (None, [vp]),
+    "sapphire_rope_device": (i32, [vp, vp]),
+    "sapphire_kv_page_bytes": (sz, [vp]),
+    "sapphire_kv_write_device": (i32, [vp, vp, vp]),
+    "sapphire_kv_read_device": (i32, [vp, vp, vp]),
+    "sapphire_attention_workspace_bytes": (sz, [vp, vp, i32, i32]),
+    "sapphire_attention_device": (i32, [vp, vp, vp]),
 }
 
 
@@ -134,6 +143,47 @@ class Gemma3Config(C.Structure):
 class Gemma3Weights(C.Structure):
     """sapphire_gemma3_weights_t (include/sapphire_decode.h)."""
     _fields_ = [("embed_bf16", vp), ("lm_head", vp), ("final_norm", vp), ("proj", vp), ("norms", vp)]
+
+
+i64 = C.c_longlong
+f64 = C.c_double
+
+
+class RopeConfig(C.Structure):
+    """sapphire_rope_config_t (include/sapphire_attention.h)."""
+    _fields_ = [("head_dim", i32), ("rot_dim", i32), ("layout", i32), ("scaling", i32), ("theta", f64),
+                ("factor", f64), ("original_context", i32), ("turns_slow", f64), ("turns_fast", f64),
+                ("attention_factor", f64)]
+
+
+class RopeArgs(C.Structure):
+    """sapphire_rope_args_t."""
+    _fields_ = [("dtype", i32), ("tokens", i32), ("positions", vp),
+                ("q", vp), ("q_out", vp), ("q_heads", i32), ("q_token_stride", i64), ("q_head_stride", i64),
+                ("q_out_token_stride", i64), ("q_out_head_stride", i64),
+                ("k", vp), ("k_out", vp), ("k_heads", i32), ("k_token_stride", i64), ("k_head_stride", i64),
+                ("k_out_token_stride", i64), ("k_out_head_stride", i64), ("inverse", i32)]
+
+
+class KvCacheStruct(C.Structure):
+    """sapphire_kv_cache_t."""
+    _fields_ = [("dtype", i32), ("page_size", i32), ("kv_heads", i32), ("head_dim", i32), ("num_pages", i32),
+                ("pages", vp)]
+
+
+class KvArgs(C.Structure):
+    """sapphire_kv_args_t."""
+    _fields_ = [("dtype", i32), ("tokens", i32), ("sequences", i32), ("cu_tokens", vp), ("start", vp),
+                ("page_table", vp), ("table_stride", i32), ("k", vp), ("v", vp), ("k_token_stride", i64),
+                ("k_head_stride", i64), ("v_token_stride", i64), ("v_head_stride", i64)]
+
+
+class AttentionArgs(C.Structure):
+    """sapphire_attention_args_t."""
+    _fields_ = [("dtype", i32), ("sequences", i32), ("heads", i32), ("q", vp), ("out", vp), ("q_seq_stride", i64),
+                ("q_head_stride", i64), ("out_seq_stride", i64), ("out_head_stride", i64), ("lse", vp),
+                ("page_table", vp), ("table_stride", i32), ("lengths", vp), ("length_offset", i32), ("window", i32),
+                ("scale", f32), ("workspace", vp), ("workspace_bytes", sz)]
 
 
 def load(path: str = LIB_PATH) -> C.CDLL:

@@ -1,0 +1,128 @@
+// attention.cuh - what the rotary, paged-cache and attention sources share
+// (include/sapphire_attention.h): element types, the cache's byte layout and
+// the checks of arguments.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "internal.cuh"
+#include "../../include/sapphire_attention.h"
+
+// Error-word bit of a page number, position or length outside the cache.
+constexpr int kErrCache = 32;
+
+// The bytes of a page (include/sapphire_attention.h): for each KV head a chunk
+// [K rows | V rows | K scales | V scales].
+struct KvLayout {
+    uint8_t *pages;
+    unsigned long long page_bytes;
+    int num_pages, page_size, kv_heads, head_dim;
+    int row_bytes;       // one row of codes or values
+    int scale_stride;    // padded scales of a row (0: dense)
+    int chunk_bytes;     // one KV head of a page
+    int v_off;           // V rows inside a chunk
+    int ks_off, vs_off;  // K and V scales inside a chunk
+};
+
+// Ragged rows (sapphire_kv_args_t).
+struct KvRows {
+    const int *cu_tokens, *start, *page_table;
+    int tokens, sequences, table_stride;
+    void *k, *v;
+    long long k_ts, k_hs, v_ts, v_hs;
+};
+
+// Whether every row starts on 16 bytes.
+inline bool rows_aligned(const void *p, long long ts, long long hs, size_t elem) {
+    return ((uintptr_t)p & 15) == 0 && (ts * (long long)elem) % 16 == 0 && (hs * (long long)elem) % 16 == 0;
+}
+
+// Fills `l` from the caller's cache; false (with the context's error set when
+// ctx is given) if the shape is not supported.
+bool kv_layout(kernel_context_t *ctx, const char *who, const sapphire_kv_cache_t *c, KvLayout *l);
+// Whether p is device memory of the context's GPU (recorded as an error if not).
+bool on_device(kernel_context_t *ctx, const char *who, const char *what, const void *p);
+
+inline size_t io_size(tensor_dtype_t dt) { return dt == DTYPE_F32 ? 4 : (dt == DTYPE_BF16 || dt == DTYPE_F16) ? 2 : 0; }
+
+// Restores the caller's device on scope exit.
+struct AttnDevice {
+    int prev = -1, dev;
+    explicit AttnDevice(int d) : dev(d) {
+        if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+        if (prev != dev) cudaSetDevice(dev);
+    }
+    ~AttnDevice() {
+        if (prev >= 0 && prev != dev) cudaSetDevice(prev);
+    }
+};
+
+#ifdef __CUDACC__
+template <typename T>
+__device__ __forceinline__ float to_f32(T x);
+template <>
+__device__ __forceinline__ float to_f32<float>(float x) {
+    return x;
+}
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 x) {
+    return __bfloat162float(x);
+}
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half x) {
+    return __half2float(x);
+}
+// One rounding, to nearest even.
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) {
+    return x;
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) {
+    return __float2bfloat16_rn(x);
+}
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) {
+    return __float2half_rn(x);
+}
+
+// N consecutive values (N * sizeof(T) a multiple of 16 when `wide`).
+template <typename T, int N>
+__device__ __forceinline__ void load_row(const T *p, bool wide, float (&x)[N]) {
+    if (wide) {
+        constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < N / kPer; ++i) {
+            const uint4 u = reinterpret_cast<const uint4 *>(p)[i];
+            T t[kPer];
+            memcpy(t, &u, 16);
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) x[i * kPer + j] = to_f32(t[j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[j] = to_f32(p[j]);
+    }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_row(T *p, bool wide, const float (&x)[N]) {
+    if (wide) {
+        constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < N / kPer; ++i) {
+            T t[kPer];
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) t[j] = from_f32<T>(x[i * kPer + j]);
+            uint4 u;
+            memcpy(&u, t, 16);
+            reinterpret_cast<uint4 *>(p)[i] = u;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) p[j] = from_f32<T>(x[j]);
+    }
+}
+#endif

@@ -274,7 +274,8 @@ int launch_product(kernel_context_t *ctx, const DevWeight &w, const float *x, in
                    int batch, cudaStream_t stream);
 // Reads and clears the error word after a synchronisation; -1 if a kernel
 // reported a failed wait (the split-tile counters are then cleared too).
-// Bits: 1 GEMV copy wait, 2/4 prefill-product waits, 8 peer-gather wait.
+// Bits: 1 GEMV copy wait, 2/4 prefill-product waits, 8 peer-gather wait, 32
+// an index outside a paged key-value cache (attention.cuh).
 int check_kernel_error(kernel_context_t *ctx, const char *who);
 
 // Tensor-core batched product of a Q4_0 weight (gemm_tc.cu), used for

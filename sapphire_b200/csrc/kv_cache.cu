@@ -1,0 +1,353 @@
+// kv_cache.cu - the paged key-value cache (include/sapphire_attention.h):
+// keys and values stored as they are or quantised, and read back dense.
+//
+// The block formulas are those of kernel_quantize_q8_0 / _q4_0 (quant.cu),
+// every float step one IEEE-rounded operation, so a row's codes and scales are
+// the same numbers; only their order inside a row differs (8 x nb words of
+// four codes, include/sapphire_attention.h).
+#include <cstring>
+
+#include "attention.cuh"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kUnit = 8;          // consecutive values of a row that one thread takes: words 2t and 2t + 1 of a block
+constexpr int kMaxTokens = 32;    // tokens of one block
+
+struct KvParams {
+    KvLayout l;
+    KvRows r;
+    int block_tokens, units;      // units: threads of one row
+    bool wide;
+    int *err;
+};
+
+// Where row `i` of ragged sequences lives: page (-1: nowhere) and slot.  A
+// row outside the table or on a page outside the cache sets the error word.
+__device__ __forceinline__ int2 kv_place(const KvLayout &l, const KvRows &r, int i, int *err) {
+    int s, j;
+    if (r.cu_tokens) {
+        // The sequence whose rows hold i: the largest s with cu_tokens[s] <= i.
+        int lo = 0, hi = r.sequences;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (__ldg(r.cu_tokens + mid) <= i) lo = mid;
+            else hi = mid - 1;
+        }
+        if (lo == r.sequences) return make_int2(-1, 0);      // behind the last sequence
+        s = lo;
+        j = i - __ldg(r.cu_tokens + s);
+        if (j < 0) return make_int2(-1, 0);                  // before the first
+    } else {
+        s = i;
+        j = 0;
+    }
+    const long long pos = (long long)j + (r.start ? __ldg(r.start + s) : 0);
+    const long long page = pos < 0 ? -1 : pos / l.page_size;
+    if (page < 0 || page >= r.table_stride) {
+        atomicOr(err, kErrCache);
+        return make_int2(-1, 0);
+    }
+    const int id = __ldg(r.page_table + (long long)s * r.table_stride + page);
+    if (id < 0 || id >= l.num_pages) {
+        atomicOr(err, kErrCache);
+        return make_int2(-1, 0);
+    }
+    return make_int2(id, (int)(pos - page * l.page_size));
+}
+
+// Lanes of one 32-value block: four neighbours, `mask` their bits.
+__device__ __forceinline__ float block_max(float v, unsigned mask) {
+    v = fmaxf(v, __shfl_xor_sync(mask, v, 1));
+    return fmaxf(v, __shfl_xor_sync(mask, v, 2));
+}
+
+// Codes of 8 values as the two words' bytes (Q8_0: one uint32 each; Q4_0: 16
+// bits each); returns the block's scale.
+__device__ __forceinline__ float quantize_q8(const float (&x)[kUnit], unsigned mask, uint32_t (&w)[2]) {
+    float a = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kUnit; ++j) a = fmaxf(a, fabsf(x[j]));
+    const float d = __fdiv_rn(block_max(a, mask), 127.0f);
+    const float id = d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        w[k] = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float t = roundf(__fmul_rn(x[4 * k + j], id));
+            const int q = (t != t) ? 0 : (t > 127.0f ? 127 : (t < -127.0f ? -127 : (int)t));
+            w[k] |= (uint32_t)(q + 128) << (8 * j);
+        }
+    }
+    return d;
+}
+__device__ __forceinline__ float quantize_q4(const float (&x)[kUnit], unsigned mask, uint32_t (&w)[2]) {
+    // The value of largest magnitude, the first of the block on ties.  A NaN
+    // never compares above, so it is not chosen.
+    float a = 0.0f, m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kUnit; ++j)
+        if (fabsf(x[j]) > a) {
+            a = fabsf(x[j]);
+            m = x[j];
+        }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        const float b = __shfl_xor_sync(mask, a, o), n = __shfl_xor_sync(mask, m, o);
+        const bool lower = (threadIdx.x & o) != 0;           // the other lane's values come first
+        if (b > a || (b == a && lower)) {
+            a = b;
+            m = n;
+        }
+    }
+    const float d = __fdiv_rn(m, -8.0f);
+    const float id = d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        w[k] = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float t = __fadd_rn(__fmul_rn(x[4 * k + j], id), 8.5f);
+            const uint32_t q = t >= 15.0f ? 15u : (t >= 1.0f ? (uint32_t)__float2int_rz(t) : 0u);
+            w[k] |= q << (4 * j);
+        }
+    }
+    return d;
+}
+
+// A block stores block_tokens tokens: K and V rows of every KV head.  A thread
+// owns one unit of a row; the four threads of a quantised block are
+// neighbours in a warp (units is a multiple of 4 for quantised formats).
+template <typename T, int kCache>
+__global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvParams p) {
+    __shared__ int2 place[kMaxTokens];
+    const int t0 = blockIdx.x * p.block_tokens, nt = min(p.block_tokens, p.r.tokens - t0);
+    const int tid = threadIdx.y * blockDim.x + threadIdx.x;
+    if (tid < nt) place[tid] = kv_place(p.l, p.r, t0 + tid, p.err);
+    __syncthreads();
+    const int u = threadIdx.x, d0 = u * kUnit, heads = p.l.kv_heads;
+    const unsigned mask = 0xfu << (tid & 28);
+    for (int i = threadIdx.y; i < nt * 2 * heads; i += blockDim.y) {
+        const int t = i / (2 * heads), c = i - t * 2 * heads;
+        const bool is_v = c >= heads;
+        const int h = is_v ? c - heads : c;
+        const int2 at = place[t];
+        if (at.x < 0) continue;
+        const T *src = (is_v ? static_cast<const T *>(p.r.v) + (long long)(t0 + t) * p.r.v_ts + (long long)h * p.r.v_hs
+                             : static_cast<const T *>(p.r.k) + (long long)(t0 + t) * p.r.k_ts + (long long)h * p.r.k_hs) + d0;
+        uint8_t *chunk = p.l.pages + (unsigned long long)at.x * p.l.page_bytes + (unsigned long long)h * p.l.chunk_bytes;
+        uint8_t *row = chunk + (is_v ? p.l.v_off : 0) + at.y * p.l.row_bytes;
+        float x[kUnit];
+        load_row<T, kUnit>(src, p.wide, x);
+        if (kCache == DTYPE_Q8_0 || kCache == DTYPE_Q4_0) {
+            const int nb = p.l.head_dim / 32, b = u >> 2, word = 2 * (u & 3);
+            uint32_t w[2];
+            float d;
+            if (kCache == DTYPE_Q8_0) {
+                d = quantize_q8(x, mask, w);
+                reinterpret_cast<uint32_t *>(row)[word * nb + b] = w[0];
+                reinterpret_cast<uint32_t *>(row)[(word + 1) * nb + b] = w[1];
+            } else {
+                d = quantize_q4(x, mask, w);
+                reinterpret_cast<uint16_t *>(row)[word * nb + b] = (uint16_t)w[0];
+                reinterpret_cast<uint16_t *>(row)[(word + 1) * nb + b] = (uint16_t)w[1];
+            }
+            if ((u & 3) == 0)
+                reinterpret_cast<float *>(chunk + (is_v ? p.l.vs_off : p.l.ks_off))[at.y * p.l.scale_stride + b] = d;
+        } else if (kCache == DTYPE_F32) {
+            store_row<float, kUnit>(reinterpret_cast<float *>(row) + d0, true, x);
+        } else if (kCache == DTYPE_BF16) {
+            store_row<__nv_bfloat16, kUnit>(reinterpret_cast<__nv_bfloat16 *>(row) + d0, true, x);
+        } else {
+            store_row<__half, kUnit>(reinterpret_cast<__half *>(row) + d0, true, x);
+        }
+    }
+}
+
+template <typename T, int kCache>
+__global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvParams p) {
+    __shared__ int2 place[kMaxTokens];
+    const int t0 = blockIdx.x * p.block_tokens, nt = min(p.block_tokens, p.r.tokens - t0);
+    const int tid = threadIdx.y * blockDim.x + threadIdx.x;
+    if (tid < nt) place[tid] = kv_place(p.l, p.r, t0 + tid, p.err);
+    __syncthreads();
+    const int u = threadIdx.x, d0 = u * kUnit, heads = p.l.kv_heads;
+    for (int i = threadIdx.y; i < nt * 2 * heads; i += blockDim.y) {
+        const int t = i / (2 * heads), c = i - t * 2 * heads;
+        const bool is_v = c >= heads;
+        const int h = is_v ? c - heads : c;
+        const int2 at = place[t];
+        if (at.x < 0) continue;
+        T *dst = (is_v ? static_cast<T *>(p.r.v) + (long long)(t0 + t) * p.r.v_ts + (long long)h * p.r.v_hs
+                       : static_cast<T *>(p.r.k) + (long long)(t0 + t) * p.r.k_ts + (long long)h * p.r.k_hs) + d0;
+        const uint8_t *chunk =
+            p.l.pages + (unsigned long long)at.x * p.l.page_bytes + (unsigned long long)h * p.l.chunk_bytes;
+        const uint8_t *row = chunk + (is_v ? p.l.v_off : 0) + at.y * p.l.row_bytes;
+        float x[kUnit];
+        if (kCache == DTYPE_Q8_0 || kCache == DTYPE_Q4_0) {
+            const int nb = p.l.head_dim / 32, b = u >> 2, word = 2 * (u & 3);
+            const float d = reinterpret_cast<const float *>(chunk + (is_v ? p.l.vs_off : p.l.ks_off))[at.y * p.l.scale_stride + b];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint32_t w = kCache == DTYPE_Q8_0 ? reinterpret_cast<const uint32_t *>(row)[(word + k) * nb + b]
+                                                        : reinterpret_cast<const uint16_t *>(row)[(word + k) * nb + b];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int q = kCache == DTYPE_Q8_0 ? (int)((w >> (8 * j)) & 255u) - 128 : (int)((w >> (4 * j)) & 15u) - 8;
+                    x[4 * k + j] = __fmul_rn((float)q, d);
+                }
+            }
+        } else if (kCache == DTYPE_F32) {
+            load_row<float, kUnit>(reinterpret_cast<const float *>(row) + d0, true, x);
+        } else if (kCache == DTYPE_BF16) {
+            load_row<__nv_bfloat16, kUnit>(reinterpret_cast<const __nv_bfloat16 *>(row) + d0, true, x);
+        } else {
+            load_row<__half, kUnit>(reinterpret_cast<const __half *>(row) + d0, true, x);
+        }
+        store_row<T, kUnit>(dst, p.wide, x);
+    }
+}
+
+template <typename T, int kCache>
+void launch_kv(const KvParams &p, bool write, dim3 grid, dim3 block, cudaStream_t st) {
+    if (write)
+        kv_write_kernel<T, kCache><<<grid, block, 0, st>>>(p);
+    else
+        kv_read_kernel<T, kCache><<<grid, block, 0, st>>>(p);
+}
+template <typename T>
+void launch_kv(tensor_dtype_t cache, const KvParams &p, bool write, dim3 grid, dim3 block, cudaStream_t st) {
+    switch (cache) {
+        case DTYPE_F32: launch_kv<T, DTYPE_F32>(p, write, grid, block, st); break;
+        case DTYPE_BF16: launch_kv<T, DTYPE_BF16>(p, write, grid, block, st); break;
+        case DTYPE_F16: launch_kv<T, DTYPE_F16>(p, write, grid, block, st); break;
+        case DTYPE_Q8_0: launch_kv<T, DTYPE_Q8_0>(p, write, grid, block, st); break;
+        default: launch_kv<T, DTYPE_Q4_0>(p, write, grid, block, st); break;
+    }
+}
+
+int kv_call(kernel_context_t *ctx, const sapphire_kv_cache_t *cache, const sapphire_kv_args_t *a, bool write) {
+    const char *who = write ? "sapphire_kv_write_device" : "sapphire_kv_read_device";
+    if (!ctx || !cache || !a) {
+        LOG_ERROR("%s: NULL argument", who);
+        return -1;
+    }
+    std::lock_guard<std::recursive_mutex> lk(ctx->exec_mutex);
+    if (!ctx->initialized) {
+        ctx_fail(ctx, who, "context not initialized");
+        return -1;
+    }
+    KvParams p{};
+    if (!kv_layout(ctx, who, cache, &p.l)) return -1;
+    const size_t size = io_size(a->dtype);
+    if (!size) {
+        ctx_fail(ctx, who, "k and v must be F32, BF16 or F16");
+        return -1;
+    }
+    if (a->tokens < 0 || a->sequences < 0 || (!a->cu_tokens && a->tokens != a->sequences)) {
+        ctx_fail(ctx, who, "%d tokens of %d sequences (without cu_tokens each has one)", a->tokens, a->sequences);
+        return -1;
+    }
+    if (a->tokens == 0 || a->sequences == 0) return 0;
+    if (a->table_stride <= 0) {
+        ctx_fail(ctx, who, "table_stride must be positive");
+        return -1;
+    }
+    if (!on_device(ctx, who, "pages", cache->pages) || !on_device(ctx, who, "k", a->k) || !on_device(ctx, who, "v", a->v) ||
+        !on_device(ctx, who, "page_table", a->page_table) ||
+        (a->cu_tokens && !on_device(ctx, who, "cu_tokens", a->cu_tokens)) ||
+        (a->start && !on_device(ctx, who, "start", a->start)))
+        return -1;
+    const long long row = (long long)cache->kv_heads * cache->head_dim;
+    p.r = {a->cu_tokens, a->start, a->page_table, a->tokens, a->sequences, a->table_stride, a->k, a->v,
+           a->k_token_stride ? a->k_token_stride : row, a->k_head_stride ? a->k_head_stride : cache->head_dim,
+           a->v_token_stride ? a->v_token_stride : row, a->v_head_stride ? a->v_head_stride : cache->head_dim};
+    p.wide = rows_aligned(a->k, p.r.k_ts, p.r.k_hs, size) && rows_aligned(a->v, p.r.v_ts, p.r.v_hs, size);
+    p.err = ctx->d_err;
+    p.units = cache->head_dim / kUnit;
+    AttnDevice g(ctx->device);
+    const int rows = kThreads / p.units, sms = sm_count(ctx->device);
+    // About four rows a thread while that still gives every SM two blocks.
+    p.block_tokens = std::min(kMaxTokens, std::max(1, 4 * rows / (2 * cache->kv_heads)));
+    while (p.block_tokens > 1 && (a->tokens + p.block_tokens - 1) / p.block_tokens < 2 * sms) p.block_tokens /= 2;
+    const dim3 grid((a->tokens + p.block_tokens - 1) / p.block_tokens), block(p.units, rows);
+    switch (a->dtype) {
+        case DTYPE_F32: launch_kv<float>(cache->dtype, p, write, grid, block, ctx->stream); break;
+        case DTYPE_BF16: launch_kv<__nv_bfloat16>(cache->dtype, p, write, grid, block, ctx->stream); break;
+        default: launch_kv<__half>(cache->dtype, p, write, grid, block, ctx->stream); break;
+    }
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) {
+        ctx_fail(ctx, who, "launch failed: %s", cudaGetErrorString(e));
+        return -1;
+    }
+    return 0;
+}
+
+// nullptr, or why the cache's shape is not supported.
+const char *kv_shape(const sapphire_kv_cache_t *c, KvLayout *l) {
+    const int d = c->head_dim;
+    if (d != 64 && d != 96 && d != 128 && d != 192 && d != 256) return "head_dim must be 64, 96, 128, 192 or 256";
+    if (c->kv_heads <= 0 || c->kv_heads > 1024) return "kv_heads must be 1 to 1024";
+    if (c->page_size <= 0 || c->page_size > 4096) return "page_size must be 1 to 4096";
+    const int nb = d / 32;
+    l->scale_stride = 0;
+    switch (c->dtype) {
+        case DTYPE_F32: l->row_bytes = 4 * d; break;
+        case DTYPE_BF16:
+        case DTYPE_F16: l->row_bytes = 2 * d; break;
+        case DTYPE_Q8_0: l->row_bytes = d; break;
+        case DTYPE_Q4_0: l->row_bytes = d / 2; break;
+        default: return "the cache's type must be F32, BF16, F16, Q8_0 or Q4_0";
+    }
+    if (c->dtype == DTYPE_Q8_0 || c->dtype == DTYPE_Q4_0) l->scale_stride = nb <= 2 ? 2 : nb <= 4 ? 4 : 8;
+    const int ps = c->page_size;
+    l->v_off = ps * l->row_bytes;
+    l->ks_off = 2 * ps * l->row_bytes;
+    l->vs_off = l->ks_off + ps * l->scale_stride * 4;
+    l->chunk_bytes = l->vs_off + ps * l->scale_stride * 4;
+    l->page_bytes = (unsigned long long)l->chunk_bytes * c->kv_heads;
+    l->page_size = ps;
+    l->kv_heads = c->kv_heads;
+    l->head_dim = d;
+    return nullptr;
+}
+
+}  // namespace
+
+bool on_device(kernel_context_t *ctx, const char *who, const char *what, const void *p) {
+    int dev = -1;
+    if (p && ptr_is_device(p, &dev) && dev == ctx->device) return true;
+    ctx_fail(ctx, who, "%s must be device memory of the context's GPU", what);
+    return false;
+}
+
+bool kv_layout(kernel_context_t *ctx, const char *who, const sapphire_kv_cache_t *c, KvLayout *l) {
+    const char *why = kv_shape(c, l);
+    l->pages = static_cast<uint8_t *>(c->pages);
+    l->num_pages = c->num_pages;
+    if (!why && c->num_pages <= 0) why = "num_pages must be positive";
+    // Row offsets are kept in units of 16 bytes in 32 bits.
+    if (!why && l->page_bytes * (unsigned long long)c->num_pages > (1ull << 36)) why = "the cache is above 64 GB";
+    if (!why && ((uintptr_t)c->pages & 15)) why = "pages must be 16-byte aligned";
+    if (!why) return true;
+    ctx_fail(ctx, who, "%s", why);
+    return false;
+}
+
+extern "C" SAPPHIRE_API size_t sapphire_kv_page_bytes(const sapphire_kv_cache_t *cache) {
+    KvLayout l{};
+    return cache && !kv_shape(cache, &l) ? (size_t)l.page_bytes : 0;
+}
+
+extern "C" SAPPHIRE_API int sapphire_kv_write_device(kernel_context_t *ctx, const sapphire_kv_cache_t *cache,
+                                                     const sapphire_kv_args_t *args) {
+    return kv_call(ctx, cache, args, true);
+}
+
+extern "C" SAPPHIRE_API int sapphire_kv_read_device(kernel_context_t *ctx, const sapphire_kv_cache_t *cache,
+                                                    const sapphire_kv_args_t *args) {
+    return kv_call(ctx, cache, args, false);
+}

@@ -1,0 +1,687 @@
+"""Rotary positions, the paged key-value cache and attention of one new token
+against plain 64-bit forms.
+
+Tolerances.  A rounding is off by at most half a step, eps(t) / 2 of the value
+(fp16 below 2^-14: 2^-25).
+
+rope: the phase is good to 2^-32 of a turn, its fp32 half turns to 2^-25 and
+sincospi to 2 ulp, so cos and sin are off by at most pi 2^-25 + 2^-22 < 2^-21.4
+(times the amplitude, itself rounded); the products and the sum round three
+times.  A turned value is off by at most (|a| + |b|) m 2^-21 before its own
+rounding.
+
+attend: q, k and p are held to at least 21 bits, sums in fp32 over at most
+2^12 terms per partial sum (tests are smaller), so a score is off by at most
+ds = scale sum|q k| 2^-19; p is off by a factor of exp(+-2 ds) (1 + 2^-18) with
+the approximate exponential (2^-21), and so out by at most
+max|v| (4 ds + 2^-17) before its rounding.
+"""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+IO = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+CACHES = ["f32", "bf16", "f16", "q8_0", "q4_0"]
+
+
+def half_step(t, y):
+    """Half a step of type t at y (fp64)."""
+    return y.abs() * (torch.finfo(t).eps / 2) + (2.0 ** -25 if t == torch.float16 else 0.0)
+
+
+def assert_within(got, want, before, what=""):
+    """got (type t) is want (fp64) off by at most `before` and one rounding."""
+    tol = before + half_step(got.dtype, want.abs() + before) * (1 if got.dtype != torch.float32 else 1)
+    bad = (got.double() - want).abs() - tol
+    assert torch.isfinite(got.double()).all(), what
+    assert bad.max().item() <= 0, f"{what}: over by {bad.max().item():.3g}, want {want.flatten()[bad.argmax()].item():.6g}"
+
+
+@pytest.fixture
+def dev_ctx(sp):
+    """A context on torch's current stream."""
+    c = sp.Context(num_threads=1)
+    c.set_stream(torch.cuda.current_stream().cuda_stream)
+    yield c
+    c.close()
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+# --------------------------------------------------------------------- rope --
+def rope_frequencies(rot, theta, scaling, factor, orig=8192):
+    i = np.arange(rot // 2, dtype=np.float64)
+    f = theta ** (-2 * i / rot)
+    m = 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "banded":
+        r = orig * f / (2 * np.pi)
+        s = np.clip((r - 1) / 3, 0, 1)
+        f = (1 - s) * f / factor + s * f
+    elif scaling == "yarn":
+        c = lambda r: rot * math.log(orig / (2 * math.pi * r)) / (2 * math.log(theta))  # noqa: E731
+        lo, hi = max(math.floor(c(32.0)), 0), min(math.ceil(c(1.0)), rot - 1)
+        g = np.clip((i - lo) / max(hi - lo, 1e-3), 0, 1)
+        f = (1 - g) * f + g * f / factor
+        m = 0.1 * math.log(factor) + 1
+    return torch.from_numpy(f).cuda(), m
+
+
+def rope_plain(x, pos, rot, layout, theta=1e4, scaling="none", factor=1.0, inverse=False):
+    """fp64 result and the error bound before rounding."""
+    f, m = rope_frequencies(rot, theta, scaling, factor)
+    a = pos.double()[:, None, None] * f
+    if inverse:
+        a = -a
+    y, e = x.double().clone(), torch.zeros_like(x, dtype=torch.float64)
+    at = (slice(0, rot // 2), slice(rot // 2, rot)) if layout == "half" else (slice(0, rot, 2), slice(1, rot, 2))
+    u, v = y[..., at[0]].clone(), y[..., at[1]].clone()
+    y[..., at[0]], y[..., at[1]] = (u * a.cos() - v * a.sin()) * m, (u * a.sin() + v * a.cos()) * m
+    e[..., at[0]] = e[..., at[1]] = (u.abs() + v.abs()) * m * 2.0 ** -21
+    return y, e
+
+
+@pytest.mark.parametrize("tokens,heads,kv_heads,dim,rot,layout,kind,scaling", [
+    (1, 4, 1, 256, 256, "half", "f32", "none"),
+    (1, 1, 0, 2, 2, "interleaved", "f32", "none"),
+    (5, 3, 1, 64, 64, "half", "bf16", "linear"),
+    (7, 5, 5, 80, 40, "half", "f16", "none"),
+    (7, 5, 5, 80, 40, "interleaved", "f16", "yarn"),
+    (33, 32, 8, 128, 128, "half", "bf16", "banded"),
+    (33, 32, 8, 128, 64, "interleaved", "bf16", "yarn"),
+    (130, 6, 2, 96, 22, "half", "f32", "banded"),
+    (130, 6, 2, 96, 22, "interleaved", "f32", "linear"),
+    (1000, 2, 1, 512, 512, "half", "f16", "yarn"),
+    (601, 40, 0, 18, 18, "interleaved", "bf16", "none"),
+])
+def test_rope(dev_ctx, tokens, heads, kv_heads, dim, rot, layout, kind, scaling):
+    from sapphire_b200.attention import Rope
+    g = gen(tokens)
+    pos = torch.randint(0, 131072, (tokens,), device="cuda", generator=g, dtype=torch.int32)
+    pos[0] = 0 if tokens > 1 else 777
+    q = torch.randn(tokens, heads, dim, device="cuda", generator=g).to(IO[kind])
+    k = torch.randn(tokens, kv_heads, dim, device="cuda", generator=g).to(IO[kind]) if kv_heads else None
+    r = Rope(dev_ctx, dim, rot_dim=rot, layout=layout, theta=5e5, scaling=scaling, factor=4.0, original_context=8192)
+    q_out = torch.full_like(q, 9.0)
+    k_out = torch.full_like(k, 9.0) if k is not None else None
+    r.apply(pos, q, k, q_out, k_out)
+    dev_ctx.synchronize()
+    for x, y in ((q, q_out), (k, k_out)):
+        if x is None:
+            continue
+        want, e = rope_plain(x, pos, rot, layout, 5e5, scaling, 4.0)
+        assert_within(y, want, e)
+        assert torch.equal(y[..., rot:], x[..., rot:])
+    r.close()
+
+
+def test_rope_far_positions(dev_ctx):
+    """Every 32-bit position, behind zero too."""
+    from sapphire_b200.attention import Rope
+    pos = torch.tensor([0, 1, -1, 2 ** 24 + 1, 10 ** 9 + 7, 2 ** 31 - 1, -2 ** 31], device="cuda", dtype=torch.int32)
+    q = torch.randn(7, 2, 64, device="cuda", generator=gen(3))
+    out = torch.empty_like(q)
+    Rope(dev_ctx, 64).apply(pos, q, q_out=out)
+    dev_ctx.synchronize()
+    # fp64 angles: 2^31 * 2^-53 = 2^-22 rad; the frequency's own rounding of 2^-53 the same again
+    want, e = rope_plain(q, pos, 64, "half")
+    assert_within(out, want, e + q.abs().max().item() * 2.0 ** -20)
+
+
+def test_rope_in_place_strided_and_back(dev_ctx):
+    from sapphire_b200.attention import Rope
+    qkv = torch.randn(9, 10, 128, device="cuda", generator=gen(4)).bfloat16()
+    before = qkv.clone()
+    pos = torch.arange(9, device="cuda", dtype=torch.int32) * 100
+    r = Rope(dev_ctx, 128, rot_dim=64)
+    q, k = qkv[:, :6], qkv[:, 6:8]
+    r.apply(pos, q, k)
+    dev_ctx.synchronize()
+    for x, y in ((before[:, :6], q), (before[:, 6:8], k)):
+        want, e = rope_plain(x, pos, 64, "half")
+        assert_within(y, want, e)
+    assert torch.equal(qkv[:, 8:], before[:, 8:])
+    # rows that do not start on 16 bytes
+    odd = torch.randn(9, 3 * 128 + 5, device="cuda", generator=gen(5)).bfloat16()
+    x = odd[:, 1:1 + 3 * 128].unflatten(1, (3, 128))
+    y = torch.empty(9, 3, 128, device="cuda", dtype=torch.bfloat16)
+    r.apply(pos, q=x, q_out=y)
+    dev_ctx.synchronize()
+    want, e = rope_plain(x, pos, 64, "half")
+    assert_within(y, want, e)
+    # the inverse of the turned values, in fp32, gives them back
+    f = torch.randn(9, 3, 128, device="cuda", generator=gen(6))
+    z = f.clone()
+    r.apply(pos, k=z)
+    r.apply(pos, k=z, inverse=True)
+    dev_ctx.synchronize()
+    assert (z - f).abs().max().item() <= 4 * f.abs().max().item() * 2.0 ** -21 * 2
+
+
+def test_rope_gradient(dev_ctx):
+    """The inverse turn is the gradient: against the formula's and against differences."""
+    from sapphire_b200.attention import Rope
+    g = gen(8)
+    pos = torch.randint(0, 5000, (6,), device="cuda", generator=g, dtype=torch.int32)
+    x = torch.randn(6, 2, 64, device="cuda", generator=g)
+    dy = torch.randn(6, 2, 64, device="cuda", generator=g)
+    r = Rope(dev_ctx, 64, rot_dim=48, layout="interleaved", scaling="yarn", factor=4.0, original_context=8192)
+    dx = torch.empty_like(x)
+    r.apply(pos, q=dy, q_out=dx, inverse=True)
+    dev_ctx.synchronize()
+    want, e = rope_plain(dy, pos, 48, "interleaved", scaling="yarn", factor=4.0, inverse=True)
+    assert_within(dx, want, e)
+    u = torch.randn(6, 2, 64, device="cuda", generator=g, dtype=torch.float64)
+    f = lambda v: (rope_plain(v, pos, 48, "interleaved", scaling="yarn", factor=4.0)[0] * dy.double()).sum()  # noqa: E731
+    diff = (f(x.double() + 1e-3 * u) - f(x.double() - 1e-3 * u)) / 2e-3
+    # the turn is linear: differences are exact but for the kernel's own error
+    assert abs(diff.item() - (dx.double() * u).sum().item()) <= (e.sum() * u.abs().max()).item() + 1e-6
+
+
+def test_rope_refusals(sp, dev_ctx):
+    from sapphire_b200.attention import Rope
+    r = Rope(dev_ctx, 64)
+    q = torch.zeros(4, 2, 64, device="cuda")
+    pos = torch.zeros(4, device="cuda", dtype=torch.int32)
+    with pytest.raises(sp.SapphireError, match="int32"):
+        r.apply(pos.long(), q)
+    with pytest.raises(sp.SapphireError, match="shape"):
+        r.apply(pos[:3], q)
+    with pytest.raises(sp.SapphireError, match="float32"):
+        r.apply(pos, q.double())
+    with pytest.raises(sp.SapphireError, match="one type"):
+        r.apply(pos, q, q.bfloat16())
+    with pytest.raises(sp.SapphireError, match="shape"):
+        r.apply(pos, torch.zeros(4, 2, 32, device="cuda"))
+    with pytest.raises(sp.SapphireError, match="contiguous"):
+        r.apply(pos, torch.zeros(4, 64, 2, device="cuda").transpose(1, 2))
+    with pytest.raises(sp.SapphireError, match="broadcast"):
+        r.apply(pos, torch.zeros(1, 2, 64, device="cuda").expand(4, 2, 64))
+    with pytest.raises(sp.SapphireError, match="device memory"):
+        r.apply(pos, q.cpu())
+    with pytest.raises(sp.SapphireError, match="device memory"):
+        r.apply(pos.cpu(), q)
+    with pytest.raises(sp.SapphireError, match="in place"):
+        r.apply(pos, q[:, :1], q_out=torch.as_strided(q, (4, 1, 64), (64, 64, 1)))
+    r.apply(pos[:0], q[:0])
+    dev_ctx.synchronize()
+
+
+# -------------------------------------------------------------------- cache --
+def layout(dtype, dim, page):
+    """(row bytes, padded scales, offsets of K, V, K scales, V scales, chunk bytes)."""
+    nb = dim // 32
+    row = {"f32": 4 * dim, "bf16": 2 * dim, "f16": 2 * dim, "q8_0": dim, "q4_0": dim // 2}[dtype]
+    ns = (2 if nb <= 2 else 4 if nb <= 4 else 8) if dtype[0] == "q" else 0
+    at = [0, page * row, 2 * page * row, 2 * page * row + 4 * page * ns]
+    return row, ns, at, at[3] + 4 * page * ns
+
+
+def cache_values(pages, dtype, page, heads, dim, j):
+    """fp64 [pages, heads, page, dim] of the K (0) or V (1) rows; quantised rows as code * scale."""
+    row, ns, at, chunk = layout(dtype, dim, page)
+    p = pages.reshape(-1, heads, chunk)
+    rows = p[..., at[j]:at[j] + page * row].reshape(-1, heads, page, row)
+    if not ns:
+        return rows.contiguous().view(IO[dtype]).double()
+    nb = dim // 32
+    if dtype == "q4_0":
+        rows = torch.stack((rows & 15, rows >> 4), -1).flatten(-2)
+    codes = rows.reshape(*rows.shape[:-1], 8, nb, 4).transpose(-3, -2).flatten(-2).double() - (128 if dtype == "q8_0" else 8)
+    sc = p[..., at[2 + j]:at[2 + j] + 4 * ns * page].contiguous().view(torch.float32).reshape(-1, heads, page, ns)
+    return (codes * sc[..., :nb, None].double()).flatten(-2)
+
+
+def make_cache(ctx, dtype, page, heads, dim, num_pages, fill=0):
+    from sapphire_b200.attention import KVCache, kv_page_bytes
+    pages = torch.full((num_pages, kv_page_bytes(dtype, page, heads, dim)), fill, dtype=torch.uint8, device="cuda")
+    return KVCache(ctx, dtype, page, heads, dim, pages)
+
+
+def make_table(lengths, page, num_pages, g, width=None):
+    """Random pages for sequences of these lengths; unused entries -1."""
+    need = [-(-n // page) for n in lengths]
+    order = torch.randperm(num_pages, device="cuda", generator=g)[:sum(need)].cpu().int()
+    t = torch.full((len(lengths), width or max(1, max(need))), -1, dtype=torch.int32)
+    a = 0
+    for i, m in enumerate(need):
+        t[i, :m] = order[a:a + m]
+        a += m
+    return t.cuda()
+
+
+def ragged(lens):
+    return torch.tensor([0] + list(np.cumsum(lens)), dtype=torch.int32, device="cuda")
+
+
+def expected_store(sp, ctx, x, dtype):
+    """fp64 values that the cache should hold of x, quantised by the library's quantiser."""
+    if dtype in IO:
+        return x.to(IO[dtype]).double()
+    code = sp.DTYPE_Q8_0 if dtype == "q8_0" else sp.DTYPE_Q4_0
+    flat = np.ascontiguousarray(x.float().cpu().numpy().reshape(-1, x.shape[-1]))
+    packed = sp.quantize(ctx, code, flat)
+    t = sp.Tensor(code, flat.shape, packed)
+    size = 36 if dtype == "q8_0" else 20
+    blocks = packed.reshape(-1, size)
+    scale = blocks[:, :4].copy().view(np.float32).astype(np.float64)
+    body = blocks[:, 4:]
+    codes = body.view(np.int8).astype(np.float64) if dtype == "q8_0" else \
+        np.stack((body & 15, body >> 4), -1).reshape(len(blocks), 32).astype(np.float64) - 8
+    t.release()
+    return torch.from_numpy((codes * scale).reshape(x.shape)).cuda()
+
+
+@pytest.mark.parametrize("dtype", CACHES)
+@pytest.mark.parametrize("kind,dim,page,heads", [("bf16", 128, 16, 8), ("f32", 256, 7, 1), ("f16", 96, 1, 3),
+                                                 ("bf16", 64, 100, 2), ("f32", 192, 24, 5)])
+def test_write_and_read(sp, dev_ctx, ctx, dtype, kind, dim, page, heads):
+    """Ragged chunks behind what was there, rows that belong to no sequence,
+    values stored as the library's quantisers store them, and read back."""
+    g = gen(dim + page)
+    before, new = [0, 3, 2 * page, 5], [11, 0, page + 1, 2]
+    total = [a + b for a, b in zip(before, new)]
+    pages = sum(-(-n // page) for n in total) + 2
+    kv = make_cache(dev_ctx, dtype, page, heads, dim, pages, fill=0xA5)
+    table = make_table(total, page, pages, g)
+    rows = sum(new) + 3
+    k = torch.randn(rows, heads, dim, device="cuda", generator=g)
+    k[1] = 0.0                                            # scale 0
+    k[2, :, 3] = -k[2, :, 7].abs().clamp(min=4.0)         # a tie in magnitude, the negative one first
+    k[2, :, 7] = -k[2, :, 3]
+    k[3] *= 1e-30
+    k, v = k.to(IO[kind]), torch.randn(rows, heads, dim, device="cuda", generator=g).to(IO[kind])
+    old = kv.pages.clone()
+    start = torch.tensor(before, dtype=torch.int32, device="cuda")
+    kv.write(k, v, table, start=start, cu_tokens=ragged(new))
+    dev_ctx.synchronize()
+    # place of every stored token
+    where, row = [], 0
+    for s, (b, m) in enumerate(zip(before, new)):
+        for j in range(m):
+            where.append((row, int(table[s, (b + j) // page]), (b + j) % page))
+            row += 1
+    r, pg, slot = (torch.tensor(c, device="cuda") for c in zip(*where))
+    for j, x in ((0, k), (1, v)):
+        got = cache_values(kv.pages, dtype, page, heads, dim, j)[pg, :, slot]
+        assert torch.equal(got, expected_store(sp, ctx, x, dtype)[r])
+    # nothing else changed: put the written slots' old bytes back and compare
+    rb, ns, at, chunk = layout(dtype, dim, page)
+    a, b = (t.reshape(-1, heads, chunk).clone() for t in (kv.pages, old))
+    for _, p_, s_ in where:
+        for o, n in ((at[0] + s_ * rb, rb), (at[1] + s_ * rb, rb), (at[2] + 4 * s_ * ns, 4 * (dim // 32) * (ns > 0)),
+                     (at[3] + 4 * s_ * ns, 4 * (dim // 32) * (ns > 0))):
+            a[p_, :, o:o + n] = 0
+            b[p_, :, o:o + n] = 0
+    assert torch.equal(a, b)
+    # read back: one fp32 product, rounded once
+    ko, vo = torch.full_like(k, 7.0), torch.full_like(v, 7.0)
+    kv.read(ko, vo, table, start=start, cu_tokens=ragged(new))
+    dev_ctx.synchronize()
+    for j, out in ((0, ko), (1, vo)):
+        want = cache_values(kv.pages, dtype, page, heads, dim, j)[pg, :, slot].float().to(IO[kind])
+        assert torch.equal(out[:sum(new)], want)
+        assert (out[sum(new):] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", CACHES)
+def test_one_token_each_strided(sp, dev_ctx, ctx, dtype):
+    """A decoding step out of a fused projection, rows not on 16 bytes."""
+    g = gen(5)
+    lens, page, heads, dim = [0, 15, 16, 40], 16, 2, 64
+    kv = make_cache(dev_ctx, dtype, page, heads, dim, 12)
+    table = make_table([n + 1 for n in lens], page, 12, g)
+    buf = torch.randn(4, 6 * dim + 3, device="cuda", generator=g).bfloat16()
+    k = buf[:, 1:1 + 2 * dim].unflatten(1, (2, dim))
+    v = buf[:, 3 + 4 * dim:3 + 6 * dim].unflatten(1, (2, dim))
+    start = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    kv.write(k, v, table, start=start)
+    ko, vo = torch.empty(4, 2, dim, device="cuda"), torch.empty(4, 2, dim, device="cuda")
+    kv.read(ko, vo, table, start=start)
+    dev_ctx.synchronize()
+    assert torch.equal(ko, expected_store(sp, ctx, k, dtype).float())
+    assert torch.equal(vo, expected_store(sp, ctx, v, dtype).float())
+
+
+def test_nan_and_infinity_quantise_as_documented(sp, dev_ctx, ctx):
+    for dtype in ("q8_0", "q4_0"):
+        x = torch.randn(2, 1, 64, device="cuda", generator=gen(9))
+        x[0, 0, 3], x[0, 0, 40], x[1, 0, 5] = math.nan, -math.inf, math.inf
+        kv = make_cache(dev_ctx, dtype, 4, 1, 64, 2)
+        table = torch.tensor([[0], [1]], dtype=torch.int32, device="cuda")
+        kv.write(x, x, table)
+        dev_ctx.synchronize()
+        got = cache_values(kv.pages, dtype, 4, 1, 64, 0)[:, :, 0]
+        want = expected_store(sp, ctx, x, dtype)
+        assert torch.equal(torch.nan_to_num(got, 7.0, 8.0, 9.0), torch.nan_to_num(want, 7.0, 8.0, 9.0))
+
+
+def test_bad_places_are_skipped_and_reported(sp, dev_ctx):
+    kv = make_cache(dev_ctx, "bf16", 4, 1, 64, 3, fill=0)
+    x = torch.ones(4, 1, 64, device="cuda", dtype=torch.bfloat16)
+    table = torch.tensor([[0, 1], [3, 1], [-1, 1], [2, 2]], dtype=torch.int32, device="cuda")
+    start = torch.tensor([0, 0, 0, 8], dtype=torch.int32, device="cuda")
+    kv.write(x, x, table, start=start)
+    with pytest.raises(sp.SapphireError, match="paged key-value cache"):
+        dev_ctx.synchronize()
+    got = cache_values(kv.pages, "bf16", 4, 1, 64, 0)
+    assert got[0, 0, 0].eq(1).all() and got.sum().item() == 64
+    out = torch.full_like(x, 5.0)
+    kv.read(out, out.clone(), table, start=start)
+    with pytest.raises(sp.SapphireError, match="paged key-value cache"):
+        dev_ctx.synchronize()
+    assert out[0].eq(1).all() and out[1:].eq(5).all()
+    start[3] = -1
+    kv.write(x[3:], x[3:], table[3:], start=start[3:])
+    with pytest.raises(sp.SapphireError, match="paged key-value cache"):
+        dev_ctx.synchronize()
+    kv.write(x[:1], x[:1], table[:1])                # the context works on
+    dev_ctx.synchronize()
+
+
+def test_cache_refusals(sp, dev_ctx):
+    from sapphire_b200.attention import KVCache
+    kv = make_cache(dev_ctx, "q8_0", 4, 2, 64, 3)
+    x = torch.zeros(2, 2, 64, device="cuda")
+    table = torch.zeros(2, 1, device="cuda", dtype=torch.int32)
+    for bad, match in (((x[:1], x, table), "shape"), ((x, x[..., :32], table), "shape"), ((x, x.half(), table), "one type"),
+                       ((x, x, table.long()), "int32"), ((x, x, table[:1]), "without cu_tokens"),
+                       ((x.cpu(), x, table), "device memory"), ((x, x, table.cpu()), "device memory")):
+        with pytest.raises(sp.SapphireError, match=match):
+            kv.write(*bad)
+    with pytest.raises(sp.SapphireError, match="shape"):
+        kv.write(x, x, table, cu_tokens=torch.zeros(2, device="cuda", dtype=torch.int32))
+    with pytest.raises(sp.SapphireError, match="byte tensor"):
+        KVCache(dev_ctx, "q8_0", 4, 2, 64, kv.pages[:, :-1])
+    with pytest.raises(sp.SapphireError, match="16-byte"):
+        flat = torch.zeros(kv.pages.numel() + 16, device="cuda", dtype=torch.uint8)
+        KVCache(dev_ctx, "q8_0", 4, 2, 64, flat[8:8 + kv.pages.numel()].view_as(kv.pages)).write(x, x, table)
+    kv.write(x[:0], x[:0], table[:0])
+    dev_ctx.synchronize()
+
+
+# ------------------------------------------------------------------- attend --
+def attend_plain(kv, q, table, lengths, page, heads, dim, dtype, window=0, scale=None):
+    """fp64 out, lse and the error bound before rounding."""
+    k, v = (cache_values(kv.pages, dtype, page, heads, dim, j) for j in (0, 1))
+    out, bound = torch.zeros_like(q, dtype=torch.float64), torch.zeros_like(q, dtype=torch.float64)
+    lse = torch.full(q.shape[:2], -math.inf, dtype=torch.float64, device="cuda")
+    lse_bound = torch.zeros_like(lse)
+    group = q.shape[1] // heads
+    scale = dim ** -0.5 if scale is None else scale
+    for s, n in enumerate(lengths):
+        first = max(0, n - window) if window else 0
+        if n <= first:
+            continue
+        t = torch.arange(first, n, device="cuda")
+        pg, slot = table[s].long()[t // page], t % page
+        for h in range(heads):
+            x = q[s, h * group:(h + 1) * group].double()
+            ks, vs = k[pg, h, slot], v[pg, h, slot]
+            score = x @ ks.T * scale
+            ds = (x.abs() @ ks.abs().T * abs(scale)).amax(-1) * 2.0 ** -19
+            out[s, h * group:(h + 1) * group] = torch.softmax(score, -1) @ vs
+            bound[s, h * group:(h + 1) * group] = vs.abs().max() * (4 * ds + 2.0 ** -17)[:, None]
+            lse[s, h * group:(h + 1) * group] = torch.logsumexp(score, -1)
+            lse_bound[s, h * group:(h + 1) * group] = 2 * ds + 2.0 ** -17
+    return out, bound, lse, lse_bound
+
+
+def attend_case(ctx, dtype, kind, lengths, heads, group, dim, page, window=0, seed=0, scale=None, fill=0xFF, loud=1.0):
+    """A filled cache; slots that no sequence holds are 0xFF bytes (NaN in every
+    dense type and in every scale)."""
+    g = gen(seed)
+    pages = sum(-(-n // page) for n in lengths) + 2
+    kv = make_cache(ctx, dtype, page, heads, dim, pages, fill=fill)
+    table = make_table(lengths, page, pages, g)
+    n = sum(lengths)
+    if n:
+        k = torch.randn(n, heads, dim, device="cuda", generator=g)
+        k[..., ::17] *= 4 * loud
+        v = torch.randn(n, heads, dim, device="cuda", generator=g) * torch.rand(n, heads, 1, device="cuda", generator=g) * loud
+        kv.write(k.to(IO[kind]), v.to(IO[kind]), table, cu_tokens=ragged(lengths))
+    q = torch.randn(len(lengths), heads * group, dim, device="cuda", generator=g).to(IO[kind])
+    return kv, table, q
+
+
+def check_attend(ctx, dtype, kind, lengths, heads, group, dim, page, window=0, seed=0, scale=None, loud=1.0):
+    kv, table, q = attend_case(ctx, dtype, kind, lengths, heads, group, dim, page, window, seed, scale, loud=loud)
+    out, lse = torch.full_like(q, 3.0), torch.full(q.shape[:2], 3.0, device="cuda")
+    kv.attend(q, table, torch.tensor(lengths, dtype=torch.int32, device="cuda"), out, window=window, lse=lse,
+              scale=0.0 if scale is None else scale)
+    ctx.synchronize()
+    want, bound, want_lse, lse_bound = attend_plain(kv, q, table, lengths, page, heads, dim, dtype, window, scale)
+    assert_within(out, want, bound, f"{dtype} {kind}")
+    empty = torch.tensor([n == 0 for n in lengths], device="cuda")
+    assert (out[empty] == 0).all() and (lse[empty] == -math.inf).all()
+    if (~empty).any():
+        assert_within(lse[~empty], want_lse[~empty], lse_bound[~empty], "lse")
+    return kv, table, q, out
+
+
+@pytest.mark.parametrize("dtype", CACHES)
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("dim,heads,group", [(64, 2, 1), (96, 1, 3), (128, 3, 4), (192, 2, 8), (256, 1, 5)])
+def test_attend_types_and_heads(dev_ctx, dtype, kind, dim, heads, group):
+    check_attend(dev_ctx, dtype, kind, [37, 0, 1, 200, 16, 65], heads, group, dim, 16, seed=dim)
+
+
+@pytest.mark.parametrize("dtype", CACHES)
+@pytest.mark.parametrize("page", [1, 3, 16, 24, 100, 4096])
+def test_attend_pages(dev_ctx, dtype, page):
+    check_attend(dev_ctx, dtype, "f32", [1, 15, 33, 257, 1000], 2, 4, 128, page, seed=page)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "q8_0"])
+@pytest.mark.parametrize("window", [1, 16, 100, 513, 5000])
+def test_attend_window(dev_ctx, dtype, window):
+    check_attend(dev_ctx, dtype, "f32", [0, 1, 16, 99, 100, 101, 700, 1501], 1, 2, 64, 16, window=window, seed=window)
+
+
+@pytest.mark.parametrize("dtype", CACHES)
+@pytest.mark.parametrize("group", [2, 6, 7, 9, 12, 16, 33])
+def test_attend_groups(dev_ctx, dtype, group):
+    check_attend(dev_ctx, dtype, "bf16", [130, 7], 2, group, 128, 16, seed=group)
+
+
+@pytest.mark.parametrize("dtype", CACHES)
+def test_attend_long_and_many(dev_ctx, dtype):
+    check_attend(dev_ctx, dtype, "f32", [20011], 1, 4, 64, 64, seed=1)
+    check_attend(dev_ctx, dtype, "bf16", [3 * i % 97 for i in range(300)], 2, 4, 64, 16, seed=2)
+
+
+@pytest.mark.parametrize("dtype", CACHES)
+@pytest.mark.parametrize("scale", [0.0078125, 1.5])
+def test_attend_scale_and_range(dev_ctx, dtype, scale):
+    """Loud keys and values; scores far apart, so single positions win."""
+    check_attend(dev_ctx, dtype, "f32", [300, 41], 1, 4, 128, 16, seed=3, scale=scale, loud=30.0)
+
+
+@pytest.mark.parametrize("dtype", ["q8_0", "q4_0"])
+def test_attend_scales_that_grow(dev_ctx, dtype):
+    """Values whose block scales rise by many powers of two along the sequence."""
+    g = gen(12)
+    n, heads, dim, page = 400, 1, 128, 16
+    kv = make_cache(dev_ctx, dtype, page, heads, dim, 30)
+    table = make_table([n], page, 30, g)
+    k = torch.randn(n, heads, dim, device="cuda", generator=g)
+    v = torch.randn(n, heads, dim, device="cuda", generator=g) * torch.logspace(-12, 12, n, base=2, device="cuda")[:, None, None]
+    kv.write(k, v, table, cu_tokens=ragged([n]))
+    q, out = torch.randn(1, 4, dim, device="cuda", generator=g), torch.empty(1, 4, dim, device="cuda")
+    kv.attend(q, table, torch.tensor([n], dtype=torch.int32, device="cuda"), out)
+    dev_ctx.synchronize()
+    want, bound, _, _ = attend_plain(kv, q, table, [n], page, heads, dim, dtype)
+    assert_within(out, want, bound)
+
+
+def test_attend_q_far_from_one(dev_ctx):
+    """Queries of large and small magnitude against every cache type."""
+    for dtype in CACHES:
+        kv, table, q = attend_case(dev_ctx, dtype, "f32", [90, 33], 1, 4, 64, 16, seed=4)
+        lengths = torch.tensor([90, 33], dtype=torch.int32, device="cuda")
+        for size, scale in ((2.0 ** 40, 2.0 ** -43), (2.0 ** -60, 2.0 ** 57)):
+            x, out = q * size, torch.empty_like(q)
+            kv.attend(x, table, lengths, out, scale=scale)
+            dev_ctx.synchronize()
+            want, bound, _, _ = attend_plain(kv, x, table, [90, 33], 16, 1, 64, dtype, scale=scale)
+            assert_within(out, want, bound, f"{dtype} {size}")
+
+
+def test_attend_strides_offset_and_shared_pages(dev_ctx):
+    kv, table, _ = attend_case(dev_ctx, "bf16", "f16", [40, 70], 2, 3, 64, 16, seed=5)
+    buf = torch.randn(2, 6 * 64 * 2 + 1, device="cuda", generator=gen(6)).half()
+    q = buf[:, 1:].unflatten(1, (12, 64))[:, ::2]
+    res = torch.full((2, 8, 64), 2.0, device="cuda", dtype=torch.float16)
+    out = res[:, 1:7]
+    table[1, 0] = table[0, 0]                                  # a prefix both sequences hold
+    kv.attend(q, table, torch.tensor([38, 68], dtype=torch.int32, device="cuda"), out, length_offset=2)
+    dev_ctx.synchronize()
+    want, bound, _, _ = attend_plain(kv, q, table, [40, 70], 16, 2, 64, "bf16")
+    assert_within(out, want, bound)
+    assert (res[:, 0] == 2).all() and (res[:, 7] == 2).all()
+
+
+def test_attend_is_repeatable(dev_ctx):
+    kv, table, q = attend_case(dev_ctx, "q8_0", "bf16", [3000, 17, 999], 2, 4, 128, 16, seed=7)
+    n = torch.tensor([3000, 17, 999], dtype=torch.int32, device="cuda")
+    a, b = torch.empty_like(q), torch.empty_like(q)
+    kv.attend(q, table, n, a)
+    for _ in range(5):
+        kv.attend(q, table, n, b)
+        dev_ctx.synchronize()
+        assert torch.equal(a, b)
+
+
+def test_attend_far_offsets(dev_ctx):
+    """Pages behind 4 GB, and rows behind 2^31 elements."""
+    from sapphire_b200.attention import KVCache, kv_page_bytes
+    per = kv_page_bytes("bf16", 64, 8, 128)
+    count = (5 << 30) // per
+    kv = KVCache(dev_ctx, "bf16", 64, 8, 128, torch.empty(count, per, dtype=torch.uint8, device="cuda"))
+    n = [130, 64]
+    table = torch.tensor([[count - 1, 0, count - 2], [count - 3, -1, -1]], dtype=torch.int32, device="cuda")
+    g = gen(13)
+    k, v = (torch.randn(194, 8, 128, device="cuda", generator=g).bfloat16() for _ in range(2))
+    kv.write(k, v, table, cu_tokens=ragged(n))
+    q, out = torch.randn(2, 32, 128, device="cuda", generator=g).bfloat16(), torch.empty(2, 32, 128, device="cuda").bfloat16()
+    kv.attend(q, table, torch.tensor(n, dtype=torch.int32, device="cuda"), out)
+    ko, vo = torch.empty_like(k), torch.empty_like(v)
+    kv.read(ko, vo, table, cu_tokens=ragged(n))
+    dev_ctx.synchronize()
+    assert torch.equal(ko, k) and torch.equal(vo, v)
+    small = make_cache(dev_ctx, "bf16", 64, 8, 128, 4)
+    near = torch.tensor([[3, 0, 2], [1, -1, -1]], dtype=torch.int32, device="cuda")
+    small.write(k, v, near, cu_tokens=ragged(n))
+    again = torch.empty_like(out)
+    small.attend(q, near, torch.tensor(n, dtype=torch.int32, device="cuda"), again)
+    dev_ctx.synchronize()
+    assert torch.equal(out, again)
+
+
+def test_attend_bad_places(sp, dev_ctx):
+    """A page outside the cache counts as not attended, a length outside the
+    table is clamped; both are reported, and the context works on."""
+    kv, table, q = attend_case(dev_ctx, "bf16", "f32", [40, 20], 1, 2, 64, 16, seed=8)
+    good = table.clone()
+    lengths = torch.tensor([40, 20], dtype=torch.int32, device="cuda")
+    out, ref = torch.empty_like(q), torch.empty_like(q)
+    kv.attend(q, good, lengths, ref)
+    dev_ctx.synchronize()
+    for bad in (-5, kv.pages.shape[0], 2 ** 31 - 1):
+        table[0, 1] = bad
+        kv.attend(q, table, lengths, out)
+        with pytest.raises(sp.SapphireError, match="paged key-value cache"):
+            dev_ctx.synchronize()
+        assert torch.equal(out[1], ref[1]) and torch.isfinite(out[0]).all()
+    for bad in (-1, 49, 2 ** 31 - 1):
+        kv.attend(q, good, torch.tensor([bad, 20], dtype=torch.int32, device="cuda"), out)
+        with pytest.raises(sp.SapphireError, match="paged key-value cache"):
+            dev_ctx.synchronize()
+        assert torch.equal(out[1], ref[1])
+        assert bad > 0 or (out[0] == 0).all()
+    kv.attend(q, good, lengths, out)
+    dev_ctx.synchronize()
+    assert torch.equal(out, ref)
+
+
+def test_attend_refusals(sp, dev_ctx):
+    kv, table, q = attend_case(dev_ctx, "f32", "f32", [4, 5], 2, 2, 64, 16)
+    n, out = torch.tensor([4, 5], dtype=torch.int32, device="cuda"), torch.empty_like(q)
+    for args, kw, match in (((q[:, :3], table, n, out[:, :3]), {}, "query heads"), ((q, table, n, out.half()), {}, "one type"),
+                            ((q, table, n[:1], out), {}, "shape"), ((q, table[:1], n, out), {}, "shape"),
+                            ((q, table, n.long(), out), {}, "int32"), ((q, table, n, out), {"window": -1}, "window"),
+                            ((q, table, n, out), {"scale": math.inf}, "scale"), ((q.cpu(), table, n, out), {}, "device memory"),
+                            ((q, table, n, out.cpu()), {}, "device memory"), ((q, table, n.cpu(), out), {}, "device memory"),
+                            ((q, table, n, out), {"lse": torch.zeros(2, 3, device="cuda")}, "lse")):
+        with pytest.raises(sp.SapphireError, match=match):
+            kv.attend(*args, **kw)
+    kv.attend(q[:0], table[:0], n[:0], out[:0])
+    dev_ctx.synchronize()
+
+
+# ----------------------------------------------------------------- together --
+@pytest.mark.parametrize("dtype", CACHES)
+def test_decoding_steps_together(dev_ctx, dtype):
+    """rope, write and attend as a serving loop runs them: a ragged prompt, then
+    steps of one token each, against the dense 64-bit computation."""
+    from sapphire_b200.attention import Rope
+    g = gen(21)
+    heads, group, dim, page, steps = 2, 3, 64, 8, 5
+    prompt = [9, 1, 20]
+    total = [n + steps for n in prompt]
+    kv = make_cache(dev_ctx, dtype, page, heads, dim, 20, fill=0xFF)
+    table = make_table(total, page, 20, g)
+    rope = Rope(dev_ctx, dim, theta=1e4)
+    pos = torch.cat([torch.arange(n, device="cuda", dtype=torch.int32) for n in prompt])
+    k, v = (torch.randn(sum(prompt), heads, dim, device="cuda", generator=g) for _ in range(2))
+    rope.apply(pos, k=k)
+    kv.write(k, v, table, cu_tokens=ragged(prompt))
+    lengths = torch.tensor(prompt, dtype=torch.int32, device="cuda")
+    for step in range(steps):
+        q, k, v = (torch.randn(3, h, dim, device="cuda", generator=g) for h in (heads * group, heads, heads))
+        q0, k0 = q.clone(), k.clone()
+        rope.apply(lengths, q, k)
+        kv.write(k, v, table, start=lengths)
+        out = torch.empty_like(q)
+        kv.attend(q, table, lengths, out, length_offset=1)
+        now = [n + step + 1 for n in prompt]
+        dev_ctx.synchronize()
+        for x, x0 in ((q, q0), (k, k0)):
+            want, e = rope_plain(x0, lengths, dim, "half")
+            assert_within(x, want, e)
+        want, bound, _, _ = attend_plain(kv, q, table, now, page, heads, dim, dtype)
+        assert_within(out, want, bound)
+        lengths += 1
+
+
+def test_another_stream_and_device_guard(sp):
+    """Two contexts on streams of their own, each with its cache."""
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ctxs, runs = [], []
+    for i, st in enumerate(streams):
+        c = sp.Context(num_threads=1)
+        c.set_stream(st.cuda_stream)
+        ctxs.append(c)
+        with torch.cuda.stream(st):
+            lengths = [2500, 0, 300 + i]
+            kv, table, q = attend_case(c, "q8_0", "f32", lengths, 2, 4, 64, 16, seed=30 + i)
+            runs.append((kv, table, q, torch.tensor(lengths, dtype=torch.int32, device="cuda"), torch.empty_like(q), lengths))
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for kv, table, q, n, out, _ in runs:
+            kv.attend(q, table, n, out)
+    for c, (kv, table, q, n, out, lengths) in zip(ctxs, runs):
+        c.synchronize()
+        want, bound, _, _ = attend_plain(kv, q, table, lengths, 16, 2, 64, "q8_0")
+        assert_within(out, want, bound)
+        c.close()
