@@ -112,6 +112,8 @@ struct sapphire_context {
     int *h_err = nullptr;    int *d_err = nullptr;
     // bf16 copy of the activations for the tensor-core batched product.
     float *d_xb = nullptr;   size_t d_xb_cap = 0;
+    // Partial results of split sequences (attention.cu).
+    float *d_attn = nullptr; size_t d_attn_cap = 0;
 
     HostPool *pool = nullptr;
 

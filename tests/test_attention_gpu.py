@@ -685,3 +685,53 @@ def test_another_stream_and_device_guard(sp):
         want, bound, _, _ = attend_plain(kv, q, table, lengths, 16, 2, 64, "q8_0")
         assert_within(out, want, bound)
         c.close()
+
+
+def test_captured_calls_keep_workspaces_of_their_own(sp, dev_ctx):
+    """Two captured graphs replayed at the same time; new lengths take effect."""
+    st = torch.cuda.Stream()
+    dev_ctx.set_stream(st.cuda_stream)
+    sets = []
+    for i in range(2):
+        kv, table, q = attend_case(dev_ctx, "q8_0", "bf16", [1500, 900, 40], 2, 4, 128, 16, seed=40 + i)
+        n = torch.tensor([1500, 900, 40], dtype=torch.int32, device="cuda")
+        ws = torch.full((kv.workspace_bytes(3, 8),), 0xEE, dtype=torch.uint8, device="cuda")
+        sets.append((kv, table, q, n, torch.empty_like(q), ws))
+    dev_ctx.synchronize()
+    graphs = []
+    for kv, table, q, n, out, ws in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            with pytest.raises(sp.SapphireError, match="workspace"):
+                kv.attend(q, table, n, out)
+            kv.attend(q, table, n, out, workspace=ws)
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for lengths in ([1500, 900, 40], [3, 899, 0], [1400, 1, 40]):
+        for *_, n, out, ws in sets:
+            n.copy_(torch.tensor(lengths, dtype=torch.int32, device="cuda"))
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for graph, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    graph.replay()
+        torch.cuda.synchronize()
+        dev_ctx.synchronize()
+        for kv, table, q, n, out, ws in sets:
+            want, bound, _, _ = attend_plain(kv, q, table, lengths, 16, 2, 128, "q8_0")
+            assert_within(out, want, bound)
+
+
+def test_workspace_refusals(sp, dev_ctx):
+    kv, table, q = attend_case(dev_ctx, "bf16", "bf16", [4], 1, 2, 64, 16)
+    n, out = torch.tensor([4], dtype=torch.int32, device="cuda"), torch.empty_like(q)
+    need = kv.workspace_bytes(1, 2)
+    for ws in (torch.zeros(need - 1, dtype=torch.uint8, device="cuda"), torch.zeros(need + 16, dtype=torch.uint8, device="cuda")[8:]):
+        with pytest.raises(sp.SapphireError, match="workspace"):
+            kv.attend(q, table, n, out, workspace=ws)
+    with pytest.raises(sp.SapphireError, match="device memory"):
+        kv.attend(q, table, n, out, workspace=torch.zeros(need, dtype=torch.uint8).contiguous())
+    with pytest.raises(sp.SapphireError, match="query heads"):
+        kv.workspace_bytes(1, 0)
+    kv.attend(q, table, n, out, workspace=torch.zeros(need, dtype=torch.uint8, device="cuda"))
+    dev_ctx.synchronize()
