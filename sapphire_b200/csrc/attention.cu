@@ -63,6 +63,11 @@ extern "C" SAPPHIRE_API int sapphire_attention_device(kernel_context_t *ctx, con
         !on_device(ctx, who, "out", a->out) || !on_device(ctx, who, "page_table", a->page_table) ||
         !on_device(ctx, who, "lengths", a->lengths) || (a->lse && !on_device(ctx, who, "lse", a->lse)))
         return -1;
+    // The kernels number tiles (of 64 tokens or more) in 31 bits.
+    if ((double)a->sequences * a->heads * ((double)a->table_stride * cache->page_size / 64 + 1) >= 2147483648.0) {
+        ctx_fail(ctx, who, "%d sequences of up to %d pages are more tiles than 2^31", a->sequences, a->table_stride);
+        return -1;
+    }
     p.q = a->q;
     p.out = a->out;
     p.lse = a->lse;
@@ -85,6 +90,11 @@ extern "C" SAPPHIRE_API int sapphire_attention_device(kernel_context_t *ctx, con
     p.head_tiles = (p.group + attn_tile_heads(p.group) - 1) / attn_tile_heads(p.group);
     p.page_mul = (1ull << 32) / cache->page_size + 1;
     p.blocks = attn_blocks(ctx, cache);
+    p.aligned = cache->page_size % 16 == 0;
+    p.device = ctx->device;
+    const long long items = (long long)a->sequences * cache->kv_heads * p.head_tiles;
+    p.by_item = items <= p.blocks;
+    p.joins = (int)std::min<long long>(items, p.blocks);
     AttnDevice g(ctx->device);
     const size_t need = attn_workspace(ctx, cache, p.group);
     char *ws = static_cast<char *>(a->workspace);

@@ -33,10 +33,16 @@
 //   P (B operand): a movmatrix of the packed (high, low) pairs.
 //
 // Quantised rows are kept as words of 4 codes in the order [8][nb], so the same
-// lanes read consecutive bytes; codes become fp16 exactly (1024 + code - 1152,
-// or - 1032).  K's scale multiplies the 32-dim partial score; V's scale is
-// multiplied into the probability (one B operand per 32 dims), brought into
-// fp16's range by a power of two per warp that grows with the scales seen.
+// lanes read consecutive bytes.  Under a bf16 output codes are multiplied as
+// the integers they are: the query becomes 15-bit integers (two signed bytes),
+// and a tile's probabilities times V's scales become 15-bit integers relative
+// to the tile's largest, per head and block of 32 dims; sums are exact, the
+// codes' offsets come off with an MMA of ones, and one conversion and product
+// per sum brings it to fp32.  That is a third of the instructions of converting
+// codes to fp16, which fp32 and fp16 outputs take (1024 + code - 1152 or - 1032,
+// exactly): there K's scale multiplies the 32-dim partial score and V's scale the
+// probability, brought into fp16's range by a power of two per warp that grows
+// with the scales seen.
 //
 // Split.  The tiles (64 tokens of one KV head and up to 8 query heads) of all
 // sequences are numbered in a row and cut into as many equal ranges as the GPU
@@ -47,7 +53,7 @@
 #include "attention.cuh"
 
 constexpr int kAttnWarps = 4;
-constexpr int kAttnTile = 16 * kAttnWarps;    // tokens of one tile
+constexpr int kAttnSmem = 224 * 1024;         // shared memory that an SM's blocks divide
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttnParams {
@@ -63,26 +69,40 @@ struct AttnParams {
     int table_stride, length_offset, window;
     float scale;                   // scores times log2 e
     unsigned long long page_mul;   // floor(2^32 / page_size) + 1
+    int tile_pages, tile_slots;    // a block's tile of tokens as whole pages and the rest
+    bool aligned;                  // pages of a multiple of 16 tokens
+    int device;
     int blocks;
     float *part;                   // [blocks][2][GH * (HD + 2)]
-    int4 *piece;                   // [blocks] (sequence, head tile, blocks it spans, -)
+    // Items that several blocks hold: (sequence, head tile, blocks, first
+    // block), by item where there are no more of them than blocks (by_item),
+    // else by first block; 0 blocks where there is nothing to join.
+    int4 *piece;
+    bool by_item;
+    int joins;                     // entries of piece
     int *err;
 };
 
 // Query heads of a tile for a group of this size.
 inline bool attn_wide(int group) { return group > 4; }
 inline int attn_tile_heads(int group) { return attn_wide(group) ? 8 : 4; }
-// Resident blocks per SM that each variant is compiled for.
+// MMA tiles (16 tokens) of a warp's tile, and resident blocks per SM.
+constexpr int attn_m_tiles(int cache, int hd) { return cache == DTYPE_Q4_0 || cache == DTYPE_Q8_0 ? 2 : 1; }
 constexpr int attn_blocks_per_sm(int cache, int hd) {
-    const bool quant = cache == DTYPE_Q8_0 || cache == DTYPE_Q4_0;
-    return quant ? (hd <= 128 ? 4 : hd <= 192 ? 3 : 2) : (hd <= 96 ? 4 : hd <= 192 ? 3 : 2);
+    if (cache == DTYPE_F32) return hd <= 64 ? 3 : hd <= 128 ? 2 : 1;
+    if (cache == DTYPE_Q4_0) return hd <= 64 ? 4 : hd <= 128 ? 3 : 2;
+    if (cache == DTYPE_Q8_0) return hd <= 64 ? 4 : hd <= 128 ? 3 : 2;
+    return hd <= 64 ? 4 : hd <= 128 ? 3 : 2;
 }
 
 #ifdef __CUDACC__
 
+// Codes are multiplied as integers where the output's rounding allows.
+template <int kCache, bool kExact>
+constexpr bool kAttnInt = (kCache == DTYPE_Q8_0 || kCache == DTYPE_Q4_0) && !kExact;
 // 2^(p + kBias): probabilities use the upper end of fp16 where the MMA is fp16.
-template <int kCache>
-constexpr float kAttnBias = (kCache == DTYPE_BF16 || kCache == DTYPE_F32) ? 0.0f : 14.0f;
+template <int kCache, bool kExact>
+constexpr float kAttnBias = (kCache == DTYPE_BF16 || kCache == DTYPE_F32 || kAttnInt<kCache, kExact>) ? 0.0f : 14.0f;
 
 __device__ __forceinline__ float attn_exp2(float x) {
     float y;
@@ -113,6 +133,31 @@ __device__ __forceinline__ uint32_t round_tf32(float x) {
     uint32_t y;
     asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(y) : "f"(x));
     return y;
+}
+// d = a b + c on 32 unsigned (kSigned: signed) bytes of a and signed bytes of b.
+template <bool kSigned>
+__device__ __forceinline__ void mma8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                     uint32_t b1, const int (&c)[4]) {
+    if (kSigned)
+        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                     : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
+    else
+        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                     : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
+}
+// The power of two that brings a value with these (absolute) bits to [2^6, 2^7),
+// and its inverse, NaN for infinities and NaN.
+__device__ __forceinline__ float unit_of(uint32_t bits, float &inverse) {
+    const int e = (int)(bits >> 23), c = min(max(e, 7), 253);
+    inverse = __uint_as_float(e == 255 ? 0x7fc00000u : (uint32_t)(c - 6) << 23);
+    return __uint_as_float((uint32_t)(260 - c) << 23);
+}
+__device__ __forceinline__ uint32_t max_over_rows(uint32_t x) {
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) x = max(x, __shfl_xor_sync(0xffffffffu, x, o));
+    return x;
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
@@ -169,48 +214,57 @@ __device__ __forceinline__ uint32_t nibbles_to_half2(uint32_t w) {
     return *reinterpret_cast<const uint32_t *>(&v);
 }
 
-// N bytes at p (aligned to the largest power of two up to 16 that divides N)
-// into 32-bit words; zeros where !ok.
+__device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// 16 (8) bytes from global to shared memory, zeros where bytes is 0.
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t *src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy8(uint32_t dst, const uint8_t *src, int bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
-__device__ __forceinline__ void load_bytes(const uint8_t *p, bool ok, uint32_t *w) {
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// N bytes of shared memory at p (aligned to the largest power of two up to 16
+// that divides N) as 32-bit words.
+template <int N>
+__device__ __forceinline__ void read_bytes(const uint8_t *p, uint32_t *w) {
     if constexpr (N % 16 == 0) {
 #pragma unroll
         for (int i = 0; i < N / 16; ++i) {
-            uint4 u = make_uint4(0, 0, 0, 0);
-            if (ok)
-                asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                             : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
-                             : "l"(p + 16 * i));
+            const uint4 u = reinterpret_cast<const uint4 *>(p)[i];
             w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
         }
     } else if constexpr (N % 8 == 0) {
 #pragma unroll
         for (int i = 0; i < N / 8; ++i) {
-            uint2 u = make_uint2(0, 0);
-            if (ok) u = __ldg(reinterpret_cast<const uint2 *>(p) + i);
+            const uint2 u = reinterpret_cast<const uint2 *>(p)[i];
             w[2 * i] = u.x, w[2 * i + 1] = u.y;
         }
     } else if constexpr (N % 4 == 0) {
 #pragma unroll
-        for (int i = 0; i < N / 4; ++i) w[i] = ok ? __ldg(reinterpret_cast<const uint32_t *>(p) + i) : 0u;
+        for (int i = 0; i < N / 4; ++i) w[i] = reinterpret_cast<const uint32_t *>(p)[i];
     } else {
         static_assert(N % 2 == 0, "");
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) {
-            const uint32_t h = ok ? __ldg(reinterpret_cast<const uint16_t *>(p) + i) : 0u;
+            const uint32_t h = reinterpret_cast<const uint16_t *>(p)[i];
             if (i % 2 == 0) w[i / 2] = h;
             else w[i / 2] |= h << 16;
         }
     }
 }
 template <int N>
-__device__ __forceinline__ void load_scales(const uint8_t *p, bool ok, float (&s)[N]) {
+__device__ __forceinline__ void read_scales(const uint8_t *p, float (&s)[N]) {
     constexpr int kPad = N <= 2 ? 2 : N <= 4 ? 4 : 8;
     float f[kPad];
-    load_bytes<kPad * 4>(p, ok, reinterpret_cast<uint32_t *>(f));
+    read_bytes<kPad * 4>(p, reinterpret_cast<uint32_t *>(f));
 #pragma unroll
     for (int i = 0; i < N; ++i) s[i] = f[i];
 }
+#endif  // __CUDACC__
 
 // Shapes of one variant.
 template <int kCache, int HD>
@@ -219,24 +273,41 @@ struct AttnShape {
     static constexpr bool kF32 = kCache == DTYPE_F32;
     static constexpr bool kBf16 = kCache == DTYPE_BF16;
     static constexpr int NB = HD / 32;
-    // Dims of one register chunk: 32 registers of K (or V) a lane.
-    static constexpr int kChunk = kQuant ? HD : kF32 ? 64 : 128;
-    static constexpr int kChunks = (HD + kChunk - 1) / kChunk;
-    // Registers of a chunk: 2 K rows (4 lanes share a row) or 4 V rows (8 lanes).
-    static constexpr int kRegs = kCache == DTYPE_Q8_0 ? HD / 8 : kCache == DTYPE_Q4_0 ? (HD / 16 < 8 ? 8 : HD / 16) : 32;
-    static constexpr int kScaleBytes = NB <= 2 ? 8 : NB <= 4 ? 16 : 32;
-    static constexpr int kChunkBytes = 256;                       // of a dense row
     static constexpr int kRowBytes = kCache == DTYPE_Q8_0 ? HD : kCache == DTYPE_Q4_0 ? HD / 2 : kF32 ? 4 * HD : 2 * HD;
-    // Query parts in shared memory: rows of 8 columns, padded so that the rows
-    // of neighbouring lanes fall on the other half of the banks.
+    static constexpr int kScaleBytes = !kQuant ? 0 : NB <= 2 ? 8 : NB <= 4 ? 16 : 32;
+    // Tokens of a warp's tile: two MMA tiles where rows are short.
+    static constexpr int MT = attn_m_tiles(kCache, HD);
+    static constexpr int kTok = 16 * MT;
+    // A slot of a warp's ring: the K or the V rows of a tile, each row padded
+    // off the banks of its neighbours, their scales, and the tokens that count.
+    static constexpr int kStride = kRowBytes + (kF32 ? 32 : 16);
+    static constexpr int kScaleOff = kTok * kStride;
+    static constexpr int kMaskOff = kScaleOff + kTok * kScaleBytes;
+    static constexpr int kSlot = kMaskOff + 16;
+    static constexpr int kBlocks = attn_blocks_per_sm(kCache, HD);
+    // Query parts: rows of 8 columns, padded so that the rows of neighbouring
+    // lanes fall on the other half of the banks.
     static constexpr int kQElem = kF32 ? 4 : 2;
     static constexpr int kQStride = (HD * kQElem) % 128 == 0 ? HD * kQElem + 64 : HD * kQElem;
+    // Slots that fit beside the query's parts, of what an SM has for each block.
+    static constexpr int kDigitStride = HD % 128 == 96 ? HD : HD + 32;        // of a row of query bytes
+    static constexpr int kMaxQS = kBf16 ? 3 : 2;
+    static constexpr int kFit = (kAttnSmem / kBlocks - kMaxQS * 8 * kQStride - 2048) / (kAttnWarps * kSlot);
+    static constexpr int R = kFit > 6 ? 6 : kFit;
+    static_assert(R >= 2, "a ring of K and V rows does not fit");
 };
 
+#ifdef __CUDACC__
+// What an item costs besides its tiles (its query, the filling of the rings and
+// the joining of the warps), in tiles: the ranges of blocks are cut in these
+// units, so one that meets many short sequences takes fewer tiles.
+constexpr int kAttnItemUnits = 2;
 // The positions a sequence's new token attends to, as tiles.
 struct AttnSpan {
-    int first, end, tile0, tiles;
+    int first, end, tile0, tiles, units;
 };
+// (tiles of kTile tokens)
+template <int kTile>
 __device__ __forceinline__ AttnSpan attn_span(const AttnParams &p, int s, bool report) {
     long long n = (long long)__ldg(p.lengths + s) + p.length_offset;
     const long long room = min((long long)p.table_stride * p.l.page_size, 0x7fffffc0ll);
@@ -247,65 +318,81 @@ __device__ __forceinline__ AttnSpan attn_span(const AttnParams &p, int s, bool r
     AttnSpan a;
     a.end = (int)n;
     a.first = p.window > 0 && a.end > p.window ? a.end - p.window : 0;
-    a.tile0 = a.first / kAttnTile;
-    a.tiles = max(1, (a.end + kAttnTile - 1) / kAttnTile - a.tile0);      // an empty sequence still writes its zeros
+    a.tile0 = a.first / kTile;
+    a.tiles = max(1, (a.end + kTile - 1) / kTile - a.tile0);      // an empty sequence still writes its zeros
+    a.units = a.tiles + kAttnItemUnits;
     return a;
 }
 
-// kQS, kPS: B operands of a query and of a probability (narrow: one holds two
-// parts, two hold three; wide: one part each).  kAligned: pages hold a multiple
-// of 16 tokens, so a warp's tile lies in one page.
-template <int kCache, int HD, bool kWide, int kQS, int kPS, bool kAligned>
+// Parts of a query and of a probability, as B operands (narrow: one holds two
+// parts, two hold three; wide: one part each).  kExact: fp32 and fp16 queries.
+template <int kCache, bool kWide, bool kExact>
+struct AttnParts {
+    static constexpr int kQS = !kWide ? (kCache == DTYPE_BF16 && kExact ? 2 : 1)
+                               : kCache == DTYPE_F32 ? 2 : kCache == DTYPE_BF16 ? (kExact ? 3 : 1) : kExact ? 2 : 1;
+    static constexpr bool kInt = kAttnInt<kCache, kExact>;        // wide: two signed bytes, an MMA each
+    static constexpr int kSets = kInt ? (kWide ? 2 : 1) : kQS;    // rows of 8 columns of the query
+    static constexpr int kPS = !kWide ? kQS : kCache == DTYPE_F32 ? 2 : kCache == DTYPE_BF16 ? (kExact ? 3 : 2) : kExact ? 2 : 1;
+};
+
+template <int kCache, int HD, bool kWide, bool kExact>
 __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD)) attend_kernel(const AttnParams p) {
     using Sh = AttnShape<kCache, HD>;
+    using Pt = AttnParts<kCache, kWide, kExact>;
     constexpr int GH = kWide ? 8 : 4, HL = kWide ? 2 : 1;         // heads of a tile, and of a lane
-    constexpr int NB = Sh::NB, kRegs = Sh::kRegs, kMTiles = HD / 16, C = Sh::kChunks;
+    constexpr int NB = Sh::NB, MT = Sh::MT, R = Sh::R, kTok = Sh::kTok, kTile = kTok * kAttnWarps, kMTiles = HD / 16;
+    constexpr int kQS = Pt::kQS, kPS = Pt::kPS, NA = kAttnInt<kCache, kExact> && !kWide ? 2 : 4;
+    constexpr bool kInt = kAttnInt<kCache, kExact>;
     constexpr bool kBf16 = Sh::kBf16, kF32 = Sh::kF32;
-    constexpr float kBias = kAttnBias<kCache>;
-    // The query's parts; at the end of an item, the warps' outputs.
-    constexpr int kQBytes = kQS * 8 * Sh::kQStride, kAccBytes = kAttnWarps * GH * HD * 4;
-    __shared__ __align__(16) uint8_t sq[kQBytes > kAccBytes ? kQBytes : kAccBytes];
-    float *const sacc = reinterpret_cast<float *>(sq);            // [warp][head][dim]
+    constexpr float kBias = kAttnBias<kCache, kExact>;
+    extern __shared__ __align__(16) uint8_t shared[];
+    uint8_t *const sq = shared;                                   // the query's parts
+    uint8_t *const rings = shared + Pt::kSets * 8 * Sh::kQStride;  // [warp][R] slots; at the end of an item the
+    float *const sacc = reinterpret_cast<float *>(rings);         // warps' outputs [warp][head][dim]
+    static_assert(R * Sh::kSlot >= GH * HD * 4, "the warps' outputs do not fit the rings");
     __shared__ float sm_m[kAttnWarps][GH], sm_l[kAttnWarps][GH];
     __shared__ float qmul[GH];
-    __shared__ long long warp_sum[kAttnWarps];
+    __shared__ unsigned warp_sum[kAttnWarps];
     __shared__ int found_seq;
-    __shared__ long long found_base;
+    __shared__ unsigned found_base;
+    __shared__ int qoff[kInt ? GH : 1][NB];                       // what the codes' offsets add to a block's integer score
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     pdl_trigger();
 
-    // ---- this block's range of tiles [lo, hi) of all sequences' ----
+    // ---- this block's range [lo, hi) of all items' units (fewer than 2^31,
+    //      checked on the host) ----
     const int per_thread = (p.sequences + kAttnWarps * 32 - 1) / (kAttnWarps * 32);
     const int s0 = min(tid * per_thread, p.sequences), s1 = min(s0 + per_thread, p.sequences);
     const int rows = p.l.kv_heads * p.head_tiles;                 // items of a sequence
-    long long mine = 0;
-    for (int s = s0; s < s1; ++s) mine += attn_span(p, s, blockIdx.x == 0).tiles;
-    long long incl = mine;
+    unsigned mine = 0;
+    for (int s = s0; s < s1; ++s) mine += attn_span<kTile>(p, s, blockIdx.x == 0).units;
+    unsigned incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+        const unsigned v = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += v;
     }
     if (lane == 31) warp_sum[warp] = incl;
     __syncthreads();
-    long long total = 0, before = 0;
+    unsigned total = 0, base = incl - mine;
 #pragma unroll
     for (int w = 0; w < kAttnWarps; ++w) {
-        if (w < warp) before += warp_sum[w];
+        if (w < warp) base += warp_sum[w];
         total += warp_sum[w];
     }
-    long long base = (before + incl - mine) * rows;
+    base *= rows;
     total *= rows;
-    const int blocks = (int)min((long long)p.blocks, total);
-    const int bid = blockIdx.x;
+    const unsigned blocks = min((unsigned)p.blocks, total), bid = blockIdx.x;
     if (bid >= blocks) {
-        if (tid == 0) p.piece[bid] = make_int4(0, 0, 0, 0);
+        if (tid == 0 && !p.by_item) p.piece[bid] = make_int4(0, 0, 0, 0);
         return;
     }
-    const long long lo = bid * total / blocks, hi = (bid + 1) * total / blocks;
-    if (lo >= base && lo < base + mine * rows) {
+    // The first `longer` blocks take each + 1 units, the others each.
+    const unsigned each = total / blocks, longer = total - each * blocks;
+    const unsigned lo = bid * each + min(bid, longer), hi = lo + each + (bid < longer ? 1 : 0);
+    if (lo >= base && lo - base < mine * rows) {
         for (int s = s0; s < s1; ++s) {
-            const long long n = (long long)attn_span(p, s, false).tiles * rows;
+            const unsigned n = (unsigned)attn_span<kTile>(p, s, false).units * rows;
             if (lo < base + n) {
                 found_seq = s;
                 found_base = base;
@@ -316,141 +403,178 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
     }
     __syncthreads();
     int seq = found_seq;
-    long long seq_base = found_base;
+    unsigned seq_base = found_base;
     int4 piece = make_int4(0, 0, 0, 0);
 
-    long long pos = lo;
+    unsigned pos = lo;
     while (pos < hi) {
-        AttnSpan sp = attn_span(p, seq, false);
-        if (pos >= seq_base + (long long)sp.tiles * rows) {
-            seq_base += (long long)sp.tiles * rows;
+        AttnSpan sp = attn_span<kTile>(p, seq, false);
+        if (pos - seq_base >= (unsigned)sp.units * rows) {
+            seq_base += (unsigned)sp.units * rows;
             ++seq;
             continue;
         }
-        const int item = (int)((pos - seq_base) / sp.tiles);      // (KV head, head tile)
-        const long long item0 = seq_base + (long long)item * sp.tiles;
-        const long long end = min(hi, item0 + sp.tiles);
+        const int item = (int)((pos - seq_base) / (unsigned)sp.units);        // (KV head, head tile)
+        // The item's tiles are its last units; this block takes those in its range.
+        const unsigned tile_unit = seq_base + (unsigned)(item * sp.units) + kAttnItemUnits;
+        const unsigned end = min(hi, tile_unit + sp.tiles);
+        if (end <= tile_unit) break;                              // the next block has its first tile
+        const int piece0 = pos > tile_unit ? (int)(pos - tile_unit) : 0, piece1 = (int)(end - tile_unit);
         const int kh = item / p.head_tiles, ht = item - kh * p.head_tiles;
         const int nh = min(GH, p.group - ht * GH);                // heads of this tile
         const int head0 = kh * p.group + ht * GH;
         const uint8_t *head = p.l.pages + (unsigned long long)kh * p.l.chunk_bytes;
         const int *table = p.page_table + (long long)seq * p.table_stride;
         const unsigned page16 = (unsigned)(p.l.page_bytes >> 4);
-        const int tile_first = sp.tile0 + (int)(pos - item0), tile_end = sp.tile0 + (int)(end - item0);
+        const int tile_first = sp.tile0 + piece0, tile_end = sp.tile0 + piece1;
+
+        const bool aligned = p.aligned;
 
         // ---- where a tile's tokens are ----
-        // A tile's page ids are fetched a tile ahead (fetch) and then resolved
-        // to the 16-byte offset of the page, the slot and the tokens that
-        // count.  Lane l looks up token l % 16; pages of a multiple of 16
-        // tokens need one look-up, which every lane makes alike.
-        int entry, slot, tok0;
-        auto fetch = [&](int tile) {
-            tok0 = tile * kAttnTile + warp * 16;
-            const int tok = kAligned ? tok0 : tok0 + (lane & 15);
-            int pg = (int)(((unsigned long long)(unsigned)tok * p.page_mul) >> 32);
-            slot = tok - pg * p.l.page_size;
-            if (slot < 0) {
-                --pg;
-                slot += p.l.page_size;
-            }
-            const bool inside = kAligned ? tok0 + 16 > sp.first && tok0 < sp.end : tok >= sp.first && tok < sp.end;
-            entry = inside ? __ldg(table + pg) : -1;
+        // A tile's page ids are fetched ahead and resolved when its rows are
+        // copied, to offsets in units of 16 bytes and the tokens that count.
+        // Pages of a multiple of 16 tokens (aligned): each MMA tile is a run
+        // of rows, looked up by every lane alike.  Others: lane l looks up
+        // token l, and the copying lanes ask it.  Tiles are fetched in order.
+        struct Entry {
+            int page[MT], slot[MT];
         };
-        unsigned at16 = 0, valid = 0;
-        int at_slot = 0;
-        const uint8_t *at_page = head;
-        auto resolve = [&]() {
-            const bool ok = (unsigned)entry < (unsigned)p.l.num_pages;
-            const int l0 = max(sp.first - tok0, 0), l1 = min(sp.end - tok0, 16);
-            unsigned inside = l1 > l0 ? (0xffffu >> (16 - l1)) & (0xffffu << l0) : 0u;
-            at_slot = slot;
-            if constexpr (kAligned) {
-                if (inside && !ok) {
-                    if (lane == 0) atomicOr(p.err, kErrCache);
-                    inside = 0;
+        int next_tok = tile_first * kTile + warp * kTok, next_page, next_slot;
+        {
+            const int tok = next_tok + (aligned ? 0 : lane);
+            next_page = (int)(((unsigned long long)(unsigned)tok * p.page_mul) >> 32);
+            next_slot = tok - next_page * p.l.page_size;
+            if (next_slot < 0) {
+                --next_page;
+                next_slot += p.l.page_size;
+            }
+        }
+        const int tok_end = min(sp.end, tile_end * kTile);
+        auto fetch = [&]() {
+            Entry e;
+            int pg = next_page, sl = next_slot;
+            if (aligned) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    const int tok = next_tok + 16 * i;
+                    e.page[i] = tok + 16 > sp.first && tok < tok_end ? __ldg(table + pg) : -1;
+                    e.slot[i] = sl;
+                    sl += 16;
+                    if (sl >= p.l.page_size) {
+                        sl -= p.l.page_size;
+                        ++pg;
+                    }
                 }
-                valid = inside;
-                at_page = head + (ok ? (unsigned long long)((unsigned)entry * page16) << 4 : 0ull);
             } else {
-                valid = __ballot_sync(0xffffffffu, ok) & inside;
-                if (lane < 16 && ((inside >> lane) & 1) && !ok) atomicOr(p.err, kErrCache);
-                at16 = ok ? (unsigned)entry * page16 : 0u;
+                const int tok = next_tok + lane;
+                e.page[0] = lane < kTok && tok >= sp.first && tok < tok_end ? __ldg(table + pg) : -1;
+                e.slot[0] = sl;
+                if (MT == 2) e.page[MT - 1] = e.slot[MT - 1] = 0;
             }
+            // kTile tokens on
+            next_tok += kTile;
+            next_page += p.tile_pages;
+            next_slot += p.tile_slots;
+            if (next_slot >= p.l.page_size) {
+                next_slot -= p.l.page_size;
+                ++next_page;
+            }
+            return e;
         };
-        auto row_ptr = [&](int token, int off, int stride) {
-            if constexpr (kAligned) return at_page + (off + (at_slot + token) * stride);
-            const unsigned o16 = __shfl_sync(0xffffffffu, at16, token);
-            const int sl = __shfl_sync(0xffffffffu, at_slot, token);
-            return head + ((unsigned long long)o16 << 4) + (unsigned)(off + sl * stride);
+        constexpr unsigned kAll = kTok == 32 ? 0xffffffffu : 0xffffu;
+        unsigned row16[MT], page_at[MT], valid = 0;               // offsets of the first row and of its page
+        int first_slot[MT], load_tok = next_tok;
+        auto resolve = [&](const Entry &e) {
+            unsigned inside = kAll;
+            if (load_tok < sp.first || load_tok + kTok > tok_end) {
+                const int l0 = max(sp.first - load_tok, 0), l1 = min(tok_end - load_tok, kTok);
+                inside = l1 > l0 ? (0xffffffffu >> (32 - l1)) & (0xffffffffu << l0) : 0u;
+            }
+            load_tok += kTile;
+            valid = inside;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const bool ok = (unsigned)e.page[i] < (unsigned)p.l.num_pages;
+                page_at[i] = ok ? (unsigned)e.page[i] * page16 : 0u;
+                first_slot[i] = e.slot[i];
+                row16[i] = page_at[i] + (unsigned)(e.slot[i] * (Sh::kRowBytes / 16));
+                if (aligned) {
+                    if (!ok) valid &= ~(0xffffu << (16 * i));
+                } else if (i == 0) {
+                    valid &= __ballot_sync(0xffffffffu, ok);
+                }
+            }
+            if (valid != inside && lane == 0) atomicOr(p.err, kErrCache);
         };
 
-        // ---- rows to registers: chunk c of K (c < C) and of V (c - C) ----
-        uint32_t buf[2][kRegs];
-        float ks[2][NB], vs[2][NB];
-        auto load = [&](int i) {
-            uint32_t *w = buf[i & 1];
-            if (i < C) {
+        // ---- K or V rows of a tile into slot `at` of the warp's ring ----
+        uint8_t *const ring = rings + warp * R * Sh::kSlot;
+        auto copy_rows = [&](int at, bool is_v) {
+            uint8_t *const slot = ring + at * Sh::kSlot;
+            const uint32_t dst = smem_addr(slot);
+            constexpr int PR = Sh::kRowBytes / 16, kCopies = kTok * PR / 32;  // pieces of a row, copies of a lane
+            static_assert(kTok * PR % 32 == 0, "");
+            // Piece 32 j + lane of the rows: its row and its place in the slot.
+            auto row_of = [&](int j) { return 32 % PR == 0 ? j * (32 / PR) + lane / PR : PR % 32 == 0 ? j / (PR / 32) : (32 * j + lane) / PR; };
+            auto to = [&](int j) {
+                const int col = 32 % PR == 0 ? lane % PR : PR % 32 == 0 ? 32 * (j % (PR / 32 > 0 ? PR / 32 : 1)) + lane : (32 * j + lane) % PR;
+                return dst + row_of(j) * Sh::kStride + col * 16;
+            };
+            const uint8_t *base = head + (is_v ? p.l.v_off : 0), *sbase = head + (is_v ? p.l.vs_off : p.l.ks_off);
+            constexpr int kPer = Sh::kScaleBytes == 32 ? 2 : 1, kPiece = Sh::kScaleBytes == 8 ? 8 : 16;   // of a token's scales
+            auto copy_scales = [&](const uint8_t *src, int i, int row) {
+                const uint32_t d = dst + Sh::kScaleOff + i * kPiece;
+                if (kPiece == 8) copy8(d, src, (valid >> row) & 1 ? 8 : 0);
+                else copy16(d, src, (valid >> row) & 1 ? 16 : 0);
+            };
+            if (!valid) {
+                // nothing of this tile counts
+            } else if (aligned) {
+                const uint8_t *src[MT];
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const bool ok = (valid >> (g + 8 * r)) & 1;
-                    const uint8_t *row = row_ptr(g + 8 * r, 0, Sh::kRowBytes);
-                    if constexpr (Sh::kQuant) {
-                        constexpr int kBytes = Sh::kRowBytes / 4;
-                        load_bytes<kBytes>(row + t * kBytes, ok, w + r * (kBytes / 4));
-                        load_scales<NB>(row_ptr(g + 8 * r, p.l.ks_off, Sh::kScaleBytes), ok, ks[r]);
-                    } else {
-                        // 64 bytes of the row at a time, 16 of them this lane's
+                for (int i = 0; i < MT; ++i) src[i] = base + ((unsigned long long)row16[i] << 4) + lane * 16 - i * 16 * Sh::kRowBytes;
+                if (valid == kAll) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            if (i * Sh::kChunkBytes + 64 * j < Sh::kRowBytes)
-                                load_bytes<16>(row + i * Sh::kChunkBytes + 64 * j + 16 * t, ok, w + r * 16 + 4 * j);
-                    }
-                }
-            } else {
+                    for (int j = 0; j < kCopies; ++j)
+                        copy16(to(j), (MT == 1 || row_of(j) < 16 ? src[0] : src[MT - 1]) + 512 * j, 16);
+                } else {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int tok = kF32 ? t + 4 * r : 2 * t + (r & 1) + 8 * (r >> 1);
-                    const bool ok = (valid >> tok) & 1;
-                    const uint8_t *row = row_ptr(tok, p.l.v_off, Sh::kRowBytes);
-                    if constexpr (Sh::kQuant) {
-                        constexpr int kBytes = Sh::kRowBytes / 8;
-                        load_bytes<kBytes>(row + g * kBytes, ok, w + r * ((kBytes + 3) / 4));
-                    } else {
-                        // 128 bytes of the row at a time (64 where the head ends), 16 (8) of them this lane's
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            const int off = (i - C) * Sh::kChunkBytes + 128 * j;
-                            if (off + 128 <= Sh::kRowBytes) load_bytes<16>(row + off + 16 * g, ok, w + r * 8 + 4 * j);
-                            else if (off + 64 <= Sh::kRowBytes) load_bytes<8>(row + off + 8 * g, ok, w + r * 8 + 4 * j);
-                        }
-                    }
+                    for (int j = 0; j < kCopies; ++j)
+                        copy16(to(j), (MT == 1 || row_of(j) < 16 ? src[0] : src[MT - 1]) + 512 * j, (valid >> row_of(j)) & 1 ? 16 : 0);
                 }
                 if constexpr (Sh::kQuant) {
 #pragma unroll
-                    for (int r = 0; r < 2; ++r)
-                        load_scales<NB>(row_ptr(g + 8 * r, p.l.vs_off, Sh::kScaleBytes), (valid >> (g + 8 * r)) & 1, vs[r]);
+                    for (int j = 0; j < kTok * kPer / 32; ++j) {
+                        const int i = 32 * j + lane, row = i / kPer;
+                        const unsigned o = row < 16 ? page_at[0] : page_at[MT - 1];
+                        const int sl = row < 16 ? first_slot[0] : first_slot[MT - 1] - 16;
+                        copy_scales(sbase + ((unsigned long long)o << 4) + sl * Sh::kScaleBytes + i * kPiece, i, row);
+                    }
+                }
+            } else {
+                for (int j = 0; j < kCopies; ++j) {
+                    const int i = 32 * j + lane, row = i / PR, col = i - row * PR;
+                    const unsigned o = __shfl_sync(0xffffffffu, row16[0], row) + col;
+                    copy16(dst + row * Sh::kStride + col * 16, base + ((unsigned long long)o << 4), (valid >> row) & 1 ? 16 : 0);
+                }
+                if constexpr (Sh::kQuant) {
+                    for (int j = 0; j < kTok * kPer / 32; ++j) {
+                        const int i = 32 * j + lane, row = i / kPer;
+                        const unsigned o = __shfl_sync(0xffffffffu, page_at[0], row);
+                        const int sl = __shfl_sync(0xffffffffu, first_slot[0], row);
+                        copy_scales(sbase + ((unsigned long long)o << 4) + sl * Sh::kScaleBytes + (i - row * kPer) * kPiece, i, row);
+                    }
                 }
             }
-        };
-        // After chunk i is used, its registers take chunk i + 2, of the next
-        // tile where this one has no more.
-        auto load_after = [&](int i, int tile) {
-            if (i + 2 < 2 * C) {
-                load(i + 2);
-            } else if (tile + 1 < tile_end) {
-                if (i == 2 * C - 2) {
-                    resolve();
-                    load(0);
-                    if (tile + 2 < tile_end) fetch(tile + 2);
-                } else {
-                    load(1);
-                }
-            }
+            if (!is_v && lane == 0) *reinterpret_cast<unsigned *>(slot + Sh::kMaskOff) = valid;
+            copies_commit();
         };
 
-        // ---- the first tile's rows on their way, then the query's parts in
-        //      shared memory in B operand order ----
-        fetch(tile_first);
+        // ---- the query's values, and the ring's first copies ----
+        constexpr int kAhead = (R + 1) / 2;                       // tiles whose copies a full ring holds
+        Entry next[kAhead + 1];
+#pragma unroll
+        for (int i = 0; i <= kAhead; ++i) next[i] = fetch();
         constexpr int kPerWarp = GH / kAttnWarps;
         float x[kPerWarp][NB];
 #pragma unroll
@@ -464,20 +588,20 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                           : p.io == DTYPE_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(p.q)[off + 32 * b])
                                                : __half2float(static_cast<const __half *>(p.q)[off + 32 * b]);
         }
-        resolve();
-        load(0);
-        load(1);
-        if (tile_first + 1 < tile_end) fetch(tile_first + 1);
-        __syncthreads();                                          // the last item's readers
+        __syncthreads();                                          // the last item's readers of the rings
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            if (i % 2 == 0) resolve(next[i / 2]);
+            copy_rows(i, i % 2 == 1);
+        }
 #pragma unroll
         for (int k = 0; k < kPerWarp; ++k) {
             const int j = warp + k * kAttnWarps;
-            float up = 1.0f, mul = p.scale;
+            float up = 1.0f, mul = p.scale, top = 0.0f;
             if (!kBf16 && !kF32) {
                 // fp16 parts: the head's largest value goes to [2^14, 2^15).
-                float top = 0.0f;
 #pragma unroll
-                for (int b = 0; b < NB; ++b) top = fmaxf(top, fabsf(x[k][b]));
+                for (int b = 0; b < NB; ++b) top = x[k][b] == x[k][b] ? fmaxf(top, fabsf(x[k][b])) : INFINITY;
 #pragma unroll
                 for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                 if (top > 0.0f && top < INFINITY) {
@@ -486,8 +610,28 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                     mul = p.scale * ldexpf(1.0f, -e);
                 }
             }
-            if (lane == 0) qmul[j] = mul;
             const int col = kWide ? j : 2 * j;
+            if constexpr (kInt) {
+                // 15-bit integers: the head's largest value goes to [2^13, 2^14);
+                // a head with an infinity or a NaN has no score.
+                if (!(top < INFINITY)) mul = __uint_as_float(0x7fc00000u);
+                up *= 0.5f;
+                mul *= 2.0f;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    const int y = top < INFINITY ? __float2int_rn(x[k][b] * up) : 0;
+                    const int sum = __reduce_add_sync(0xffffffffu, y);
+                    if (lane == 0) qoff[j][b] = -(kCache == DTYPE_Q8_0 ? 128 : 8) * sum;
+                    int d = 32 * b + lane;
+                    if (kCache == DTYPE_Q4_0) d = (d & ~7) | ((d & 1) << 2) | ((d >> 1) & 3);   // evens, odds
+                    uint8_t *to = sq + col * Sh::kDigitStride + d;
+                    to[0] = (uint8_t)y;
+                    to[(kWide ? 8 : 1) * Sh::kDigitStride] = (uint8_t)((y + 128) >> 8);
+                }
+                if (lane == 0) qmul[j] = mul;
+                continue;
+            }
+            if (lane == 0) qmul[j] = mul;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 float y = x[k][b] * up;
@@ -513,7 +657,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
         for (int j = 0; j < HL; ++j) qm[j] = qmul[HL * t + j];
 
         // ---- the pass over this block's tiles of the item ----
-        float acc[kMTiles][4], m[HL], l[HL];
+        // acc: M tile of 16 dims, rows g and g + 8, of the lane's columns (of its
+        // head, where integers join a head's two).
+        float acc[kMTiles][NA], m[HL], l[HL];
 #pragma unroll
         for (int j = 0; j < HL; ++j) {
             m[j] = -INFINITY;
@@ -522,112 +668,208 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
 #pragma unroll
         for (int i = 0; i < kMTiles; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
+            for (int j = 0; j < NA; ++j) acc[i][j] = 0.0f;
+        int qo[HL][NB];
+        if constexpr (kInt)
+#pragma unroll
+            for (int j = 0; j < HL; ++j)
+#pragma unroll
+                for (int b = 0; b < NB; ++b) qo[j][b] = qoff[HL * t + j][b];
         float vlim = 0.0f, vinv = 0.0f;                           // V scales: largest that fits, and the power of two
+        // Adds what an accumulator of its own holds: an MMA truncates its
+        // sums, so where that shows (kExact) only a tile's products share one.
+        auto add_up = [](float (&to)[4], const float (&c)[4]) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) to[j] += c[j];
+        };
+        int at = 0;                                               // the ring's oldest slot
+        auto advance = [&](bool after_v) {
+            // The slot's rows are used: copy the half tile R behind into it.
+            __syncwarp();
+            if ((R & 1) == (after_v ? 1 : 0)) {
+                // its K rows: a tile not yet looked at
+                resolve(next[kAhead]);
+                copy_rows(at, false);
+                next[kAhead] = fetch();
+            } else {
+                copy_rows(at, true);
+            }
+            at = at + 1 == R ? 0 : at + 1;
+        };
         for (int tile = tile_first; tile < tile_end; ++tile) {
-            const bool ok0 = (valid >> g) & 1, ok1 = (valid >> (g + 8)) & 1;
-            // ---- scores of 16 tokens: lane (g, t) has tokens g, g + 8 of its heads ----
-            float s[HL][2];
+            copies_wait<R - 1>();
+            __syncwarp();
+            const uint8_t *slot = ring + at * Sh::kSlot;
+            const unsigned now = *reinterpret_cast<const unsigned *>(slot + Sh::kMaskOff);
+            // ---- scores: lane (g, t) has tokens 16 i + g, + 8 of its heads ----
+            float s[HL][2 * MT];
             if constexpr (Sh::kQuant) {
-                const uint32_t *kr = buf[0];
+                constexpr int kBytes = Sh::kRowBytes / 4, kW = kBytes / 4;        // of a row in this lane
+                uint32_t kr[MT][2][kW];
+                float ks[MT][2][NB];
 #pragma unroll
-                for (int j = 0; j < HL; ++j) s[j][0] = s[j][1] = 0.0f;
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    uint32_t a[2][4];
-                    constexpr int kW = Sh::kRowBytes / 16;            // words of a row in this lane
+                for (int i = 0; i < MT; ++i)
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        if constexpr (kCache == DTYPE_Q8_0) {
+                        const int row = 16 * i + 8 * r + g;
+                        read_bytes<kBytes>(slot + row * Sh::kStride + t * kBytes, kr[i][r]);
+                        read_scales<NB>(slot + Sh::kScaleOff + row * Sh::kScaleBytes, ks[i][r]);
+                    }
 #pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                const uint32_t w = kr[r * kW + i * NB + b];
-                                a[i][r] = bytes_to_half2(w, 0x4140);
-                                a[i][2 + r] = bytes_to_half2(w, 0x4342);
+                for (int j = 0; j < HL; ++j)
+#pragma unroll
+                    for (int r = 0; r < 2 * MT; ++r) s[j][r] = 0.0f;
+                if constexpr (kInt) {
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        uint2 q[Pt::kSets];
+#pragma unroll
+                        for (int set = 0; set < Pt::kSets; ++set)
+                            q[set] = *reinterpret_cast<const uint2 *>(sq + (set * 8 + g) * Sh::kDigitStride + 32 * b + 8 * t);
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) {
+                            uint32_t a[4];
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) {
+                                if constexpr (kCache == DTYPE_Q8_0) {
+                                    a[r] = kr[i][r][b];
+                                    a[2 + r] = kr[i][r][NB + b];
+                                } else {
+                                    const uint32_t u = kr[i][r][b / 2], v = kr[i][r][(NB + b) / 2];
+                                    const uint32_t w = __byte_perm(u, v, (b & 1 ? 0x32 : 0x10) | ((NB + b) & 1 ? 0x7600 : 0x5400));
+                                    a[r] = w & 0x0f0f0f0fu;
+                                    a[2 + r] = (w >> 4) & 0x0f0f0f0fu;
+                                }
                             }
-                        } else {
-                            // halfwords b and NB + b: codes 0-3 of words 2t and 2t + 1
-                            const uint32_t u = kr[r * kW + b / 2], v = kr[r * kW + (NB + b) / 2];
-                            const uint32_t w = __byte_perm(u, v, (b & 1 ? 0x32 : 0x10) | ((NB + b) & 1 ? 0x7600 : 0x5400));
-                            a[0][r] = nibbles_to_half2<0>(w);
-                            a[0][2 + r] = nibbles_to_half2<4>(w);
-                            a[1][r] = nibbles_to_half2<0>(w >> 8);
-                            a[1][2 + r] = nibbles_to_half2<4>(w >> 8);
+                            const int zero[4] = {0, 0, 0, 0};
+                            int c[Pt::kSets][4];
+#pragma unroll
+                            for (int set = 0; set < Pt::kSets; ++set) mma8<false>(c[set], a[0], a[1], a[2], a[3], q[set].x, q[set].y, zero);
+#pragma unroll
+                            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                                for (int j = 0; j < HL; ++j) {
+                                    const int v = kWide ? c[0][2 * r + j] + c[Pt::kSets - 1][2 * r + j] * 256 : c[0][2 * r] + c[0][2 * r + 1] * 256;
+                                    s[j][2 * i + r] = fmaf(ks[i][r][b], (float)(v + qo[j][b]), s[j][2 * i + r]);
+                                }
                         }
                     }
-                    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                } else {
 #pragma unroll
-                    for (int set = 0; set < kQS; ++set) {
-                        const uint4 q = *reinterpret_cast<const uint4 *>(sq + (set * 8 + g) * Sh::kQStride + 64 * b + 16 * t);
-                        mma16<false>(c, a[0][0], a[0][1], a[0][2], a[0][3], q.x, q.y);
-                        mma16<false>(c, a[1][0], a[1][1], a[1][2], a[1][3], q.z, q.w);
-                    }
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        if constexpr (kWide) {
-                            s[0][r] = fmaf(ks[r][b], c[2 * r], s[0][r]);
-                            s[1][r] = fmaf(ks[r][b], c[2 * r + 1], s[1][r]);
-                        } else {
-                            s[0][r] = fmaf(ks[r][b], c[2 * r] + c[2 * r + 1], s[0][r]);
+                    for (int b = 0; b < NB; ++b) {
+                        uint4 q[kQS];
+    #pragma unroll
+                        for (int set = 0; set < kQS; ++set)
+                            q[set] = *reinterpret_cast<const uint4 *>(sq + (set * 8 + g) * Sh::kQStride + 64 * b + 16 * t);
+    #pragma unroll
+                        for (int i = 0; i < MT; ++i) {
+                            uint32_t a[2][4];
+    #pragma unroll
+                            for (int r = 0; r < 2; ++r) {
+                                if constexpr (kCache == DTYPE_Q8_0) {
+    #pragma unroll
+                                    for (int h = 0; h < 2; ++h) {
+                                        const uint32_t w = kr[i][r][h * NB + b];
+                                        a[h][r] = bytes_to_half2(w, 0x4140);
+                                        a[h][2 + r] = bytes_to_half2(w, 0x4342);
+                                    }
+                                } else {
+                                    // halfwords b and NB + b: codes 0-3 of words 2t and 2t + 1
+                                    const uint32_t u = kr[i][r][b / 2], v = kr[i][r][(NB + b) / 2];
+                                    const uint32_t w = __byte_perm(u, v, (b & 1 ? 0x32 : 0x10) | ((NB + b) & 1 ? 0x7600 : 0x5400));
+                                    a[0][r] = nibbles_to_half2<0>(w);
+                                    a[0][2 + r] = nibbles_to_half2<4>(w);
+                                    a[1][r] = nibbles_to_half2<0>(w >> 8);
+                                    a[1][2 + r] = nibbles_to_half2<4>(w >> 8);
+                                }
+                            }
+                            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    #pragma unroll
+                            for (int set = 0; set < kQS; ++set) {
+                                mma16<false>(c, a[0][0], a[0][1], a[0][2], a[0][3], q[set].x, q[set].y);
+                                mma16<false>(c, a[1][0], a[1][1], a[1][2], a[1][3], q[set].z, q[set].w);
+                            }
+    #pragma unroll
+                            for (int r = 0; r < 2; ++r) {
+                                if constexpr (kWide) {
+                                    s[0][2 * i + r] = fmaf(ks[i][r][b], c[2 * r], s[0][2 * i + r]);
+                                    s[HL - 1][2 * i + r] = fmaf(ks[i][r][b], c[2 * r + 1], s[HL - 1][2 * i + r]);
+                                } else {
+                                    s[0][2 * i + r] = fmaf(ks[i][r][b], c[2 * r] + c[2 * r + 1], s[0][2 * i + r]);
+                                }
+                            }
                         }
                     }
                 }
-                load_after(0, tile);
             } else {
-                float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                float c[MT][4];
 #pragma unroll
-                for (int ch = 0; ch < C; ++ch) {
-                    const uint32_t *kr = buf[ch & 1];
+                for (int i = 0; i < MT; ++i)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int off = ch * Sh::kChunkBytes + 64 * i;            // bytes into the row
-                        if (off >= Sh::kRowBytes) continue;
-                        const uint32_t *u = kr + 4 * i, *v = kr + 16 + 4 * i;
+                    for (int j = 0; j < 4; ++j) c[i][j] = 0.0f;
+#pragma unroll
+                for (int off = 0; off < Sh::kRowBytes; off += 64) {               // 64 bytes of a row, 16 this lane's
+                    uint4 q[kQS];
+#pragma unroll
+                    for (int set = 0; set < kQS; ++set)
+                        q[set] = *reinterpret_cast<const uint4 *>(sq + (set * 8 + g) * Sh::kQStride + off + 16 * t);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        uint32_t u[4], v[4];
+                        read_bytes<16>(slot + (16 * i + g) * Sh::kStride + off + 16 * t, u);
+                        read_bytes<16>(slot + (16 * i + g + 8) * Sh::kStride + off + 16 * t, v);
+                        float own[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        float(&to)[4] = kExact ? own : c[i];
                         uint32_t uh[4], ul[4], vh[4], vl[4];
                         if constexpr (kF32) {
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
-                                float a = __uint_as_float(u[j]), b = __uint_as_float(v[j]);
-                                uh[j] = __float_as_uint(take_tf32(a));
-                                vh[j] = __float_as_uint(take_tf32(b));
-                                ul[j] = round_tf32(a);
-                                vl[j] = round_tf32(b);
+                                float x0 = __uint_as_float(u[j]), x1 = __uint_as_float(v[j]);
+                                uh[j] = __float_as_uint(take_tf32(x0));
+                                vh[j] = __float_as_uint(take_tf32(x1));
+                                ul[j] = round_tf32(x0);
+                                vl[j] = round_tf32(x1);
                             }
                         }
 #pragma unroll
                         for (int set = 0; set < kQS; ++set) {
-                            const uint4 q = *reinterpret_cast<const uint4 *>(sq + (set * 8 + g) * Sh::kQStride + off + 16 * t);
                             if constexpr (kF32) {
-                                mma_tf32(c, ul[0], vl[0], ul[1], vl[1], q.x, q.y);
-                                mma_tf32(c, ul[2], vl[2], ul[3], vl[3], q.z, q.w);
-                                mma_tf32(c, uh[0], vh[0], uh[1], vh[1], q.x, q.y);
-                                mma_tf32(c, uh[2], vh[2], uh[3], vh[3], q.z, q.w);
+                                mma_tf32(to, ul[0], vl[0], ul[1], vl[1], q[set].x, q[set].y);
+                                mma_tf32(to, ul[2], vl[2], ul[3], vl[3], q[set].z, q[set].w);
+                                mma_tf32(to, uh[0], vh[0], uh[1], vh[1], q[set].x, q[set].y);
+                                mma_tf32(to, uh[2], vh[2], uh[3], vh[3], q[set].z, q[set].w);
                             } else {
-                                mma16<kBf16>(c, u[0], v[0], u[1], v[1], q.x, q.y);
-                                mma16<kBf16>(c, u[2], v[2], u[3], v[3], q.z, q.w);
+                                mma16<kBf16>(to, u[0], v[0], u[1], v[1], q[set].x, q[set].y);
+                                mma16<kBf16>(to, u[2], v[2], u[3], v[3], q[set].z, q[set].w);
                             }
                         }
+                        if (kExact) add_up(c[i], own);
                     }
-                    load_after(ch, tile);
                 }
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    if constexpr (kWide) {
-                        s[0][r] = c[2 * r];
-                        s[1][r] = c[2 * r + 1];
-                    } else {
-                        s[0][r] = c[2 * r] + c[2 * r + 1];
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        if constexpr (kWide) {
+                            s[0][2 * i + r] = c[i][2 * r];
+                            s[HL - 1][2 * i + r] = c[i][2 * r + 1];
+                        } else {
+                            s[0][2 * i + r] = c[i][2 * r] + c[i][2 * r + 1];
+                        }
                     }
-                }
             }
+            advance(false);
             // ---- probabilities ----
-            float pr[HL][2], top[HL];
+            float pr[HL][2 * MT], top[HL];
             bool grew = false;
 #pragma unroll
             for (int j = 0; j < HL; ++j) {
-                s[j][0] = ok0 ? s[j][0] * qm[j] : -INFINITY;
-                s[j][1] = ok1 ? s[j][1] * qm[j] : -INFINITY;
-                top[j] = fmaxf(s[j][0], s[j][1]);
+                top[j] = -INFINITY;
+#pragma unroll
+                for (int r = 0; r < 2 * MT; ++r) {
+                    s[j][r] = (now >> (8 * r + g)) & 1 ? s[j][r] * qm[j] : -INFINITY;
+                    top[j] = fmaxf(top[j], s[j][r]);
+                }
                 grew = grew || top[j] > m[j];
             }
             if (__any_sync(0xffffffffu, grew)) {
@@ -644,16 +886,18 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
 #pragma unroll
                 for (int i = 0; i < kMTiles; ++i)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] *= keep[kWide ? j & 1 : 0];
+                    for (int j = 0; j < NA; ++j) acc[i][j] *= keep[kWide ? j & 1 : 0];
             }
 #pragma unroll
             for (int j = 0; j < HL; ++j) {
                 const float ref = m[j] == -INFINITY ? 0.0f : m[j] - kBias;
-                pr[j][0] = attn_exp2(s[j][0] - ref);
-                pr[j][1] = attn_exp2(s[j][1] - ref);
-                l[j] += pr[j][0] + pr[j][1];
+#pragma unroll
+                for (int r = 0; r < 2 * MT; ++r) {
+                    pr[j][r] = attn_exp2(s[j][r] - ref);
+                    l[j] += pr[j][r];
+                }
             }
-            // The 16-bit B operands of w (tokens g and g + 8 of the lane's heads).
+            // The 16-bit B operands of MMA tile i of w.
             auto operand = [&](const float (&w)[HL][2], uint32_t (&b0)[kPS], uint32_t (&b1)[kPS]) {
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
@@ -664,27 +908,130 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                     for (int set = 0; set < kPS; ++set) {
                         uint32_t u;
                         if constexpr (kWide) {
-                            u = pack16<kBf16>(y[0], y[1]);
+                            u = pack16<kBf16>(y[0], y[HL - 1]);
                             if (set + 1 < kPS) {
                                 take16<kBf16>(y[0]);
-                                take16<kBf16>(y[1]);
+                                take16<kBf16>(y[HL - 1]);
                             }
                         } else {
-                            const float hi2 = take16<kBf16>(y[0]);
-                            u = pack16<kBf16>(hi2, y[0]);
+                            const float high = take16<kBf16>(y[0]);
+                            u = pack16<kBf16>(high, set == 0 ? y[0] : 0.0f);
                             if (set + 1 < kPS) take16<kBf16>(y[0]);
-                            if (set == 1) u = pack16<kBf16>(hi2, 0.0f);
                         }
                         (r ? b1 : b0)[set] = transpose8x8(u);
                     }
                 }
             };
             // ---- acc += V^T P^T ----
-            if constexpr (Sh::kQuant) {
-                const uint32_t *vr = buf[1];
-                float big = 0.0f;
+            copies_wait<R - 1>();
+            __syncwarp();
+            slot = ring + at * Sh::kSlot;
+            if constexpr (kInt) {
+                if (now) {
+                    constexpr int kBytes = Sh::kRowBytes / 8, kW = (kBytes + 3) / 4;      // of a row in this lane
+                    static_assert(MT == 2, "an integer MMA takes 32 tokens");
+                    uint32_t vr[MT][4][kW];
+                    float vs[MT][2][NB];
 #pragma unroll
-                for (int b = 0; b < NB; ++b) big = fmaxf(big, fmaxf(fabsf(vs[0][b]), fabsf(vs[1][b])));
+                    for (int i = 0; i < MT; ++i) {
+#pragma unroll
+                        for (int r = 0; r < 2; ++r)
+                            read_scales<NB>(slot + Sh::kScaleOff + (16 * i + 8 * r + g) * Sh::kScaleBytes, vs[i][r]);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            read_bytes<kBytes>(slot + (16 * i + 2 * t + (r & 1) + 8 * (r >> 1)) * Sh::kStride + g * kBytes, vr[i][r]);
+                    }
+                    // Probabilities in [0, 2^7) of the tile's largest of each head.
+                    float pinv[HL];
+#pragma unroll
+                    for (int j = 0; j < HL; ++j) {
+                        uint32_t top = 0;
+#pragma unroll
+                        for (int r = 0; r < 2 * MT; ++r) top = max(top, __float_as_uint(pr[j][r]));
+                        const float f = unit_of(max_over_rows(top), pinv[j]);
+#pragma unroll
+                        for (int r = 0; r < 2 * MT; ++r) pr[j][r] *= f;
+                    }
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        // The block's scales likewise; the products round to integers below 2^14.
+                        uint32_t top = 0;
+#pragma unroll
+                        for (int r = 0; r < 2 * MT; ++r) top = max(top, __float_as_uint(fabsf(vs[r >> 1][r & 1][b])));
+                        float sinv;
+                        const float f = unit_of(max_over_rows(top), sinv);
+                        uint32_t bo[Pt::kSets][MT];                           // B operands: signed bytes of 16 tokens
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) {
+                            uint32_t w[HL];
+#pragma unroll
+                            for (int j = 0; j < HL; ++j) {
+                                // 1.5 * 2^23 + 128 + w: the low two bytes are w's
+                                const uint32_t u = __float_as_uint(fmaf(pr[j][2 * i], vs[i][0][b] * f, 12583040.0f));
+                                const uint32_t v = __float_as_uint(fmaf(pr[j][2 * i + 1], vs[i][1][b] * f, 12583040.0f));
+                                w[j] = __byte_perm(u, v, 0x5140);             // low bytes of tokens g and g + 8, high bytes
+                            }
+                            if constexpr (kWide) {
+                                bo[0][i] = transpose8x8(__byte_perm(w[0], w[HL - 1], 0x5410) ^ 0x80808080u);
+                                bo[Pt::kSets - 1][i] = transpose8x8(__byte_perm(w[0], w[HL - 1], 0x7632));
+                            } else {
+                                bo[0][i] = transpose8x8(w[0] ^ 0x00008080u);
+                            }
+                        }
+                        // Bytes 4t .. 4t + 3 of the MMA's 32: tokens 2t, 2t + 8, 2t + 1, 2t + 9 of each 16.
+                        uint32_t a[4][MT];                                    // dims 4g .. 4g + 3
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) {
+                            if constexpr (kCache == DTYPE_Q8_0) {
+                                const uint32_t t0 = __byte_perm(vr[i][0][b], vr[i][2][b], 0x5140), t1 = __byte_perm(vr[i][0][b], vr[i][2][b], 0x7362);
+                                const uint32_t t2 = __byte_perm(vr[i][1][b], vr[i][3][b], 0x5140), t3 = __byte_perm(vr[i][1][b], vr[i][3][b], 0x7362);
+                                a[0][i] = __byte_perm(t0, t2, 0x5410);
+                                a[1][i] = __byte_perm(t0, t2, 0x7632);
+                                a[2][i] = __byte_perm(t1, t3, 0x5410);
+                                a[3][i] = __byte_perm(t1, t3, 0x7632);
+                            } else {
+                                const uint32_t y0 = __byte_perm(vr[i][0][b / 2], vr[i][2][b / 2], b & 1 ? 0x7632 : 0x5410);
+                                const uint32_t y1 = __byte_perm(vr[i][1][b / 2], vr[i][3][b / 2], b & 1 ? 0x7632 : 0x5410);
+                                const uint32_t l0 = y0 & 0x0f0f0f0fu, l1 = y1 & 0x0f0f0f0fu;
+                                const uint32_t h0 = (y0 >> 4) & 0x0f0f0f0fu, h1 = (y1 >> 4) & 0x0f0f0f0fu;
+                                a[0][i] = __byte_perm(l0, l1, 0x6420);
+                                a[1][i] = __byte_perm(h0, h1, 0x6420);
+                                a[2][i] = __byte_perm(l0, l1, 0x7531);
+                                a[3][i] = __byte_perm(h0, h1, 0x7531);
+                            }
+                        }
+                        constexpr uint32_t kOff = kCache == DTYPE_Q8_0 ? 0x80808080u : 0xf8f8f8f8u;      // - 128, - 8
+                        const int zero[4] = {0, 0, 0, 0};
+                        int c[Pt::kSets][2][4];
+#pragma unroll
+                        for (int set = 0; set < Pt::kSets; ++set) {
+                            int off[4];
+                            mma8<true>(off, kOff, kOff, kOff, kOff, bo[set][0], bo[set][MT - 1], zero);
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+                                mma8<false>(c[set][h], a[2 * h][0], a[2 * h + 1][0], a[2 * h][MT - 1], a[2 * h + 1][MT - 1], bo[set][0], bo[set][MT - 1], off);
+                        }
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int j = 0; j < NA; ++j) {
+                                const int v = kWide ? c[0][h][j] + c[Pt::kSets - 1][h][j] * 256 : c[0][h][(2 * j) & 3] + c[0][h][(2 * j + 1) & 3] * 256;
+                                acc[2 * b + h][j] = fmaf((float)v, pinv[kWide ? j & 1 : 0] * sinv, acc[2 * b + h][j]);
+                            }
+                    }
+                }
+            } else if constexpr (Sh::kQuant) {
+                constexpr int kBytes = Sh::kRowBytes / 8, kW = (kBytes + 3) / 4;  // of a row in this lane
+                float vs[MT][2][NB], big = 0.0f;
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        read_scales<NB>(slot + Sh::kScaleOff + (16 * i + 8 * r + g) * Sh::kScaleBytes, vs[i][r]);
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) big = fmaxf(big, fabsf(vs[i][r][b]));
+                    }
+                if (!now) big = 0.0f;                             // nothing was copied
                 if (__any_sync(0xffffffffu, big > vlim)) {
                     // A larger scale than fits: a new power of two that brings it to [1/2, 1).
 #pragma unroll
@@ -699,46 +1046,60 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
 #pragma unroll
                         for (int j = 0; j < 4; ++j) acc[i][j] *= f;
                 }
-                constexpr int kW = (Sh::kRowBytes / 8 + 3) / 4;       // words of a row in this lane
+                uint32_t vr[MT][4][kW];
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    uint32_t a[2][4];
+                for (int i = 0; i < MT; ++i)
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        if constexpr (kCache == DTYPE_Q8_0) {
-                            const uint32_t u = vr[(2 * r) * kW + b], v = vr[(2 * r + 1) * kW + b];
-                            const uint32_t lo2 = __byte_perm(u, v, 0x5140), hi2 = __byte_perm(u, v, 0x7362);
-                            a[0][2 * r] = bytes_to_half2(lo2, 0x4140);
-                            a[0][2 * r + 1] = bytes_to_half2(lo2, 0x4342);
-                            a[1][2 * r] = bytes_to_half2(hi2, 0x4140);
-                            a[1][2 * r + 1] = bytes_to_half2(hi2, 0x4342);
-                        } else {
-                            const uint32_t w = __byte_perm(vr[(2 * r) * kW + b / 2], vr[(2 * r + 1) * kW + b / 2],
-                                                           b & 1 ? 0x7632 : 0x5410);
-                            a[0][2 * r] = nibbles_to_half2<0>(w);
-                            a[0][2 * r + 1] = nibbles_to_half2<4>(w);
-                            a[1][2 * r] = nibbles_to_half2<0>(w >> 8);
-                            a[1][2 * r + 1] = nibbles_to_half2<4>(w >> 8);
+                    for (int r = 0; r < 4; ++r)
+                        read_bytes<kBytes>(slot + (16 * i + 2 * t + (r & 1) + 8 * (r >> 1)) * Sh::kStride + g * kBytes, vr[i][r]);
+                if (now) {
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        float own[2][4] = {};
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) {
+                            uint32_t a[2][4];
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) {
+                                if constexpr (kCache == DTYPE_Q8_0) {
+                                    const uint32_t u = vr[i][2 * r][b], v = vr[i][2 * r + 1][b];
+                                    const uint32_t lo2 = __byte_perm(u, v, 0x5140), hi2 = __byte_perm(u, v, 0x7362);
+                                    a[0][2 * r] = bytes_to_half2(lo2, 0x4140);
+                                    a[0][2 * r + 1] = bytes_to_half2(lo2, 0x4342);
+                                    a[1][2 * r] = bytes_to_half2(hi2, 0x4140);
+                                    a[1][2 * r + 1] = bytes_to_half2(hi2, 0x4342);
+                                } else {
+                                    const uint32_t w = __byte_perm(vr[i][2 * r][b / 2], vr[i][2 * r + 1][b / 2], b & 1 ? 0x7632 : 0x5410);
+                                    a[0][2 * r] = nibbles_to_half2<0>(w);
+                                    a[0][2 * r + 1] = nibbles_to_half2<4>(w);
+                                    a[1][2 * r] = nibbles_to_half2<0>(w >> 8);
+                                    a[1][2 * r + 1] = nibbles_to_half2<4>(w >> 8);
+                                }
+                            }
+                            const float f0 = vs[i][0][b] * vinv, f1 = vs[i][1][b] * vinv;
+                            float w[HL][2];
+#pragma unroll
+                            for (int j = 0; j < HL; ++j) {
+                                w[j][0] = pr[j][2 * i] * f0;
+                                w[j][1] = pr[j][2 * i + 1] * f1;
+                            }
+                            uint32_t b0[kPS], b1[kPS];
+                            operand(w, b0, b1);
+#pragma unroll
+                            for (int set = 0; set < kPS; ++set)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h)
+                                    mma16<false>(kExact ? own[h] : acc[2 * b + h], a[h][0], a[h][1], a[h][2], a[h][3], b0[set], b1[set]);
+                        }
+                        if (kExact) {
+                            add_up(acc[2 * b], own[0]);
+                            add_up(acc[2 * b + 1], own[1]);
                         }
                     }
-                    const float f0 = vs[0][b] * vinv, f1 = vs[1][b] * vinv;
-                    float w[HL][2];
-#pragma unroll
-                    for (int j = 0; j < HL; ++j) {
-                        w[j][0] = pr[j][0] * f0;
-                        w[j][1] = pr[j][1] * f1;
-                    }
-                    uint32_t b0[kPS], b1[kPS];
-                    operand(w, b0, b1);
-#pragma unroll
-                    for (int set = 0; set < kPS; ++set) {
-                        mma16<false>(acc[2 * b], a[0][0], a[0][1], a[0][2], a[0][3], b0[set], b1[set]);
-                        mma16<false>(acc[2 * b + 1], a[1][0], a[1][1], a[1][2], a[1][3], b0[set], b1[set]);
-                    }
                 }
-                load_after(1, tile);
             } else if constexpr (kF32) {
                 // 32-bit B operands: column g is head g's part (wide), or part g % 2 of head g / 2.
+                static_assert(MT == 1, "");
                 uint32_t pb[kPS][2][2];                               // [set][8 tokens][k = t, t + 4]
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
@@ -757,63 +1118,83 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                         }
                     }
                 }
+                if (now) {
 #pragma unroll
-                for (int ch = 0; ch < C; ++ch) {
-                    const uint32_t *vr = buf[(C + ch) & 1];
+                    for (int d32 = 0; d32 < NB; ++d32) {
+                        uint32_t x[4][4];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {                     // 32 dims
-                        const int d32 = ch * 2 + i;
-                        if (d32 >= NB) continue;
+                        for (int r = 0; r < 4; ++r) read_bytes<16>(slot + (t + 4 * r) * Sh::kStride + 128 * d32 + 16 * g, x[r]);
 #pragma unroll
-                        for (int j = 0; j < 2; ++j)
+                        for (int j = 0; j < 2; ++j) {
+                            float own[4] = {};
 #pragma unroll
                             for (int r = 0; r < 2; ++r) {             // tokens 8r .. 8r + 7
                                 uint32_t h[4], lw[4];
 #pragma unroll
                                 for (int k = 0; k < 4; ++k) {
-                                    float y = __uint_as_float(vr[(2 * r + (k >> 1)) * 8 + 4 * i + 2 * j + (k & 1)]);
+                                    float y = __uint_as_float(x[2 * r + (k >> 1)][2 * j + (k & 1)]);
                                     h[k] = __float_as_uint(take_tf32(y));
                                     lw[k] = round_tf32(y);
                                 }
 #pragma unroll
                                 for (int set = 0; set < kPS; ++set) {
-                                    mma_tf32(acc[2 * d32 + j], lw[0], lw[1], lw[2], lw[3], pb[set][r][0], pb[set][r][1]);
-                                    mma_tf32(acc[2 * d32 + j], h[0], h[1], h[2], h[3], pb[set][r][0], pb[set][r][1]);
+                                    mma_tf32(own, lw[0], lw[1], lw[2], lw[3], pb[set][r][0], pb[set][r][1]);
+                                    mma_tf32(own, h[0], h[1], h[2], h[3], pb[set][r][0], pb[set][r][1]);
                                 }
                             }
+                            add_up(acc[2 * d32 + j], own);
+                        }
                     }
-                    load_after(C + ch, tile);
                 }
             } else {
-                uint32_t b0[kPS], b1[kPS];
-                operand(pr, b0, b1);
+                uint32_t b0[MT][kPS], b1[MT][kPS];
 #pragma unroll
-                for (int ch = 0; ch < C; ++ch) {
-                    const uint32_t *vr = buf[(C + ch) & 1];
+                for (int i = 0; i < MT; ++i) {
+                    float w[HL][2];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int off = ch * Sh::kChunkBytes + 128 * i;           // bytes into the row
-                        if (off >= Sh::kRowBytes) continue;
+                    for (int j = 0; j < HL; ++j) {
+                        w[j][0] = pr[j][2 * i];
+                        w[j][1] = pr[j][2 * i + 1];
+                    }
+                    operand(w, b0[i], b1[i]);
+                }
+                if (now) {
+#pragma unroll
+                    for (int off = 0; off < Sh::kRowBytes; off += 128) {
+                        constexpr int kTail = Sh::kRowBytes % 128;                // 64 where the head ends
                         const int pairs = off + 128 <= Sh::kRowBytes ? 4 : 2;     // dims 2j, 2j + 1 of this lane
+                        uint32_t x[MT][4][4];
+#pragma unroll
+                        for (int i = 0; i < MT; ++i)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const uint8_t *row = slot + (16 * i + 2 * t + (r & 1) + 8 * (r >> 1)) * Sh::kStride + off;
+                                if (kTail && off + 128 > Sh::kRowBytes) read_bytes<8>(row + 8 * g, x[i][r]);
+                                else read_bytes<16>(row + 16 * g, x[i][r]);
+                            }
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             if (j >= pairs) continue;
-                            const uint32_t x0 = vr[0 * 8 + 4 * i + j], x1 = vr[1 * 8 + 4 * i + j];
-                            const uint32_t y0 = vr[2 * 8 + 4 * i + j], y1 = vr[3 * 8 + 4 * i + j];
-                            const uint32_t a0 = __byte_perm(x0, x1, 0x5410), a1 = __byte_perm(x0, x1, 0x7632);
-                            const uint32_t a2 = __byte_perm(y0, y1, 0x5410), a3 = __byte_perm(y0, y1, 0x7632);
+                            float own[4] = {};
+                            float(&to)[4] = kExact ? own : acc[off / 32 + j];
 #pragma unroll
-                            for (int set = 0; set < kPS; ++set)
-                                mma16<kBf16>(acc[off / 32 + j], a0, a1, a2, a3, b0[set], b1[set]);
+                            for (int i = 0; i < MT; ++i) {
+                                const uint32_t a0 = __byte_perm(x[i][0][j], x[i][1][j], 0x5410), a1 = __byte_perm(x[i][0][j], x[i][1][j], 0x7632);
+                                const uint32_t a2 = __byte_perm(x[i][2][j], x[i][3][j], 0x5410), a3 = __byte_perm(x[i][2][j], x[i][3][j], 0x7632);
+#pragma unroll
+                                for (int set = 0; set < kPS; ++set) mma16<kBf16>(to, a0, a1, a2, a3, b0[i][set], b1[i][set]);
+                            }
+                            if (kExact) add_up(acc[off / 32 + j], own);
                         }
                     }
-                    load_after(C + ch, tile);
                 }
             }
+            advance(true);
         }
+        copies_wait<0>();
 
         // ---- join the warps ----
-        const float unit = Sh::kQuant ? (vinv == 0.0f ? 0.0f : 1.0f / vinv) : 1.0f;
+        const float unit = Sh::kQuant && !kInt ? (vinv == 0.0f ? 0.0f : 1.0f / vinv) : 1.0f;
 #pragma unroll
         for (int j = 0; j < HL; ++j) {
 #pragma unroll
@@ -847,12 +1228,14 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
             if constexpr (kWide) {
                 to[0] = make_float2(acc[i][0] * f[0], acc[i][2] * f[0]);
                 to[HD / 2] = make_float2(acc[i][1] * f[1], acc[i][3] * f[1]);
+            } else if constexpr (kInt) {
+                to[0] = make_float2(acc[i][0] * f[0], acc[i][1] * f[0]);
             } else {
                 to[0] = make_float2((acc[i][0] + acc[i][1]) * f[0], (acc[i][2] + acc[i][3]) * f[0]);
             }
         }
-        const bool whole = pos == item0 && end == item0 + sp.tiles;
-        float *part = p.part + (size_t)(2 * bid + (pos == item0 ? 1 : 0)) * GH * (HD + 2);
+        const bool whole = piece0 == 0 && piece1 == sp.tiles;
+        float *part = p.part + (size_t)(2 * bid + (piece0 == 0 ? 1 : 0)) * GH * (HD + 2);
         if (warp == 0 && g == 0) {
 #pragma unroll
             for (int j = 0; j < HL; ++j) {
@@ -884,84 +1267,128 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                 else static_cast<__half *>(p.out)[off] = __float2half_rn(o);
             }
         }
-        if (pos == item0 && !whole) {
-            // The blocks of this item: this one and all up to the one that holds its last tile.
-            const long long last = ((item0 + sp.tiles) * blocks - 1) / total;
-            piece = make_int4(seq, item, (int)(last - bid) + 1, 0);
+        if (piece0 == 0) {
+            int4 mine_holds = make_int4(0, 0, 0, 0);
+            if (!whole) {
+                // The blocks of this item: this one and all up to the one that holds its last tile.
+                const unsigned x = tile_unit + sp.tiles - 1, split = longer * (each + 1);
+                const unsigned last = x < split ? x / (each + 1) : longer + (x - split) / each;
+                mine_holds = make_int4(seq, item, (int)(last - bid) + 1, (int)bid);
+                piece = mine_holds;
+            }
+            if (p.by_item && tid == 0) p.piece[seq * rows + item] = mine_holds;
         }
         pos = end;
     }
-    if (tid == 0) p.piece[bid] = piece;
+    if (tid == 0 && !p.by_item) p.piece[bid] = piece;
 }
 
-// Adds up an item that several blocks hold, one block per first holder, one
-// warp per query head.
-template <int HD, int GH>
-__global__ void __launch_bounds__(GH * 32) attend_join_kernel(const AttnParams p, float bias) {
+// Adds up the items that several blocks hold: one block per item and query
+// head, its warps taking every eighth holder, eight of them in flight.
+constexpr int kJoinWarps = 8;
+template <int HD>
+__global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const AttnParams p, int tile_heads, float bias) {
+    constexpr int kVals = HD / 32;
+    __shared__ float so[kJoinWarps][HD], sl[kJoinWarps];
     pdl_wait();
     const int4 piece = __ldcg(p.piece + blockIdx.x);
     if (piece.z == 0) return;
-    const int h = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int kh = piece.y / p.head_tiles, ht = piece.y - kh * p.head_tiles;
-    if (h >= min(GH, p.group - ht * GH)) return;
-    constexpr int kStride = GH * (HD + 2), kVals = HD / 32;
+    if (h >= min(tile_heads, p.group - ht * tile_heads)) return;
+    const size_t stride = (size_t)tile_heads * (HD + 2);
     // Holder i's partial: the second slot of the first block, the first of the others.
-    const float *part = p.part + (size_t)(2 * blockIdx.x + 1) * kStride;
+    const float *part = p.part + (2 * (size_t)piece.w + 1) * stride + h;
+    auto of = [&](int i) { return part + (i ? 2 * i - 1 : 0) * stride; };
     float M = -INFINITY;
-    for (int i = lane; i < piece.z; i += 32) M = fmaxf(M, __ldcg(part + (size_t)(i ? 2 * i - 1 : 0) * kStride + h));
+    for (int i = lane; i < piece.z; i += 32) M = fmaxf(M, __ldcg(of(i)));
+#pragma unroll
     for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     float L = 0.0f, o[kVals];
 #pragma unroll
     for (int j = 0; j < kVals; ++j) o[j] = 0.0f;
-#pragma unroll 4
-    for (int i = 0; i < piece.z; ++i) {
-        const float *x = part + (size_t)(i ? 2 * i - 1 : 0) * kStride;
-        const float w = M == -INFINITY ? 1.0f : attn_exp2(__ldcg(x + h) - M);
-        L = fmaf(w, __ldcg(x + GH + h), L);
+#pragma unroll 8
+    for (int i = warp; i < piece.z; i += kJoinWarps) {
+        const float *x = of(i);
+        const float w = M == -INFINITY ? 1.0f : attn_exp2(__ldcg(x) - M);
+        L = fmaf(w, __ldcg(x + tile_heads), L);
 #pragma unroll
-        for (int j = 0; j < kVals; ++j) o[j] = fmaf(w, __ldcg(x + 2 * GH + h * HD + 32 * j + lane), o[j]);
+        for (int j = 0; j < kVals; ++j) o[j] = fmaf(w, __ldcg(x - h + 2 * tile_heads + h * HD + 32 * j + lane), o[j]);
     }
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    const int head = kh * p.group + ht * GH + h;
-    if (p.lse && lane == 0)
-        p.lse[(long long)piece.x * p.heads + head] = L == 0.0f ? -INFINITY : (M - bias + log2f(L)) * 0.6931471805599453f;
-    const long long off = piece.x * p.out_ss + (long long)head * p.out_hs + lane;
 #pragma unroll
-    for (int j = 0; j < kVals; ++j) {
-        const float y = o[j] * inv;
-        if (p.io == DTYPE_F32) static_cast<float *>(p.out)[off + 32 * j] = y;
-        else if (p.io == DTYPE_BF16) static_cast<__nv_bfloat16 *>(p.out)[off + 32 * j] = __float2bfloat16_rn(y);
-        else static_cast<__half *>(p.out)[off + 32 * j] = __float2half_rn(y);
+    for (int j = 0; j < kVals; ++j) so[warp][32 * j + lane] = o[j];
+    if (lane == 0) sl[warp] = L;
+    __syncthreads();
+    L = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) L += sl[w];
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    const int head = kh * p.group + ht * tile_heads + h;
+    if (p.lse && threadIdx.x == 0)
+        p.lse[(long long)piece.x * p.heads + head] = L == 0.0f ? -INFINITY : (M - bias + log2f(L)) * 0.6931471805599453f;
+    const long long off = piece.x * p.out_ss + (long long)head * p.out_hs;
+    for (int d = threadIdx.x; d < HD; d += kJoinWarps * 32) {
+        float y = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) y += so[w][d];
+        y *= inv;
+        if (p.io == DTYPE_F32) static_cast<float *>(p.out)[off + d] = y;
+        else if (p.io == DTYPE_BF16) static_cast<__nv_bfloat16 *>(p.out)[off + d] = __float2bfloat16_rn(y);
+        else static_cast<__half *>(p.out)[off + d] = __float2half_rn(y);
     }
 }
 
-// The variant of a cache type for a head size: narrow or wide by the group,
-// pages of a multiple of 16 tokens or any.
-template <int kCache, int HD, bool kWide, int kQS, int kPS>
-cudaError_t attn_launch(const AttnParams &p, cudaStream_t st) {
-    if (p.l.page_size % 16 == 0)
-        attend_kernel<kCache, HD, kWide, kQS, kPS, true><<<p.blocks, kAttnWarps * 32, 0, st>>>(p);
-    else
-        attend_kernel<kCache, HD, kWide, kQS, kPS, false><<<p.blocks, kAttnWarps * 32, 0, st>>>(p);
-    const cudaError_t e = cudaGetLastError();
+// Allows a kernel its dynamic shared memory, once on each device.
+template <typename K>
+cudaError_t attn_allow(K *kernel, size_t bytes, int device, std::atomic<unsigned long long> &done) {
+    const unsigned long long bit = 1ull << (device & 63);
+    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
+}
+
+template <int kCache, int HD, bool kWide, bool kExact>
+cudaError_t attn_launch(AttnParams p, cudaStream_t st) {
+    using Sh = AttnShape<kCache, HD>;
+    constexpr int kTile = Sh::kTok * kAttnWarps;
+    p.tile_pages = kTile / p.l.page_size;
+    p.tile_slots = kTile % p.l.page_size;
+    constexpr size_t kBytes = AttnParts<kCache, kWide, kExact>::kSets * 8 * Sh::kQStride + kAttnWarps * Sh::R * Sh::kSlot;
+    static std::atomic<unsigned long long> done{0};
+    cudaError_t e = attn_allow(attend_kernel<kCache, HD, kWide, kExact>, kBytes, p.device, done);
+    if (e != cudaSuccess) return e;
+    attend_kernel<kCache, HD, kWide, kExact><<<p.blocks, kAttnWarps * 32, kBytes, st>>>(p);
+    e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     constexpr int GH = kWide ? 8 : 4;
-    return launch_pdl(attend_join_kernel<HD, GH>, dim3(p.blocks), dim3(GH * 32), 0, st, p, kAttnBias<kCache>);
+    return launch_pdl(attend_join_kernel<HD>, dim3(p.joins, std::min(GH, p.group)), dim3(kJoinWarps * 32), 0, st, p, GH,
+                      kAttnBias<kCache, kExact>);
 }
-template <int kCache, bool kWide, int kQS, int kPS>
+template <int kCache, bool kWide, bool kExact>
 cudaError_t attn_launch(const AttnParams &p, cudaStream_t st) {
     switch (p.l.head_dim) {
-        case 64: return attn_launch<kCache, 64, kWide, kQS, kPS>(p, st);
-        case 96: return attn_launch<kCache, 96, kWide, kQS, kPS>(p, st);
-        case 128: return attn_launch<kCache, 128, kWide, kQS, kPS>(p, st);
-        case 192: return attn_launch<kCache, 192, kWide, kQS, kPS>(p, st);
-        default: return attn_launch<kCache, 256, kWide, kQS, kPS>(p, st);
+        case 64: return attn_launch<kCache, 64, kWide, kExact>(p, st);
+        case 96: return attn_launch<kCache, 96, kWide, kExact>(p, st);
+        case 128: return attn_launch<kCache, 128, kWide, kExact>(p, st);
+        case 192: return attn_launch<kCache, 192, kWide, kExact>(p, st);
+        default: return attn_launch<kCache, 256, kWide, kExact>(p, st);
     }
+}
+// The variant of a cache type: narrow or wide by the group; sums of their own
+// and more parts (kExact) unless query and output are bf16, whose rounding hides
+// what these save.
+template <int kCache>
+cudaError_t attn_launch(const AttnParams &p, cudaStream_t st) {
+    if constexpr (kCache != DTYPE_F32) {
+        if (p.io == DTYPE_BF16)
+            return attn_wide(p.group) ? attn_launch<kCache, true, false>(p, st) : attn_launch<kCache, false, false>(p, st);
+    }
+    return attn_wide(p.group) ? attn_launch<kCache, true, true>(p, st) : attn_launch<kCache, false, true>(p, st);
 }
 #endif
 
-// One cache type each (attention_<type>.cu).  A bf16 query and output need
-// fewer parts than the others where noted there.
+// One cache type each (attention_<type>.cu).
 cudaError_t attn_run_f32(const AttnParams &p, cudaStream_t st);
 cudaError_t attn_run_bf16(const AttnParams &p, cudaStream_t st);
 cudaError_t attn_run_f16(const AttnParams &p, cudaStream_t st);

@@ -1,9 +1,4 @@
-// attention_q4_0.cu - the attention kernels of Q4_0 caches.  Two fp16 parts hold
-// 24 bits; a bf16 query is one exactly, and one of the probability (2^-12) is
-// enough under a bf16 output.
+// attention_q4_0.cu - the attention kernels of Q4_0 caches.
 #include "attention_kernel.cuh"
 
-cudaError_t attn_run_q4_0(const AttnParams &p, cudaStream_t st) {
-    if (!attn_wide(p.group)) return attn_launch<DTYPE_Q4_0, false, 1, 1>(p, st);
-    return p.io == DTYPE_BF16 ? attn_launch<DTYPE_Q4_0, true, 1, 1>(p, st) : attn_launch<DTYPE_Q4_0, true, 2, 2>(p, st);
-}
+cudaError_t attn_run_q4_0(const AttnParams &p, cudaStream_t st) { return attn_launch<DTYPE_Q4_0>(p, st); }

@@ -15,6 +15,13 @@ attend: q, k and p are held to at least 21 bits, sums in fp32 over at most
 ds = scale sum|q k| 2^-19; p is off by a factor of exp(+-2 ds) (1 + 2^-18) with
 the approximate exponential (2^-21), and so out by at most
 max|v| (4 ds + 2^-17) before its rounding.
+
+Quantised caches under bf16 queries are multiplied in integers: a query value is
+off by at most half of max|q| 2^-13, so ds grows by scale max|q| sum|k| 2^-14.  A
+tile's weight p s rounds to half a unit where the largest p times the largest s
+is at least 2^12, so each of its 32 tokens is off by at most 2^-13 max p max|v|,
+and as l is at least the sum of the tiles' largest p, out by at most
+32 2^-13 max|v| = 2^-8 max|v|.
 """
 from __future__ import annotations
 
@@ -430,8 +437,11 @@ def attend_plain(kv, q, table, lengths, page, heads, dim, dtype, window=0, scale
             ks, vs = k[pg, h, slot], v[pg, h, slot]
             score = x @ ks.T * scale
             ds = (x.abs() @ ks.abs().T * abs(scale)).amax(-1) * 2.0 ** -19
+            integers = dtype[0] == "q" and q.dtype == torch.bfloat16
+            if integers:
+                ds = ds + abs(scale) * x.abs().amax(-1) * ks.abs().sum(-1).amax() * 2.0 ** -14
             out[s, h * group:(h + 1) * group] = torch.softmax(score, -1) @ vs
-            bound[s, h * group:(h + 1) * group] = vs.abs().max() * (4 * ds + 2.0 ** -17)[:, None]
+            bound[s, h * group:(h + 1) * group] = vs.abs().max() * (4 * ds + 2.0 ** -17 + integers * 2.0 ** -8)[:, None]
             lse[s, h * group:(h + 1) * group] = torch.logsumexp(score, -1)
             lse_bound[s, h * group:(h + 1) * group] = 2 * ds + 2.0 ** -17
     return out, bound, lse, lse_bound
