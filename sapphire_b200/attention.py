@@ -17,6 +17,7 @@ from ._lib import (DTYPE_BF16, DTYPE_F16, DTYPE_F32, DTYPE_NAMES, AttentionArgs,
 _BY_NAME = {name.lower(): dt for dt, name in DTYPE_NAMES.items()}
 _IO = {"float32": DTYPE_F32, "bfloat16": DTYPE_BF16, "float16": DTYPE_F16}
 _io_seen: dict = {}          # dtype object -> tensor_dtype_t
+_int_seen: dict = {}         # dtype object -> whether it is int32
 
 LAYOUTS = {"half": 0, "interleaved": 1}
 SCALINGS = {"none": 0, "linear": 1, "banded": 2, "yarn": 3}
@@ -57,9 +58,17 @@ def _heads(x, what: str, rows: int | None, heads: int | None, dim: int) -> tuple
     return a, b
 
 
-def _ints(x, what: str, n: int | None):
-    if str(x.dtype).rsplit(".", 1)[-1] != "int32":
+def _int32(x, what: str) -> None:
+    """Raises unless x is int32."""
+    ok = _int_seen.get(x.dtype)
+    if ok is None:
+        ok = _int_seen[x.dtype] = str(x.dtype).rsplit(".", 1)[-1] == "int32"
+    if not ok:
         raise SapphireError(f"{what} must be int32, not {x.dtype}")
+
+
+def _ints(x, what: str, n: int | None):
+    _int32(x, what)
     if n is not None and (len(x.shape) != 1 or x.shape[0] != n):
         raise SapphireError(f"{what} has shape {tuple(x.shape)}, not [{n}]")
     if not x.is_contiguous():
@@ -69,8 +78,7 @@ def _ints(x, what: str, n: int | None):
 
 def _table(x, sequences: int):
     """(address, pages a sequence, row stride) of an int32 page table [sequences, pages]."""
-    if str(x.dtype).rsplit(".", 1)[-1] != "int32":
-        raise SapphireError(f"page_table must be int32, not {x.dtype}")
+    _int32(x, "page_table")
     if len(x.shape) != 2 or x.shape[0] != sequences:
         raise SapphireError(f"page_table has shape {tuple(x.shape)}, not [{sequences}, pages]")
     if not x.is_contiguous():

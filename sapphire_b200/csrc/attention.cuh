@@ -89,40 +89,46 @@ __device__ __forceinline__ __half from_f32<__half>(float x) {
     return __float2half_rn(x);
 }
 
-// N consecutive values (N * sizeof(T) a multiple of 16 when `wide`).
-template <typename T, int N>
-__device__ __forceinline__ void load_row(const T *p, bool wide, float (&x)[N]) {
-    if (wide) {
-        constexpr int kPer = 16 / sizeof(T);
+// Eight consecutive values as they lie in memory, so that loads in flight hold
+// no more registers than their bytes.
+template <typename T>
+struct Raw8 {
+    static constexpr int N = 8 * sizeof(T) / 16;
+    uint4 v[N];
+    // wide: p is on 16 bytes
+    __device__ __forceinline__ void load(const T *p, bool wide) {
+        if (wide) {
 #pragma unroll
-        for (int i = 0; i < N / kPer; ++i) {
-            const uint4 u = reinterpret_cast<const uint4 *>(p)[i];
-            T t[kPer];
-            memcpy(t, &u, 16);
+            for (int i = 0; i < N; ++i) v[i] = reinterpret_cast<const uint4 *>(p)[i];
+        } else {
+            T t[8];
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) x[i * kPer + j] = to_f32(t[j]);
+            for (int j = 0; j < 8; ++j) t[j] = p[j];
+            memcpy(v, t, sizeof v);
         }
-    } else {
-#pragma unroll
-        for (int j = 0; j < N; ++j) x[j] = to_f32(p[j]);
     }
-}
-template <typename T, int N>
-__device__ __forceinline__ void store_row(T *p, bool wide, const float (&x)[N]) {
-    if (wide) {
-        constexpr int kPer = 16 / sizeof(T);
+    __device__ __forceinline__ void store(T *p, bool wide) const {
+        if (wide) {
 #pragma unroll
-        for (int i = 0; i < N / kPer; ++i) {
-            T t[kPer];
+            for (int i = 0; i < N; ++i) reinterpret_cast<uint4 *>(p)[i] = v[i];
+        } else {
+            T t[8];
+            memcpy(t, v, sizeof v);
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) t[j] = from_f32<T>(x[i * kPer + j]);
-            uint4 u;
-            memcpy(&u, t, 16);
-            reinterpret_cast<uint4 *>(p)[i] = u;
+            for (int j = 0; j < 8; ++j) p[j] = t[j];
         }
-    } else {
-#pragma unroll
-        for (int j = 0; j < N; ++j) p[j] = from_f32<T>(x[j]);
     }
-}
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+        T t[8];
+        memcpy(t, v, sizeof v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = to_f32(t[j]);
+    }
+    __device__ __forceinline__ void set(const float (&x)[8]) {
+        T t[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[j] = from_f32<T>(x[j]);
+        memcpy(v, t, sizeof v);
+    }
+};
 #endif

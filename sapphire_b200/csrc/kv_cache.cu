@@ -19,13 +19,22 @@ struct KvParams {
     KvLayout l;
     KvRows r;
     int block_tokens, units;      // units: threads of one row
+    int row_heads;                // of K and V together, that the rows of a block take at a time
     bool wide;
     int *err;
 };
 
-// Where row `i` of ragged sequences lives: page (-1: nowhere) and slot.  A
-// row outside the table or on a page outside the cache sets the error word.
-__device__ __forceinline__ int2 kv_place(const KvLayout &l, const KvRows &r, int i, int *err) {
+// Where a token lives, in units of 16 bytes from a head's first row (row) and
+// from its first page (page), and its slot; slot -1: nowhere.
+struct KvPlace {
+    unsigned row, page;
+    int slot;
+};
+
+// The place of row `i` of ragged sequences.  A row outside the table or on a
+// page outside the cache sets the error word.
+__device__ __forceinline__ KvPlace kv_place(const KvLayout &l, const KvRows &r, int i, int *err) {
+    const KvPlace nowhere = {0, 0, -1};
     int s, j;
     if (r.cu_tokens) {
         // The sequence whose rows hold i: the largest s with cu_tokens[s] <= i.
@@ -35,10 +44,10 @@ __device__ __forceinline__ int2 kv_place(const KvLayout &l, const KvRows &r, int
             if (__ldg(r.cu_tokens + mid) <= i) lo = mid;
             else hi = mid - 1;
         }
-        if (lo == r.sequences) return make_int2(-1, 0);      // behind the last sequence
+        if (lo == r.sequences) return nowhere;               // behind the last sequence
         s = lo;
         j = i - __ldg(r.cu_tokens + s);
-        if (j < 0) return make_int2(-1, 0);                  // before the first
+        if (j < 0) return nowhere;                           // before the first
     } else {
         s = i;
         j = 0;
@@ -47,14 +56,18 @@ __device__ __forceinline__ int2 kv_place(const KvLayout &l, const KvRows &r, int
     const long long page = pos < 0 ? -1 : pos / l.page_size;
     if (page < 0 || page >= r.table_stride) {
         atomicOr(err, kErrCache);
-        return make_int2(-1, 0);
+        return nowhere;
     }
     const int id = __ldg(r.page_table + (long long)s * r.table_stride + page);
     if (id < 0 || id >= l.num_pages) {
         atomicOr(err, kErrCache);
-        return make_int2(-1, 0);
+        return nowhere;
     }
-    return make_int2(id, (int)(pos - page * l.page_size));
+    KvPlace at;
+    at.slot = (int)(pos - page * l.page_size);
+    at.page = (unsigned)id * (unsigned)(l.page_bytes >> 4);
+    at.row = at.page + (unsigned)(at.slot * (l.row_bytes >> 4));
+    return at;
 }
 
 // Lanes of one 32-value block: four neighbours, `mask` their bits.
@@ -66,21 +79,36 @@ __device__ __forceinline__ float block_max(float v, unsigned mask) {
 // Codes of 8 values as the two words' bytes (Q8_0: one uint32 each; Q4_0: 16
 // bits each); returns the block's scale.
 __device__ __forceinline__ float quantize_q8(const float (&x)[kUnit], unsigned mask, uint32_t (&w)[2]) {
-    float a = 0.0f;
+    float a = 0.0f, odd = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kUnit; ++j) a = fmaxf(a, fabsf(x[j]));
+    for (int j = 0; j < kUnit; ++j) {
+        a = fmaxf(a, fabsf(x[j]));
+        odd = fmaf(x[j], 0.0f, odd);      // NaN where a value is none or infinite
+    }
     const float d = __fdiv_rn(block_max(a, mask), 127.0f);
     const float id = d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
+    uint32_t q[kUnit];
+    if (odd == 0.0f && id < INFINITY) {
+        // |x| id is at most 127 and a rounding, so no code is clamped.  Half
+        // away from zero is the whole part of |t| + 1/2: both sums truncate,
+        // so neither rounds a value below a half up.
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        w[k] = 0;
+        for (int j = 0; j < kUnit; ++j) {
+            const float t = __fmul_rn(x[j], id);
+            const int n = (int)__float_as_uint(__fadd_rz(__fadd_rz(fabsf(t), 0.5f), 8388608.0f));
+            const int sign = (int)__float_as_uint(t) >> 31;
+            q[j] = (uint32_t)((n ^ sign) - sign + 128);
+        }
+    } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float t = roundf(__fmul_rn(x[4 * k + j], id));
-            const int q = (t != t) ? 0 : (t > 127.0f ? 127 : (t < -127.0f ? -127 : (int)t));
-            w[k] |= (uint32_t)(q + 128) << (8 * j);
+        for (int j = 0; j < kUnit; ++j) {
+            const float t = roundf(__fmul_rn(x[j], id));
+            q[j] = (uint32_t)(((t != t) ? 0 : (t > 127.0f ? 127 : (t < -127.0f ? -127 : (int)t))) + 128);
         }
     }
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+        w[k] = __byte_perm(__byte_perm(q[4 * k], q[4 * k + 1], 0x0040), __byte_perm(q[4 * k + 2], q[4 * k + 3], 0x0040), 0x5410);
     return d;
 }
 __device__ __forceinline__ float quantize_q4(const float (&x)[kUnit], unsigned mask, uint32_t (&w)[2]) {
@@ -109,104 +137,192 @@ __device__ __forceinline__ float quantize_q4(const float (&x)[kUnit], unsigned m
         w[k] = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float t = __fadd_rn(__fmul_rn(x[4 * k + j], id), 8.5f);
-            const uint32_t q = t >= 15.0f ? 15u : (t >= 1.0f ? (uint32_t)__float2int_rz(t) : 0u);
-            w[k] |= q << (4 * j);
+            // a NaN becomes 0; the truncating sum leaves the whole part
+            const float t = fminf(fmaxf(__fadd_rn(__fmul_rn(x[4 * k + j], id), 8.5f), 0.0f), 15.0f);
+            w[k] |= (__float_as_uint(__fadd_rz(t, 8388608.0f)) & 15u) << (4 * j);
         }
     }
     return d;
 }
 
-// A block stores block_tokens tokens: K and V rows of every KV head.  A thread
-// owns one unit of a row; the four threads of a quantised block are
-// neighbours in a warp (units is a multiple of 4 for quantised formats).
+// Rows of a block: K and V of every KV head of block_tokens tokens.  A thread
+// owns one unit of a row and one row of blockDim.y: K or V of KV head y %
+// row_heads (V behind K), token y / row_heads; it walks down the tokens, kBatch
+// at a time with their loads in flight together, and then the heads.  The four
+// threads of a quantised block are neighbours in a warp (units is a multiple of 4).
+constexpr int kBatch = 2;
+
+// The type of a dense cache's values (unused for quantised ones).
+template <int kCache>
+struct KvType {
+    using type = float;
+};
+template <>
+struct KvType<DTYPE_BF16> {
+    using type = __nv_bfloat16;
+};
+template <>
+struct KvType<DTYPE_F16> {
+    using type = __half;
+};
+
+// What a thread needs of its head: its unit of the block's first token, and the
+// head's rows and scales in the first page.
+template <typename T>
+struct KvHead {
+    T *io;
+    long long ts;
+    uint8_t *rows, *scales;
+};
+template <typename T>
+__device__ __forceinline__ KvHead<T> kv_head(const KvParams &p, int c, int t0, int d0) {
+    const bool is_v = c >= p.l.kv_heads;
+    const int h = is_v ? c - p.l.kv_heads : c;
+    KvHead<T> r;
+    r.ts = is_v ? p.r.v_ts : p.r.k_ts;
+    r.io = static_cast<T *>(is_v ? p.r.v : p.r.k) + (long long)t0 * r.ts + (long long)h * (is_v ? p.r.v_hs : p.r.k_hs) + d0;
+    uint8_t *chunk = p.l.pages + (unsigned long long)h * p.l.chunk_bytes;
+    r.rows = chunk + (is_v ? p.l.v_off : 0);
+    r.scales = chunk + (is_v ? p.l.vs_off : p.l.ks_off);
+    return r;
+}
+__device__ __forceinline__ uint8_t *kv_at(uint8_t *p, unsigned off16) { return p + (unsigned long long)off16 * 16; }
+
 template <typename T, int kCache>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvParams p) {
-    __shared__ int2 place[kMaxTokens];
+    __shared__ KvPlace place[kMaxTokens];
     const int t0 = blockIdx.x * p.block_tokens, nt = min(p.block_tokens, p.r.tokens - t0);
     const int tid = threadIdx.y * blockDim.x + threadIdx.x;
-    if (tid < nt) place[tid] = kv_place(p.l, p.r, t0 + tid, p.err);
-    __syncthreads();
-    const int u = threadIdx.x, d0 = u * kUnit, heads = p.l.kv_heads;
+    const int u = threadIdx.x, token_rows = blockDim.y / p.row_heads, heads = 2 * p.l.kv_heads;
+    const int ty = threadIdx.y / p.row_heads, cy = threadIdx.y - ty * p.row_heads;
+    const int nb = p.l.head_dim / 32, b = u >> 2, word = 2 * (u & 3);
     const unsigned mask = 0xfu << (tid & 28);
-    for (int i = threadIdx.y; i < nt * 2 * heads; i += blockDim.y) {
-        const int t = i / (2 * heads), c = i - t * 2 * heads;
-        const bool is_v = c >= heads;
-        const int h = is_v ? c - heads : c;
-        const int2 at = place[t];
-        if (at.x < 0) continue;
-        const T *src = (is_v ? static_cast<const T *>(p.r.v) + (long long)(t0 + t) * p.r.v_ts + (long long)h * p.r.v_hs
-                             : static_cast<const T *>(p.r.k) + (long long)(t0 + t) * p.r.k_ts + (long long)h * p.r.k_hs) + d0;
-        uint8_t *chunk = p.l.pages + (unsigned long long)at.x * p.l.page_bytes + (unsigned long long)h * p.l.chunk_bytes;
-        uint8_t *row = chunk + (is_v ? p.l.v_off : 0) + at.y * p.l.row_bytes;
-        float x[kUnit];
-        load_row<T, kUnit>(src, p.wide, x);
-        if (kCache == DTYPE_Q8_0 || kCache == DTYPE_Q4_0) {
-            const int nb = p.l.head_dim / 32, b = u >> 2, word = 2 * (u & 3);
-            uint32_t w[2];
-            float d;
-            if (kCache == DTYPE_Q8_0) {
-                d = quantize_q8(x, mask, w);
-                reinterpret_cast<uint32_t *>(row)[word * nb + b] = w[0];
-                reinterpret_cast<uint32_t *>(row)[(word + 1) * nb + b] = w[1];
-            } else {
-                d = quantize_q4(x, mask, w);
-                reinterpret_cast<uint16_t *>(row)[word * nb + b] = (uint16_t)w[0];
-                reinterpret_cast<uint16_t *>(row)[(word + 1) * nb + b] = (uint16_t)w[1];
+    bool looked = false;
+    for (int c = cy; c < heads; c += p.row_heads) {
+        const KvHead<T> r = kv_head<T>(p, c, t0, u * kUnit);
+        // kBatch tokens at a time, the next ones' loads in flight.
+        Raw8<T> x[kBatch];
+        const T *io = r.io + ty * r.ts;
+        const long long step = token_rows * r.ts;
+        auto load = [&](int t) {
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k, io += step)
+                if (t + k * token_rows < nt) x[k].load(io, p.wide);
+        };
+        load(ty);
+        if (!looked) {                    // the first rows do not wait for their places
+            if (tid < nt) place[tid] = kv_place(p.l, p.r, t0 + tid, p.err);
+            __syncthreads();
+            looked = true;
+        }
+        for (int t = ty; t < nt; t += kBatch * token_rows) {
+            Raw8<T> y[kBatch];
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) y[k] = x[k];
+            load(t + kBatch * token_rows);
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                if (t + k * token_rows >= nt) continue;
+                const KvPlace at = place[t + k * token_rows];
+                if (at.slot < 0) continue;
+                uint8_t *row = kv_at(r.rows, at.row);
+                float v[kUnit];
+                y[k].get(v);
+                if (kCache == DTYPE_Q8_0 || kCache == DTYPE_Q4_0) {
+                    uint32_t q[2];
+                    float d;
+                    if (kCache == DTYPE_Q8_0) {
+                        d = quantize_q8(v, mask, q);
+                        reinterpret_cast<uint32_t *>(row)[word * nb + b] = q[0];
+                        reinterpret_cast<uint32_t *>(row)[(word + 1) * nb + b] = q[1];
+                    } else {
+                        d = quantize_q4(v, mask, q);
+                        reinterpret_cast<uint16_t *>(row)[word * nb + b] = (uint16_t)q[0];
+                        reinterpret_cast<uint16_t *>(row)[(word + 1) * nb + b] = (uint16_t)q[1];
+                    }
+                    if ((u & 3) == 0) reinterpret_cast<float *>(kv_at(r.scales, at.page))[at.slot * p.l.scale_stride + b] = d;
+                } else {
+                    using C = typename KvType<kCache>::type;
+                    Raw8<C> z;
+                    z.set(v);
+                    z.store(reinterpret_cast<C *>(row) + u * kUnit, true);
+                }
             }
-            if ((u & 3) == 0)
-                reinterpret_cast<float *>(chunk + (is_v ? p.l.vs_off : p.l.ks_off))[at.y * p.l.scale_stride + b] = d;
-        } else if (kCache == DTYPE_F32) {
-            store_row<float, kUnit>(reinterpret_cast<float *>(row) + d0, true, x);
-        } else if (kCache == DTYPE_BF16) {
-            store_row<__nv_bfloat16, kUnit>(reinterpret_cast<__nv_bfloat16 *>(row) + d0, true, x);
-        } else {
-            store_row<__half, kUnit>(reinterpret_cast<__half *>(row) + d0, true, x);
         }
     }
 }
 
 template <typename T, int kCache>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvParams p) {
-    __shared__ int2 place[kMaxTokens];
+    constexpr bool kQuant = kCache == DTYPE_Q8_0 || kCache == DTYPE_Q4_0;
+    using C = typename KvType<kCache>::type;
+    __shared__ KvPlace place[kMaxTokens];
     const int t0 = blockIdx.x * p.block_tokens, nt = min(p.block_tokens, p.r.tokens - t0);
     const int tid = threadIdx.y * blockDim.x + threadIdx.x;
+    const int u = threadIdx.x, token_rows = blockDim.y / p.row_heads, heads = 2 * p.l.kv_heads;
+    const int ty = threadIdx.y / p.row_heads, cy = threadIdx.y - ty * p.row_heads;
+    const int nb = p.l.head_dim / 32, b = u >> 2, word = 2 * (u & 3);
+    const int at_u = kCache == DTYPE_Q8_0 ? 4 * (word * nb + b) : kCache == DTYPE_Q4_0 ? 2 * (word * nb + b) : u * kUnit * (int)sizeof(C);
+    // What a thread loads of a row: a block's scale and the bytes of two words, or values.
+    struct Unit {
+        bool ok;
+        float d;
+        uint32_t w[2];
+        Raw8<C> x;
+    };
     if (tid < nt) place[tid] = kv_place(p.l, p.r, t0 + tid, p.err);
     __syncthreads();
-    const int u = threadIdx.x, d0 = u * kUnit, heads = p.l.kv_heads;
-    for (int i = threadIdx.y; i < nt * 2 * heads; i += blockDim.y) {
-        const int t = i / (2 * heads), c = i - t * 2 * heads;
-        const bool is_v = c >= heads;
-        const int h = is_v ? c - heads : c;
-        const int2 at = place[t];
-        if (at.x < 0) continue;
-        T *dst = (is_v ? static_cast<T *>(p.r.v) + (long long)(t0 + t) * p.r.v_ts + (long long)h * p.r.v_hs
-                       : static_cast<T *>(p.r.k) + (long long)(t0 + t) * p.r.k_ts + (long long)h * p.r.k_hs) + d0;
-        const uint8_t *chunk =
-            p.l.pages + (unsigned long long)at.x * p.l.page_bytes + (unsigned long long)h * p.l.chunk_bytes;
-        const uint8_t *row = chunk + (is_v ? p.l.v_off : 0) + at.y * p.l.row_bytes;
-        float x[kUnit];
-        if (kCache == DTYPE_Q8_0 || kCache == DTYPE_Q4_0) {
-            const int nb = p.l.head_dim / 32, b = u >> 2, word = 2 * (u & 3);
-            const float d = reinterpret_cast<const float *>(chunk + (is_v ? p.l.vs_off : p.l.ks_off))[at.y * p.l.scale_stride + b];
+    for (int c = cy; c < heads; c += p.row_heads) {
+        const KvHead<T> r = kv_head<T>(p, c, t0, u * kUnit);
+        uint8_t *const rows = r.rows + at_u, *const scales = r.scales + 4 * b;
+        Unit x[kBatch];
+        auto load = [&](int t) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const uint32_t w = kCache == DTYPE_Q8_0 ? reinterpret_cast<const uint32_t *>(row)[(word + k) * nb + b]
-                                                        : reinterpret_cast<const uint16_t *>(row)[(word + k) * nb + b];
+            for (int k = 0; k < kBatch; ++k) {
+                x[k].ok = false;
+                if (t + k * token_rows >= nt) continue;
+                const KvPlace at = place[t + k * token_rows];
+                x[k].ok = at.slot >= 0;
+                if (!x[k].ok) continue;
+                const uint8_t *row = kv_at(rows, at.row);
+                if constexpr (kQuant) {
+                    x[k].d = *reinterpret_cast<const float *>(kv_at(scales, at.page) + at.slot * p.l.scale_stride * 4);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int q = kCache == DTYPE_Q8_0 ? (int)((w >> (8 * j)) & 255u) - 128 : (int)((w >> (4 * j)) & 15u) - 8;
-                    x[4 * k + j] = __fmul_rn((float)q, d);
+                    for (int j = 0; j < 2; ++j)
+                        x[k].w[j] = kCache == DTYPE_Q8_0 ? reinterpret_cast<const uint32_t *>(row)[j * nb] : reinterpret_cast<const uint16_t *>(row)[j * nb];
+                } else {
+                    x[k].x.load(reinterpret_cast<const C *>(row), true);
                 }
             }
-        } else if (kCache == DTYPE_F32) {
-            load_row<float, kUnit>(reinterpret_cast<const float *>(row) + d0, true, x);
-        } else if (kCache == DTYPE_BF16) {
-            load_row<__nv_bfloat16, kUnit>(reinterpret_cast<const __nv_bfloat16 *>(row) + d0, true, x);
-        } else {
-            load_row<__half, kUnit>(reinterpret_cast<const __half *>(row) + d0, true, x);
+        };
+        load(ty);
+        T *io = r.io + ty * r.ts;
+        const long long step = token_rows * r.ts;
+        for (int t = ty; t < nt; t += kBatch * token_rows) {
+            Unit y[kBatch];
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) y[k] = x[k];
+            load(t + kBatch * token_rows);
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k, io += step) {
+                if (!y[k].ok) continue;
+                float v[kUnit];
+                if constexpr (kQuant) {
+                    // 2^23 + code by its bytes, and the offset off again: exact
+#pragma unroll
+                    for (int j = 0; j < kUnit; ++j) {
+                        const uint32_t q = kCache == DTYPE_Q8_0 ? __byte_perm(y[k].w[j / 4], 0x4b000000u, 0x7440 + (j & 3))
+                                                                : ((y[k].w[j / 4] >> (4 * (j & 3))) & 15u) | 0x4b000000u;
+                        v[j] = __fmul_rn(__fadd_rn(__uint_as_float(q), kCache == DTYPE_Q8_0 ? -8388736.0f : -8388616.0f), y[k].d);
+                    }
+                } else {
+                    y[k].x.get(v);
+                }
+                Raw8<T> z;
+                z.set(v);
+                z.store(io, p.wide);
+            }
         }
-        store_row<T, kUnit>(dst, p.wide, x);
     }
 }
 
@@ -268,11 +384,18 @@ int kv_call(kernel_context_t *ctx, const sapphire_kv_cache_t *cache, const sapph
     p.err = ctx->d_err;
     p.units = cache->head_dim / kUnit;
     AttnDevice g(ctx->device);
-    const int rows = kThreads / p.units, sms = sm_count(ctx->device);
-    // About four rows a thread while that still gives every SM two blocks.
-    p.block_tokens = std::min(kMaxTokens, std::max(1, 4 * rows / (2 * cache->kv_heads)));
-    while (p.block_tokens > 1 && (a->tokens + p.block_tokens - 1) / p.block_tokens < 2 * sms) p.block_tokens /= 2;
-    const dim3 grid((a->tokens + p.block_tokens - 1) / p.block_tokens), block(p.units, rows);
+    const int rows = kThreads / p.units, sms = sm_count(ctx->device), heads = 2 * cache->kv_heads;
+    // A block's rows are heads of one token, evenly divided where there are
+    // more than rows, or heads of several tokens.  It looks its tokens up
+    // first, so it takes eight batches of them behind that, while every SM still
+    // gets four blocks; fewer tokens are cut finer.
+    const int steps = (heads + rows - 1) / rows;
+    p.row_heads = (heads + steps - 1) / steps;
+    const int token_rows = rows / p.row_heads;
+    p.block_tokens = std::min(kMaxTokens, 8 * kBatch * token_rows);
+    while (p.block_tokens > 1 && (a->tokens + p.block_tokens - 1) / p.block_tokens < 4 * sms) p.block_tokens /= 2;
+    const dim3 grid((a->tokens + p.block_tokens - 1) / p.block_tokens);
+    const dim3 block(p.units, p.row_heads * std::min(token_rows, p.block_tokens));
     switch (a->dtype) {
         case DTYPE_F32: launch_kv<float>(cache->dtype, p, write, grid, block, ctx->stream); break;
         case DTYPE_BF16: launch_kv<__nv_bfloat16>(cache->dtype, p, write, grid, block, ctx->stream); break;

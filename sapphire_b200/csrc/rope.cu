@@ -26,6 +26,7 @@ namespace {
 constexpr int kRopeMaxDim = 512;
 constexpr int kThreads = 256;
 constexpr int kUnit = 8;                  // values of a head that a thread takes from each half
+constexpr int kBatch = 2;                 // rows of a thread in flight
 constexpr int kMaxTokens = 16;            // tokens of one block (its cos and sin rows in shared memory)
 
 struct RopeHeads {
@@ -41,88 +42,128 @@ struct RopeParams {
     int tokens, q_heads, heads;           // heads: query and key heads together
     int head_dim, half;                   // half: rot_dim / 2
     int block_tokens, block_heads;
-    int units;                            // threads of one head: pair units, then copy units
+    int row_heads;                        // heads that the rows of a block take at a time
     int pair_units;
     float amplitude, direction;           // direction: 1, or -1 to turn back
     bool wide, copy_tail;
 };
 
-// A block turns block_tokens tokens x block_heads heads; a thread owns one
-// unit of a head (8 values of the first half and their 8 partners, or 8
-// interleaved values) and walks down the heads.
+// A block turns block_tokens tokens x its heads.  A thread owns one unit of a
+// head (8 values of the first half and their 8 partners, 8 interleaved values,
+// or 8 values behind the rotated part) and one row of blockDim.y: head h0 + y %
+// row_heads, token y / row_heads; it walks down the tokens and then the heads.
+// The block's cos and sin lie in shared memory as [token][pair of pairs][unit],
+// so that neighbouring units read neighbouring 16 bytes.
 template <typename T, bool kInterleaved>
 __global__ void __launch_bounds__(kThreads) rope_kernel(const RopeParams p) {
-    extern __shared__ float2 turn[];      // [block_tokens][half] (cos, sin)
-    const int t0 = blockIdx.x * p.block_tokens, nt = min(p.block_tokens, p.tokens - t0);
+    constexpr int kPairs = kInterleaved ? kUnit / 2 : kUnit;
+    extern __shared__ float4 turn[];
+    const int t0 = blockIdx.x * p.block_tokens, nt = min(p.block_tokens, p.tokens - t0), units = p.pair_units;
     const int tid = threadIdx.y * blockDim.x + threadIdx.x, nthreads = blockDim.x * blockDim.y;
+    const int u = threadIdx.x, token_rows = blockDim.y / p.row_heads;
+    const int h0 = blockIdx.y * p.block_heads, h_end = min(h0 + p.block_heads, p.heads);
+    const int ty = threadIdx.y / p.row_heads, hy = threadIdx.y - ty * p.row_heads;
+    const bool tail = u >= units;         // behind the rotated part
+    const int m0 = u * kPairs, d_tail = 2 * p.half + (u - units) * kUnit;
+    const int at_a = tail ? d_tail : kInterleaved ? 2 * m0 : m0, at_b = p.half + m0;
+    const bool short_unit = tail ? d_tail + kUnit > p.head_dim : m0 + kPairs > p.half;
+    auto input = [&](int h, int t) {
+        const RopeHeads &x = h >= p.q_heads ? p.k : p.q;
+        return static_cast<const T *>(x.in) + (long long)(t0 + t) * x.in_ts + (long long)(h >= p.q_heads ? h - p.q_heads : h) * x.in_hs;
+    };
+    auto output = [&](int h, int t) {
+        const RopeHeads &x = h >= p.q_heads ? p.k : p.q;
+        return static_cast<T *>(x.out) + (long long)(t0 + t) * x.out_ts + (long long)(h >= p.q_heads ? h - p.q_heads : h) * x.out_hs;
+    };
+    // kBatch tokens of a head at a time, the next ones' loads in flight.
+    struct Batch {
+        Raw8<T> a[kBatch], b[kInterleaved ? 1 : kBatch];
+    };
+    auto load = [&](Batch &x, int h, int t1) {
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const int t = t1 + k * token_rows;
+            if (t >= nt) continue;
+            const T *in = input(h, t);
+            x.a[k].load(in + at_a, p.wide);
+            if constexpr (!kInterleaved)
+                if (!tail) x.b[k].load(in + at_b, p.wide);
+        }
+    };
+    int h = h0 + hy, t1 = ty;
+    bool more = !short_unit && h < h_end && t1 < nt;
+    Batch x;
+    if (more) load(x, h, t1);
     for (int i = tid; i < nt * p.half; i += nthreads) {
-        const int t = i / p.half, m = i - t * p.half;
+        const int t = i / p.half, m = i - t * p.half, j = m % kPairs;
         const unsigned long long phase = (unsigned long long)(long long)p.positions[t0 + t] * p.freq[m];
         float s, c;
         sincospif((float)(int)(phase >> 32) * 0x1p-31f, &s, &c);
-        turn[i] = make_float2(c * p.amplitude, s * p.amplitude * p.direction);
+        reinterpret_cast<float2 *>(turn)[((t * (kPairs / 2) + j / 2) * units + m / kPairs) * 2 + j % 2] =
+            make_float2(c * p.amplitude, s * p.amplitude * p.direction);
     }
     __syncthreads();
-    const int h0 = blockIdx.y * p.block_heads, nh = min(p.block_heads, p.heads - h0);
-    const int u = threadIdx.x;
-    for (int r = threadIdx.y; r < nt * nh; r += blockDim.y) {
-        const int t = r / nh;
-        int h = h0 + r - t * nh;
-        const RopeHeads &x = h < p.q_heads ? p.q : p.k;
-        if (h >= p.q_heads) h -= p.q_heads;
-        const T *in = static_cast<const T *>(x.in) + (long long)(t0 + t) * x.in_ts + (long long)h * x.in_hs;
-        T *out = static_cast<T *>(x.out) + (long long)(t0 + t) * x.out_ts + (long long)h * x.out_hs;
-        if (u >= p.pair_units) {          // behind the rotated part
-            const int d0 = 2 * p.half + (u - p.pair_units) * kUnit;
-            if (d0 + kUnit <= p.head_dim) {
-                float a[kUnit];
-                load_row<T, kUnit>(in + d0, p.wide, a);
-                store_row<T, kUnit>(out + d0, p.wide, a);
-            } else {
-                for (int d = d0; d < p.head_dim; ++d) out[d] = in[d];
-            }
-        } else if (kInterleaved) {
-            const int m0 = u * (kUnit / 2), n = min(kUnit / 2, p.half - m0);
-            const float2 *cs = turn + t * p.half + m0;
-            if (n == kUnit / 2) {
-                float a[kUnit], y[kUnit];
-                load_row<T, kUnit>(in + 2 * m0, p.wide, a);
-#pragma unroll
-                for (int j = 0; j < kUnit / 2; ++j) {
-                    y[2 * j] = a[2 * j] * cs[j].x - a[2 * j + 1] * cs[j].y;
-                    y[2 * j + 1] = a[2 * j] * cs[j].y + a[2 * j + 1] * cs[j].x;
+    if (short_unit) {
+        // The end of a part: value by value.
+        for (; h < h_end; h += p.row_heads)
+            for (int t = ty; t < nt; t += token_rows) {
+                const T *a = input(h, t);
+                T *o = output(h, t);
+                if (tail) {
+                    for (int d = d_tail; d < p.head_dim; ++d) o[d] = a[d];
+                    continue;
                 }
-                store_row<T, kUnit>(out + 2 * m0, p.wide, y);
-            } else {
-                for (int j = 0; j < n; ++j) {
-                    const float a = to_f32(in[2 * (m0 + j)]), b = to_f32(in[2 * (m0 + j) + 1]);
-                    out[2 * (m0 + j)] = from_f32<T>(a * cs[j].x - b * cs[j].y);
-                    out[2 * (m0 + j) + 1] = from_f32<T>(a * cs[j].y + b * cs[j].x);
+                for (int m = m0; m < p.half; ++m) {
+                    const float2 cs = reinterpret_cast<const float2 *>(turn)[((t * (kPairs / 2) + (m - m0) / 2) * units + u) * 2 + (m - m0) % 2];
+                    const int i = kInterleaved ? 2 * m : m, j = kInterleaved ? 2 * m + 1 : p.half + m;
+                    const float v0 = to_f32(a[i]), v1 = to_f32(a[j]);
+                    o[i] = from_f32<T>(v0 * cs.x - v1 * cs.y);
+                    o[j] = from_f32<T>(v0 * cs.y + v1 * cs.x);
                 }
             }
-        } else {
-            const int m0 = u * kUnit, n = min(kUnit, p.half - m0);
-            const float2 *cs = turn + t * p.half + m0;
-            if (n == kUnit) {
-                float a[kUnit], b[kUnit];
-                load_row<T, kUnit>(in + m0, p.wide, a);
-                load_row<T, kUnit>(in + p.half + m0, p.wide, b);
-#pragma unroll
-                for (int j = 0; j < kUnit; ++j) {
-                    const float x0 = a[j], x1 = b[j];
-                    a[j] = x0 * cs[j].x - x1 * cs[j].y;
-                    b[j] = x0 * cs[j].y + x1 * cs[j].x;
-                }
-                store_row<T, kUnit>(out + m0, p.wide, a);
-                store_row<T, kUnit>(out + p.half + m0, p.wide, b);
-            } else {
-                for (int j = 0; j < n; ++j) {
-                    const float a = to_f32(in[m0 + j]), b = to_f32(in[p.half + m0 + j]);
-                    out[m0 + j] = from_f32<T>(a * cs[j].x - b * cs[j].y);
-                    out[p.half + m0 + j] = from_f32<T>(a * cs[j].y + b * cs[j].x);
-                }
-            }
+        return;
+    }
+    while (more) {
+        int h2 = h, t2 = t1 + kBatch * token_rows;
+        if (t2 >= nt) {
+            t2 = ty;
+            h2 += p.row_heads;
         }
+        more = h2 < h_end;
+        Batch next;
+        if (more) load(next, h2, t2);
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const int t = t1 + k * token_rows;
+            if (t >= nt) continue;
+            T *out = output(h, t);
+            if (!tail) {
+                float a[kUnit], b[kUnit];
+                x.a[k].get(a);
+                if constexpr (!kInterleaved) x.b[k].get(b);
+#pragma unroll
+                for (int j = 0; j < kPairs; j += 2) {
+                    const float4 cs = turn[(t * (kPairs / 2) + j / 2) * units + u];
+                    const float c2[4] = {cs.x, cs.y, cs.z, cs.w};
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float &v = kInterleaved ? a[(2 * (j + i)) & 7] : a[j + i], &w = kInterleaved ? a[(2 * (j + i) + 1) & 7] : b[j + i];
+                        const float v0 = v, v1 = w;
+                        v = v0 * c2[2 * i] - v1 * c2[2 * i + 1];
+                        w = v0 * c2[2 * i + 1] + v1 * c2[2 * i];
+                    }
+                }
+                x.a[k].set(a);
+                if constexpr (!kInterleaved) {
+                    x.b[k].set(b);
+                    x.b[k].store(out + at_b, p.wide);
+                }
+            }
+            x.a[k].store(out + at_a, p.wide);
+        }
+        x = next;
+        h = h2;
+        t1 = t2;
     }
 }
 
@@ -299,21 +340,27 @@ extern "C" SAPPHIRE_API int sapphire_rope_device(sapphire_rope_t *rope, const sa
     p.wide = p.wide && (c.rot_dim * (int)size) % 16 == 0 && (inter || (p.half * (int)size) % 16 == 0);
     p.pair_units = inter ? (p.half + kUnit / 2 - 1) / (kUnit / 2) : (p.half + kUnit - 1) / kUnit;
     const int tail = p.copy_tail ? (c.head_dim - c.rot_dim + kUnit - 1) / kUnit : 0;
-    p.units = p.pair_units + tail;
-    const int rows = std::max(1, kThreads / p.units);
-    // A block takes as many tokens as give each of its rows about four heads;
-    // few tokens are cut by heads instead, each block computing its own turns.
+    const int units = p.pair_units + tail;      // threads of one head
+    const int rows = std::max(1, kThreads / units);
+    // A block's rows are heads of one token, evenly divided where there are
+    // more than rows, or heads of several tokens; each row then walks down
+    // about four tokens, so a block's cos and sin serve every head.  Few tokens
+    // are cut by heads, each block computing its own turns.
     AttnDevice g(ctx->device);
     const int sms = sm_count(ctx->device);
+    auto cut = [](int n, int most) { return (n + (n + most - 1) / most - 1) / ((n + most - 1) / most); };
     p.block_heads = p.heads;
-    p.block_tokens = std::min(kMaxTokens, std::max(1, 4 * rows / p.heads));
+    p.row_heads = cut(p.heads, rows);
+    const int token_rows = rows / p.row_heads;
+    p.block_tokens = std::min(kMaxTokens, 4 * kBatch * token_rows);
     while (p.block_tokens > 1 && (p.tokens + p.block_tokens - 1) / p.block_tokens < 2 * sms) p.block_tokens /= 2;
     if (p.block_tokens == 1)
         while (p.block_heads > rows && (long long)p.tokens * ((p.heads + p.block_heads - 1) / p.block_heads) < 2 * sms)
             p.block_heads = (p.block_heads + 1) / 2;
+    p.row_heads = std::min(p.row_heads, p.block_heads);
     const dim3 grid((p.tokens + p.block_tokens - 1) / p.block_tokens, (p.heads + p.block_heads - 1) / p.block_heads);
-    const dim3 block(p.units, rows);
-    const size_t smem = (size_t)p.block_tokens * p.half * sizeof(float2);
+    const dim3 block(units, p.row_heads * std::min(token_rows, p.block_tokens));
+    const size_t smem = (size_t)p.block_tokens * p.pair_units * (inter ? kUnit / 2 : kUnit) * sizeof(float2);
     cudaError_t e = a->dtype == DTYPE_F32    ? launch_rope<float>(p, inter, grid, block, smem, ctx->stream)
                     : a->dtype == DTYPE_BF16 ? launch_rope<__nv_bfloat16>(p, inter, grid, block, smem, ctx->stream)
                                              : launch_rope<__half>(p, inter, grid, block, smem, ctx->stream);
