@@ -33,16 +33,13 @@
 //   P (B operand): a movmatrix of the packed (high, low) pairs.
 //
 // Quantised rows are kept as words of 4 codes in the order [8][nb], so the same
-// lanes read consecutive bytes.  Under a bf16 output codes are multiplied as
-// the integers they are: the query becomes 15-bit integers (two signed bytes),
-// and a tile's probabilities times V's scales become 15-bit integers relative
-// to the tile's largest, per head and block of 32 dims; sums are exact, the
-// codes' offsets come off with an MMA of ones, and one conversion and product
-// per sum brings it to fp32.  That is a third of the instructions of converting
-// codes to fp16, which fp32 and fp16 outputs take (1024 + code - 1152 or - 1032,
-// exactly): there K's scale multiplies the 32-dim partial score and V's scale the
-// probability, brought into fp16's range by a power of two per warp that grows
-// with the scales seen.
+// lanes read consecutive bytes.  V's codes become fp16 exactly (1024 + code - 1152,
+// or - 1032), and V's scale multiplies the probability, brought into fp16's range
+// by a power of two per warp that grows with the scales seen.  K's codes become
+// fp16 the same way under fp32 and fp16 outputs; under a bf16 output they are
+// multiplied as the integers they are by the query as 15-bit integers (two
+// signed bytes), the sums exact and started at what the codes' offset adds, and
+// one conversion and product with K's scale brings a block's sum to fp32.
 //
 // Split.  The tiles (64 tokens of one KV head and up to 8 query heads) of all
 // sequences are numbered in a row and cut into as many equal ranges as the GPU
@@ -97,12 +94,12 @@ constexpr int attn_blocks_per_sm(int cache, int hd) {
 
 #ifdef __CUDACC__
 
-// Codes are multiplied as integers where the output's rounding allows.
+// K's codes are multiplied as integers where the output's rounding allows.
 template <int kCache, bool kExact>
 constexpr bool kAttnInt = (kCache == DTYPE_Q8_0 || kCache == DTYPE_Q4_0) && !kExact;
 // 2^(p + kBias): probabilities use the upper end of fp16 where the MMA is fp16.
-template <int kCache, bool kExact>
-constexpr float kAttnBias = (kCache == DTYPE_BF16 || kCache == DTYPE_F32 || kAttnInt<kCache, kExact>) ? 0.0f : 14.0f;
+template <int kCache>
+constexpr float kAttnBias = (kCache == DTYPE_BF16 || kCache == DTYPE_F32) ? 0.0f : 14.0f;
 
 __device__ __forceinline__ float attn_exp2(float x) {
     float y;
@@ -134,30 +131,12 @@ __device__ __forceinline__ uint32_t round_tf32(float x) {
     asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(y) : "f"(x));
     return y;
 }
-// d = a b + c on 32 unsigned (kSigned: signed) bytes of a and signed bytes of b.
-template <bool kSigned>
+// d = a b + c on 32 unsigned bytes of a and signed bytes of b.
 __device__ __forceinline__ void mma8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                     uint32_t b1, const int (&c)[4]) {
-    if (kSigned)
-        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
-                     : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
-    else
-        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
-                     : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
-}
-// The power of two that brings a value with these (absolute) bits to [2^6, 2^7),
-// and its inverse, NaN for infinities and NaN.
-__device__ __forceinline__ float unit_of(uint32_t bits, float &inverse) {
-    const int e = (int)(bits >> 23), c = min(max(e, 7), 253);
-    inverse = __uint_as_float(e == 255 ? 0x7fc00000u : (uint32_t)(c - 6) << 23);
-    return __uint_as_float((uint32_t)(260 - c) << 23);
-}
-__device__ __forceinline__ uint32_t max_over_rows(uint32_t x) {
-#pragma unroll
-    for (int o = 4; o < 32; o <<= 1) x = max(x, __shfl_xor_sync(0xffffffffu, x, o));
-    return x;
+                                     uint32_t b1, int c0, int c1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c0), "r"(c1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
@@ -341,10 +320,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
     using Pt = AttnParts<kCache, kWide, kExact>;
     constexpr int GH = kWide ? 8 : 4, HL = kWide ? 2 : 1;         // heads of a tile, and of a lane
     constexpr int NB = Sh::NB, MT = Sh::MT, R = Sh::R, kTok = Sh::kTok, kTile = kTok * kAttnWarps, kMTiles = HD / 16;
-    constexpr int kQS = Pt::kQS, kPS = Pt::kPS, NA = kAttnInt<kCache, kExact> && !kWide ? 2 : 4;
+    constexpr int kQS = Pt::kQS, kPS = Pt::kPS;
     constexpr bool kInt = kAttnInt<kCache, kExact>;
     constexpr bool kBf16 = Sh::kBf16, kF32 = Sh::kF32;
-    constexpr float kBias = kAttnBias<kCache, kExact>;
+    constexpr float kBias = kAttnBias<kCache>;
     extern __shared__ __align__(16) uint8_t shared[];
     uint8_t *const sq = shared;                                   // the query's parts
     uint8_t *const rings = shared + Pt::kSets * 8 * Sh::kQStride;  // [warp][R] slots; at the end of an item the
@@ -358,6 +337,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
     __shared__ int qoff[kInt ? GH : 1][NB];                       // what the codes' offsets add to a block's integer score
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     pdl_trigger();
+    pdl_wait();
 
     // ---- this block's range [lo, hi) of all items' units (fewer than 2^31,
     //      checked on the host) ----
@@ -597,7 +577,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
 #pragma unroll
         for (int k = 0; k < kPerWarp; ++k) {
             const int j = warp + k * kAttnWarps;
-            float up = 1.0f, mul = p.scale, top = 0.0f;
+            // Scores grow with the products: a negative scale turns the query.
+            float up = p.scale < 0.0f ? -1.0f : 1.0f, mul = fmaxf(fabsf(p.scale), 1.2e-38f), top = 0.0f;
             if (!kBf16 && !kF32) {
                 // fp16 parts: the head's largest value goes to [2^14, 2^15).
 #pragma unroll
@@ -606,8 +587,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                 for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                 if (top > 0.0f && top < INFINITY) {
                     const int e = min(max(14 - ilogbf(top), -126), 126);
-                    up = ldexpf(1.0f, e);
-                    mul = p.scale * ldexpf(1.0f, -e);
+                    up *= ldexpf(1.0f, e);
+                    mul = fmaxf(mul * ldexpf(1.0f, -e), 1.2e-38f);
                 }
             }
             const int col = kWide ? j : 2 * j;
@@ -657,9 +638,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
         for (int j = 0; j < HL; ++j) qm[j] = qmul[HL * t + j];
 
         // ---- the pass over this block's tiles of the item ----
-        // acc: M tile of 16 dims, rows g and g + 8, of the lane's columns (of its
-        // head, where integers join a head's two).
-        float acc[kMTiles][NA], m[HL], l[HL];
+        // acc: M tile of 16 dims, rows g and g + 8, of the lane's two columns.
+        float acc[kMTiles][4], m[HL], l[HL];
 #pragma unroll
         for (int j = 0; j < HL; ++j) {
             m[j] = -INFINITY;
@@ -668,7 +648,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
 #pragma unroll
         for (int i = 0; i < kMTiles; ++i)
 #pragma unroll
-            for (int j = 0; j < NA; ++j) acc[i][j] = 0.0f;
+            for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
         int qo[HL][NB];
         if constexpr (kInt)
 #pragma unroll
@@ -741,16 +721,16 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                                     a[2 + r] = (w >> 4) & 0x0f0f0f0fu;
                                 }
                             }
-                            const int zero[4] = {0, 0, 0, 0};
+                            // The sums start at what the codes' offset adds.
                             int c[Pt::kSets][4];
-#pragma unroll
-                            for (int set = 0; set < Pt::kSets; ++set) mma8<false>(c[set], a[0], a[1], a[2], a[3], q[set].x, q[set].y, zero);
+                            mma8(c[0], a[0], a[1], a[2], a[3], q[0].x, q[0].y, qo[0][b], kWide ? qo[HL - 1][b] : 0);
+                            if constexpr (kWide) mma8(c[Pt::kSets - 1], a[0], a[1], a[2], a[3], q[Pt::kSets - 1].x, q[Pt::kSets - 1].y, 0, 0);
 #pragma unroll
                             for (int r = 0; r < 2; ++r)
 #pragma unroll
                                 for (int j = 0; j < HL; ++j) {
                                     const int v = kWide ? c[0][2 * r + j] + c[Pt::kSets - 1][2 * r + j] * 256 : c[0][2 * r] + c[0][2 * r + 1] * 256;
-                                    s[j][2 * i + r] = fmaf(ks[i][r][b], (float)(v + qo[j][b]), s[j][2 * i + r]);
+                                    s[j][2 * i + r] = fmaf(ks[i][r][b], (float)v, s[j][2 * i + r]);
                                 }
                         }
                     }
@@ -862,14 +842,19 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
             // ---- probabilities ----
             float pr[HL][2 * MT], top[HL];
             bool grew = false;
+            if (now != kAll) {
+#pragma unroll
+                for (int j = 0; j < HL; ++j)
+#pragma unroll
+                    for (int r = 0; r < 2 * MT; ++r)
+                        if (!((now >> (8 * r + g)) & 1)) s[j][r] = -INFINITY;
+            }
 #pragma unroll
             for (int j = 0; j < HL; ++j) {
-                top[j] = -INFINITY;
+                top[j] = s[j][0];
 #pragma unroll
-                for (int r = 0; r < 2 * MT; ++r) {
-                    s[j][r] = (now >> (8 * r + g)) & 1 ? s[j][r] * qm[j] : -INFINITY;
-                    top[j] = fmaxf(top[j], s[j][r]);
-                }
+                for (int r = 1; r < 2 * MT; ++r) top[j] = fmaxf(top[j], s[j][r]);
+                top[j] *= qm[j];
                 grew = grew || top[j] > m[j];
             }
             if (__any_sync(0xffffffffu, grew)) {
@@ -886,14 +871,14 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
 #pragma unroll
                 for (int i = 0; i < kMTiles; ++i)
 #pragma unroll
-                    for (int j = 0; j < NA; ++j) acc[i][j] *= keep[kWide ? j & 1 : 0];
+                    for (int j = 0; j < 4; ++j) acc[i][j] *= keep[kWide ? j & 1 : 0];
             }
 #pragma unroll
             for (int j = 0; j < HL; ++j) {
-                const float ref = m[j] == -INFINITY ? 0.0f : m[j] - kBias;
+                const float ref = m[j] == -INFINITY ? 0.0f : kBias - m[j];
 #pragma unroll
                 for (int r = 0; r < 2 * MT; ++r) {
-                    pr[j][r] = attn_exp2(s[j][r] - ref);
+                    pr[j][r] = now ? attn_exp2(fmaf(s[j][r], qm[j], ref)) : 0.0f;
                     l[j] += pr[j][r];
                 }
             }
@@ -907,7 +892,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
 #pragma unroll
                     for (int set = 0; set < kPS; ++set) {
                         uint32_t u;
-                        if constexpr (kWide) {
+                        if constexpr (kInt && !kWide) {
+                            u = pack16<kBf16>(y[0], 0.0f);        // one part
+                        } else if constexpr (kWide) {
                             u = pack16<kBf16>(y[0], y[HL - 1]);
                             if (set + 1 < kPS) {
                                 take16<kBf16>(y[0]);
@@ -926,101 +913,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
             copies_wait<R - 1>();
             __syncwarp();
             slot = ring + at * Sh::kSlot;
-            if constexpr (kInt) {
-                if (now) {
-                    constexpr int kBytes = Sh::kRowBytes / 8, kW = (kBytes + 3) / 4;      // of a row in this lane
-                    static_assert(MT == 2, "an integer MMA takes 32 tokens");
-                    uint32_t vr[MT][4][kW];
-                    float vs[MT][2][NB];
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) {
-#pragma unroll
-                        for (int r = 0; r < 2; ++r)
-                            read_scales<NB>(slot + Sh::kScaleOff + (16 * i + 8 * r + g) * Sh::kScaleBytes, vs[i][r]);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            read_bytes<kBytes>(slot + (16 * i + 2 * t + (r & 1) + 8 * (r >> 1)) * Sh::kStride + g * kBytes, vr[i][r]);
-                    }
-                    // Probabilities in [0, 2^7) of the tile's largest of each head.
-                    float pinv[HL];
-#pragma unroll
-                    for (int j = 0; j < HL; ++j) {
-                        uint32_t top = 0;
-#pragma unroll
-                        for (int r = 0; r < 2 * MT; ++r) top = max(top, __float_as_uint(pr[j][r]));
-                        const float f = unit_of(max_over_rows(top), pinv[j]);
-#pragma unroll
-                        for (int r = 0; r < 2 * MT; ++r) pr[j][r] *= f;
-                    }
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        // The block's scales likewise; the products round to integers below 2^14.
-                        uint32_t top = 0;
-#pragma unroll
-                        for (int r = 0; r < 2 * MT; ++r) top = max(top, __float_as_uint(fabsf(vs[r >> 1][r & 1][b])));
-                        float sinv;
-                        const float f = unit_of(max_over_rows(top), sinv);
-                        uint32_t bo[Pt::kSets][MT];                           // B operands: signed bytes of 16 tokens
-#pragma unroll
-                        for (int i = 0; i < MT; ++i) {
-                            uint32_t w[HL];
-#pragma unroll
-                            for (int j = 0; j < HL; ++j) {
-                                // 1.5 * 2^23 + 128 + w: the low two bytes are w's
-                                const uint32_t u = __float_as_uint(fmaf(pr[j][2 * i], vs[i][0][b] * f, 12583040.0f));
-                                const uint32_t v = __float_as_uint(fmaf(pr[j][2 * i + 1], vs[i][1][b] * f, 12583040.0f));
-                                w[j] = __byte_perm(u, v, 0x5140);             // low bytes of tokens g and g + 8, high bytes
-                            }
-                            if constexpr (kWide) {
-                                bo[0][i] = transpose8x8(__byte_perm(w[0], w[HL - 1], 0x5410) ^ 0x80808080u);
-                                bo[Pt::kSets - 1][i] = transpose8x8(__byte_perm(w[0], w[HL - 1], 0x7632));
-                            } else {
-                                bo[0][i] = transpose8x8(w[0] ^ 0x00008080u);
-                            }
-                        }
-                        // Bytes 4t .. 4t + 3 of the MMA's 32: tokens 2t, 2t + 8, 2t + 1, 2t + 9 of each 16.
-                        uint32_t a[4][MT];                                    // dims 4g .. 4g + 3
-#pragma unroll
-                        for (int i = 0; i < MT; ++i) {
-                            if constexpr (kCache == DTYPE_Q8_0) {
-                                const uint32_t t0 = __byte_perm(vr[i][0][b], vr[i][2][b], 0x5140), t1 = __byte_perm(vr[i][0][b], vr[i][2][b], 0x7362);
-                                const uint32_t t2 = __byte_perm(vr[i][1][b], vr[i][3][b], 0x5140), t3 = __byte_perm(vr[i][1][b], vr[i][3][b], 0x7362);
-                                a[0][i] = __byte_perm(t0, t2, 0x5410);
-                                a[1][i] = __byte_perm(t0, t2, 0x7632);
-                                a[2][i] = __byte_perm(t1, t3, 0x5410);
-                                a[3][i] = __byte_perm(t1, t3, 0x7632);
-                            } else {
-                                const uint32_t y0 = __byte_perm(vr[i][0][b / 2], vr[i][2][b / 2], b & 1 ? 0x7632 : 0x5410);
-                                const uint32_t y1 = __byte_perm(vr[i][1][b / 2], vr[i][3][b / 2], b & 1 ? 0x7632 : 0x5410);
-                                const uint32_t l0 = y0 & 0x0f0f0f0fu, l1 = y1 & 0x0f0f0f0fu;
-                                const uint32_t h0 = (y0 >> 4) & 0x0f0f0f0fu, h1 = (y1 >> 4) & 0x0f0f0f0fu;
-                                a[0][i] = __byte_perm(l0, l1, 0x6420);
-                                a[1][i] = __byte_perm(h0, h1, 0x6420);
-                                a[2][i] = __byte_perm(l0, l1, 0x7531);
-                                a[3][i] = __byte_perm(h0, h1, 0x7531);
-                            }
-                        }
-                        constexpr uint32_t kOff = kCache == DTYPE_Q8_0 ? 0x80808080u : 0xf8f8f8f8u;      // - 128, - 8
-                        const int zero[4] = {0, 0, 0, 0};
-                        int c[Pt::kSets][2][4];
-#pragma unroll
-                        for (int set = 0; set < Pt::kSets; ++set) {
-                            int off[4];
-                            mma8<true>(off, kOff, kOff, kOff, kOff, bo[set][0], bo[set][MT - 1], zero);
-#pragma unroll
-                            for (int h = 0; h < 2; ++h)
-                                mma8<false>(c[set][h], a[2 * h][0], a[2 * h + 1][0], a[2 * h][MT - 1], a[2 * h + 1][MT - 1], bo[set][0], bo[set][MT - 1], off);
-                        }
-#pragma unroll
-                        for (int h = 0; h < 2; ++h)
-#pragma unroll
-                            for (int j = 0; j < NA; ++j) {
-                                const int v = kWide ? c[0][h][j] + c[Pt::kSets - 1][h][j] * 256 : c[0][h][(2 * j) & 3] + c[0][h][(2 * j + 1) & 3] * 256;
-                                acc[2 * b + h][j] = fmaf((float)v, pinv[kWide ? j & 1 : 0] * sinv, acc[2 * b + h][j]);
-                            }
-                    }
-                }
-            } else if constexpr (Sh::kQuant) {
+            if constexpr (Sh::kQuant) {
                 constexpr int kBytes = Sh::kRowBytes / 8, kW = (kBytes + 3) / 4;  // of a row in this lane
                 float vs[MT][2][NB], big = 0.0f;
 #pragma unroll
@@ -1194,7 +1087,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
         copies_wait<0>();
 
         // ---- join the warps ----
-        const float unit = Sh::kQuant && !kInt ? (vinv == 0.0f ? 0.0f : 1.0f / vinv) : 1.0f;
+        const float unit = Sh::kQuant ? (vinv == 0.0f ? 0.0f : 1.0f / vinv) : 1.0f;
 #pragma unroll
         for (int j = 0; j < HL; ++j) {
 #pragma unroll
@@ -1228,8 +1121,6 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
             if constexpr (kWide) {
                 to[0] = make_float2(acc[i][0] * f[0], acc[i][2] * f[0]);
                 to[HD / 2] = make_float2(acc[i][1] * f[1], acc[i][3] * f[1]);
-            } else if constexpr (kInt) {
-                to[0] = make_float2(acc[i][0] * f[0], acc[i][1] * f[0]);
             } else {
                 to[0] = make_float2((acc[i][0] + acc[i][1]) * f[0], (acc[i][2] + acc[i][3]) * f[0]);
             }
@@ -1358,12 +1249,11 @@ cudaError_t attn_launch(AttnParams p, cudaStream_t st) {
     static std::atomic<unsigned long long> done{0};
     cudaError_t e = attn_allow(attend_kernel<kCache, HD, kWide, kExact>, kBytes, p.device, done);
     if (e != cudaSuccess) return e;
-    attend_kernel<kCache, HD, kWide, kExact><<<p.blocks, kAttnWarps * 32, kBytes, st>>>(p);
-    e = cudaGetLastError();
+    e = launch_pdl(attend_kernel<kCache, HD, kWide, kExact>, dim3(p.blocks), dim3(kAttnWarps * 32), kBytes, st, p);
     if (e != cudaSuccess) return e;
     constexpr int GH = kWide ? 8 : 4;
     return launch_pdl(attend_join_kernel<HD>, dim3(p.joins, std::min(GH, p.group)), dim3(kJoinWarps * 32), 0, st, p, GH,
-                      kAttnBias<kCache, kExact>);
+                      kAttnBias<kCache>);
 }
 template <int kCache, bool kWide, bool kExact>
 cudaError_t attn_launch(const AttnParams &p, cudaStream_t st) {

@@ -191,6 +191,8 @@ __device__ __forceinline__ uint8_t *kv_at(uint8_t *p, unsigned off16) { return p
 template <typename T, int kCache>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvParams p) {
     __shared__ KvPlace place[kMaxTokens];
+    pdl_trigger();
+    pdl_wait();
     const int t0 = blockIdx.x * p.block_tokens, nt = min(p.block_tokens, p.r.tokens - t0);
     const int tid = threadIdx.y * blockDim.x + threadIdx.x;
     const int u = threadIdx.x, token_rows = blockDim.y / p.row_heads, heads = 2 * p.l.kv_heads;
@@ -257,6 +259,8 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvParams p) {
     constexpr bool kQuant = kCache == DTYPE_Q8_0 || kCache == DTYPE_Q4_0;
     using C = typename KvType<kCache>::type;
     __shared__ KvPlace place[kMaxTokens];
+    pdl_trigger();
+    pdl_wait();
     const int t0 = blockIdx.x * p.block_tokens, nt = min(p.block_tokens, p.r.tokens - t0);
     const int tid = threadIdx.y * blockDim.x + threadIdx.x;
     const int u = threadIdx.x, token_rows = blockDim.y / p.row_heads, heads = 2 * p.l.kv_heads;
@@ -327,20 +331,18 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvParams p) {
 }
 
 template <typename T, int kCache>
-void launch_kv(const KvParams &p, bool write, dim3 grid, dim3 block, cudaStream_t st) {
-    if (write)
-        kv_write_kernel<T, kCache><<<grid, block, 0, st>>>(p);
-    else
-        kv_read_kernel<T, kCache><<<grid, block, 0, st>>>(p);
+cudaError_t launch_kv(const KvParams &p, bool write, dim3 grid, dim3 block, cudaStream_t st) {
+    return write ? launch_pdl(kv_write_kernel<T, kCache>, grid, block, 0, st, p)
+                 : launch_pdl(kv_read_kernel<T, kCache>, grid, block, 0, st, p);
 }
 template <typename T>
-void launch_kv(tensor_dtype_t cache, const KvParams &p, bool write, dim3 grid, dim3 block, cudaStream_t st) {
+cudaError_t launch_kv(tensor_dtype_t cache, const KvParams &p, bool write, dim3 grid, dim3 block, cudaStream_t st) {
     switch (cache) {
-        case DTYPE_F32: launch_kv<T, DTYPE_F32>(p, write, grid, block, st); break;
-        case DTYPE_BF16: launch_kv<T, DTYPE_BF16>(p, write, grid, block, st); break;
-        case DTYPE_F16: launch_kv<T, DTYPE_F16>(p, write, grid, block, st); break;
-        case DTYPE_Q8_0: launch_kv<T, DTYPE_Q8_0>(p, write, grid, block, st); break;
-        default: launch_kv<T, DTYPE_Q4_0>(p, write, grid, block, st); break;
+        case DTYPE_F32: return launch_kv<T, DTYPE_F32>(p, write, grid, block, st);
+        case DTYPE_BF16: return launch_kv<T, DTYPE_BF16>(p, write, grid, block, st);
+        case DTYPE_F16: return launch_kv<T, DTYPE_F16>(p, write, grid, block, st);
+        case DTYPE_Q8_0: return launch_kv<T, DTYPE_Q8_0>(p, write, grid, block, st);
+        default: return launch_kv<T, DTYPE_Q4_0>(p, write, grid, block, st);
     }
 }
 
@@ -396,13 +398,11 @@ int kv_call(kernel_context_t *ctx, const sapphire_kv_cache_t *cache, const sapph
     while (p.block_tokens > 1 && (a->tokens + p.block_tokens - 1) / p.block_tokens < 4 * sms) p.block_tokens /= 2;
     const dim3 grid((a->tokens + p.block_tokens - 1) / p.block_tokens);
     const dim3 block(p.units, p.row_heads * std::min(token_rows, p.block_tokens));
-    switch (a->dtype) {
-        case DTYPE_F32: launch_kv<float>(cache->dtype, p, write, grid, block, ctx->stream); break;
-        case DTYPE_BF16: launch_kv<__nv_bfloat16>(cache->dtype, p, write, grid, block, ctx->stream); break;
-        default: launch_kv<__half>(cache->dtype, p, write, grid, block, ctx->stream); break;
-    }
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = a->dtype == DTYPE_F32    ? launch_kv<float>(cache->dtype, p, write, grid, block, ctx->stream)
+                          : a->dtype == DTYPE_BF16 ? launch_kv<__nv_bfloat16>(cache->dtype, p, write, grid, block, ctx->stream)
+                                                   : launch_kv<__half>(cache->dtype, p, write, grid, block, ctx->stream);
     if (e != cudaSuccess) {
+        cudaGetLastError();
         ctx_fail(ctx, who, "launch failed: %s", cudaGetErrorString(e));
         return -1;
     }

@@ -58,6 +58,8 @@ template <typename T, bool kInterleaved>
 __global__ void __launch_bounds__(kThreads) rope_kernel(const RopeParams p) {
     constexpr int kPairs = kInterleaved ? kUnit / 2 : kUnit;
     extern __shared__ float4 turn[];
+    pdl_trigger();
+    pdl_wait();
     const int t0 = blockIdx.x * p.block_tokens, nt = min(p.block_tokens, p.tokens - t0), units = p.pair_units;
     const int tid = threadIdx.y * blockDim.x + threadIdx.x, nthreads = blockDim.x * blockDim.y;
     const int u = threadIdx.x, token_rows = blockDim.y / p.row_heads;
@@ -216,11 +218,8 @@ const char *rope_config_error(const sapphire_rope_config_t &c) {
 
 template <typename T>
 cudaError_t launch_rope(const RopeParams &p, bool interleaved, dim3 grid, dim3 block, size_t smem, cudaStream_t st) {
-    if (interleaved)
-        rope_kernel<T, true><<<grid, block, smem, st>>>(p);
-    else
-        rope_kernel<T, false><<<grid, block, smem, st>>>(p);
-    return cudaGetLastError();
+    if (interleaved) return launch_pdl(rope_kernel<T, true>, grid, block, smem, st, p);
+    return launch_pdl(rope_kernel<T, false>, grid, block, smem, st, p);
 }
 
 }  // namespace
@@ -365,6 +364,7 @@ extern "C" SAPPHIRE_API int sapphire_rope_device(sapphire_rope_t *rope, const sa
                     : a->dtype == DTYPE_BF16 ? launch_rope<__nv_bfloat16>(p, inter, grid, block, smem, ctx->stream)
                                              : launch_rope<__half>(p, inter, grid, block, smem, ctx->stream);
     if (e != cudaSuccess) {
+        cudaGetLastError();
         ctx_fail(ctx, who, "launch failed: %s", cudaGetErrorString(e));
         return -1;
     }

@@ -16,12 +16,10 @@ ds = scale sum|q k| 2^-19; p is off by a factor of exp(+-2 ds) (1 + 2^-18) with
 the approximate exponential (2^-21), and so out by at most
 max|v| (4 ds + 2^-17) before its rounding.
 
-Quantised caches under bf16 queries are multiplied in integers: a query value is
-off by at most half of max|q| 2^-13, so ds grows by scale max|q| sum|k| 2^-14.  A
-tile's weight p s rounds to half a unit where the largest p times the largest s
-is at least 2^12, so each of its 32 tokens is off by at most 2^-13 max p max|v|,
-and as l is at least the sum of the tiles' largest p, out by at most
-32 2^-13 max|v| = 2^-8 max|v|.
+Quantised caches under bf16 queries multiply the query as integers: a value is off
+by at most half of max|q| 2^-13, so ds grows by scale max|q| sum|k| 2^-14.  These
+and fp16 caches under bf16 queries round a probability to fp16 once, 2^-12 of it,
+so out is off by 2^-12 max|v| more.
 """
 from __future__ import annotations
 
@@ -437,11 +435,11 @@ def attend_plain(kv, q, table, lengths, page, heads, dim, dtype, window=0, scale
             ks, vs = k[pg, h, slot], v[pg, h, slot]
             score = x @ ks.T * scale
             ds = (x.abs() @ ks.abs().T * abs(scale)).amax(-1) * 2.0 ** -19
-            integers = dtype[0] == "q" and q.dtype == torch.bfloat16
-            if integers:
+            one_part = dtype in ("q8_0", "q4_0", "f16") and q.dtype == torch.bfloat16
+            if one_part and dtype[0] == "q":
                 ds = ds + abs(scale) * x.abs().amax(-1) * ks.abs().sum(-1).amax() * 2.0 ** -14
             out[s, h * group:(h + 1) * group] = torch.softmax(score, -1) @ vs
-            bound[s, h * group:(h + 1) * group] = vs.abs().max() * (4 * ds + 2.0 ** -17 + integers * 2.0 ** -8)[:, None]
+            bound[s, h * group:(h + 1) * group] = vs.abs().max() * (4 * ds + 2.0 ** -17 + one_part * 2.0 ** -12)[:, None]
             lse[s, h * group:(h + 1) * group] = torch.logsumexp(score, -1)
             lse_bound[s, h * group:(h + 1) * group] = 2 * ds + 2.0 ** -17
     return out, bound, lse, lse_bound
@@ -511,7 +509,7 @@ def test_attend_long_and_many(dev_ctx, dtype):
 
 
 @pytest.mark.parametrize("dtype", CACHES)
-@pytest.mark.parametrize("scale", [0.0078125, 1.5])
+@pytest.mark.parametrize("scale", [0.0078125, 1.5, -0.05])
 def test_attend_scale_and_range(dev_ctx, dtype, scale):
     """Loud keys and values; scores far apart, so single positions win."""
     check_attend(dev_ctx, dtype, "f32", [300, 41], 1, 4, 128, 16, seed=3, scale=scale, loud=30.0)
