@@ -66,7 +66,6 @@ struct AttnParams {
     int table_stride, length_offset, window;
     float scale;                   // scores times log2 e
     unsigned long long page_mul;   // floor(2^32 / page_size) + 1
-    int tile_pages, tile_slots;    // a block's tile of tokens as whole pages and the rest
     bool aligned;                  // pages of a multiple of 16 tokens
     int device;
     int blocks;
@@ -194,12 +193,18 @@ __device__ __forceinline__ uint32_t nibbles_to_half2(uint32_t w) {
 }
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-// 16 (8) bytes from global to shared memory, zeros where bytes is 0.
-__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t *src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+// N (16 or 8) bytes from global to shared memory, on their way until copies_wait.
+template <int N>
+__device__ __forceinline__ void copy_bytes(uint32_t dst, const uint8_t *src) {
+    if (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void copy8(uint32_t dst, const uint8_t *src, int bytes) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+// The same where ok, else zeros.
+template <int N>
+__device__ __forceinline__ void copy_or_zero(uint32_t dst, const uint8_t *src, bool ok) {
+    if (ok) copy_bytes<N>(dst, src);
+    else if (N == 16) asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(dst), "r"(0) : "memory");
+    else asm volatile("st.shared.v2.u32 [%0], {%1,%1};" ::"r"(dst), "r"(0) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -258,11 +263,10 @@ struct AttnShape {
     static constexpr int MT = attn_m_tiles(kCache, HD);
     static constexpr int kTok = 16 * MT;
     // A slot of a warp's ring: the K or the V rows of a tile, each row padded
-    // off the banks of its neighbours, their scales, and the tokens that count.
+    // off the banks of its neighbours, and their scales.
     static constexpr int kStride = kRowBytes + (kF32 ? 32 : 16);
     static constexpr int kScaleOff = kTok * kStride;
-    static constexpr int kMaskOff = kScaleOff + kTok * kScaleBytes;
-    static constexpr int kSlot = kMaskOff + 16;
+    static constexpr int kSlot = kScaleOff + kTok * kScaleBytes;
     static constexpr int kBlocks = attn_blocks_per_sm(kCache, HD);
     // Query parts: rows of 8 columns, padded so that the rows of neighbouring
     // lanes fall on the other half of the banks.
@@ -411,150 +415,130 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
         const bool aligned = p.aligned;
 
         // ---- where a tile's tokens are ----
-        // A tile's page ids are fetched ahead and resolved when its rows are
-        // copied, to offsets in units of 16 bytes and the tokens that count.
-        // Pages of a multiple of 16 tokens (aligned): each MMA tile is a run
-        // of rows, looked up by every lane alike.  Others: lane l looks up
-        // token l, and the copying lanes ask it.  Tiles are fetched in order.
-        struct Entry {
-            int page[MT], slot[MT];
-        };
-        int next_tok = tile_first * kTile + warp * kTok, next_page, next_slot;
-        {
-            const int tok = next_tok + (aligned ? 0 : lane);
-            next_page = (int)(((unsigned long long)(unsigned)tok * p.page_mul) >> 32);
-            next_slot = tok - next_page * p.l.page_size;
-            if (next_slot < 0) {
-                --next_page;
-                next_slot += p.l.page_size;
-            }
-        }
+        // Pages of a multiple of 16 tokens (aligned): an MMA tile is a run of
+        // rows of one page, a group.  Lane l looks up group l % MT of tile l / MT
+        // of the next 32 / MT tiles, so a look-up of the table serves many
+        // tiles, and the page ids of the ones behind are on their way.  Others:
+        // lane l looks up token l of a tile, a tile ahead, and the copying lanes
+        // ask it.  Either gives offsets of rows and K's scales in units of 16
+        // bytes from the head (scales of tokens: their page's and the slot); V's
+        // lie at fixed distances.
+        constexpr int kBatch = 32 / MT;                           // tiles of one look-up
         const int tok_end = min(sp.end, tile_end * kTile);
+        int look_tok = tile_first * kTile + warp * kTok + (aligned ? lane / MT * kTile + lane % MT * 16 : lane);
+        const int look_step = aligned ? kBatch * kTile : kTile;
+        int entry, slot;
         auto fetch = [&]() {
-            Entry e;
-            int pg = next_page, sl = next_slot;
-            if (aligned) {
-#pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    const int tok = next_tok + 16 * i;
-                    e.page[i] = tok + 16 > sp.first && tok < tok_end ? __ldg(table + pg) : -1;
-                    e.slot[i] = sl;
-                    sl += 16;
-                    if (sl >= p.l.page_size) {
-                        sl -= p.l.page_size;
-                        ++pg;
-                    }
-                }
-            } else {
-                const int tok = next_tok + lane;
-                e.page[0] = lane < kTok && tok >= sp.first && tok < tok_end ? __ldg(table + pg) : -1;
-                e.slot[0] = sl;
-                if (MT == 2) e.page[MT - 1] = e.slot[MT - 1] = 0;
+            int pg = (int)(((unsigned long long)(unsigned)look_tok * p.page_mul) >> 32);
+            slot = look_tok - pg * p.l.page_size;
+            if (slot < 0) {
+                --pg;
+                slot += p.l.page_size;
             }
-            // kTile tokens on
-            next_tok += kTile;
-            next_page += p.tile_pages;
-            next_slot += p.tile_slots;
-            if (next_slot >= p.l.page_size) {
-                next_slot -= p.l.page_size;
-                ++next_page;
-            }
-            return e;
+            const bool want = aligned ? look_tok + 16 > sp.first && look_tok < tok_end
+                                      : lane < kTok && look_tok >= sp.first && look_tok < tok_end;
+            entry = want ? __ldg(table + pg) : -1;
+            look_tok += look_step;
         };
         constexpr unsigned kAll = kTok == 32 ? 0xffffffffu : 0xffffu;
-        unsigned row16[MT], page_at[MT], valid = 0;               // offsets of the first row and of its page
-        int first_slot[MT], load_tok = next_tok;
-        auto resolve = [&](const Entry &e) {
+        unsigned row16 = 0, scale16 = 0, found = 0, valid = 0;
+        int token_slot = 0, load_tok = tile_first * kTile + warp * kTok, tiles_found = 0;
+        const uint8_t *rows_at[MT], *scales_at[MT];               // of the tile that is copied, aligned
+        auto resolve = [&]() {
+            if (!aligned || tiles_found == 0) {
+                const bool ok = (unsigned)entry < (unsigned)p.l.num_pages;
+                const unsigned page_at = ok ? (unsigned)entry * page16 : 0u;
+                row16 = page_at + (unsigned)(slot * (Sh::kRowBytes / 16));
+                scale16 = aligned ? page_at + (unsigned)(slot * Sh::kScaleBytes / 16) : page_at;
+                token_slot = slot;
+                found = __ballot_sync(0xffffffffu, ok);
+                tiles_found = kBatch;
+                fetch();
+            }
             unsigned inside = kAll;
             if (load_tok < sp.first || load_tok + kTok > tok_end) {
                 const int l0 = max(sp.first - load_tok, 0), l1 = min(tok_end - load_tok, kTok);
                 inside = l1 > l0 ? (0xffffffffu >> (32 - l1)) & (0xffffffffu << l0) : 0u;
             }
             load_tok += kTile;
-            valid = inside;
+            if (aligned) {
+                const int at = kBatch - tiles_found;
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const bool ok = (unsigned)e.page[i] < (unsigned)p.l.num_pages;
-                page_at[i] = ok ? (unsigned)e.page[i] * page16 : 0u;
-                first_slot[i] = e.slot[i];
-                row16[i] = page_at[i] + (unsigned)(e.slot[i] * (Sh::kRowBytes / 16));
-                if (aligned) {
-                    if (!ok) valid &= ~(0xffffu << (16 * i));
-                } else if (i == 0) {
-                    valid &= __ballot_sync(0xffffffffu, ok);
+                for (int i = 0; i < MT; ++i) {
+                    const unsigned r = __shfl_sync(0xffffffffu, row16, at * MT + i);
+                    rows_at[i] = head + ((unsigned long long)r << 4) + (lane * 16 - i * 16 * Sh::kRowBytes);
+                    if constexpr (Sh::kQuant) {
+                        const unsigned sc = __shfl_sync(0xffffffffu, scale16, at * MT + i);
+                        scales_at[i] = head + p.l.ks_off + ((unsigned long long)sc << 4) + (lane * (Sh::kScaleBytes == 8 ? 8 : 16) - i * 16 * Sh::kScaleBytes);
+                    }
                 }
+                const unsigned here = found >> (at * MT);
+                valid = (here & 1 ? 0xffffu : 0u) | (MT == 2 && (here & 2) ? 0xffff0000u : 0u);
+                --tiles_found;
+            } else {
+                valid = found;
             }
+            valid &= inside;
             if (valid != inside && lane == 0) atomicOr(p.err, kErrCache);
         };
 
         // ---- K or V rows of a tile into slot `at` of the warp's ring ----
+        constexpr int PR = Sh::kRowBytes / 16, kCopies = kTok * PR / 32;      // pieces of a row, copies of a lane
+        static_assert(kTok * PR % 32 == 0, "");
+        constexpr int kPer = Sh::kScaleBytes == 32 ? 2 : 1, kPiece = Sh::kScaleBytes == 8 ? 8 : 16;       // of a token's scales
+        constexpr int kScaleCopies = Sh::kQuant ? kTok * kPer / 32 : 0;
         uint8_t *const ring = rings + warp * R * Sh::kSlot;
+        const uint32_t ring_at = smem_addr(ring);
+        const int v_scales = p.l.vs_off - p.l.ks_off;
+        // Piece 32 j + lane of the rows: its row and its place in the slot.
+        auto row_of = [&](int j) { return 32 % PR == 0 ? j * (32 / PR) + lane / PR : PR % 32 == 0 ? j / (PR / 32) : (32 * j + lane) / PR; };
+        auto to = [&](int j) {
+            const int col = 32 % PR == 0 ? lane % PR : PR % 32 == 0 ? 32 * (j % (PR / 32 > 0 ? PR / 32 : 1)) + lane : (32 * j + lane) % PR;
+            return row_of(j) * Sh::kStride + col * 16;
+        };
         auto copy_rows = [&](int at, bool is_v) {
-            uint8_t *const slot = ring + at * Sh::kSlot;
-            const uint32_t dst = smem_addr(slot);
-            constexpr int PR = Sh::kRowBytes / 16, kCopies = kTok * PR / 32;  // pieces of a row, copies of a lane
-            static_assert(kTok * PR % 32 == 0, "");
-            // Piece 32 j + lane of the rows: its row and its place in the slot.
-            auto row_of = [&](int j) { return 32 % PR == 0 ? j * (32 / PR) + lane / PR : PR % 32 == 0 ? j / (PR / 32) : (32 * j + lane) / PR; };
-            auto to = [&](int j) {
-                const int col = 32 % PR == 0 ? lane % PR : PR % 32 == 0 ? 32 * (j % (PR / 32 > 0 ? PR / 32 : 1)) + lane : (32 * j + lane) % PR;
-                return dst + row_of(j) * Sh::kStride + col * 16;
-            };
-            const uint8_t *base = head + (is_v ? p.l.v_off : 0), *sbase = head + (is_v ? p.l.vs_off : p.l.ks_off);
-            constexpr int kPer = Sh::kScaleBytes == 32 ? 2 : 1, kPiece = Sh::kScaleBytes == 8 ? 8 : 16;   // of a token's scales
-            auto copy_scales = [&](const uint8_t *src, int i, int row) {
-                const uint32_t d = dst + Sh::kScaleOff + i * kPiece;
-                if (kPiece == 8) copy8(d, src, (valid >> row) & 1 ? 8 : 0);
-                else copy16(d, src, (valid >> row) & 1 ? 16 : 0);
-            };
+            const uint32_t dst = ring_at + at * Sh::kSlot, sdst = dst + Sh::kScaleOff + lane * kPiece;
             if (!valid) {
                 // nothing of this tile counts
             } else if (aligned) {
-                const uint8_t *src[MT];
+                const uint8_t *src[MT], *ssrc = nullptr;
 #pragma unroll
-                for (int i = 0; i < MT; ++i) src[i] = base + ((unsigned long long)row16[i] << 4) + lane * 16 - i * 16 * Sh::kRowBytes;
+                for (int i = 0; i < MT; ++i) src[i] = rows_at[i] + (is_v ? p.l.v_off : 0);
+                auto from = [&](int j) { return (MT == 1 || row_of(j) < 16 ? src[0] : src[MT - 1]) + 512 * j; };
+                if constexpr (kScaleCopies == 1) ssrc = (lane < 16 ? scales_at[0] : scales_at[MT - 1]) + (is_v ? v_scales : 0);
+                auto sfrom = [&](int j) { return kScaleCopies == 1 ? ssrc : scales_at[j * MT / 2] + (is_v ? v_scales : 0) + 512 * j; };
                 if (valid == kAll) {
 #pragma unroll
-                    for (int j = 0; j < kCopies; ++j)
-                        copy16(to(j), (MT == 1 || row_of(j) < 16 ? src[0] : src[MT - 1]) + 512 * j, 16);
+                    for (int j = 0; j < kCopies; ++j) copy_bytes<16>(dst + to(j), from(j));
+#pragma unroll
+                    for (int j = 0; j < kScaleCopies; ++j) copy_bytes<kPiece>(sdst + 512 * j, sfrom(j));
                 } else {
 #pragma unroll
-                    for (int j = 0; j < kCopies; ++j)
-                        copy16(to(j), (MT == 1 || row_of(j) < 16 ? src[0] : src[MT - 1]) + 512 * j, (valid >> row_of(j)) & 1 ? 16 : 0);
-                }
-                if constexpr (Sh::kQuant) {
+                    for (int j = 0; j < kCopies; ++j) copy_or_zero<16>(dst + to(j), from(j), (valid >> row_of(j)) & 1);
 #pragma unroll
-                    for (int j = 0; j < kTok * kPer / 32; ++j) {
-                        const int i = 32 * j + lane, row = i / kPer;
-                        const unsigned o = row < 16 ? page_at[0] : page_at[MT - 1];
-                        const int sl = row < 16 ? first_slot[0] : first_slot[MT - 1] - 16;
-                        copy_scales(sbase + ((unsigned long long)o << 4) + sl * Sh::kScaleBytes + i * kPiece, i, row);
-                    }
+                    for (int j = 0; j < kScaleCopies; ++j) copy_or_zero<kPiece>(sdst + 512 * j, sfrom(j), (valid >> ((32 * j + lane) / kPer)) & 1);
                 }
             } else {
+                const uint8_t *base = head + (is_v ? p.l.v_off : 0), *sbase = head + (is_v ? p.l.vs_off : p.l.ks_off);
                 for (int j = 0; j < kCopies; ++j) {
                     const int i = 32 * j + lane, row = i / PR, col = i - row * PR;
-                    const unsigned o = __shfl_sync(0xffffffffu, row16[0], row) + col;
-                    copy16(dst + row * Sh::kStride + col * 16, base + ((unsigned long long)o << 4), (valid >> row) & 1 ? 16 : 0);
+                    const unsigned o = __shfl_sync(0xffffffffu, row16, row) + col;
+                    copy_or_zero<16>(dst + row * Sh::kStride + col * 16, base + ((unsigned long long)o << 4), (valid >> row) & 1);
                 }
-                if constexpr (Sh::kQuant) {
-                    for (int j = 0; j < kTok * kPer / 32; ++j) {
-                        const int i = 32 * j + lane, row = i / kPer;
-                        const unsigned o = __shfl_sync(0xffffffffu, page_at[0], row);
-                        const int sl = __shfl_sync(0xffffffffu, first_slot[0], row);
-                        copy_scales(sbase + ((unsigned long long)o << 4) + sl * Sh::kScaleBytes + (i - row * kPer) * kPiece, i, row);
-                    }
+                for (int j = 0; j < kScaleCopies; ++j) {
+                    const int i = 32 * j + lane, row = i / kPer;
+                    const unsigned o = __shfl_sync(0xffffffffu, scale16, row);
+                    const int sl = __shfl_sync(0xffffffffu, token_slot, row);
+                    copy_or_zero<kPiece>(sdst + 512 * j, sbase + ((unsigned long long)o << 4) + sl * Sh::kScaleBytes + (i - row * kPer) * kPiece, (valid >> row) & 1);
                 }
             }
-            if (!is_v && lane == 0) *reinterpret_cast<unsigned *>(slot + Sh::kMaskOff) = valid;
             copies_commit();
         };
 
         // ---- the query's values, and the ring's first copies ----
         constexpr int kAhead = (R + 1) / 2;                       // tiles whose copies a full ring holds
-        Entry next[kAhead + 1];
-#pragma unroll
-        for (int i = 0; i <= kAhead; ++i) next[i] = fetch();
+        unsigned counts[kAhead];                                  // tokens that count, of the tiles copied
+        fetch();
         constexpr int kPerWarp = GH / kAttnWarps;
         float x[kPerWarp][NB];
 #pragma unroll
@@ -571,7 +555,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
         __syncthreads();                                          // the last item's readers of the rings
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            if (i % 2 == 0) resolve(next[i / 2]);
+            if (i % 2 == 0) {
+                resolve();
+                counts[i / 2] = valid;
+            }
             copy_rows(i, i % 2 == 1);
         }
 #pragma unroll
@@ -668,9 +655,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
             __syncwarp();
             if ((R & 1) == (after_v ? 1 : 0)) {
                 // its K rows: a tile not yet looked at
-                resolve(next[kAhead]);
+                resolve();
+                counts[kAhead - 1] = valid;
                 copy_rows(at, false);
-                next[kAhead] = fetch();
             } else {
                 copy_rows(at, true);
             }
@@ -680,7 +667,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
             copies_wait<R - 1>();
             __syncwarp();
             const uint8_t *slot = ring + at * Sh::kSlot;
-            const unsigned now = *reinterpret_cast<const unsigned *>(slot + Sh::kMaskOff);
+            const unsigned now = counts[0];
+#pragma unroll
+            for (int i = 0; i + 1 < kAhead; ++i) counts[i] = counts[i + 1];
             // ---- scores: lane (g, t) has tokens 16 i + g, + 8 of its heads ----
             float s[HL][2 * MT];
             if constexpr (Sh::kQuant) {
@@ -929,7 +918,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                     // A larger scale than fits: a new power of two that brings it to [1/2, 1).
 #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-                    const int e = min(max((int)((__float_as_uint(big) >> 23) & 255) - 126, -126), 126);
+                    const int e = min(max((int)((__float_as_uint(big) >> 23) & 255) - 126, -100), 126);
                     const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
                     const float f = vinv == 0.0f ? 0.0f : inv / vinv;
                     vinv = inv;
@@ -939,6 +928,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
 #pragma unroll
                         for (int j = 0; j < 4; ++j) acc[i][j] *= f;
                 }
+#pragma unroll
+                for (int j = 0; j < HL; ++j)
+#pragma unroll
+                    for (int r = 0; r < 2 * MT; ++r) pr[j][r] *= vinv;
                 uint32_t vr[MT][4][kW];
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
@@ -969,12 +962,11 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                                     a[1][2 * r + 1] = nibbles_to_half2<4>(w >> 8);
                                 }
                             }
-                            const float f0 = vs[i][0][b] * vinv, f1 = vs[i][1][b] * vinv;
                             float w[HL][2];
 #pragma unroll
                             for (int j = 0; j < HL; ++j) {
-                                w[j][0] = pr[j][2 * i] * f0;
-                                w[j][1] = pr[j][2 * i + 1] * f1;
+                                w[j][0] = pr[j][2 * i] * vs[i][0][b];
+                                w[j][1] = pr[j][2 * i + 1] * vs[i][1][b];
                             }
                             uint32_t b0[kPS], b1[kPS];
                             operand(w, b0, b1);
@@ -1240,11 +1232,8 @@ cudaError_t attn_allow(K *kernel, size_t bytes, int device, std::atomic<unsigned
 }
 
 template <int kCache, int HD, bool kWide, bool kExact>
-cudaError_t attn_launch(AttnParams p, cudaStream_t st) {
+cudaError_t attn_launch(const AttnParams &p, cudaStream_t st) {
     using Sh = AttnShape<kCache, HD>;
-    constexpr int kTile = Sh::kTok * kAttnWarps;
-    p.tile_pages = kTile / p.l.page_size;
-    p.tile_slots = kTile % p.l.page_size;
     constexpr size_t kBytes = AttnParts<kCache, kWide, kExact>::kSets * 8 * Sh::kQStride + kAttnWarps * Sh::R * Sh::kSlot;
     static std::atomic<unsigned long long> done{0};
     cudaError_t e = attn_allow(attend_kernel<kCache, HD, kWide, kExact>, kBytes, p.device, done);
