@@ -77,6 +77,7 @@ struct AttnParams {
     bool by_item;
     int joins;                     // entries of piece
     int *err;
+    unsigned nibble[4];            // NibbleConst, where the compiler does not see constants
 };
 
 // Query heads of a tile for a group of this size.
@@ -86,7 +87,7 @@ inline int attn_tile_heads(int group) { return attn_wide(group) ? 8 : 4; }
 constexpr int attn_m_tiles(int cache, int hd) { return cache == DTYPE_Q4_0 || cache == DTYPE_Q8_0 ? 2 : 1; }
 constexpr int attn_blocks_per_sm(int cache, int hd) {
     if (cache == DTYPE_F32) return hd <= 64 ? 3 : hd <= 128 ? 2 : 1;
-    if (cache == DTYPE_Q4_0) return hd <= 64 ? 4 : hd <= 128 ? 3 : 2;
+    if (cache == DTYPE_Q4_0) return hd <= 128 ? 4 : 2;
     if (cache == DTYPE_Q8_0) return hd <= 64 ? 4 : hd <= 128 ? 3 : 2;
     return hd <= 64 ? 4 : hd <= 128 ? 3 : 2;
 }
@@ -178,18 +179,18 @@ __device__ __forceinline__ uint32_t bytes_to_half2(uint32_t w, uint32_t sel) {
     const __half2 v = __hsub2(*reinterpret_cast<const __half2 *>(&x), __half2half2(__ushort_as_half(0x6480)));   // - 1152
     return *reinterpret_cast<const uint32_t *>(&v);
 }
+// What unpacking nibbles keeps in registers: an instruction takes one constant.
+struct NibbleConst {
+    uint32_t magic, sub, div, sub16;      // 1024; 1032; 1 / 16; 72, twice each
+};
 // Nibbles 0 and 4 (kShift = 0), or 1 and 5 (kShift = 4), of w as fp16 integers - 8.
 template <int kShift>
-__device__ __forceinline__ uint32_t nibbles_to_half2(uint32_t w) {
-    if (kShift == 0) {
-        const uint32_t x = (w & 0x000f000fu) | 0x64006400u;       // 1024 + code
-        const __half2 v = __hsub2(*reinterpret_cast<const __half2 *>(&x), __half2half2(__ushort_as_half(0x6408)));
-        return *reinterpret_cast<const uint32_t *>(&v);
-    }
-    const uint32_t x = (w & 0x00f000f0u) | 0x64006400u;           // 1024 + 16 code
-    const __half2 v = __hfma2(*reinterpret_cast<const __half2 *>(&x), __half2half2(__ushort_as_half(0x2c00)),
-                              __half2half2(__ushort_as_half(0xd480)));   // / 16 - 72
-    return *reinterpret_cast<const uint32_t *>(&v);
+__device__ __forceinline__ uint32_t nibbles_to_half2(uint32_t w, const NibbleConst &k) {
+    uint32_t x, v;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(x) : "r"(w), "n"(kShift ? 0x00f000f0 : 0x000f000f), "r"(k.magic));   // (w & mask) | 1024
+    if (kShift == 0) asm("sub.f16x2 %0, %1, %2;" : "=r"(v) : "r"(x), "r"(k.sub));                     // 1024 + code - 1032
+    else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(v) : "r"(x), "r"(k.div), "r"(k.sub16));            // (1024 + 16 code) / 16 - 72
+    return v;
 }
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -389,6 +390,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
     int seq = found_seq;
     unsigned seq_base = found_base;
     int4 piece = make_int4(0, 0, 0, 0);
+    const NibbleConst nib = {p.nibble[0], p.nibble[1], p.nibble[2], p.nibble[3]};
 
     unsigned pos = lo;
     while (pos < hi) {
@@ -441,56 +443,54 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
             look_tok += look_step;
         };
         constexpr unsigned kAll = kTok == 32 ? 0xffffffffu : 0xffffu;
+        constexpr int PR = Sh::kRowBytes / 16, kCopies = kTok * PR / 32;      // pieces of a row, copies of a lane
+        static_assert(kTok * PR % 32 == 0, "");
+        constexpr int kPer = Sh::kScaleBytes == 32 ? 2 : 1, kPiece = Sh::kScaleBytes == 8 ? 8 : 16;       // of a token's scales
+        constexpr int kScaleCopies = Sh::kQuant ? kTok * kPer / 32 : 0;
         unsigned row16 = 0, scale16 = 0, found = 0, valid = 0;
         int token_slot = 0, load_tok = tile_first * kTile + warp * kTok, tiles_found = 0;
-        const uint8_t *rows_at[MT], *scales_at[MT];               // of the tile that is copied, aligned
+        unsigned group16[MT], scales16[kScaleCopies > 0 ? kScaleCopies : 1];  // of the tile that is copied, aligned
         auto resolve = [&]() {
             if (!aligned || tiles_found == 0) {
                 const bool ok = (unsigned)entry < (unsigned)p.l.num_pages;
                 const unsigned page_at = ok ? (unsigned)entry * page16 : 0u;
-                row16 = page_at + (unsigned)(slot * (Sh::kRowBytes / 16));
+                row16 = page_at + (unsigned)(slot * PR);
                 scale16 = aligned ? page_at + (unsigned)(slot * Sh::kScaleBytes / 16) : page_at;
                 token_slot = slot;
                 found = __ballot_sync(0xffffffffu, ok);
                 tiles_found = kBatch;
                 fetch();
             }
-            unsigned inside = kAll;
-            if (load_tok < sp.first || load_tok + kTok > tok_end) {
+            valid = found;
+            if (aligned) {
+                const int at = (kBatch - tiles_found) * MT;
+#pragma unroll
+                for (int i = 0; i < MT; ++i) group16[i] = __shfl_sync(0xffffffffu, row16, at + i);
+#pragma unroll
+                for (int j = 0; j < kScaleCopies; ++j)            // each lane its token's group
+                    scales16[j] = __shfl_sync(0xffffffffu, scale16, at + (32 * j + lane) / kPer / 16);
+                const unsigned here = (found >> at) & (MT == 2 ? 3u : 1u);
+                valid = here == (MT == 2 ? 3u : 1u) ? kAll : (here & 1 ? 0xffffu : 0u) | (here & 2 ? 0xffff0000u : 0u);
+                --tiles_found;
+            }
+            if (load_tok < sp.first || load_tok + kTok > tok_end || (aligned && valid != kAll)) {
                 const int l0 = max(sp.first - load_tok, 0), l1 = min(tok_end - load_tok, kTok);
-                inside = l1 > l0 ? (0xffffffffu >> (32 - l1)) & (0xffffffffu << l0) : 0u;
+                const unsigned inside = l1 > l0 ? (0xffffffffu >> (32 - l1)) & (0xffffffffu << l0) : 0u;
+                if ((valid & inside) != inside && lane == 0) atomicOr(p.err, kErrCache);
+                valid &= inside;
+            } else if (!aligned && valid != kAll) {
+                if (lane == 0) atomicOr(p.err, kErrCache);
             }
             load_tok += kTile;
-            if (aligned) {
-                const int at = kBatch - tiles_found;
-#pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    const unsigned r = __shfl_sync(0xffffffffu, row16, at * MT + i);
-                    rows_at[i] = head + ((unsigned long long)r << 4) + (lane * 16 - i * 16 * Sh::kRowBytes);
-                    if constexpr (Sh::kQuant) {
-                        const unsigned sc = __shfl_sync(0xffffffffu, scale16, at * MT + i);
-                        scales_at[i] = head + p.l.ks_off + ((unsigned long long)sc << 4) + (lane * (Sh::kScaleBytes == 8 ? 8 : 16) - i * 16 * Sh::kScaleBytes);
-                    }
-                }
-                const unsigned here = found >> (at * MT);
-                valid = (here & 1 ? 0xffffu : 0u) | (MT == 2 && (here & 2) ? 0xffff0000u : 0u);
-                --tiles_found;
-            } else {
-                valid = found;
-            }
-            valid &= inside;
-            if (valid != inside && lane == 0) atomicOr(p.err, kErrCache);
         };
 
         // ---- K or V rows of a tile into slot `at` of the warp's ring ----
-        constexpr int PR = Sh::kRowBytes / 16, kCopies = kTok * PR / 32;      // pieces of a row, copies of a lane
-        static_assert(kTok * PR % 32 == 0, "");
-        constexpr int kPer = Sh::kScaleBytes == 32 ? 2 : 1, kPiece = Sh::kScaleBytes == 8 ? 8 : 16;       // of a token's scales
-        constexpr int kScaleCopies = Sh::kQuant ? kTok * kPer / 32 : 0;
         uint8_t *const ring = rings + warp * R * Sh::kSlot;
         const uint32_t ring_at = smem_addr(ring);
-        const int v_scales = p.l.vs_off - p.l.ks_off;
-        // Piece 32 j + lane of the rows: its row and its place in the slot.
+        const uint8_t *const k_rows = head + lane * 16, *const v_rows = k_rows + p.l.v_off;
+        const uint8_t *const k_scales = head + p.l.ks_off + lane * kPiece, *const v_scales = k_scales + (p.l.vs_off - p.l.ks_off);
+        // Piece 32 j + lane of the rows: its row, its place in the slot, and its
+        // place in the group's run of rows.
         auto row_of = [&](int j) { return 32 % PR == 0 ? j * (32 / PR) + lane / PR : PR % 32 == 0 ? j / (PR / 32) : (32 * j + lane) / PR; };
         auto to = [&](int j) {
             const int col = 32 % PR == 0 ? lane % PR : PR % 32 == 0 ? 32 * (j % (PR / 32 > 0 ? PR / 32 : 1)) + lane : (32 * j + lane) % PR;
@@ -501,22 +501,27 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
             if (!valid) {
                 // nothing of this tile counts
             } else if (aligned) {
-                const uint8_t *src[MT], *ssrc = nullptr;
+                const uint8_t *src[MT], *ssrc[kScaleCopies > 0 ? kScaleCopies : 1];
 #pragma unroll
-                for (int i = 0; i < MT; ++i) src[i] = rows_at[i] + (is_v ? p.l.v_off : 0);
-                auto from = [&](int j) { return (MT == 1 || row_of(j) < 16 ? src[0] : src[MT - 1]) + 512 * j; };
-                if constexpr (kScaleCopies == 1) ssrc = (lane < 16 ? scales_at[0] : scales_at[MT - 1]) + (is_v ? v_scales : 0);
-                auto sfrom = [&](int j) { return kScaleCopies == 1 ? ssrc : scales_at[j * MT / 2] + (is_v ? v_scales : 0) + 512 * j; };
+                for (int i = 0; i < MT; ++i) src[i] = (is_v ? v_rows : k_rows) + (unsigned long long)group16[i] * 16;
+#pragma unroll
+                for (int j = 0; j < kScaleCopies; ++j)            // lane's token of its group
+                    ssrc[j] = (is_v ? v_scales : k_scales) + (unsigned long long)scales16[j] * 16 + 512 * j - (32 * j + lane) / kPer / 16 * 16 * Sh::kScaleBytes;
+                auto from = [&](int j) {
+                    constexpr bool kWhole = 16 * PR % 32 == 0;    // a copy lies in one group
+                    const int i = kWhole ? 2 * j / PR : row_of(j) / 16;
+                    return (i == 0 ? src[0] : src[MT - 1]) + (512 * j - i * 16 * Sh::kRowBytes);
+                };
                 if (valid == kAll) {
 #pragma unroll
                     for (int j = 0; j < kCopies; ++j) copy_bytes<16>(dst + to(j), from(j));
 #pragma unroll
-                    for (int j = 0; j < kScaleCopies; ++j) copy_bytes<kPiece>(sdst + 512 * j, sfrom(j));
+                    for (int j = 0; j < kScaleCopies; ++j) copy_bytes<kPiece>(sdst + 512 * j, ssrc[j]);
                 } else {
 #pragma unroll
                     for (int j = 0; j < kCopies; ++j) copy_or_zero<16>(dst + to(j), from(j), (valid >> row_of(j)) & 1);
 #pragma unroll
-                    for (int j = 0; j < kScaleCopies; ++j) copy_or_zero<kPiece>(sdst + 512 * j, sfrom(j), (valid >> ((32 * j + lane) / kPer)) & 1);
+                    for (int j = 0; j < kScaleCopies; ++j) copy_or_zero<kPiece>(sdst + 512 * j, ssrc[j], (valid >> ((32 * j + lane) / kPer)) & 1);
                 }
             } else {
                 const uint8_t *base = head + (is_v ? p.l.v_off : 0), *sbase = head + (is_v ? p.l.vs_off : p.l.ks_off);
@@ -746,10 +751,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                                     // halfwords b and NB + b: codes 0-3 of words 2t and 2t + 1
                                     const uint32_t u = kr[i][r][b / 2], v = kr[i][r][(NB + b) / 2];
                                     const uint32_t w = __byte_perm(u, v, (b & 1 ? 0x32 : 0x10) | ((NB + b) & 1 ? 0x7600 : 0x5400));
-                                    a[0][r] = nibbles_to_half2<0>(w);
-                                    a[0][2 + r] = nibbles_to_half2<4>(w);
-                                    a[1][r] = nibbles_to_half2<0>(w >> 8);
-                                    a[1][2 + r] = nibbles_to_half2<4>(w >> 8);
+                                    a[0][r] = nibbles_to_half2<0>(w, nib);
+                                    a[0][2 + r] = nibbles_to_half2<4>(w, nib);
+                                    a[1][r] = nibbles_to_half2<0>(w >> 8, nib);
+                                    a[1][2 + r] = nibbles_to_half2<4>(w >> 8, nib);
                                 }
                             }
                             float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -956,10 +961,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                                     a[1][2 * r + 1] = bytes_to_half2(hi2, 0x4342);
                                 } else {
                                     const uint32_t w = __byte_perm(vr[i][2 * r][b / 2], vr[i][2 * r + 1][b / 2], b & 1 ? 0x7632 : 0x5410);
-                                    a[0][2 * r] = nibbles_to_half2<0>(w);
-                                    a[0][2 * r + 1] = nibbles_to_half2<4>(w);
-                                    a[1][2 * r] = nibbles_to_half2<0>(w >> 8);
-                                    a[1][2 * r + 1] = nibbles_to_half2<4>(w >> 8);
+                                    a[0][2 * r] = nibbles_to_half2<0>(w, nib);
+                                    a[0][2 * r + 1] = nibbles_to_half2<4>(w, nib);
+                                    a[1][2 * r] = nibbles_to_half2<0>(w >> 8, nib);
+                                    a[1][2 * r + 1] = nibbles_to_half2<4>(w >> 8, nib);
                                 }
                             }
                             float w[HL][2];
