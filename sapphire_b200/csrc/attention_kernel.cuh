@@ -84,7 +84,9 @@ struct AttnParams {
 inline bool attn_wide(int group) { return group > 4; }
 inline int attn_tile_heads(int group) { return attn_wide(group) ? 8 : 4; }
 // MMA tiles (16 tokens) of a warp's tile, and resident blocks per SM.
-constexpr int attn_m_tiles(int cache, int hd) { return cache == DTYPE_Q4_0 || cache == DTYPE_Q8_0 ? 2 : 1; }
+constexpr int attn_m_tiles(int cache, int hd) {
+    return cache == DTYPE_Q4_0 || cache == DTYPE_Q8_0 || (hd <= 64 && cache != DTYPE_F32) ? 2 : 1;
+}
 constexpr int attn_blocks_per_sm(int cache, int hd) {
     if (cache == DTYPE_F32) return hd <= 64 ? 3 : hd <= 128 ? 2 : 1;
     if (cache == DTYPE_Q4_0) return hd <= 128 ? 4 : 2;
@@ -1172,12 +1174,13 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
 }
 
 // Adds up the items that several blocks hold: one block per item and query
-// head, its warps taking every eighth holder, eight of them in flight.
-constexpr int kJoinWarps = 8;
+// head.  Its warps take every eighth holder, kJoinBatch of them in flight (maxima,
+// sums and values together), and are joined like the blocks' warps.
+constexpr int kJoinWarps = 8, kJoinBatch = 4;
 template <int HD>
 __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const AttnParams p, int tile_heads, float bias) {
     constexpr int kVals = HD / 32;
-    __shared__ float so[kJoinWarps][HD], sl[kJoinWarps];
+    __shared__ float so[kJoinWarps][HD], sm[kJoinWarps], sl[kJoinWarps];
     pdl_wait();
     const int4 piece = __ldcg(p.piece + blockIdx.x);
     if (piece.z == 0) return;
@@ -1186,30 +1189,61 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Attn
     if (h >= min(tile_heads, p.group - ht * tile_heads)) return;
     const size_t stride = (size_t)tile_heads * (HD + 2);
     // Holder i's partial: the second slot of the first block, the first of the others.
-    const float *part = p.part + (2 * (size_t)piece.w + 1) * stride + h;
-    auto of = [&](int i) { return part + (i ? 2 * i - 1 : 0) * stride; };
-    float M = -INFINITY;
-    for (int i = lane; i < piece.z; i += 32) M = fmaxf(M, __ldcg(of(i)));
-#pragma unroll
-    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    float L = 0.0f, o[kVals];
+    const float *part = p.part + (2 * (size_t)piece.w + 1) * stride;
+    float M = -INFINITY, L = 0.0f, o[kVals];
 #pragma unroll
     for (int j = 0; j < kVals; ++j) o[j] = 0.0f;
-#pragma unroll 8
-    for (int i = warp; i < piece.z; i += kJoinWarps) {
-        const float *x = of(i);
-        const float w = M == -INFINITY ? 1.0f : attn_exp2(__ldcg(x) - M);
-        L = fmaf(w, __ldcg(x + tile_heads), L);
+    for (int i0 = warp; i0 < piece.z; i0 += kJoinWarps * kJoinBatch) {
+        float m[kJoinBatch], l[kJoinBatch], x[kJoinBatch][kVals], top = M;
 #pragma unroll
-        for (int j = 0; j < kVals; ++j) o[j] = fmaf(w, __ldcg(x - h + 2 * tile_heads + h * HD + 32 * j + lane), o[j]);
+        for (int k = 0; k < kJoinBatch; ++k) {
+            const int i = i0 + k * kJoinWarps;
+            m[k] = -INFINITY;
+            l[k] = 0.0f;
+            if (i >= piece.z) {
+#pragma unroll
+                for (int j = 0; j < kVals; ++j) x[k][j] = 0.0f;
+                continue;
+            }
+            const float *from = part + (i ? 2 * i - 1 : 0) * stride;
+            m[k] = __ldcg(from + h);
+            l[k] = __ldcg(from + tile_heads + h);
+#pragma unroll
+            for (int j = 0; j < kVals; ++j) x[k][j] = __ldcg(from + 2 * tile_heads + h * HD + 32 * j + lane);
+        }
+#pragma unroll
+        for (int k = 0; k < kJoinBatch; ++k) top = fmaxf(top, m[k]);
+        const float ref = top == -INFINITY ? 0.0f : top, keep = attn_exp2(M - ref);
+        M = top;
+        L *= keep;
+#pragma unroll
+        for (int j = 0; j < kVals; ++j) o[j] *= keep;
+#pragma unroll
+        for (int k = 0; k < kJoinBatch; ++k) {
+            const float w = l[k] != l[k] ? l[k] : attn_exp2(m[k] - ref);      // a NaN's maximum says nothing
+            L = fmaf(w, l[k], L);
+#pragma unroll
+            for (int j = 0; j < kVals; ++j) o[j] = fmaf(w, x[k][j], o[j]);
+        }
     }
 #pragma unroll
     for (int j = 0; j < kVals; ++j) so[warp][32 * j + lane] = o[j];
-    if (lane == 0) sl[warp] = L;
+    if (lane == 0) {
+        sm[warp] = M;
+        sl[warp] = L;
+    }
     __syncthreads();
+    float w[kJoinWarps];
+    M = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kJoinWarps; ++i) M = fmaxf(M, sm[i]);
+    const float ref = M == -INFINITY ? 0.0f : M;
     L = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) L += sl[w];
+    for (int i = 0; i < kJoinWarps; ++i) {
+        w[i] = sl[i] != sl[i] ? sl[i] : attn_exp2(sm[i] - ref);
+        L = fmaf(w[i], sl[i], L);
+    }
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     const int head = kh * p.group + ht * tile_heads + h;
     if (p.lse && threadIdx.x == 0)
@@ -1218,7 +1252,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Attn
     for (int d = threadIdx.x; d < HD; d += kJoinWarps * 32) {
         float y = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kJoinWarps; ++w) y += so[w][d];
+        for (int i = 0; i < kJoinWarps; ++i) y = fmaf(w[i], so[i][d], y);
         y *= inv;
         if (p.io == DTYPE_F32) static_cast<float *>(p.out)[off + d] = y;
         else if (p.io == DTYPE_BF16) static_cast<__nv_bfloat16 *>(p.out)[off + d] = __float2bfloat16_rn(y);
