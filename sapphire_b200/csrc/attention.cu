@@ -90,10 +90,10 @@ extern "C" SAPPHIRE_API int sapphire_attention_device(kernel_context_t *ctx, con
     p.head_tiles = (p.group + attn_tile_heads(p.group) - 1) / attn_tile_heads(p.group);
     p.page_mul = (1ull << 32) / cache->page_size + 1;
     p.blocks = attn_blocks(ctx, cache);
-    p.nibble[0] = 0x64006400u;
-    p.nibble[1] = 0x64086408u;
-    p.nibble[2] = 0x2c002c00u;
-    p.nibble[3] = 0xd480d480u;
+    p.code[0] = 0x64006400u;
+    p.code[1] = cache->dtype == DTYPE_Q8_0 ? 0x64806480u : 0x64086408u;
+    p.code[2] = 0x2c002c00u;
+    p.code[3] = 0xd480d480u;
     p.aligned = cache->page_size % 16 == 0;
     p.device = ctx->device;
     const long long items = (long long)a->sequences * cache->kv_heads * p.head_tiles;

@@ -77,7 +77,7 @@ struct AttnParams {
     bool by_item;
     int joins;                     // entries of piece
     int *err;
-    unsigned nibble[4];            // NibbleConst, where the compiler does not see constants
+    unsigned code[4];              // CodeConst, where the compiler does not see constants
 };
 
 // Query heads of a tile for a group of this size.
@@ -174,20 +174,22 @@ __device__ __forceinline__ float take_tf32(float &x) {
     return hi;
 }
 
-// Two bytes of `w` (selected by sel's low nibbles of positions 0 and 2) as fp16
-// integers - 128.
-__device__ __forceinline__ uint32_t bytes_to_half2(uint32_t w, uint32_t sel) {
-    const uint32_t x = __byte_perm(w, 0x64646464u, sel);          // 1024 + code
-    const __half2 v = __hsub2(*reinterpret_cast<const __half2 *>(&x), __half2half2(__ushort_as_half(0x6480)));   // - 1152
-    return *reinterpret_cast<const uint32_t *>(&v);
-}
-// What unpacking nibbles keeps in registers: an instruction takes one constant.
-struct NibbleConst {
-    uint32_t magic, sub, div, sub16;      // 1024; 1032; 1 / 16; 72, twice each
+// What unpacking codes keeps in registers: an instruction takes one constant.
+struct CodeConst {
+    uint32_t magic, sub, div, sub16;      // 1024; 1152 (Q8_0) or 1032; 1 / 16; 72, twice each
 };
+// Two bytes of `w` (selected by sel's low nibbles of positions 0 and 2; the
+// others take magic's high byte) as fp16 integers - 128.
+template <uint32_t kSel>
+__device__ __forceinline__ uint32_t bytes_to_half2(uint32_t w, const CodeConst &k) {
+    uint32_t x, v;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(x) : "r"(w), "r"(k.magic), "n"(kSel));                     // 1024 + code
+    asm("sub.f16x2 %0, %1, %2;" : "=r"(v) : "r"(x), "r"(k.sub));
+    return v;
+}
 // Nibbles 0 and 4 (kShift = 0), or 1 and 5 (kShift = 4), of w as fp16 integers - 8.
 template <int kShift>
-__device__ __forceinline__ uint32_t nibbles_to_half2(uint32_t w, const NibbleConst &k) {
+__device__ __forceinline__ uint32_t nibbles_to_half2(uint32_t w, const CodeConst &k) {
     uint32_t x, v;
     asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(x) : "r"(w), "n"(kShift ? 0x00f000f0 : 0x000f000f), "r"(k.magic));   // (w & mask) | 1024
     if (kShift == 0) asm("sub.f16x2 %0, %1, %2;" : "=r"(v) : "r"(x), "r"(k.sub));                     // 1024 + code - 1032
@@ -392,7 +394,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
     int seq = found_seq;
     unsigned seq_base = found_base;
     int4 piece = make_int4(0, 0, 0, 0);
-    const NibbleConst nib = {p.nibble[0], p.nibble[1], p.nibble[2], p.nibble[3]};
+    const CodeConst codes = {p.code[0], p.code[1], p.code[2], p.code[3]};
 
     unsigned pos = lo;
     while (pos < hi) {
@@ -746,17 +748,17 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
     #pragma unroll
                                     for (int h = 0; h < 2; ++h) {
                                         const uint32_t w = kr[i][r][h * NB + b];
-                                        a[h][r] = bytes_to_half2(w, 0x4140);
-                                        a[h][2 + r] = bytes_to_half2(w, 0x4342);
+                                        a[h][r] = bytes_to_half2<0x5150>(w, codes);
+                                        a[h][2 + r] = bytes_to_half2<0x5352>(w, codes);
                                     }
                                 } else {
                                     // halfwords b and NB + b: codes 0-3 of words 2t and 2t + 1
                                     const uint32_t u = kr[i][r][b / 2], v = kr[i][r][(NB + b) / 2];
                                     const uint32_t w = __byte_perm(u, v, (b & 1 ? 0x32 : 0x10) | ((NB + b) & 1 ? 0x7600 : 0x5400));
-                                    a[0][r] = nibbles_to_half2<0>(w, nib);
-                                    a[0][2 + r] = nibbles_to_half2<4>(w, nib);
-                                    a[1][r] = nibbles_to_half2<0>(w >> 8, nib);
-                                    a[1][2 + r] = nibbles_to_half2<4>(w >> 8, nib);
+                                    a[0][r] = nibbles_to_half2<0>(w, codes);
+                                    a[0][2 + r] = nibbles_to_half2<4>(w, codes);
+                                    a[1][r] = nibbles_to_half2<0>(w >> 8, codes);
+                                    a[1][2 + r] = nibbles_to_half2<4>(w >> 8, codes);
                                 }
                             }
                             float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -957,16 +959,16 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                                 if constexpr (kCache == DTYPE_Q8_0) {
                                     const uint32_t u = vr[i][2 * r][b], v = vr[i][2 * r + 1][b];
                                     const uint32_t lo2 = __byte_perm(u, v, 0x5140), hi2 = __byte_perm(u, v, 0x7362);
-                                    a[0][2 * r] = bytes_to_half2(lo2, 0x4140);
-                                    a[0][2 * r + 1] = bytes_to_half2(lo2, 0x4342);
-                                    a[1][2 * r] = bytes_to_half2(hi2, 0x4140);
-                                    a[1][2 * r + 1] = bytes_to_half2(hi2, 0x4342);
+                                    a[0][2 * r] = bytes_to_half2<0x5150>(lo2, codes);
+                                    a[0][2 * r + 1] = bytes_to_half2<0x5352>(lo2, codes);
+                                    a[1][2 * r] = bytes_to_half2<0x5150>(hi2, codes);
+                                    a[1][2 * r + 1] = bytes_to_half2<0x5352>(hi2, codes);
                                 } else {
                                     const uint32_t w = __byte_perm(vr[i][2 * r][b / 2], vr[i][2 * r + 1][b / 2], b & 1 ? 0x7632 : 0x5410);
-                                    a[0][2 * r] = nibbles_to_half2<0>(w, nib);
-                                    a[0][2 * r + 1] = nibbles_to_half2<4>(w, nib);
-                                    a[1][2 * r] = nibbles_to_half2<0>(w >> 8, nib);
-                                    a[1][2 * r + 1] = nibbles_to_half2<4>(w >> 8, nib);
+                                    a[0][2 * r] = nibbles_to_half2<0>(w, codes);
+                                    a[0][2 * r + 1] = nibbles_to_half2<4>(w, codes);
+                                    a[1][2 * r] = nibbles_to_half2<0>(w >> 8, codes);
+                                    a[1][2 * r + 1] = nibbles_to_half2<4>(w >> 8, codes);
                                 }
                             }
                             float w[HL][2];
