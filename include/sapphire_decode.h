@@ -71,6 +71,17 @@ typedef struct {
  *  the same order with the same arguments. */
 SAPPHIRE_API sapphire_decoder_t *sapphire_decoder_create(kernel_context_t *ctx, const sapphire_gemma3_config_t *cfg,
                                                          const sapphire_gemma3_weights_t *w);
+/** Like sapphire_decoder_create with the KV cache in pages (sapphire_attention.h)
+ *  of page_size positions of type kv_dtype: F32, BF16, F16, or Q8_0 / Q4_0, which
+ *  hold 3.6 / 6.4 times the context of F32 in the same memory.  The context may
+ *  reach 2^20 positions (4096 otherwise).  Every stage is its own kernel (9 per
+ *  layer): QK-norm, rotation, cache write and attention are the operators of
+ *  sapphire_attention.h, angles exact at far positions instead of the
+ *  reference's fp32 tables. */
+SAPPHIRE_API sapphire_decoder_t *sapphire_decoder_create_paged(kernel_context_t *ctx,
+                                                               const sapphire_gemma3_config_t *cfg,
+                                                               const sapphire_gemma3_weights_t *w,
+                                                               tensor_dtype_t kv_dtype, int page_size);
 /** Greedy generation as the reference's perform_inference orders it
  *  (inference.c:238-325): prompt[0..n_prompt-2] fill the KV cache at
  *  positions 0..n_prompt-2, then prompt[n_prompt-1] at position n_prompt-1

@@ -114,6 +114,7 @@ _SIGNATURES = {
     "sapphire_test_decode_stall": (i32, [i32]),
     # include/sapphire_decode.h
     "sapphire_decoder_create": (vp, [vp, vp, vp]),
+    "sapphire_decoder_create_paged": (vp, [vp, vp, vp, i32, i32]),
     "sapphire_decoder_generate": (i32, [vp, vp, i32, i32, vp, vp]),
     "sapphire_decoder_last_logits": (i32, [vp, vp]),
     "sapphire_decoder_last_times": (i32, [vp, C.POINTER(f32), C.POINTER(f32)]),

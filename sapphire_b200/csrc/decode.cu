@@ -35,6 +35,11 @@
 // and a step is captured once into a CUDA graph per step kind (prompt step,
 // generated step); a generation is a sequence of graph launches with no host
 // round trip.
+//
+// A decoder with a paged cache (sapphire_decoder_create_paged) replaces the
+// attention stage by the serving operators: qk_norm_kernel, then
+// sapphire_rope_device, sapphire_kv_write_device and sapphire_attention_device
+// on the layer's pages, captured like the rest (9 kernels per layer).
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
@@ -42,6 +47,7 @@
 
 #include "internal.cuh"
 #include "decode_common.cuh"
+#include "../../include/sapphire_attention.h"
 #include "../../include/sapphire_decode.h"
 #include "../../include/sapphire_safetensors.h"
 
@@ -333,6 +339,23 @@ __global__ void __launch_bounds__(kAttnThreads) attention_kernel(
     if (threadIdx.x == 0) *counter = 0;
 }
 
+// rmsnorm_delta of each query and key head of qkv in place, one warp a head
+// (what attention_kernel does on the way in; the rotation follows on its own).
+__global__ void qk_norm_kernel(float *qkv, int heads, int kv_heads, int hd, const float *q_norm, const float *k_norm,
+                               float eps) {
+    pdl_trigger();
+    pdl_wait();
+    const int h = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (h >= heads + kv_heads) return;
+    float *x = qkv + (size_t)h * hd;
+    const float *w = h < heads ? q_norm : k_norm;
+    float ss = 0.0f;
+    for (int i = lane; i < hd; i += 32) ss += x[i] * x[i];
+    ss = warp_sum(ss);
+    const float r = 1.0f / sqrtf(ss / (float)hd + eps);
+    for (int i = lane; i < hd; i += 32) x[i] = (x[i] * r) * (1.0f + (w ? w[i] : 0.0f));
+}
+
 // Top-1 (value, lowest index on ties) and top-2 value.
 struct Top2 {
     float v1;
@@ -568,6 +591,16 @@ struct sapphire_decoder {
     unsigned epochs = 0;
     float *logits_all = nullptr;    // [world * ceil(vocab / world)] gathered logits (last_logits)
 
+    // Paged cache (sapphire_decoder_create_paged): one cache per layer, page i
+    // of each holding positions i * page_size .. in order.
+    bool paged = false;
+    std::vector<sapphire_kv_cache_t> kv;
+    int *page_table = nullptr;
+    int table_pages = 0;
+    sapphire_rope_t *rope_g = nullptr, *rope_l = nullptr;
+    void *attn_ws = nullptr;
+    size_t attn_ws_bytes = 0;
+
     // Persistent step (decode_persistent.cu): used when the model fits its
     // plan, unless SAPPHIRE_DECODE_PERSISTENT=0.  Projections live in its
     // row layout only; the LM head stays a context weight.
@@ -697,6 +730,50 @@ int enqueue_head(sapphire_decoder_t *d, cudaStream_t st) {
     return 2;
 }
 
+// The attention stage over the layer's pages: the current token at state->pos.
+int enqueue_paged_attention(sapphire_decoder_t *d, int l, float scale, cudaStream_t st) {
+    const sapphire_gemma3_config_t &c = d->cfg;
+    const sapphire_decoder::Layer &L = d->layers[l];
+    float *k = d->qkv + d->q_dim, *v = k + d->kv_dim;
+    const int *pos = &d->state->pos;
+    launch_pdl(qk_norm_kernel, dim3((c.heads + c.kv_heads + 7) / 8), dim3(256), 0, st, d->qkv, c.heads, c.kv_heads,
+               c.head_dim, (const float *)L.w_q, (const float *)L.w_k, c.rms_eps);
+    if (check_launch(d, "QK norm")) return -1;
+    sapphire_rope_args_t r{};
+    r.dtype = DTYPE_F32;
+    r.tokens = 1;
+    r.positions = pos;
+    r.q = r.q_out = d->qkv;
+    r.q_heads = c.heads;
+    r.k = r.k_out = k;
+    r.k_heads = c.kv_heads;
+    if (sapphire_rope_device(L.global ? d->rope_g : d->rope_l, &r)) return -1;
+    sapphire_kv_args_t w{};
+    w.dtype = DTYPE_F32;
+    w.tokens = w.sequences = 1;
+    w.start = pos;
+    w.page_table = d->page_table;
+    w.table_stride = d->table_pages;
+    w.k = k;
+    w.v = v;
+    if (sapphire_kv_write_device(d->ctx, &d->kv[l], &w)) return -1;
+    sapphire_attention_args_t a{};
+    a.dtype = DTYPE_F32;
+    a.sequences = 1;
+    a.heads = c.heads;
+    a.q = d->qkv;
+    a.out = d->attn;
+    a.page_table = d->page_table;
+    a.table_stride = d->table_pages;
+    a.lengths = pos;
+    a.length_offset = 1;
+    a.window = L.global ? 0 : c.sliding_window > 0 ? c.sliding_window : 1024;
+    a.scale = scale;
+    a.workspace = d->attn_ws;
+    a.workspace_bytes = d->attn_ws_bytes;
+    return sapphire_attention_device(d->ctx, &d->kv[l], &a);
+}
+
 int enqueue_step(sapphire_decoder_t *d, bool generate, cudaStream_t st) {
     const sapphire_gemma3_config_t &c = d->cfg;
     kernel_context_t *ctx = d->ctx;
@@ -741,15 +818,20 @@ int enqueue_step(sapphire_decoder_t *d, bool generate, cudaStream_t st) {
                 return -1;
             std::swap(cur, other);
         }
-        float *kc = d->kcache + (size_t)l * c.kv_heads * c.context * c.head_dim;
-        float *vc = d->vcache + (size_t)l * c.kv_heads * c.context * c.head_dim;
-        launch_pdl(attention_kernel, dim3(kAttnSplit), dim3(kAttnThreads), 0, st, (const DecState *)d->state,
-                   (const float *)d->qkv, kc, vc, d->attn, d->attn_part, d->counters, c.heads, c.kv_heads,
-                   c.head_dim, c.context, c.sliding_window > 0 ? c.sliding_window : 1024, L.global ? 1 : 0,
-                   att_scale, (const float *)L.w_q, (const float *)L.w_k, eps,
-                   (const float *)(L.global ? d->rope_cos_g : d->rope_cos_l),
-                   (const float *)(L.global ? d->rope_sin_g : d->rope_sin_l));
-        if (check_launch(d, "attention")) return -1;
+        if (d->paged) {
+            if (enqueue_paged_attention(d, l, att_scale, st)) return -1;
+            launches += 4;
+        } else {
+            float *kc = d->kcache + (size_t)l * c.kv_heads * c.context * c.head_dim;
+            float *vc = d->vcache + (size_t)l * c.kv_heads * c.context * c.head_dim;
+            launch_pdl(attention_kernel, dim3(kAttnSplit), dim3(kAttnThreads), 0, st, (const DecState *)d->state,
+                       (const float *)d->qkv, kc, vc, d->attn, d->attn_part, d->counters, c.heads, c.kv_heads,
+                       c.head_dim, c.context, c.sliding_window > 0 ? c.sliding_window : 1024, L.global ? 1 : 0,
+                       att_scale, (const float *)L.w_q, (const float *)L.w_k, eps,
+                       (const float *)(L.global ? d->rope_cos_g : d->rope_cos_l),
+                       (const float *)(L.global ? d->rope_sin_g : d->rope_sin_l));
+            if (check_launch(d, "attention")) return -1;
+        }
         if (launch_gemv_direct(ctx, *o, d->attn, d->tmp, st)) return -1;
         // gu = W_gu . rmsnorm_delta(h + rmsnorm_delta(o_out, attn_post), ffn)
         if (launch_gemv_direct_resnorm(ctx, *gu, d->tmp, L.w_attn_post, cur, L.w_ffn, other, eps, d->gu, st))
@@ -824,15 +906,52 @@ extern "C" SAPPHIRE_API void sapphire_decoder_destroy(sapphire_decoder_t *d) {
             if (e) cudaEventDestroy(e);
         for (void *p : d->allocations) cudaFree(p);
         if (d->exch_local) shard_unmap_buffers(d->ctx, d->exch_local, d->exch_peers);
+        sapphire_rope_destroy(d->rope_g);
+        sapphire_rope_destroy(d->rope_l);
         if (prev >= 0) cudaSetDevice(prev);
     }
     for (tensor_t *t : d->tensors) tensor_release(t);   // drops the device copies
     delete d;
 }
 
-extern "C" SAPPHIRE_API sapphire_decoder_t *sapphire_decoder_create(kernel_context_t *ctx,
-                                                                    const sapphire_gemma3_config_t *cfg,
-                                                                    const sapphire_gemma3_weights_t *w) {
+namespace {
+
+// Pages, table, rotation plans and workspace of a paged decoder.
+int create_pages(sapphire_decoder_t *d, tensor_dtype_t kv_dtype, int page_size) {
+    const sapphire_gemma3_config_t &c = d->cfg;
+    sapphire_kv_cache_t kv{kv_dtype, page_size, c.kv_heads, c.head_dim, 0, nullptr};
+    const size_t per = sapphire_kv_page_bytes(&kv);
+    if (!per) {
+        ctx_fail(d->ctx, "sapphire_decoder_create_paged", "no cache of this type, page size and head size");
+        return -1;
+    }
+    d->table_pages = (c.context + page_size - 1) / page_size;
+    kv.num_pages = d->table_pages;
+    for (int l = 0; l < c.layers; ++l) {
+        if (dev_alloc(d, &kv.pages, per * kv.num_pages)) return -1;
+        d->kv.push_back(kv);
+    }
+    std::vector<int> table(d->table_pages);
+    for (int i = 0; i < d->table_pages; ++i) table[i] = i;
+    if (dev_alloc(d, (void **)&d->page_table, table.size() * sizeof(int))) return -1;
+    if (cudaMemcpy(d->page_table, table.data(), table.size() * sizeof(int), cudaMemcpyHostToDevice) != cudaSuccess) {
+        ctx_fail(d->ctx, "sapphire_decoder_create_paged", "page table upload failed");
+        return -1;
+    }
+    sapphire_rope_config_t r{};
+    r.head_dim = c.head_dim;
+    r.layout = SAPPHIRE_ROPE_HALF;
+    r.theta = c.rope_theta;
+    if (!(d->rope_g = sapphire_rope_create(d->ctx, &r))) return -1;
+    r.theta = c.rope_local_theta;
+    if (!(d->rope_l = sapphire_rope_create(d->ctx, &r))) return -1;
+    d->attn_ws_bytes = sapphire_attention_workspace_bytes(d->ctx, &d->kv[0], 1, c.heads);
+    return dev_alloc(d, &d->attn_ws, d->attn_ws_bytes);
+}
+
+sapphire_decoder_t *create_decoder(kernel_context_t *ctx, const sapphire_gemma3_config_t *cfg,
+                                   const sapphire_gemma3_weights_t *w, bool paged, tensor_dtype_t kv_dtype,
+                                   int page_size) {
     if (!ctx || !cfg || !w || !w->embed_bf16 || !w->lm_head || !w->proj) {
         LOG_ERROR("sapphire_decoder_create: NULL argument");
         return nullptr;
@@ -840,10 +959,10 @@ extern "C" SAPPHIRE_API sapphire_decoder_t *sapphire_decoder_create(kernel_conte
     const sapphire_gemma3_config_t &c = *cfg;
     if (c.layers <= 0 || c.hidden <= 0 || c.ffn <= 0 || c.heads <= 0 || c.kv_heads <= 0 || c.heads % c.kv_heads ||
         c.heads / c.kv_heads > kMaxGroup || c.heads > kMaxHeads || c.head_dim <= 0 || c.head_dim > kMaxHeadDim || c.head_dim % 64 ||
-        c.vocab <= 0 || c.context <= 0 || c.context > kMaxContext || c.rms_eps < 0.0f) {
+        c.vocab <= 0 || c.context <= 0 || c.context > (paged ? kMaxPagedContext : kMaxContext) || c.rms_eps < 0.0f) {
         ctx_fail(ctx, "sapphire_decoder_create",
                  "unsupported shape (heads %% kv_heads == 0, group <= %d, head_dim a multiple of 64 up to %d, "
-                 "context <= %d)", kMaxGroup, kMaxHeadDim, kMaxContext);
+                 "context <= %d)", kMaxGroup, kMaxHeadDim, paged ? kMaxPagedContext : kMaxContext);
         return nullptr;
     }
     std::lock_guard<std::recursive_mutex> lk(ctx->exec_mutex);
@@ -858,6 +977,7 @@ extern "C" SAPPHIRE_API sapphire_decoder_t *sapphire_decoder_create(kernel_conte
     d->ctx = ctx;
     d->cfg = c;
     d->sharded = ctx->world > 1;
+    d->paged = paged;
     d->q_dim = c.heads * c.head_dim;
     d->kv_dim = c.kv_heads * c.head_dim;
     bool ok = false;
@@ -893,7 +1013,7 @@ extern "C" SAPPHIRE_API sapphire_decoder_t *sapphire_decoder_create(kernel_conte
             lb += (unsigned long long)pp.stage_rows[s] * pp.stage_stride[s];
         }
         pp.layer_bytes = lb;
-        {
+        if (!paged) {
             const char *why = nullptr;
             const char *env = getenv("SAPPHIRE_DECODE_PERSISTENT");
             d->plan = persist_plan(ctx->device, pp, &why);
@@ -1007,16 +1127,20 @@ extern "C" SAPPHIRE_API sapphire_decoder_t *sapphire_decoder_create(kernel_conte
             ctx_fail(ctx, "sapphire_decoder_create", "embedding upload failed");
             break;
         }
-        std::vector<float> cs, sn;
-        const size_t rope_n = (size_t)c.context * c.head_dim;
-        rope_table(cs, sn, c.head_dim, c.context, c.rope_theta);
-        if (upload_floats(d, &d->rope_cos_g, cs.data(), rope_n) || upload_floats(d, &d->rope_sin_g, sn.data(), rope_n))
-            break;
-        rope_table(cs, sn, c.head_dim, c.context, c.rope_local_theta);
-        if (upload_floats(d, &d->rope_cos_l, cs.data(), rope_n) || upload_floats(d, &d->rope_sin_l, sn.data(), rope_n))
-            break;
-        const size_t kv = (size_t)c.layers * c.kv_heads * c.context * c.head_dim;
-        if (upload_floats(d, &d->kcache, nullptr, kv) || upload_floats(d, &d->vcache, nullptr, kv)) break;
+        if (paged) {
+            if (create_pages(d, kv_dtype, page_size)) break;
+        } else {
+            std::vector<float> cs, sn;
+            const size_t rope_n = (size_t)c.context * c.head_dim;
+            rope_table(cs, sn, c.head_dim, c.context, c.rope_theta);
+            if (upload_floats(d, &d->rope_cos_g, cs.data(), rope_n) || upload_floats(d, &d->rope_sin_g, sn.data(), rope_n))
+                break;
+            rope_table(cs, sn, c.head_dim, c.context, c.rope_local_theta);
+            if (upload_floats(d, &d->rope_cos_l, cs.data(), rope_n) || upload_floats(d, &d->rope_sin_l, sn.data(), rope_n))
+                break;
+            const size_t kv = (size_t)c.layers * c.kv_heads * c.context * c.head_dim;
+            if (upload_floats(d, &d->kcache, nullptr, kv) || upload_floats(d, &d->vcache, nullptr, kv)) break;
+        }
         if (dev_alloc(d, (void **)&d->hidden, c.hidden * 4) || dev_alloc(d, (void **)&d->hidden2, c.hidden * 4) ||
             dev_alloc(d, (void **)&d->norm, c.hidden * 4) ||
             dev_alloc(d, (void **)&d->qkv, (size_t)(d->q_dim + 2 * d->kv_dim) * 4) ||
@@ -1142,6 +1266,21 @@ extern "C" SAPPHIRE_API sapphire_decoder_t *sapphire_decoder_create(kernel_conte
         return nullptr;
     }
     return d;
+}
+
+}  // namespace
+
+extern "C" SAPPHIRE_API sapphire_decoder_t *sapphire_decoder_create(kernel_context_t *ctx,
+                                                                    const sapphire_gemma3_config_t *cfg,
+                                                                    const sapphire_gemma3_weights_t *w) {
+    return create_decoder(ctx, cfg, w, false, DTYPE_F32, 0);
+}
+
+extern "C" SAPPHIRE_API sapphire_decoder_t *sapphire_decoder_create_paged(kernel_context_t *ctx,
+                                                                          const sapphire_gemma3_config_t *cfg,
+                                                                          const sapphire_gemma3_weights_t *w,
+                                                                          tensor_dtype_t kv_dtype, int page_size) {
+    return create_decoder(ctx, cfg, w, true, kv_dtype, page_size);
 }
 
 extern "C" SAPPHIRE_API int sapphire_decoder_generate(sapphire_decoder_t *d, const int *prompt, int n_prompt,

@@ -10,6 +10,7 @@ constexpr int kMaxGroup = 8;          // query heads per KV head
 constexpr int kMaxHeads = 32;
 constexpr int kMaxHeadDim = 256;
 constexpr int kMaxContext = 4096;
+constexpr int kMaxPagedContext = 1 << 20;   // with a paged cache
 
 // Device-side step state.
 struct DecState {

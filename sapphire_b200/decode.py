@@ -22,16 +22,24 @@ def config_struct(cfg) -> Gemma3Config:
 
 
 class Decoder:
-    """Uploads `model` (workloads.make_decode_model) to the context's GPU."""
+    """Uploads `model` (workloads.make_decode_model) to the context's GPU.
 
-    def __init__(self, ctx, cfg, model):
+    kv_dtype (a DTYPE_* number or its name: F32, BF16, F16, Q8_0, Q4_0) selects
+    a paged cache of kv_page_size positions a page (sapphire_decoder_create_paged)."""
+
+    def __init__(self, ctx, cfg, model, kv_dtype=None, kv_page_size: int = 64):
         self.ctx, self.cfg = ctx, cfg
         ptrs = [addr(layer[name]) for layer in model["layers"] for name, _, _ in cfg.projections()]
         self._proj = (C.c_void_p * len(ptrs))(*ptrs)
         w = Gemma3Weights(addr(model["embed"]), addr(model["lm_head"]), None,
                           C.cast(self._proj, C.c_void_p), None)
         c = config_struct(cfg)
-        self.handle = lib.sapphire_decoder_create(ctx.handle, C.byref(c), C.byref(w))
+        if kv_dtype is None:
+            self.handle = lib.sapphire_decoder_create(ctx.handle, C.byref(c), C.byref(w))
+        else:
+            from .attention import _dtype
+            self.handle = lib.sapphire_decoder_create_paged(ctx.handle, C.byref(c), C.byref(w), _dtype(kv_dtype),
+                                                            kv_page_size)
         if not self.handle:
             raise SapphireError(f"sapphire_decoder_create failed: {ctx.last_error}")
 

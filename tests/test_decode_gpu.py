@@ -205,3 +205,74 @@ def test_long_prompt_paths_agree(sp, ctx, decoder, monkeypatch):
     top2 = np.sort(logits_s)[-2:]
     if top2[1] - top2[0] > 1e-3:
         assert ids_p[0] == ids_s[0]
+
+
+# ------------------------------------------------------------- paged cache --
+def test_paged_decoder_matches_reference(sp, ctx, decoder, golden):
+    """The decoder over fp32 pages (the rope, cache and attention operators in
+    place of its own attention) gives the reference's ids."""
+    from sapphire_b200.decode import Decoder
+    cfg, model, _ = decoder
+    for page in (16, 24):
+        dec = Decoder(ctx, cfg, model, kv_dtype="f32", kv_page_size=page)
+        ids, margins = dec.generate(model["prompt"], cfg.generate)
+        assert np.array_equal(ids, golden["tokens"])
+        # angles are exact here and fp32 products there: half a step of an angle of up to 575
+        assert np.max(np.abs(margins - golden["margins"])) < 2e-3
+        assert dec.launches_per_token == 9 * cfg.layers + 4
+        dec.close()
+
+
+@pytest.mark.parametrize("kv", ["bf16", "f16", "q8_0", "q4_0"])
+def test_paged_decoder_types(sp, ctx, decoder, golden, kv):
+    """Other cache types: the first position attends to itself alone, so its
+    logits move by no more than the rounding of its values does; generation
+    repeats itself, and the cache is the prompt's alone."""
+    from sapphire_b200.decode import Decoder
+    cfg, model, ref = decoder
+    dec = Decoder(ctx, cfg, model, kv_dtype=kv, kv_page_size=32)
+    a, _ = dec.generate(model["prompt"][:40], 8)
+    first = dec.last_logits()
+    dec.generate(model["prompt"][40:90], 4)
+    b, _ = dec.generate(model["prompt"][:40], 8)
+    assert np.array_equal(a, b) and np.array_equal(first, dec.last_logits())
+    # One token: every attention output is v itself, rounded by the type (half a
+    # step relative to the block's largest value).  An RMS norm follows each, so
+    # a relative error e of the output of one of 18 layers moves the residual
+    # stream by at most e of its own added part, and the sum of 18 parts by 18 e.
+    step = {"bf16": 2.0 ** -9, "f16": 2.0 ** -12, "q8_0": 0.5 / 127 * 4, "q4_0": 0.5 / 8 * 4}[kv]
+    ref.generate(model["prompt"][:1], 1)
+    want = ref.last_logits().astype(np.float64)
+    dec.generate(model["prompt"][:1], 1)
+    got = dec.last_logits().astype(np.float64)
+    assert np.linalg.norm(got - want) <= 18 * step * np.linalg.norm(want)
+    dec.close()
+
+
+def test_paged_decoder_long_context(sp, ctx):
+    """A context above the dense cache's 4096: windowed and global layers past it."""
+    from sapphire_b200 import workloads
+    from sapphire_b200.decode import Decoder
+    cfg = dataclasses.replace(workloads.GQA_TINY, context=6000)
+    model = workloads.make_decode_model(cfg, lambda a: sp.quantize(ctx, Q4_0, a), seed=3)
+    with pytest.raises(sp.SapphireError):
+        Decoder(ctx, cfg, model)
+    prompt = np.resize(model["prompt"], 4500)
+    ids = {}
+    for kv, page in (("f32", 64), ("f32", 50)):
+        dec = Decoder(ctx, cfg, model, kv_dtype=kv, kv_page_size=page)
+        ids[page], _ = dec.generate(prompt, 8)
+        with pytest.raises(sp.SapphireError):
+            dec.generate(prompt, 1501)
+        dec.close()
+    assert np.array_equal(ids[64], ids[50])
+
+
+def test_paged_decoder_refusals(sp, ctx):
+    from sapphire_b200 import workloads
+    from sapphire_b200.decode import Decoder
+    cfg = workloads.GQA_TINY
+    model = workloads.make_decode_model(cfg, lambda a: sp.quantize(ctx, Q4_0, a), seed=3)
+    for kv, page in (("tq2_0", 16), ("f32", 0), ("q8_0", 5000)):
+        with pytest.raises(sp.SapphireError, match="no cache of this type"):
+            Decoder(ctx, cfg, model, kv_dtype=kv, kv_page_size=page)
