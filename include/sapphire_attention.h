@@ -84,7 +84,7 @@ typedef struct {
     tensor_dtype_t dtype;    /* F32, BF16 or F16, of q, k and their outputs */
     int tokens;
     const int *positions;    /* [tokens] */
-    /* [tokens, q_heads, head_dim]; q_heads 0: none.  q_out may be q (same strides). */
+    /* [tokens, q_heads, head_dim]; q_heads 0: none.  q_out is q (same strides) or does not overlap it. */
     const void *q;
     void *q_out;
     int q_heads;
@@ -93,7 +93,8 @@ typedef struct {
     void *k_out;
     int k_heads;
     long long k_token_stride, k_head_stride, k_out_token_stride, k_out_head_stride;
-    int inverse;             /* != 0: turn back (also the gradient of the forward turn) */
+    int inverse;             /* != 0: turn by the negative angles, cos and sin still times
+                                attention_factor: the gradient of the turn */
 } sapphire_rope_args_t;
 
 SAPPHIRE_API int sapphire_rope_device(sapphire_rope_t *rope, const sapphire_rope_args_t *args);
@@ -160,7 +161,7 @@ typedef struct {
     int sequences;
     int heads;               /* a multiple of kv_heads */
     const void *q;           /* [sequences, heads, head_dim] */
-    void *out;               /* the same */
+    void *out;               /* the same, not overlapping q */
     long long q_seq_stride, q_head_stride, out_seq_stride, out_head_stride;
     float *lse;              /* [sequences, heads] log of the softmax's sum, or NULL */
     const int *page_table;   /* [sequences, table_stride] */

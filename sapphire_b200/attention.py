@@ -42,20 +42,22 @@ def _io(x, what: str) -> int:
     return dt
 
 
-def _heads(x, what: str, rows: int | None, heads: int | None, dim: int) -> tuple[int, int]:
-    """(row stride, head stride) of x [rows, heads, dim]."""
+def _heads(x, what: str, rows: int | None, heads: int | None, dim: int, dt: int) -> tuple[int, int, int]:
+    """(address, row stride, head stride) of x [rows, heads, dim] of type dt."""
     shape = x.shape
     if len(shape) != 3 or shape[2] != dim or (rows is not None and shape[0] != rows) or \
             (heads is not None and shape[1] != heads):
         want = ["any" if n is None else n for n in (rows, heads, dim)]
         raise SapphireError(f"{what} has shape {tuple(shape)}, not {want}")
+    if _io_seen.get(x.dtype) != dt and _io(x, what) != dt:
+        raise SapphireError(f"the tensors of a call must have one type: {what} is {x.dtype}")
     a, b, c = x.stride()
-    if c != 1 and dim > 1:
+    if c != 1:
         raise SapphireError(f"{what}: the last dimension must be contiguous")
-    # A dimension of one row has no stride that matters; 0 would mean contiguous.
+    # To the library a stride of 0 is a contiguous one.
     if (a == 0 and shape[0] > 1) or (b == 0 and shape[1] > 1):
         raise SapphireError(f"{what}: broadcast dimensions are not supported")
-    return a, b
+    return x.data_ptr(), a, b
 
 
 def _int32(x, what: str) -> None:
@@ -113,19 +115,21 @@ class Rope:
         x = q if q is not None else k
         if x is None:
             return
-        n, dt = x.shape[0], _io(x, "q" if q is not None else "k")
-        sides = []
-        for name, a, o in (("q", q, q_out), ("k", k, k_out)):
-            if a is None:
-                sides += [0, 0, 0, 0, 0, 0, 0]
-                continue
-            o = a if o is None else o
-            if _io(a, name) != dt or _io(o, name + "_out") != dt:
-                raise SapphireError("q, k and their outputs must have one type")
-            ts, hs = _heads(a, name, n, None, self.head_dim)
-            ots, ohs = _heads(o, name + "_out", n, a.shape[1], self.head_dim)
-            sides += [a.data_ptr(), o.data_ptr(), a.shape[1], ts, hs, ots, ohs]
-        args = RopeArgs(dt, n, _ints(positions, "positions", n), *sides, int(inverse))
+        n, dim = x.shape[0], self.head_dim
+        dt = _io_seen.get(x.dtype)
+        if dt is None:
+            dt = _io(x, "q" if q is not None else "k")
+        qh = kh = qp = kp = qop = kop = qt = qs = kt = ks = qot = qos = kot = kos = 0
+        if q is not None:
+            qh = q.shape[1]
+            qp, qt, qs = _heads(q, "q", n, None, dim, dt)
+            qop, qot, qos = (qp, qt, qs) if q_out is None else _heads(q_out, "q_out", n, qh, dim, dt)
+        if k is not None:
+            kh = k.shape[1]
+            kp, kt, ks = _heads(k, "k", n, None, dim, dt)
+            kop, kot, kos = (kp, kt, ks) if k_out is None else _heads(k_out, "k_out", n, kh, dim, dt)
+        args = RopeArgs(dt, n, _ints(positions, "positions", n), qp, qop, qh, qt, qs, qot, qos, kp, kop, kh, kt, ks, kot,
+                        kos, inverse)
         if lib.sapphire_rope_device(self.handle, C.byref(args)) != 0:
             raise SapphireError(f"sapphire_rope_device failed: {self.ctx.last_error}")
 
@@ -163,17 +167,16 @@ class KVCache:
         self._ref = C.byref(self._struct)
 
     def _rows(self, fn, what, k, v, page_table, start, cu_tokens) -> None:
-        n = k.shape[0]
-        kts, khs = _heads(k, "k", n, self.kv_heads, self.head_dim)
-        vts, vhs = _heads(v, "v", n, self.kv_heads, self.head_dim)
-        dt = _io(k, "k")
-        if _io(v, "v") != dt:
-            raise SapphireError("k and v must have one type")
+        n, heads, dim = k.shape[0], self.kv_heads, self.head_dim
+        dt = _io_seen.get(k.dtype)
+        if dt is None:
+            dt = _io(k, "k")
+        kp, kt, kh = _heads(k, "k", n, heads, dim, dt)
+        vp, vt, vh = _heads(v, "v", n, heads, dim, dt)
         seqs = page_table.shape[0]
         table, stride = _table(page_table, seqs)
-        args = KvArgs(dt, n, seqs, 0 if cu_tokens is None else _ints(cu_tokens, "cu_tokens", seqs + 1),
-                      0 if start is None else _ints(start, "start", seqs), table, stride, k.data_ptr(), v.data_ptr(),
-                      kts, khs, vts, vhs)
+        args = KvArgs(dt, n, seqs, None if cu_tokens is None else _ints(cu_tokens, "cu_tokens", seqs + 1),
+                      None if start is None else _ints(start, "start", seqs), table, stride, kp, vp, kt, kh, vt, vh)
         if fn(self.ctx.handle, self._ref, C.byref(args)) != 0:
             raise SapphireError(f"{what} failed: {self.ctx.last_error}")
 
@@ -200,16 +203,16 @@ class KVCache:
         `window` of them, if set).  lse: float32 [sequences, heads] or None.
         workspace: a byte tensor of workspace_bytes(...) (required when the
         call is captured into a graph)."""
-        n, heads = q.shape[0], q.shape[1]
-        qs, qh = _heads(q, "q", n, None, self.head_dim)
-        os, oh = _heads(out, "out", n, heads, self.head_dim)
-        dt = _io(q, "q")
-        if _io(out, "out") != dt:
-            raise SapphireError("q and out must have one type")
+        n, heads, dim = q.shape[0], q.shape[1], self.head_dim
+        dt = _io_seen.get(q.dtype)
+        if dt is None:
+            dt = _io(q, "q")
+        qp, qs, qh = _heads(q, "q", n, None, dim, dt)
+        op, os, oh = _heads(out, "out", n, heads, dim, dt)
         if lse is not None and (tuple(lse.shape) != (n, heads) or _io(lse, "lse") != DTYPE_F32 or not lse.is_contiguous()):
             raise SapphireError(f"lse must be contiguous float32 [{n}, {heads}]")
         table, stride = _table(page_table, n)
-        args = AttentionArgs(dt, n, heads, q.data_ptr(), out.data_ptr(), qs, qh, os, oh,
+        args = AttentionArgs(dt, n, heads, qp, op, qs, qh, os, oh,
                              0 if lse is None else lse.data_ptr(), table, stride, _ints(lengths, "lengths", n),
                              length_offset, window, scale, addr(workspace),
                              0 if workspace is None else workspace.numel() * workspace.element_size())

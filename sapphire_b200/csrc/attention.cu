@@ -9,13 +9,13 @@
 namespace {
 
 // Blocks of one launch: all that the GPU holds at a time.
-int attn_blocks(kernel_context_t *ctx, const sapphire_kv_cache_t *c) {
-    return sm_count(ctx->device) * attn_blocks_per_sm(c->dtype, c->head_dim);
+int attn_blocks(kernel_context_t *ctx, const sapphire_kv_cache_t *c, int group) {
+    return sm_count(ctx->device) * attn_blocks_per_sm(c->dtype, c->head_dim, attn_wide(group));
 }
 
 // Workspace: the pieces' descriptions, then two partial results a block.
 size_t attn_workspace(kernel_context_t *ctx, const sapphire_kv_cache_t *c, int group) {
-    const size_t blocks = attn_blocks(ctx, c), heads = attn_tile_heads(group);
+    const size_t blocks = attn_blocks(ctx, c, group), heads = attn_tile_heads(group);
     return blocks * (sizeof(int4) + 2 * heads * (c->head_dim + 2) * sizeof(float));
 }
 
@@ -63,8 +63,9 @@ extern "C" SAPPHIRE_API int sapphire_attention_device(kernel_context_t *ctx, con
         !on_device(ctx, who, "out", a->out) || !on_device(ctx, who, "page_table", a->page_table) ||
         !on_device(ctx, who, "lengths", a->lengths) || (a->lse && !on_device(ctx, who, "lse", a->lse)))
         return -1;
-    // The kernels number tiles (of 64 tokens or more) in 31 bits.
-    if ((double)a->sequences * a->heads * ((double)a->table_stride * cache->page_size / 64 + 1) >= 2147483648.0) {
+    // The kernels number tiles (of 64 tokens or more, and what an item costs besides) in 31 bits.
+    if ((double)a->sequences * a->heads * ((double)a->table_stride * cache->page_size / 64 + 1 + kAttnItemUnits) >=
+        2147483648.0) {
         ctx_fail(ctx, who, "%d sequences of up to %d pages are more tiles than 2^31", a->sequences, a->table_stride);
         return -1;
     }
@@ -89,7 +90,7 @@ extern "C" SAPPHIRE_API int sapphire_attention_device(kernel_context_t *ctx, con
     p.group = a->heads / cache->kv_heads;
     p.head_tiles = (p.group + attn_tile_heads(p.group) - 1) / attn_tile_heads(p.group);
     p.page_mul = (1ull << 32) / cache->page_size + 1;
-    p.blocks = attn_blocks(ctx, cache);
+    p.blocks = attn_blocks(ctx, cache, p.group);
     p.code[0] = 0x64006400u;
     p.code[1] = cache->dtype == DTYPE_Q8_0 ? 0x64806480u : 0x64086408u;
     p.code[2] = 0x2c002c00u;

@@ -34,8 +34,8 @@
 //
 // Quantised rows are kept as words of 4 codes in the order [8][nb], so the same
 // lanes read consecutive bytes.  V's codes become fp16 exactly (1024 + code - 1152,
-// or - 1032), and V's scale multiplies the probability, brought into fp16's range
-// by a power of two per warp that grows with the scales seen.  K's codes become
+// or - 1032), and V's scale multiplies the probability, the product brought into
+// fp16's range by a power of two per warp that follows the largest seen.  K's codes become
 // fp16 the same way under fp32 and fp16 outputs; under a bf16 output they are
 // multiplied as the integers they are by the query as 15-bit integers (two
 // signed bytes), the sums exact and started at what the codes' offset adds, and
@@ -52,6 +52,11 @@
 constexpr int kAttnWarps = 4;
 constexpr int kAttnSmem = 224 * 1024;         // shared memory that an SM's blocks divide
 constexpr float kLog2e = 1.4426950408889634f;
+
+// What an item costs besides its tiles (its query, the filling of the rings and
+// the joining of the warps), in tiles: the ranges of blocks are cut in these
+// units, so one that meets many short sequences takes fewer tiles.
+constexpr int kAttnItemUnits = 2;
 
 struct AttnParams {
     KvLayout l;
@@ -87,9 +92,9 @@ inline int attn_tile_heads(int group) { return attn_wide(group) ? 8 : 4; }
 constexpr int attn_m_tiles(int cache, int hd) {
     return cache == DTYPE_Q4_0 || cache == DTYPE_Q8_0 || (hd <= 64 && cache != DTYPE_F32) ? 2 : 1;
 }
-constexpr int attn_blocks_per_sm(int cache, int hd) {
+constexpr int attn_blocks_per_sm(int cache, int hd, bool wide) {
     if (cache == DTYPE_F32) return hd <= 64 ? 3 : hd <= 128 ? 2 : 1;
-    if (cache == DTYPE_Q4_0) return hd <= 128 ? 4 : 2;
+    if (cache == DTYPE_Q4_0) return hd <= 64 ? 4 : hd <= 128 ? (wide ? 3 : 4) : 2;
     if (cache == DTYPE_Q8_0) return hd <= 64 ? 4 : hd <= 128 ? 3 : 2;
     return hd <= 64 ? 4 : hd <= 128 ? 3 : 2;
 }
@@ -99,9 +104,9 @@ constexpr int attn_blocks_per_sm(int cache, int hd) {
 // K's codes are multiplied as integers where the output's rounding allows.
 template <int kCache, bool kExact>
 constexpr bool kAttnInt = (kCache == DTYPE_Q8_0 || kCache == DTYPE_Q4_0) && !kExact;
-// 2^(p + kBias): probabilities use the upper end of fp16 where the MMA is fp16.
+// 2^(p + kBias): probabilities use the upper end of fp16 over fp16 caches.
 template <int kCache>
-constexpr float kAttnBias = (kCache == DTYPE_BF16 || kCache == DTYPE_F32) ? 0.0f : 14.0f;
+constexpr float kAttnBias = kCache == DTYPE_F16 ? 14.0f : 0.0f;
 
 __device__ __forceinline__ float attn_exp2(float x) {
     float y;
@@ -256,7 +261,7 @@ __device__ __forceinline__ void read_scales(const uint8_t *p, float (&s)[N]) {
 #endif  // __CUDACC__
 
 // Shapes of one variant.
-template <int kCache, int HD>
+template <int kCache, int HD, bool kWide>
 struct AttnShape {
     static constexpr bool kQuant = kCache == DTYPE_Q8_0 || kCache == DTYPE_Q4_0;
     static constexpr bool kF32 = kCache == DTYPE_F32;
@@ -272,7 +277,7 @@ struct AttnShape {
     static constexpr int kStride = kRowBytes + (kF32 ? 32 : 16);
     static constexpr int kScaleOff = kTok * kStride;
     static constexpr int kSlot = kScaleOff + kTok * kScaleBytes;
-    static constexpr int kBlocks = attn_blocks_per_sm(kCache, HD);
+    static constexpr int kBlocks = attn_blocks_per_sm(kCache, HD, kWide);
     // Query parts: rows of 8 columns, padded so that the rows of neighbouring
     // lanes fall on the other half of the banks.
     static constexpr int kQElem = kF32 ? 4 : 2;
@@ -286,10 +291,6 @@ struct AttnShape {
 };
 
 #ifdef __CUDACC__
-// What an item costs besides its tiles (its query, the filling of the rings and
-// the joining of the warps), in tiles: the ranges of blocks are cut in these
-// units, so one that meets many short sequences takes fewer tiles.
-constexpr int kAttnItemUnits = 2;
 // The positions a sequence's new token attends to, as tiles.
 struct AttnSpan {
     int first, end, tile0, tiles, units;
@@ -324,8 +325,8 @@ struct AttnParts {
 };
 
 template <int kCache, int HD, bool kWide, bool kExact>
-__global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD)) attend_kernel(const AttnParams p) {
-    using Sh = AttnShape<kCache, HD>;
+__global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD, kWide)) attend_kernel(const AttnParams p) {
+    using Sh = AttnShape<kCache, HD, kWide>;
     using Pt = AttnParts<kCache, kWide, kExact>;
     constexpr int GH = kWide ? 8 : 4, HL = kWide ? 2 : 1;         // heads of a tile, and of a lane
     constexpr int NB = Sh::NB, MT = Sh::MT, R = Sh::R, kTok = Sh::kTok, kTile = kTok * kAttnWarps, kMTiles = HD / 16;
@@ -651,7 +652,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
             for (int j = 0; j < HL; ++j)
 #pragma unroll
                 for (int b = 0; b < NB; ++b) qo[j][b] = qoff[HL * t + j][b];
-        float vlim = 0.0f, vinv = 0.0f;                           // V scales: largest that fits, and the power of two
+        float vlim = 0.0f, vinv = 0.0f;                           // p times V's scale: largest that fits, and the power of two
         // Adds what an accumulator of its own holds: an MMA truncates its
         // sums, so where that shows (kExact) only a tile's products share one.
         auto add_up = [](float (&to)[4], const float (&c)[4]) {
@@ -919,23 +920,42 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
                         read_scales<NB>(slot + Sh::kScaleOff + (16 * i + 8 * r + g) * Sh::kScaleBytes, vs[i][r]);
+                        float top_s = 0.0f;
 #pragma unroll
-                        for (int b = 0; b < NB; ++b) big = fmaxf(big, fabsf(vs[i][r][b]));
+                        for (int b = 0; b < NB; ++b) top_s = fmaxf(top_s, fabsf(vs[i][r][b]));
+#pragma unroll
+                        for (int j = 0; j < HL; ++j) big = fmaxf(big, pr[j][2 * i + r] * top_s);
                     }
                 if (!now) big = 0.0f;                             // nothing was copied
                 if (__any_sync(0xffffffffu, big > vlim)) {
-                    // A larger scale than fits: a new power of two that brings it to [1/2, 1).
+                    // A larger product of probability and scale than fits: a new
+                    // power of two that brings it to [2^13, 2^14).  An infinite
+                    // scale is its block's alone.
+                    big = 0.0f;
 #pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-                    const int e = min(max((int)((__float_as_uint(big) >> 23) & 255) - 126, -100), 126);
-                    const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-                    const float f = vinv == 0.0f ? 0.0f : inv / vinv;
-                    vinv = inv;
-                    vlim = 3.5f / inv;
+                    for (int i = 0; i < MT; ++i)
 #pragma unroll
-                    for (int i = 0; i < kMTiles; ++i)
+                        for (int r = 0; r < 2; ++r)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) acc[i][j] *= f;
+                            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                                for (int j = 0; j < HL; ++j) {
+                                    const float y = pr[j][2 * i + r] * fabsf(vs[i][r][b]);
+                                    if (y < INFINITY) big = fmaxf(big, y);
+                                }
+#pragma unroll
+                    for (int o = 16; o; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+                    if (big > vlim) {
+                        const int e = min(max((int)((__float_as_uint(big) >> 23) & 255) - 126, -100), 126);
+                        const float inv = __uint_as_float((uint32_t)(141 - e) << 23);
+                        const float f = vinv == 0.0f ? 0.0f : inv / vinv;
+                        vinv = inv;
+                        vlim = 57344.0f / inv;
+#pragma unroll
+                        for (int i = 0; i < kMTiles; ++i)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) acc[i][j] *= f;
+                    }
                 }
 #pragma unroll
                 for (int j = 0; j < HL; ++j)
@@ -1274,7 +1294,7 @@ cudaError_t attn_allow(K *kernel, size_t bytes, int device, std::atomic<unsigned
 
 template <int kCache, int HD, bool kWide, bool kExact>
 cudaError_t attn_launch(const AttnParams &p, cudaStream_t st) {
-    using Sh = AttnShape<kCache, HD>;
+    using Sh = AttnShape<kCache, HD, kWide>;
     constexpr size_t kBytes = AttnParts<kCache, kWide, kExact>::kSets * 8 * Sh::kQStride + kAttnWarps * Sh::R * Sh::kSlot;
     static std::atomic<unsigned long long> done{0};
     cudaError_t e = attn_allow(attend_kernel<kCache, HD, kWide, kExact>, kBytes, p.device, done);

@@ -743,3 +743,35 @@ def test_workspace_refusals(sp, dev_ctx):
         kv.workspace_bytes(1, 0)
     kv.attend(q, table, n, out, workspace=torch.zeros(need, dtype=torch.uint8, device="cuda"))
     dev_ctx.synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["q8_0", "q4_0", "f16", "bf16"])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_attend_values_beside_infinities(dev_ctx, dtype, kind):
+    """An infinite value, and one of 2^40 (2^15 in fp16) at a position whose
+    probability is zero, leave the other dims what they are."""
+    g = gen(14)
+    n, dim, page = 90, 128, 16
+    kv = make_cache(dev_ctx, dtype, page, 1, dim, 8)
+    table = make_table([n], page, 8, g)
+    q = torch.randn(1, 4, dim, device="cuda", generator=g).to(IO[kind])
+    k = torch.randn(n, 1, dim, device="cuda", generator=g)
+    v = torch.randn(n, 1, dim, device="cuda", generator=g)
+    k[50] = -1000 * q[0].float().sign().sum(0).sign()          # far below the others for every head
+    q = q.abs() * q.float().sign().sum(1, keepdim=True).sign().to(q.dtype)
+    v[50] *= 2.0 ** (12 if dtype == "f16" else 40)
+    v[20, 0, 3] = math.inf
+    kv.write(k, v, table, cu_tokens=ragged([n]))
+    out = torch.empty_like(q)
+    kv.attend(q, table, torch.tensor([n], dtype=torch.int32, device="cuda"), out)
+    dev_ctx.synchronize()
+    clean = v.clone()
+    clean[20, 0, 3] = 1.0
+    clean[50] = 0.0
+    kv.write(k, clean, table, cu_tokens=ragged([n]))
+    want, bound, _, _ = attend_plain(kv, q, table, [n], page, 1, dim, dtype)
+    hurt = slice(0, 32) if dtype[0] == "q" else slice(3, 4)
+    assert not torch.isfinite(out[..., hurt]).any()
+    keep = torch.ones(dim, dtype=torch.bool, device="cuda")
+    keep[hurt] = False
+    assert_within(out[..., keep], want[..., keep], bound[..., keep])
