@@ -100,6 +100,7 @@ extern "C" SAPPHIRE_API int sapphire_attention_device(kernel_context_t *ctx, con
     const long long items = (long long)a->sequences * cache->kv_heads * p.head_tiles;
     p.by_item = items <= p.blocks;
     p.joins = (int)std::min<long long>(items, p.blocks);
+    p.few_holders = p.blocks <= 16 * items;
     AttnDevice g(ctx->device);
     const size_t need = attn_workspace(ctx, cache, p.group);
     char *ws = static_cast<char *>(a->workspace);
