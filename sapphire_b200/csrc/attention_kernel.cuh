@@ -50,10 +50,11 @@
 #include "attention.cuh"
 
 constexpr int kAttnWarps = 4;
-constexpr int kAttnSmem = 224 * 1024;         // shared memory that an SM's blocks divide
+// Shared memory of one of an SM's `blocks` blocks (each costs 1 KB besides).
+constexpr int attn_smem(int blocks) { return 228 * 1024 / blocks - 1024; }
 constexpr float kLog2e = 1.4426950408889634f;
 
-// What an item costs besides its tiles (its query, the filling of the rings and
+// What an item costs besides its tiles (its query, the filling of the slots and
 // the joining of the warps), in tiles: the ranges of blocks are cut in these
 // units, so one that meets many short sequences takes fewer tiles.
 constexpr int kAttnItemUnits = 2;
@@ -94,10 +95,10 @@ constexpr int attn_m_tiles(int cache, int hd) {
     return cache == DTYPE_Q4_0 || cache == DTYPE_Q8_0 || (hd <= 64 && cache != DTYPE_F32) ? 2 : 1;
 }
 constexpr int attn_blocks_per_sm(int cache, int hd, bool wide) {
-    if (cache == DTYPE_F32) return hd <= 64 ? 3 : hd <= 128 ? 2 : 1;
+    if (cache == DTYPE_F32) return hd <= 64 ? 3 : 1;
     if (cache == DTYPE_Q4_0) return hd <= 64 ? 4 : hd <= 128 ? (wide ? 3 : 4) : 2;
     if (cache == DTYPE_Q8_0) return hd <= 64 ? 4 : hd <= 128 ? 3 : 2;
-    return hd <= 64 ? 4 : hd <= 128 ? 3 : 2;
+    return hd <= 128 ? 3 : 2;
 }
 
 #ifdef __CUDACC__
@@ -133,11 +134,13 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], uint32_t a0, uint32_t a1
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// The 11 leading bits of x, rounded.
-__device__ __forceinline__ uint32_t round_tf32(float x) {
-    uint32_t y;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(y) : "f"(x));
-    return y;
+// The 11 leading bits of x, rounded half away from zero (the bits of a value are
+// ordered like its magnitude): two cheap instructions where the conversion is
+// one of a quarter of their rate.
+__device__ __forceinline__ float take_tf32(float &x) {
+    const float hi = __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xffffe000u);
+    x -= hi;
+    return hi;
 }
 // d = a b + c on 32 unsigned bytes of a and signed bytes of b.
 __device__ __forceinline__ void mma8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -171,11 +174,6 @@ __device__ __forceinline__ float round16(float a) {
 template <bool kBf16>
 __device__ __forceinline__ float take16(float &x) {
     const float hi = round16<kBf16>(x);
-    x -= hi;
-    return hi;
-}
-__device__ __forceinline__ float take_tf32(float &x) {
-    const float hi = __uint_as_float(round_tf32(x));
     x -= hi;
     return hi;
 }
@@ -273,8 +271,8 @@ struct AttnShape {
     // Tokens of a warp's tile: two MMA tiles where rows are short.
     static constexpr int MT = attn_m_tiles(kCache, HD);
     static constexpr int kTok = 16 * MT;
-    // A slot of a warp's ring: the K or the V rows of a tile, each row padded
-    // off the banks of its neighbours, and their scales.
+    // A warp's two slots: the K and the V rows of a tile, each row padded off
+    // the banks of its neighbours, and their scales.
     static constexpr int kStride = kRowBytes + (kF32 ? 32 : 16);
     static constexpr int kScaleOff = kTok * kStride;
     static constexpr int kSlot = kScaleOff + kTok * kScaleBytes;
@@ -283,12 +281,9 @@ struct AttnShape {
     // lanes fall on the other half of the banks.
     static constexpr int kQElem = kF32 ? 4 : 2;
     static constexpr int kQStride = (HD * kQElem) % 128 == 0 ? HD * kQElem + 64 : HD * kQElem;
-    // Slots that fit beside the query's parts, of what an SM has for each block.
     static constexpr int kDigitStride = HD % 128 == 96 ? HD : HD + 32;        // of a row of query bytes
-    static constexpr int kMaxQS = kBf16 ? 3 : 2;
-    static constexpr int kFit = (kAttnSmem / kBlocks - kMaxQS * 8 * kQStride - 2048) / (kAttnWarps * kSlot);
-    static constexpr int R = kFit > 6 ? 6 : kFit;
-    static_assert(R >= 2, "a ring of K and V rows does not fit");
+    static constexpr int kMaxSets = (kWide ? 2 : 1) + (kBf16 ? 1 : 0);
+    static_assert(kMaxSets * 8 * kQStride + 2 * kAttnWarps * kSlot + 2048 <= attn_smem(kBlocks), "the rows do not fit");
 };
 
 #ifdef __CUDACC__
@@ -330,16 +325,16 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
     using Sh = AttnShape<kCache, HD, kWide>;
     using Pt = AttnParts<kCache, kWide, kExact>;
     constexpr int GH = kWide ? 8 : 4, HL = kWide ? 2 : 1;         // heads of a tile, and of a lane
-    constexpr int NB = Sh::NB, MT = Sh::MT, R = Sh::R, kTok = Sh::kTok, kTile = kTok * kAttnWarps, kMTiles = HD / 16;
+    constexpr int NB = Sh::NB, MT = Sh::MT, kTok = Sh::kTok, kTile = kTok * kAttnWarps, kMTiles = HD / 16;
     constexpr int kQS = Pt::kQS, kPS = Pt::kPS;
     constexpr bool kInt = kAttnInt<kCache, kExact>;
     constexpr bool kBf16 = Sh::kBf16, kF32 = Sh::kF32;
     constexpr float kBias = kAttnBias<kCache>;
     extern __shared__ __align__(16) uint8_t shared[];
     uint8_t *const sq = shared;                                   // the query's parts
-    uint8_t *const rings = shared + Pt::kSets * 8 * Sh::kQStride;  // [warp][R] slots; at the end of an item the
-    float *const sacc = reinterpret_cast<float *>(rings);         // warps' outputs [warp][head][dim]
-    static_assert(R * Sh::kSlot >= GH * HD * 4, "the warps' outputs do not fit the rings");
+    uint8_t *const slots = shared + Pt::kSets * 8 * Sh::kQStride;  // [warp][2]; at the end of an item the warps'
+    float *const sacc = reinterpret_cast<float *>(slots);         // outputs [warp][head][dim]
+    static_assert(2 * Sh::kSlot >= GH * HD * 4, "the warps' outputs do not fit the slots");
     __shared__ float sm_m[kAttnWarps][GH], sm_l[kAttnWarps][GH];
     __shared__ float qmul[GH];
     __shared__ unsigned warp_sum[kAttnWarps];
@@ -490,9 +485,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
             load_tok += kTile;
         };
 
-        // ---- K or V rows of a tile into slot `at` of the warp's ring ----
-        uint8_t *const ring = rings + warp * R * Sh::kSlot;
-        const uint32_t ring_at = smem_addr(ring);
+        // ---- K or V rows of a tile into the warp's slots ----
+        const uint8_t *const k_slot = slots + warp * 2 * Sh::kSlot, *const v_slot = k_slot + Sh::kSlot;
+        const uint32_t slots_at = smem_addr(k_slot);
         const uint8_t *const k_rows = head + lane * 16, *const v_rows = k_rows + p.l.v_off;
         const uint8_t *const k_scales = head + p.l.ks_off + lane * kPiece, *const v_scales = k_scales + (p.l.vs_off - p.l.ks_off);
         // Piece 32 j + lane of the rows: its row, its place in the slot, and its
@@ -502,8 +497,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
             const int col = 32 % PR == 0 ? lane % PR : PR % 32 == 0 ? 32 * (j % (PR / 32 > 0 ? PR / 32 : 1)) + lane : (32 * j + lane) % PR;
             return row_of(j) * Sh::kStride + col * 16;
         };
-        auto copy_rows = [&](int at, bool is_v) {
-            const uint32_t dst = ring_at + at * Sh::kSlot, sdst = dst + Sh::kScaleOff + lane * kPiece;
+        auto copy_rows = [&](bool is_v) {
+            const uint32_t dst = slots_at + (is_v ? Sh::kSlot : 0), sdst = dst + Sh::kScaleOff + lane * kPiece;
             if (!valid) {
                 // nothing of this tile counts
             } else if (aligned) {
@@ -547,9 +542,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
             copies_commit();
         };
 
-        // ---- the query's values, and the ring's first copies ----
-        constexpr int kAhead = (R + 1) / 2;                       // tiles whose copies a full ring holds
-        unsigned counts[kAhead];                                  // tokens that count, of the tiles copied
+        // ---- the first tile's rows, and the query's values ----
         fetch();
         constexpr int kPerWarp = GH / kAttnWarps;
         float x[kPerWarp][NB];
@@ -564,15 +557,11 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                           : p.io == DTYPE_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(p.q)[off + 32 * b])
                                                : __half2float(static_cast<const __half *>(p.q)[off + 32 * b]);
         }
-        __syncthreads();                                          // the last item's readers of the rings
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-            if (i % 2 == 0) {
-                resolve();
-                counts[i / 2] = valid;
-            }
-            copy_rows(i, i % 2 == 1);
-        }
+        __syncthreads();                                          // the last item's readers of the slots
+        resolve();
+        unsigned next_counts = valid;                             // tokens of the next tile that count
+        copy_rows(false);
+        copy_rows(true);
 #pragma unroll
         for (int k = 0; k < kPerWarp; ++k) {
             const int j = warp + k * kAttnWarps;
@@ -661,27 +650,15 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
 #pragma unroll
             for (int j = 0; j < 4; ++j) to[j] += c[j];
         };
-        int at = 0;                                               // the ring's oldest slot
-        auto advance = [&](bool after_v) {
-            // The slot's rows are used: copy the half tile R behind into it.
-            __syncwarp();
-            if ((R & 1) == (after_v ? 1 : 0)) {
-                // its K rows: a tile not yet looked at
-                resolve();
-                counts[kAhead - 1] = valid;
-                copy_rows(at, false);
-            } else {
-                copy_rows(at, true);
-            }
-            at = at + 1 == R ? 0 : at + 1;
-        };
+        // While V's rows are used the next K's are on their way, and the other
+        // way round.  More slots measured worse at every type and size (64 x 8192
+        // over Q8_0: 210 us with two, 217 with three; over bf16 352 and 355): the
+        // memory serves fewer streams faster.
         for (int tile = tile_first; tile < tile_end; ++tile) {
-            copies_wait<R - 1>();
+            copies_wait<1>();
             __syncwarp();
-            const uint8_t *slot = ring + at * Sh::kSlot;
-            const unsigned now = counts[0];
-#pragma unroll
-            for (int i = 0; i + 1 < kAhead; ++i) counts[i] = counts[i + 1];
+            const uint8_t *slot = k_slot;
+            const unsigned now = next_counts;
             // ---- scores: lane (g, t) has tokens 16 i + g, + 8 of its heads ----
             float s[HL][2 * MT];
             if constexpr (Sh::kQuant) {
@@ -808,8 +785,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                                 float x0 = __uint_as_float(u[j]), x1 = __uint_as_float(v[j]);
                                 uh[j] = __float_as_uint(take_tf32(x0));
                                 vh[j] = __float_as_uint(take_tf32(x1));
-                                ul[j] = round_tf32(x0);
-                                vl[j] = round_tf32(x1);
+                                ul[j] = __float_as_uint(x0);
+                                vl[j] = __float_as_uint(x1);
                             }
                         }
 #pragma unroll
@@ -839,7 +816,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                         }
                     }
             }
-            advance(false);
+            __syncwarp();
+            resolve();
+            next_counts = valid;
+            copy_rows(false);
             // ---- probabilities ----
             float pr[HL][2 * MT], top[HL];
             bool grew = false;
@@ -911,9 +891,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                 }
             };
             // ---- acc += V^T P^T ----
-            copies_wait<R - 1>();
+            copies_wait<1>();
             __syncwarp();
-            slot = ring + at * Sh::kSlot;
+            slot = v_slot;
             if constexpr (Sh::kQuant) {
                 constexpr int kBytes = Sh::kRowBytes / 8, kW = (kBytes + 3) / 4;  // of a row in this lane
                 float vs[MT][2][NB], big = 0.0f;
@@ -1025,7 +1005,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
 #pragma unroll
                     for (int set = 0; set < kPS; ++set) {
                         const float u = take_tf32(y[0]);
-                        const float v = kWide ? take_tf32(y[HL - 1]) : __uint_as_float(round_tf32(y[0]));
+                        const float v = kWide ? take_tf32(y[HL - 1]) : y[0];
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
                             const int src = (t + 4 * k) * 4 + (g >> 1);
@@ -1050,7 +1030,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                                 for (int k = 0; k < 4; ++k) {
                                     float y = __uint_as_float(x[2 * r + (k >> 1)][2 * j + (k & 1)]);
                                     h[k] = __float_as_uint(take_tf32(y));
-                                    lw[k] = round_tf32(y);
+                                    lw[k] = __float_as_uint(y);
                                 }
 #pragma unroll
                                 for (int set = 0; set < kPS; ++set) {
@@ -1105,7 +1085,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                     }
                 }
             }
-            advance(true);
+            __syncwarp();
+            copy_rows(true);
         }
         copies_wait<0>();
 
@@ -1296,7 +1277,7 @@ cudaError_t attn_allow(K *kernel, size_t bytes, int device, std::atomic<unsigned
 template <int kCache, int HD, bool kWide, bool kExact>
 cudaError_t attn_launch(const AttnParams &p, cudaStream_t st) {
     using Sh = AttnShape<kCache, HD, kWide>;
-    constexpr size_t kBytes = AttnParts<kCache, kWide, kExact>::kSets * 8 * Sh::kQStride + kAttnWarps * Sh::R * Sh::kSlot;
+    constexpr size_t kBytes = AttnParts<kCache, kWide, kExact>::kSets * 8 * Sh::kQStride + 2 * kAttnWarps * Sh::kSlot;
     static std::atomic<unsigned long long> done{0};
     cudaError_t e = attn_allow(attend_kernel<kCache, HD, kWide, kExact>, kBytes, p.device, done);
     if (e != cudaSuccess) return e;
