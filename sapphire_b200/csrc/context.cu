@@ -594,7 +594,19 @@ extern "C" SAPPHIRE_API int kernel_ctx_set_stream(kernel_context_t *ctx, void *s
     if (!ctx) return -1;
     std::lock_guard<std::recursive_mutex> lk(ctx->exec_mutex);
     DeviceGuard g(ctx->device);
-    if (ctx->stream) cudaStreamSynchronize(ctx->stream);
+    // What the old stream still runs may use the context's buffers, so it is
+    // waited for, the NULL stream too - unless it is being captured: a wait
+    // would end the capture, and nothing of it runs yet.  (Relaxed, because the
+    // wait is harmless to a capture on another stream.)
+    if (ctx->initialized) {
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(ctx->stream, &capturing) == cudaSuccess && capturing == cudaStreamCaptureStatusNone)
+            cudaStreamSynchronize(ctx->stream);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        cudaGetLastError();
+    }
     if (ctx->own_stream && ctx->stream) cudaStreamDestroy(ctx->stream);
     ctx->stream = (cudaStream_t)stream;
     ctx->own_stream = false;
