@@ -154,7 +154,14 @@ SAPPHIRE_API int sapphire_kv_read_device(kernel_context_t *ctx, const sapphire_k
  * tokens in the cache (its new one among them) and attends to positions
  * max(0, n - window) .. n - 1 (window 0: all).  Query head h uses KV head
  * h / (heads / kv_heads).  out = sum_t softmax(scale q . k_t) v_t; a sequence
- * with no position to attend to gets zeros, and -inf in lse.
+ * with no position to attend to gets zeros, and -inf in lse.  What lies in
+ * slots that are not attended to (NaN included) has no effect.  A NaN or an
+ * infinity that is attended to makes the outputs it enters NaN or infinite
+ * (an infinity may come out as NaN) and no others.  A length below 0 counts as
+ * 0, one beyond the table as the table's end, and a token on a page outside the
+ * cache does not count; each is an error at the next kernel_ctx_synchronize.
+ * The order of the sums depends on the lengths and the GPU alone: the same call
+ * gives the same bits.
  * ------------------------------------------------------------------------- */
 typedef struct {
     tensor_dtype_t dtype;    /* F32, BF16 or F16, of q and out */

@@ -90,7 +90,11 @@ extern "C" SAPPHIRE_API int sapphire_attention_device(kernel_context_t *ctx, con
     p.group = a->heads / cache->kv_heads;
     p.head_tiles = (p.group + attn_tile_heads(p.group) - 1) / attn_tile_heads(p.group);
     p.page_mul = (1ull << 32) / cache->page_size + 1;
+    // Side by side: as many head tiles as divide their number evenly, up to 8.
     p.blocks = attn_blocks(ctx, cache, p.group);
+    p.sides = std::min(std::min(p.head_tiles, 8), p.blocks);
+    while (p.head_tiles % p.sides) --p.sides;
+    p.blocks -= p.blocks % p.sides;
     p.code[0] = 0x64006400u;
     p.code[1] = cache->dtype == DTYPE_Q8_0 ? 0x64806480u : 0x64086408u;
     p.code[2] = 0x2c002c00u;

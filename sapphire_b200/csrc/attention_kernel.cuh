@@ -7,9 +7,15 @@
 // of a sequence join by weights 2^(m_piece - m).
 //
 // What bounds it: every visible K and V row is read once from HBM, so the work
-// is laid out to stream rows and to keep everything else off that path.
+// is laid out to stream rows and to keep everything else off that path.  64
+// sequences of 8192, 8 KV heads of 128, 4 query heads each (of 6554 GB/s): bf16
+// 348 us, 0.94; Q8_0 202 us, 0.91; F32 364 us at 32 sequences, 0.90.  Q4_0
+// 147 us, 0.70, and 2 x 131071 with 5 query heads 90 us, 0.57, are bound by
+// instructions: schedulers issue in 0.6 of the cycles, a third of them ALU, and
+// unpacking is the most.  Short calls are latency: one fp32 sequence of 577
+// takes 11 us, a block's chain of lengths, page table, rows and joining.
 //
-// Layout.  A warp takes 16 tokens at a time.  Scores are S^T = K Q^T and
+// Layout.  A warp takes 16 tokens at a time, or 32 where rows are short.  Scores are S^T = K Q^T and
 // outputs O^T = V^T P^T with warp MMAs whose M side is the tile (16 tokens, or
 // 16 dims) and whose N = 8 columns are query heads.  A 16-bit MMA gives fp32
 // products of more bits from parts of the query and of the probability (high,
@@ -21,14 +27,14 @@
 //     where it is exact (a bf16 query) or its rounding is far below the
 //     output's (an fp16 probability under a bf16 output: 2^-12 against 2^-9).
 // A tcgen05 tile would leave 120 of its 128 rows empty here; the MMAs below are
-// a few percent of the pass.  K and V fragments go from global memory straight
-// to registers as 16-byte loads: the order of dims inside an MMA is free as
-// long as both operands share it, so a lane's consecutive bytes of a row are
-// its fragment.
+// a few percent of the pass.  Rows come by asynchronous copies into two slots of
+// a warp, K's and V's, while the other's is used, and a lane reads its fragments
+// as vectors: the order of dims inside an MMA is free as long as both operands
+// share it, so a lane's consecutive bytes of a row are its fragment.
 //
-//   K (A operand): lane (g, t) = (lane / 4, lane % 4) loads rows g and g + 8,
+//   K (A operand): lane (g, t) = (lane / 4, lane % 4) reads rows g and g + 8,
 //     dims 8t .. 8t + 7 of each 32.
-//   V (A operand, transposed): lane (g, t) loads tokens 2t, 2t + 1, 2t + 8,
+//   V (A operand, transposed): lane (g, t) reads tokens 2t, 2t + 1, 2t + 8,
 //     2t + 9, dims 8g .. 8g + 7 of each 64, and pairs tokens with byte permutes.
 //   P (B operand): a movmatrix of the packed (high, low) pairs.
 //
@@ -43,7 +49,7 @@
 //
 // Split.  The tiles (64 tokens of one KV head and up to 8 query heads) of all
 // sequences are numbered in a row and cut into as many equal ranges as the GPU
-// holds blocks, whatever the lengths; a block's pieces that do not hold a whole
+// holds blocks (of one side, below), whatever the lengths; a block's pieces that do not hold a whole
 // sequence go to the workspace and attend_join_kernel adds them up.
 #pragma once
 
@@ -68,7 +74,8 @@ struct AttnParams {
     const int *page_table, *lengths;
     int io;                        // tensor_dtype_t of q and out
     int sequences, heads, group;   // group: query heads of a KV head
-    int head_tiles;                // tiles of 4 NT query heads of a group
+    int head_tiles;                // tiles of 4 or 8 query heads of a group
+    int sides;                     // head tiles that neighbouring blocks work on side by side
     int table_stride, length_offset, window;
     float scale;                   // scores times log2 e
     unsigned long long page_mul;   // floor(2^32 / page_size) + 1
@@ -91,6 +98,10 @@ struct AttnParams {
 inline bool attn_wide(int group) { return group > 4; }
 inline int attn_tile_heads(int group) { return attn_wide(group) ? 8 : 4; }
 // MMA tiles (16 tokens) of a warp's tile, and resident blocks per SM.
+// (MMA tiles: two of short rows share a tile's overhead.  Blocks: as many as
+// registers and shared memory allow, but rows of 512 bytes and more are served
+// faster to one block: 32 x 8192 over F32 at 128 dims 391 us with two, 364 with
+// one.)
 constexpr int attn_m_tiles(int cache, int hd) {
     return cache == DTYPE_Q4_0 || cache == DTYPE_Q8_0 || (hd <= 64 && cache != DTYPE_F32) ? 2 : 1;
 }
@@ -349,7 +360,13 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
     //      checked on the host) ----
     const int per_thread = (p.sequences + kAttnWarps * 32 - 1) / (kAttnWarps * 32);
     const int s0 = min(tid * per_thread, p.sequences), s1 = min(s0 + per_thread, p.sequences);
-    const int rows = p.l.kv_heads * p.head_tiles;                 // items of a sequence
+    // Blocks are dealt to the sides in turn: those of one rank walk the same
+    // tokens for head tiles of their own, so a row comes from HBM once and from
+    // L2 for the others (64 x 8192, 16 query heads to a KV head of 128: bf16
+    // 687 -> 454 us, Q8_0 402 -> 363 us against one tile behind another).
+    // An item: a KV head and one of this side's head tiles.
+    const int side = blockIdx.x % p.sides, side_tiles = p.head_tiles / p.sides, side_blocks = p.blocks / p.sides;
+    const int rows = p.l.kv_heads * side_tiles;                   // items of a sequence
     unsigned mine = 0;
     for (int s = s0; s < s1; ++s) mine += attn_span<kTile>(p, s, blockIdx.x == 0).units;
     unsigned incl = mine;
@@ -368,9 +385,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
     }
     base *= rows;
     total *= rows;
-    const unsigned blocks = min((unsigned)p.blocks, total), bid = blockIdx.x;
+    const unsigned blocks = min((unsigned)side_blocks, total), bid = blockIdx.x / p.sides, slot0 = side * side_blocks;
     if (bid >= blocks) {
-        if (tid == 0 && !p.by_item) p.piece[bid] = make_int4(0, 0, 0, 0);
+        if (tid == 0 && !p.by_item) p.piece[slot0 + bid] = make_int4(0, 0, 0, 0);
         return;
     }
     // The first `longer` blocks take each + 1 units, the others each.
@@ -401,13 +418,13 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
             ++seq;
             continue;
         }
-        const int item = (int)((pos - seq_base) / (unsigned)sp.units);        // (KV head, head tile)
+        const int item = (int)((pos - seq_base) / (unsigned)sp.units);
         // The item's tiles are its last units; this block takes those in its range.
         const unsigned tile_unit = seq_base + (unsigned)(item * sp.units) + kAttnItemUnits;
         const unsigned end = min(hi, tile_unit + sp.tiles);
         if (end <= tile_unit) break;                              // the next block has its first tile
         const int piece0 = pos > tile_unit ? (int)(pos - tile_unit) : 0, piece1 = (int)(end - tile_unit);
-        const int kh = item / p.head_tiles, ht = item - kh * p.head_tiles;
+        const int kh = item / side_tiles, ht = (item - kh * side_tiles) * p.sides + side;
         const int nh = min(GH, p.group - ht * GH);                // heads of this tile
         const int head0 = kh * p.group + ht * GH;
         const uint8_t *head = p.l.pages + (unsigned long long)kh * p.l.chunk_bytes;
@@ -1130,7 +1147,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
             }
         }
         const bool whole = piece0 == 0 && piece1 == sp.tiles;
-        float *part = p.part + (size_t)(2 * bid + (piece0 == 0 ? 1 : 0)) * GH * (HD + 2);
+        float *part = p.part + (size_t)(2 * (slot0 + bid) + (piece0 == 0 ? 1 : 0)) * GH * (HD + 2);
         if (warp == 0 && g == 0) {
 #pragma unroll
             for (int j = 0; j < HL; ++j) {
@@ -1168,18 +1185,20 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                 // The blocks of this item: this one and all up to the one that holds its last tile.
                 const unsigned x = tile_unit + sp.tiles - 1, split = longer * (each + 1);
                 const unsigned last = x < split ? x / (each + 1) : longer + (x - split) / each;
-                mine_holds = make_int4(seq, item, (int)(last - bid) + 1, (int)bid);
+                mine_holds = make_int4(seq, kh * p.head_tiles + ht, (int)(last - bid) + 1, (int)(slot0 + bid));
                 piece = mine_holds;
             }
-            if (p.by_item && tid == 0) p.piece[seq * rows + item] = mine_holds;
+            if (p.by_item && tid == 0) p.piece[(seq * p.l.kv_heads + kh) * p.head_tiles + ht] = mine_holds;
         }
         pos = end;
     }
-    if (tid == 0 && !p.by_item) p.piece[bid] = piece;
+    if (tid == 0 && !p.by_item) p.piece[slot0 + bid] = piece;
 }
 
 // Adds up the items that several blocks hold: one block per item and query
-// head.  Its warps take turns at the holders, kJoinBatch of them in flight
+// head.  Latency bound (4 us); it does not let the next kernel start early,
+// whose blocks would take the SMs before it is done (2 x 131071 over Q4_0 called
+// again and again: 93 -> 112 us).  Its warps take turns at the holders, kJoinBatch of them in flight
 // (maxima, sums and values together), and are joined like the blocks' warps.
 template <int HD, int kJoinWarps, int kJoinBatch>
 __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const AttnParams p, int tile_heads, float bias) {

@@ -8,7 +8,8 @@
 // F_i mod 2^64 is the phase, reduced exactly by the overflow of an integer
 // product, good to 2^-32 of a turn at any 32-bit position, and sincospi takes
 // the reduced half turns.  No table is read, so a call moves its heads once in
-// and once out.
+// and once out, and is bound by that: 16381 tokens x 40 bf16 heads of 128 take
+// 58 us, 5.8 TB/s.  Single tokens cost a launch.
 #include <cmath>
 #include <cstring>
 
@@ -347,7 +348,7 @@ extern "C" SAPPHIRE_API int sapphire_rope_device(sapphire_rope_t *rope, const sa
     // tokens (four batches of them) and heads, so a block's cos and sin serve
     // every head.  Where that gives an SM fewer than eight blocks, a row takes
     // fewer tokens, then a block fewer heads, computing its own turns (1507
-    // tokens x 96 heads of 256: 47 us with whole blocks, 27 us so).
+    // tokens x 96 heads of 256: 47 us with whole blocks, 31 us so).
     AttnDevice g(ctx->device);
     const int batch = rope_batch(inter);
     auto cut = [](int n, int most) { return (n + (n + most - 1) / most - 1) / ((n + most - 1) / most); };

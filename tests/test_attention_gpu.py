@@ -502,6 +502,14 @@ def test_attend_groups(dev_ctx, dtype, group):
     check_attend(dev_ctx, dtype, "bf16", [130, 7], 2, group, 128, 16, seed=group)
 
 
+@pytest.mark.parametrize("group", [12, 24, 40, 72, 88])
+def test_attend_head_tiles_side_by_side(dev_ctx, group):
+    """2, 3, 5, 9 and 11 tiles of 8 heads: on sides of their own, three of three, or one behind another; few
+    sequences (ranges in the middle of them) and many (items of one block each)."""
+    check_attend(dev_ctx, "q8_0", "bf16", [5003, 0, 1], 2, group, 64, 16, seed=group)
+    check_attend(dev_ctx, "bf16", "f32", [5 * i % 211 for i in range(160)], 2, group, 64, 8, seed=group)
+
+
 @pytest.mark.parametrize("dtype", CACHES)
 def test_attend_long_and_many(dev_ctx, dtype):
     check_attend(dev_ctx, dtype, "f32", [20011], 1, 4, 64, 64, seed=1)
@@ -728,6 +736,39 @@ def test_captured_calls_keep_workspaces_of_their_own(sp, dev_ctx):
         for kv, table, q, n, out, ws in sets:
             want, bound, _, _ = attend_plain(kv, q, table, lengths, 16, 2, 128, "q8_0")
             assert_within(out, want, bound)
+
+
+def test_changing_streams(sp, dev_ctx):
+    """A call on the default stream, the next on another at once (both in the
+    context's workspace), and a change of streams while one is captured."""
+    dev_ctx.set_stream(0)
+    kv, table, q = attend_case(dev_ctx, "q8_0", "f32", [9000, 4000, 40], 8, 4, 128, 16, seed=60)
+    n = torch.tensor([9000, 4000, 40], dtype=torch.int32, device="cuda")
+    outs = [torch.empty_like(q) for _ in range(4)]
+    torch.cuda.synchronize()
+    st = torch.cuda.Stream()
+    for _ in range(5):
+        dev_ctx.set_stream(0)
+        for _ in range(4):
+            kv.attend(q, table, n, outs[0])
+        dev_ctx.set_stream(st.cuda_stream)
+        kv.attend(q[:1], table[:1], n[:1], outs[1][:1])
+    dev_ctx.set_stream(0)
+    ws = torch.empty(kv.workspace_bytes(3, 32), dtype=torch.uint8, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=st):
+        dev_ctx.set_stream(st.cuda_stream)
+        kv.attend(q, table, n, outs[2], workspace=ws)
+        dev_ctx.set_stream(0)
+    kv.attend(q, table, n, outs[3])
+    graph.replay()
+    torch.cuda.synchronize()
+    dev_ctx.synchronize()
+    want, bound, _, _ = attend_plain(kv, q, table, [9000, 4000, 40], 16, 8, 128, "q8_0")
+    for i, o in enumerate(outs):
+        rows = 1 if i == 1 else 3
+        assert_within(o[:rows], want[:rows], bound[:rows] if torch.is_tensor(bound) else bound, str(i))
 
 
 def test_workspace_refusals(sp, dev_ctx):
