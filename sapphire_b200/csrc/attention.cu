@@ -1,6 +1,7 @@
 // attention.cu - attention of one new token of every sequence over its pages
 // (include/sapphire_attention.h): arguments, workspace and choice of kernel.
 // The kernels and what bounds them are in attention_kernel.cuh.
+#include <climits>
 #include <cmath>
 #include <cstring>
 
@@ -95,6 +96,7 @@ extern "C" SAPPHIRE_API int sapphire_attention_device(kernel_context_t *ctx, con
     p.sides = std::min(std::min(p.head_tiles, 8), p.blocks);
     while (p.head_tiles % p.sides) --p.sides;
     p.blocks -= p.blocks % p.sides;
+    p.side_tiles = p.head_tiles / p.sides;
     p.code[0] = 0x64006400u;
     p.code[1] = cache->dtype == DTYPE_Q8_0 ? 0x64806480u : 0x64086408u;
     p.code[2] = 0x2c002c00u;
@@ -104,7 +106,11 @@ extern "C" SAPPHIRE_API int sapphire_attention_device(kernel_context_t *ctx, con
     const long long items = (long long)a->sequences * cache->kv_heads * p.head_tiles;
     p.by_item = items <= p.blocks;
     p.joins = (int)std::min<long long>(items, p.blocks);
-    p.few_holders = p.blocks <= 16 * items;
+    // Blocks to an item: on average, and at most one for each tile that the table
+    // or the window leaves it.
+    const int tile = 16 * kAttnWarps * attn_m_tiles(cache->dtype, cache->head_dim);
+    const long long room = std::min((long long)a->table_stride * cache->page_size, a->window ? (long long)a->window + tile : INT_MAX);
+    p.few_holders = p.blocks <= 16 * items || (room + tile - 1) / tile <= 16;
     AttnDevice g(ctx->device);
     const size_t need = attn_workspace(ctx, cache, p.group);
     char *ws = static_cast<char *>(a->workspace);
@@ -121,8 +127,12 @@ extern "C" SAPPHIRE_API int sapphire_attention_device(kernel_context_t *ctx, con
             ctx_fail(ctx, who, "a captured call needs a workspace of its own");
             return -1;
         }
-        if (ensure_scratch(ctx, &ctx->d_attn, &ctx->d_attn_cap, need)) return -1;
-        ws = reinterpret_cast<char *>(ctx->d_attn);
+        // The context's own begins with zeroed counters: with few blocks to an item
+        // the last of them joins their pieces, which saves a launch.
+        const size_t counts = ((size_t)sm_count(ctx->device) * kAttnMaxBlocks * sizeof(int) + 15) & ~(size_t)15;
+        if (ensure_scratch(ctx, &ctx->d_attn, &ctx->d_attn_cap, counts + need)) return -1;
+        ws = reinterpret_cast<char *>(ctx->d_attn) + counts;
+        if (p.few_holders) p.count = reinterpret_cast<int *>(ctx->d_attn);
     }
     p.piece = reinterpret_cast<int4 *>(ws);
     p.part = reinterpret_cast<float *>(ws + (size_t)p.blocks * sizeof(int4));

@@ -9,11 +9,13 @@
 // What bounds it: every visible K and V row is read once from HBM, so the work
 // is laid out to stream rows and to keep everything else off that path.  64
 // sequences of 8192, 8 KV heads of 128, 4 query heads each (of 6554 GB/s): bf16
-// 348 us, 0.94; Q8_0 202 us, 0.91; F32 364 us at 32 sequences, 0.90.  Q4_0
-// 147 us, 0.70, and 2 x 131071 with 5 query heads 90 us, 0.57, are bound by
+// 348 us, 0.94; Q8_0 204 us, 0.90; F32 364 us at 32 sequences, 0.90.  Q4_0
+// 147 us, 0.70, and 2 x 131071 with 5 query heads 87 us, 0.59, are bound by
 // instructions: schedulers issue in 0.6 of the cycles, a third of them ALU, and
 // unpacking is the most.  Short calls are latency: one fp32 sequence of 577
-// takes 11 us, a block's chain of lengths, page table, rows and joining.
+// takes 11 us, a block's chain of lengths, page table, rows and joining (20 k
+// cycles: 2.5 k to its first item, 5 k to its first rows, 4 k for a tile, 8 k for
+// the joins of its warps and of the blocks).
 //
 // Layout.  A warp takes 16 tokens at a time, or 32 where rows are short.  Scores are S^T = K Q^T and
 // outputs O^T = V^T P^T with warp MMAs whose M side is the tile (16 tokens, or
@@ -44,13 +46,17 @@
 // fp16's range by a power of two per warp that follows the largest seen.  K's codes become
 // fp16 the same way under fp32 and fp16 outputs; under a bf16 output they are
 // multiplied as the integers they are by the query as 15-bit integers (two
-// signed bytes), the sums exact and started at what the codes' offset adds, and
-// one conversion and product with K's scale brings a block's sum to fp32.
+// signed bytes), the sums exact, and one conversion and product with K's scale
+// brings a block's sum to fp32.  Q8_0's sums start at what the codes' offset
+// adds; a Q4_0 code in the high half of a byte, its top bit turned, is 16 (code -
+// 8) as it is.
 //
 // Split.  The tiles (64 tokens of one KV head and up to 8 query heads) of all
 // sequences are numbered in a row and cut into as many equal ranges as the GPU
-// holds blocks (of one side, below), whatever the lengths; a block's pieces that do not hold a whole
-// sequence go to the workspace and attend_join_kernel adds them up.
+// holds blocks (of one side, below), whatever the lengths; a block's pieces that
+// do not hold a whole sequence go to the workspace.  The last of an item's blocks
+// adds them up in their order, or, where an item may have many blocks or the
+// workspace is the caller's (no zeroed counters), attend_join_kernel does.
 #pragma once
 
 #include "attention.cuh"
@@ -64,6 +70,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // the joining of the warps), in tiles: the ranges of blocks are cut in these
 // units, so one that meets many short sequences takes fewer tiles.
 constexpr int kAttnItemUnits = 2;
+constexpr int kAttnMaxBlocks = 4;         // on an SM, of any variant
 
 struct AttnParams {
     KvLayout l;
@@ -75,7 +82,7 @@ struct AttnParams {
     int io;                        // tensor_dtype_t of q and out
     int sequences, heads, group;   // group: query heads of a KV head
     int head_tiles;                // tiles of 4 or 8 query heads of a group
-    int sides;                     // head tiles that neighbouring blocks work on side by side
+    int sides, side_tiles;         // head tiles that blocks work on side by side, and one behind another
     int table_stride, length_offset, window;
     float scale;                   // scores times log2 e
     unsigned long long page_mul;   // floor(2^32 / page_size) + 1
@@ -89,7 +96,8 @@ struct AttnParams {
     int4 *piece;
     bool by_item;
     int joins;                     // entries of piece
-    bool few_holders;              // at most 16 blocks to an item, on average
+    bool few_holders;              // at most 16 blocks to an item, on average or at all
+    int *count;                    // [blocks] zeros (and zeros again behind the call), or nullptr: attend_join_kernel joins
     int *err;
     unsigned code[4];              // CodeConst, where the compiler does not see constants
 };
@@ -153,12 +161,18 @@ __device__ __forceinline__ float take_tf32(float &x) {
     x -= hi;
     return hi;
 }
-// d = a b + c on 32 unsigned bytes of a and signed bytes of b.
+// d = a b + c on 32 bytes of a (signed or not) and signed bytes of b.
+template <bool kSigned>
 __device__ __forceinline__ void mma8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                      uint32_t b1, int c0, int c1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
-                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c0), "r"(c1));
+    if (kSigned)
+        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+                     : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c0), "r"(c1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+                     : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c0), "r"(c1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
@@ -288,6 +302,7 @@ struct AttnShape {
     static constexpr int kScaleOff = kTok * kStride;
     static constexpr int kSlot = kScaleOff + kTok * kScaleBytes;
     static constexpr int kBlocks = attn_blocks_per_sm(kCache, HD, kWide);
+    static_assert(kBlocks <= kAttnMaxBlocks, "");
     // Query parts: rows of 8 columns, padded so that the rows of neighbouring
     // lanes fall on the other half of the banks.
     static constexpr int kQElem = kF32 ? 4 : 2;
@@ -331,6 +346,54 @@ struct AttnParts {
     static constexpr int kPS = !kWide ? kQS : kCache == DTYPE_F32 ? 2 : kCache == DTYPE_BF16 ? (kExact ? 3 : 2) : kExact ? 2 : 1;
 };
 
+// Adds holders i0, i0 + step, ... below n of head h's item to M, L and o,
+// kBatch of them in flight.  part: the first one's partial; the others' follow
+// as the first slots of the next blocks.
+template <int HD, int kBatch>
+__device__ __forceinline__ void attn_add_holders(const float *part, size_t stride, int tile_heads, int h, int i0, int step,
+                                                 int n, float &M, float &L, float (&o)[HD / 32]) {
+    constexpr int kVals = HD / 32;
+    const int lane = threadIdx.x & 31;
+    for (; i0 < n; i0 += step * kBatch) {
+        float m[kBatch], l[kBatch], x[kBatch][kVals], top = M;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const int i = i0 + k * step;
+            m[k] = -INFINITY;
+            l[k] = 0.0f;
+            if (i >= n) {
+#pragma unroll
+                for (int j = 0; j < kVals; ++j) x[k][j] = 0.0f;
+                continue;
+            }
+            const float *from = part + (i ? 2 * i - 1 : 0) * stride;
+            m[k] = __ldcg(from + h);
+            l[k] = __ldcg(from + tile_heads + h);
+#pragma unroll
+            for (int j = 0; j < kVals; ++j) x[k][j] = __ldcg(from + 2 * tile_heads + h * HD + 32 * j + lane);
+        }
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) top = fmaxf(top, m[k]);
+        const float ref = top == -INFINITY ? 0.0f : top, keep = attn_exp2(M - ref);
+        M = top;
+        L *= keep;
+#pragma unroll
+        for (int j = 0; j < kVals; ++j) o[j] *= keep;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const float w = l[k] != l[k] ? l[k] : attn_exp2(m[k] - ref);      // a NaN's maximum says nothing
+            L = fmaf(w, l[k], L);
+#pragma unroll
+            for (int j = 0; j < kVals; ++j) o[j] = fmaf(w, x[k][j], o[j]);
+        }
+    }
+}
+__device__ __forceinline__ void attn_store(const AttnParams &p, long long at, float y) {
+    if (p.io == DTYPE_F32) static_cast<float *>(p.out)[at] = y;
+    else if (p.io == DTYPE_BF16) static_cast<__nv_bfloat16 *>(p.out)[at] = __float2bfloat16_rn(y);
+    else static_cast<__half *>(p.out)[at] = __float2half_rn(y);
+}
+
 template <int kCache, int HD, bool kWide, bool kExact>
 __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD, kWide)) attend_kernel(const AttnParams p) {
     using Sh = AttnShape<kCache, HD, kWide>;
@@ -338,7 +401,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
     constexpr int GH = kWide ? 8 : 4, HL = kWide ? 2 : 1;         // heads of a tile, and of a lane
     constexpr int NB = Sh::NB, MT = Sh::MT, kTok = Sh::kTok, kTile = kTok * kAttnWarps, kMTiles = HD / 16;
     constexpr int kQS = Pt::kQS, kPS = Pt::kPS;
-    constexpr bool kInt = kAttnInt<kCache, kExact>;
+    constexpr bool kInt = kAttnInt<kCache, kExact>, kOff = kInt && kCache == DTYPE_Q8_0;
     constexpr bool kBf16 = Sh::kBf16, kF32 = Sh::kF32;
     constexpr float kBias = kAttnBias<kCache>;
     extern __shared__ __align__(16) uint8_t shared[];
@@ -351,7 +414,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
     __shared__ unsigned warp_sum[kAttnWarps];
     __shared__ int found_seq;
     __shared__ unsigned found_base;
-    __shared__ int qoff[kInt ? GH : 1][NB];                       // what the codes' offsets add to a block's integer score
+    __shared__ int qoff[kOff ? GH : 1][NB];                       // what the codes' offsets add to a block's integer score
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     pdl_trigger();
     pdl_wait();
@@ -360,15 +423,15 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
     //      checked on the host) ----
     const int per_thread = (p.sequences + kAttnWarps * 32 - 1) / (kAttnWarps * 32);
     const int s0 = min(tid * per_thread, p.sequences), s1 = min(s0 + per_thread, p.sequences);
-    // Blocks are dealt to the sides in turn: those of one rank walk the same
-    // tokens for head tiles of their own, so a row comes from HBM once and from
-    // L2 for the others (64 x 8192, 16 query heads to a KV head of 128: bf16
-    // 687 -> 454 us, Q8_0 402 -> 363 us against one tile behind another).
-    // An item: a KV head and one of this side's head tiles.
-    const int side = blockIdx.x % p.sides, side_tiles = p.head_tiles / p.sides, side_blocks = p.blocks / p.sides;
+    // The sides' blocks of one rank walk the same tokens for head tiles of their
+    // own, so a row comes from HBM once and from L2 for the others (64 x 8192, 16
+    // query heads to a KV head of 128: bf16 687 -> 454 us, Q8_0 402 -> 350 us
+    // against one tile behind another).  An item: a KV head and one of this
+    // side's head tiles.
+    const int side = blockIdx.y, side_tiles = p.side_tiles, side_blocks = gridDim.x;
     const int rows = p.l.kv_heads * side_tiles;                   // items of a sequence
     unsigned mine = 0;
-    for (int s = s0; s < s1; ++s) mine += attn_span<kTile>(p, s, blockIdx.x == 0).units;
+    for (int s = s0; s < s1; ++s) mine += attn_span<kTile>(p, s, blockIdx.x == 0 && side == 0).units;
     unsigned incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -385,9 +448,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
     }
     base *= rows;
     total *= rows;
-    const unsigned blocks = min((unsigned)side_blocks, total), bid = blockIdx.x / p.sides, slot0 = side * side_blocks;
+    const unsigned blocks = min((unsigned)side_blocks, total), bid = blockIdx.x, slot0 = side * side_blocks;
     if (bid >= blocks) {
-        if (tid == 0 && !p.by_item) p.piece[slot0 + bid] = make_int4(0, 0, 0, 0);
+        if (tid == 0 && !p.count && !p.by_item) p.piece[slot0 + bid] = make_int4(0, 0, 0, 0);
         return;
     }
     // The first `longer` blocks take each + 1 units, the others each.
@@ -578,7 +641,6 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
         resolve();
         unsigned next_counts = valid;                             // tokens of the next tile that count
         copy_rows(false);
-        copy_rows(true);
 #pragma unroll
         for (int k = 0; k < kPerWarp; ++k) {
             const int j = warp + k * kAttnWarps;
@@ -602,12 +664,14 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                 // a head with an infinity or a NaN has no score.
                 if (!(top < INFINITY)) mul = __uint_as_float(0x7fc00000u);
                 up *= 0.5f;
-                mul *= 2.0f;
+                mul *= kOff ? 2.0f : 0.125f;                      // (Q4_0's codes come times 16)
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     const int y = top < INFINITY ? __float2int_rn(x[k][b] * up) : 0;
-                    const int sum = __reduce_add_sync(0xffffffffu, y);
-                    if (lane == 0) qoff[j][b] = -(kCache == DTYPE_Q8_0 ? 128 : 8) * sum;
+                    if constexpr (kOff) {
+                        const int sum = __reduce_add_sync(0xffffffffu, y);
+                        if (lane == 0) qoff[j][b] = -128 * sum;
+                    }
                     int d = 32 * b + lane;
                     if (kCache == DTYPE_Q4_0) d = (d & ~7) | ((d & 1) << 2) | ((d >> 1) & 3);   // evens, odds
                     uint8_t *to = sq + col * Sh::kDigitStride + d;
@@ -638,6 +702,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
             }
         }
         __syncthreads();
+        copy_rows(true);                                          // behind the query's stores, which are waited for
         float qm[HL];
 #pragma unroll
         for (int j = 0; j < HL; ++j) qm[j] = qmul[HL * t + j];
@@ -655,7 +720,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
         int qo[HL][NB];
-        if constexpr (kInt)
+        if constexpr (kOff)
 #pragma unroll
             for (int j = 0; j < HL; ++j)
 #pragma unroll
@@ -712,14 +777,17 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                                 } else {
                                     const uint32_t u = kr[i][r][b / 2], v = kr[i][r][(NB + b) / 2];
                                     const uint32_t w = __byte_perm(u, v, (b & 1 ? 0x32 : 0x10) | ((NB + b) & 1 ? 0x7600 : 0x5400));
-                                    a[r] = w & 0x0f0f0f0fu;
-                                    a[2 + r] = (w >> 4) & 0x0f0f0f0fu;
+                                    a[r] = ((w << 4) & 0xf0f0f0f0u) ^ 0x80808080u;      // 16 (code - 8)
+                                    a[2 + r] = (w & 0xf0f0f0f0u) ^ 0x80808080u;
                                 }
                             }
-                            // The sums start at what the codes' offset adds.
+                            // Q8_0: the sums start at what the codes' offset adds.
                             int c[Pt::kSets][4];
-                            mma8(c[0], a[0], a[1], a[2], a[3], q[0].x, q[0].y, qo[0][b], kWide ? qo[HL - 1][b] : 0);
-                            if constexpr (kWide) mma8(c[Pt::kSets - 1], a[0], a[1], a[2], a[3], q[Pt::kSets - 1].x, q[Pt::kSets - 1].y, 0, 0);
+#pragma unroll
+                            for (int set = 0; set < Pt::kSets; ++set) {
+                                if constexpr (kOff) mma8<false>(c[set], a[0], a[1], a[2], a[3], q[set].x, q[set].y, set ? 0 : qo[0][b], kWide && !set ? qo[HL - 1][b] : 0);
+                                else mma8<true>(c[set], a[0], a[1], a[2], a[3], q[set].x, q[set].y, 0, 0);
+                            }
 #pragma unroll
                             for (int r = 0; r < 2; ++r)
 #pragma unroll
@@ -919,17 +987,14 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
                         read_scales<NB>(slot + Sh::kScaleOff + (16 * i + 8 * r + g) * Sh::kScaleBytes, vs[i][r]);
-                        float top_s = 0.0f;
 #pragma unroll
-                        for (int b = 0; b < NB; ++b) top_s = fmaxf(top_s, fabsf(vs[i][r][b]));
-#pragma unroll
-                        for (int j = 0; j < HL; ++j) big = fmaxf(big, pr[j][2 * i + r] * top_s);
+                        for (int b = 0; b < NB; ++b) big = fmaxf(big, fabsf(vs[i][r][b]));
                     }
-                if (!now) big = 0.0f;                             // nothing was copied
+                // (probabilities are at most 1)
                 if (__any_sync(0xffffffffu, big > vlim)) {
-                    // A larger product of probability and scale than fits: a new
-                    // power of two that brings it to [2^13, 2^14).  An infinite
-                    // scale is its block's alone.
+                    // Where a product of probability and scale is larger than
+                    // fits, a new power of two brings it to [2^13, 2^14).  An
+                    // infinite scale is its block's alone.
                     big = 0.0f;
 #pragma unroll
                     for (int i = 0; i < MT; ++i)
@@ -1172,31 +1237,59 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
             if (!whole) {
                 part[2 * GH + i] = o;
             } else if (h < nh) {
-                o *= qmul[h];
-                const long long off = seq * p.out_ss + (long long)(head0 + h) * p.out_hs + d;
-                if (p.io == DTYPE_F32) static_cast<float *>(p.out)[off] = o;
-                else if (p.io == DTYPE_BF16) static_cast<__nv_bfloat16 *>(p.out)[off] = __float2bfloat16_rn(o);
-                else static_cast<__half *>(p.out)[off] = __float2half_rn(o);
+                attn_store(p, seq * p.out_ss + (long long)(head0 + h) * p.out_hs + d, o * qmul[h]);
             }
         }
-        if (piece0 == 0) {
+        // The blocks of this item: from the one that holds its first tile to the
+        // one that holds its last.
+        auto block_of = [&](unsigned x) {
+            const unsigned split = longer * (each + 1);
+            return x < split ? x / (each + 1) : longer + (x - split) / each;
+        };
+        if (p.count) {
+            if (!whole) {
+                // The one that comes last joins them, in their order.
+                const unsigned first = block_of(tile_unit), holders = block_of(tile_unit + sp.tiles - 1) - first + 1;
+                int *count = p.count + slot0 + first;
+                __syncthreads();
+                if (tid == 0) {
+                    __threadfence();
+                    found_seq = atomicAdd(count, 1) == (int)holders - 1;
+                }
+                __syncthreads();
+                if (found_seq) {
+                    __threadfence();
+                    if (tid == 0) *count = 0;
+                    const float *parts = p.part + (2 * (size_t)(slot0 + first) + 1) * GH * (HD + 2);
+                    for (int h = warp; h < nh; h += kAttnWarps) {
+                        float M1 = -INFINITY, L1 = 0.0f, o1[NB];
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) o1[b] = 0.0f;
+                        attn_add_holders<HD, 8>(parts, (size_t)GH * (HD + 2), GH, h, 0, 1, (int)holders, M1, L1, o1);
+                        const float inv = L1 == 0.0f ? 0.0f : 1.0f / L1;
+                        if (p.lse && lane == 0)
+                            p.lse[(long long)seq * p.heads + head0 + h] = L1 == 0.0f ? -INFINITY : (M1 - kBias + log2f(L1)) * 0.6931471805599453f;
+#pragma unroll
+                        for (int b = 0; b < NB; ++b)
+                            attn_store(p, seq * p.out_ss + (long long)(head0 + h) * p.out_hs + 32 * b + lane, o1[b] * inv);
+                    }
+                }
+            }
+        } else if (piece0 == 0) {
             int4 mine_holds = make_int4(0, 0, 0, 0);
             if (!whole) {
-                // The blocks of this item: this one and all up to the one that holds its last tile.
-                const unsigned x = tile_unit + sp.tiles - 1, split = longer * (each + 1);
-                const unsigned last = x < split ? x / (each + 1) : longer + (x - split) / each;
-                mine_holds = make_int4(seq, kh * p.head_tiles + ht, (int)(last - bid) + 1, (int)(slot0 + bid));
+                mine_holds = make_int4(seq, kh * p.head_tiles + ht, (int)(block_of(tile_unit + sp.tiles - 1) - bid) + 1, (int)(slot0 + bid));
                 piece = mine_holds;
             }
             if (p.by_item && tid == 0) p.piece[(seq * p.l.kv_heads + kh) * p.head_tiles + ht] = mine_holds;
         }
         pos = end;
     }
-    if (tid == 0 && !p.by_item) p.piece[slot0 + bid] = piece;
+    if (tid == 0 && !p.count && !p.by_item) p.piece[slot0 + bid] = piece;
 }
 
-// Adds up the items that several blocks hold: one block per item and query
-// head.  Latency bound (4 us); it does not let the next kernel start early,
+// Adds up the items that several blocks hold, where the pass does not: one block
+// per item and query head.  Latency bound (4 us); it does not let the next kernel start early,
 // whose blocks would take the SMs before it is done (2 x 131071 over Q4_0 called
 // again and again: 93 -> 112 us).  Its warps take turns at the holders, kJoinBatch of them in flight
 // (maxima, sums and values together), and are joined like the blocks' warps.
@@ -1216,39 +1309,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Attn
     float M = -INFINITY, L = 0.0f, o[kVals];
 #pragma unroll
     for (int j = 0; j < kVals; ++j) o[j] = 0.0f;
-    for (int i0 = warp; i0 < piece.z; i0 += kJoinWarps * kJoinBatch) {
-        float m[kJoinBatch], l[kJoinBatch], x[kJoinBatch][kVals], top = M;
-#pragma unroll
-        for (int k = 0; k < kJoinBatch; ++k) {
-            const int i = i0 + k * kJoinWarps;
-            m[k] = -INFINITY;
-            l[k] = 0.0f;
-            if (i >= piece.z) {
-#pragma unroll
-                for (int j = 0; j < kVals; ++j) x[k][j] = 0.0f;
-                continue;
-            }
-            const float *from = part + (i ? 2 * i - 1 : 0) * stride;
-            m[k] = __ldcg(from + h);
-            l[k] = __ldcg(from + tile_heads + h);
-#pragma unroll
-            for (int j = 0; j < kVals; ++j) x[k][j] = __ldcg(from + 2 * tile_heads + h * HD + 32 * j + lane);
-        }
-#pragma unroll
-        for (int k = 0; k < kJoinBatch; ++k) top = fmaxf(top, m[k]);
-        const float ref = top == -INFINITY ? 0.0f : top, keep = attn_exp2(M - ref);
-        M = top;
-        L *= keep;
-#pragma unroll
-        for (int j = 0; j < kVals; ++j) o[j] *= keep;
-#pragma unroll
-        for (int k = 0; k < kJoinBatch; ++k) {
-            const float w = l[k] != l[k] ? l[k] : attn_exp2(m[k] - ref);      // a NaN's maximum says nothing
-            L = fmaf(w, l[k], L);
-#pragma unroll
-            for (int j = 0; j < kVals; ++j) o[j] = fmaf(w, x[k][j], o[j]);
-        }
-    }
+    attn_add_holders<HD, kJoinBatch>(part, stride, tile_heads, h, warp, kJoinWarps, piece.z, M, L, o);
 #pragma unroll
     for (int j = 0; j < kVals; ++j) so[warp][32 * j + lane] = o[j];
     if (lane == 0) {
@@ -1276,10 +1337,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Attn
         float y = 0.0f;
 #pragma unroll
         for (int i = 0; i < kJoinWarps; ++i) y = fmaf(w[i], so[i][d], y);
-        y *= inv;
-        if (p.io == DTYPE_F32) static_cast<float *>(p.out)[off + d] = y;
-        else if (p.io == DTYPE_BF16) static_cast<__nv_bfloat16 *>(p.out)[off + d] = __float2bfloat16_rn(y);
-        else static_cast<__half *>(p.out)[off + d] = __float2half_rn(y);
+        attn_store(p, off + d, y * inv);
     }
 }
 
@@ -1300,8 +1358,8 @@ cudaError_t attn_launch(const AttnParams &p, cudaStream_t st) {
     static std::atomic<unsigned long long> done{0};
     cudaError_t e = attn_allow(attend_kernel<kCache, HD, kWide, kExact>, kBytes, p.device, done);
     if (e != cudaSuccess) return e;
-    e = launch_pdl(attend_kernel<kCache, HD, kWide, kExact>, dim3(p.blocks), dim3(kAttnWarps * 32), kBytes, st, p);
-    if (e != cudaSuccess) return e;
+    e = launch_pdl(attend_kernel<kCache, HD, kWide, kExact>, dim3(p.blocks / p.sides, p.sides), dim3(kAttnWarps * 32), kBytes, st, p);
+    if (e != cudaSuccess || p.count) return e;
     // Items of few holders take small blocks, many at a time; items of many are
     // few, and want their holders in one or two rounds (2 x 36238 tokens of one
     // KV head, 220 holders each: 17.9 -> 15.9 us; 512 items of two with the large
