@@ -160,8 +160,7 @@ SAPPHIRE_API int sapphire_kv_read_device(kernel_context_t *ctx, const sapphire_k
  * (an infinity may come out as NaN) and no others.  A length below 0 counts as
  * 0, one beyond the table as the table's end, and a token on a page outside the
  * cache does not count; each is an error at the next kernel_ctx_synchronize.
- * The order of the sums depends on the lengths and the GPU alone: the same call
- * gives the same bits.
+ * The same call gives the same bits.
  * ------------------------------------------------------------------------- */
 typedef struct {
     tensor_dtype_t dtype;    /* F32, BF16 or F16, of q and out */

@@ -738,6 +738,29 @@ def test_captured_calls_keep_workspaces_of_their_own(sp, dev_ctx):
             assert_within(out, want, bound)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "q8_0", "q4_0"])
+@pytest.mark.parametrize("lengths", [[30001] + [9] * 70, [700, 0, 1, 650], [257] * 40])
+def test_pieces_are_joined_in_their_order(dev_ctx, dtype, lengths):
+    """Calls on the context's workspace, whose last block joins a sequence's pieces, give the same bits every time;
+    so do calls on the caller's."""
+    kv, table, q = attend_case(dev_ctx, dtype, "f32", lengths, 2, 4, 64, 16, seed=71)
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    ws = torch.full((kv.workspace_bytes(len(lengths), 8),), 0xEE, dtype=torch.uint8, device="cuda")
+    want, bound, want_lse, lse_bound = attend_plain(kv, q, table, lengths, 16, 2, 64, dtype)
+    for workspace in (None, ws):
+        first = None
+        for _ in range(12):
+            out, lse = torch.full_like(q, 3.0), torch.full(q.shape[:2], 3.0, device="cuda")
+            kv.attend(q, table, n, out, lse=lse, workspace=workspace)
+            dev_ctx.synchronize()
+            if first is None:
+                first = (out, lse)
+                assert_within(out, want, bound)
+                some = n > 0
+                assert_within(lse[some], want_lse[some], lse_bound[some])
+            assert torch.equal(out, first[0]) and torch.equal(lse, first[1])
+
+
 def test_changing_streams(sp, dev_ctx):
     """A call on the default stream, the next on another at once (both in the
     context's workspace), and a change of streams while one is captured."""
