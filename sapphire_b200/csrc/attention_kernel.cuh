@@ -653,9 +653,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
 #pragma unroll
                 for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                 if (top > 0.0f && top < INFINITY) {
-                    const int e = min(max(14 - ilogbf(top), -126), 126);
-                    up *= ldexpf(1.0f, e);
-                    mul = fmaxf(mul * ldexpf(1.0f, -e), 1.2e-38f);
+                    const int e = min(141 - (int)(__float_as_uint(top) >> 23), 126);
+                    up *= __uint_as_float((uint32_t)(127 + e) << 23);
+                    mul = fmaxf(mul * __uint_as_float((uint32_t)(127 - e) << 23), 1.2e-38f);
                 }
             }
             const int col = kWide ? j : 2 * j;
