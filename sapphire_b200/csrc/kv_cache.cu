@@ -81,39 +81,100 @@ __device__ __forceinline__ float block_max(float v, unsigned mask) {
     return fmaxf(v, __shfl_xor_sync(mask, v, 2));
 }
 
-// Codes of 8 values as the two words' bytes (Q8_0: one uint32 each; Q4_0: 16
-// bits each); returns the block's scale.
-__device__ __forceinline__ float quantize_q8(const float (&x)[kUnit], unsigned mask, uint32_t (&w)[2]) {
-    float a = 0.0f, odd = 0.0f;
+// The bits of a block's largest magnitude, at least kInfBits where a value is
+// infinite or none: magnitudes are ordered like their bits.
+template <typename T>
+struct Magnitude {
+    static constexpr uint32_t kInfBits = sizeof(T) == 4 ? 0x7f800000u : 0x7c00u;
+};
+template <>
+struct Magnitude<__nv_bfloat16> {
+    static constexpr uint32_t kInfBits = 0x7f80u;
+};
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+    uint32_t m;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+    return m;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t block_magnitude(const Raw8<T> &x, unsigned mask) {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(x.v);
+    uint32_t m = 0;
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int j = 0; j < kUnit; ++j) {
-        a = fmaxf(a, fabsf(x[j]));
-        odd = fmaf(x[j], 0.0f, odd);      // NaN where a value is none or infinite
-    }
-    const float d = __fdiv_rn(block_max(a, mask), 127.0f);
-    const float id = d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
-    uint32_t q[kUnit];
-    if (odd == 0.0f && id < INFINITY) {
-        // |x| id is at most 127 and a rounding, so no code is clamped.  Half
-        // away from zero is the whole part of |t| + 1/2: both sums truncate,
-        // so neither rounds a value below a half up.
+        for (int j = 0; j < kUnit; ++j) m = max(m, w[j] & 0x7fffffffu);
 #pragma unroll
-        for (int j = 0; j < kUnit; ++j) {
-            const float t = __fmul_rn(x[j], id);
-            const int n = (int)__float_as_uint(__fadd_rz(__fadd_rz(fabsf(t), 0.5f), 8388608.0f));
-            const int sign = (int)__float_as_uint(t) >> 31;
-            q[j] = (uint32_t)((n ^ sign) - sign + 128);
-        }
+        for (int o = 1; o < 4; o <<= 1) m = max(m, __shfl_xor_sync(mask, m, o));
+        return m;
     } else {
 #pragma unroll
-        for (int j = 0; j < kUnit; ++j) {
-            const float t = roundf(__fmul_rn(x[j], id));
-            q[j] = (uint32_t)(((t != t) ? 0 : (t > 127.0f ? 127 : (t < -127.0f ? -127 : (int)t))) + 128);
+        for (int j = 0; j < kUnit / 2; ++j) m = max_u16x2(m, w[j] & 0x7fff7fffu);
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) m = max_u16x2(m, __shfl_xor_sync(mask, m, o));
+        return max(m & 0xffffu, m >> 16);
+    }
+}
+// Four values' signs as bytes of ones or zeros.
+template <uint32_t kSel>
+__device__ __forceinline__ uint32_t permute_signs(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "n"(kSel));        // a selector's top bit spreads the sign
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t sign_bytes(const Raw8<T> &x, int k) {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(x.v);
+    if constexpr (sizeof(T) == 4)
+        return __byte_perm(permute_signs<0x00fb>(w[4 * k], w[4 * k + 1]), permute_signs<0x00fb>(w[4 * k + 2], w[4 * k + 3]), 0x5410);
+    else
+        return permute_signs<0xfdb9>(w[2 * k], w[2 * k + 1]);
+}
+
+// Codes of 8 values as the two words' bytes (Q8_0: one uint32 each; Q4_0: 16
+// bits each); returns the block's scale.
+template <typename T>
+__device__ __forceinline__ float quantize_q8(const Raw8<T> &raw, unsigned mask, uint32_t (&w)[2]) {
+    float x[kUnit];
+    raw.get(x);
+    const uint32_t bits = block_magnitude(raw, mask);
+    if (bits < Magnitude<T>::kInfBits) {
+        const T top = *reinterpret_cast<const T *>(&bits);        // (its low half for 16-bit types)
+        const float d = __fdiv_rn(to_f32(top), 127.0f);
+        const float id = d != 0.0f ? __frcp_rn(d) : 0.0f;
+        if (id < INFINITY) {
+            // |x| id is at most 127 and a rounding, so no code is clamped.  Half
+            // away from zero is the whole part of |t| + 1/2: both sums truncate,
+            // so neither rounds a value below a half up.
+            uint32_t n[kUnit];
+#pragma unroll
+            for (int j = 0; j < kUnit; ++j)
+                n[j] = __float_as_uint(__fadd_rz(__fadd_rz(fabsf(__fmul_rn(x[j], id)), 0.5f), 8388608.0f));
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                // 128 + n or 128 - n in each byte: neither carries.
+                const uint32_t m = __byte_perm(__byte_perm(n[4 * k], n[4 * k + 1], 0x0040), __byte_perm(n[4 * k + 2], n[4 * k + 3], 0x0040), 0x5410);
+                const uint32_t minus = sign_bytes(raw, k);
+                w[k] = ((0x80808080u + m) & ~minus) | ((0x80808080u - m) & minus);
+            }
+            return d;
         }
     }
+    // A block with an infinity or a NaN (not the largest, code 0), or with a
+    // scale whose reciprocal is infinite.
+    float a = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-        w[k] = __byte_perm(__byte_perm(q[4 * k], q[4 * k + 1], 0x0040), __byte_perm(q[4 * k + 2], q[4 * k + 3], 0x0040), 0x5410);
+    for (int j = 0; j < kUnit; ++j) a = fmaxf(a, fabsf(x[j]));
+    const float d = __fdiv_rn(block_max(a, mask), 127.0f);
+    const float id = d != 0.0f ? __frcp_rn(d) : 0.0f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        w[k] = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float t = roundf(__fmul_rn(x[4 * k + j], id));
+            w[k] |= (uint32_t)(((t != t) ? 0 : (t > 127.0f ? 127 : (t < -127.0f ? -127 : (int)t))) + 128) << (8 * j);
+        }
+    }
     return d;
 }
 __device__ __forceinline__ float quantize_q4(const float (&x)[kUnit], unsigned mask, uint32_t (&w)[2]) {
@@ -136,7 +197,7 @@ __device__ __forceinline__ float quantize_q4(const float (&x)[kUnit], unsigned m
         }
     }
     const float d = __fdiv_rn(m, -8.0f);
-    const float id = d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
+    const float id = d != 0.0f ? __frcp_rn(d) : 0.0f;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         w[k] = 0;
@@ -233,16 +294,16 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvParams p) {
                 const KvPlace at = place[t + k * token_rows];
                 if (at.slot < 0) continue;
                 uint8_t *row = kv_at(r.rows, at.row);
-                float v[kUnit];
-                y[k].get(v);
-                if (kCache == DTYPE_Q8_0 || kCache == DTYPE_Q4_0) {
+                if constexpr (kCache == DTYPE_Q8_0 || kCache == DTYPE_Q4_0) {
                     uint32_t q[2];
                     float d;
                     if (kCache == DTYPE_Q8_0) {
-                        d = quantize_q8(v, mask, q);
+                        d = quantize_q8(y[k], mask, q);
                         reinterpret_cast<uint32_t *>(row)[word * nb + b] = q[0];
                         reinterpret_cast<uint32_t *>(row)[(word + 1) * nb + b] = q[1];
                     } else {
+                        float v[kUnit];
+                        y[k].get(v);
                         d = quantize_q4(v, mask, q);
                         reinterpret_cast<uint16_t *>(row)[word * nb + b] = (uint16_t)q[0];
                         reinterpret_cast<uint16_t *>(row)[(word + 1) * nb + b] = (uint16_t)q[1];
@@ -250,6 +311,8 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvParams p) {
                     if ((u & 3) == 0) reinterpret_cast<float *>(kv_at(r.scales, at.page))[at.slot * p.l.scale_stride + b] = d;
                 } else {
                     using C = typename KvType<kCache>::type;
+                    float v[kUnit];
+                    y[k].get(v);
                     Raw8<C> z;
                     z.set(v);
                     z.store(reinterpret_cast<C *>(row) + u * kUnit, true);
