@@ -33,9 +33,9 @@ struct KvRows {
     long long k_ts, k_hs, v_ts, v_hs;
 };
 
-// Whether every row starts on 16 bytes.
-inline bool rows_aligned(const void *p, long long ts, long long hs, size_t elem) {
-    return ((uintptr_t)p & 15) == 0 && (ts * (long long)elem) % 16 == 0 && (hs * (long long)elem) % 16 == 0;
+// Whether every row starts on `bytes` bytes.
+inline bool rows_aligned(const void *p, long long ts, long long hs, size_t elem, int bytes = 16) {
+    return (uintptr_t)p % bytes == 0 && (ts * (long long)elem) % bytes == 0 && (hs * (long long)elem) % bytes == 0;
 }
 
 // Fills `l` from the caller's cache; false (with the context's error set when
@@ -89,46 +89,57 @@ __device__ __forceinline__ __half from_f32<__half>(float x) {
     return __float2half_rn(x);
 }
 
-// Eight consecutive values as they lie in memory, so that loads in flight hold
-// no more registers than their bytes.
-template <typename T>
-struct Raw8 {
-    static constexpr int N = 8 * sizeof(T) / 16;
-    uint4 v[N];
-    // wide: p is on 16 bytes
+// kCount (8 or 4) consecutive values as they lie in memory, so that loads in
+// flight hold no more registers than their bytes.
+template <int kBytes>
+struct RawWord {
+    using type = uint4;
+};
+template <>
+struct RawWord<8> {
+    using type = uint2;
+};
+template <typename T, int kCount>
+struct Raw {
+    using Word = typename RawWord<kCount * sizeof(T)>::type;
+    static constexpr int N = kCount * sizeof(T) / sizeof(Word);
+    Word v[N];
+    // wide: p is on 16 bytes (8 where that is all)
     __device__ __forceinline__ void load(const T *p, bool wide) {
         if (wide) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = reinterpret_cast<const uint4 *>(p)[i];
+            for (int i = 0; i < N; ++i) v[i] = reinterpret_cast<const Word *>(p)[i];
         } else {
-            T t[8];
+            T t[kCount];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) t[j] = p[j];
+            for (int j = 0; j < kCount; ++j) t[j] = p[j];
             memcpy(v, t, sizeof v);
         }
     }
     __device__ __forceinline__ void store(T *p, bool wide) const {
         if (wide) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) reinterpret_cast<uint4 *>(p)[i] = v[i];
+            for (int i = 0; i < N; ++i) reinterpret_cast<Word *>(p)[i] = v[i];
         } else {
-            T t[8];
+            T t[kCount];
             memcpy(t, v, sizeof v);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) p[j] = t[j];
+            for (int j = 0; j < kCount; ++j) p[j] = t[j];
         }
     }
-    __device__ __forceinline__ void get(float (&x)[8]) const {
-        T t[8];
+    __device__ __forceinline__ void get(float (&x)[kCount]) const {
+        T t[kCount];
         memcpy(t, v, sizeof v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = to_f32(t[j]);
+        for (int j = 0; j < kCount; ++j) x[j] = to_f32(t[j]);
     }
-    __device__ __forceinline__ void set(const float (&x)[8]) {
-        T t[8];
+    __device__ __forceinline__ void set(const float (&x)[kCount]) {
+        T t[kCount];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) t[j] = from_f32<T>(x[j]);
+        for (int j = 0; j < kCount; ++j) t[j] = from_f32<T>(x[j]);
         memcpy(v, t, sizeof v);
     }
 };
+template <typename T>
+using Raw8 = Raw<T, 8>;
 #endif

@@ -26,9 +26,12 @@ namespace {
 
 constexpr int kRopeMaxDim = 512;
 constexpr int kThreads = 256;
-constexpr int kUnit = 8;                  // values of a head that a thread takes from each half
-// Tokens of a thread in flight, and the next ones behind them: 64 bytes of 16-bit values either way.
-constexpr int rope_batch(bool interleaved) { return interleaved ? 4 : 2; }
+// Values of a head that a thread takes (from each half where these are paired):
+// 8, or 4 where the halves have a multiple of 4 and not of 8, whose ends would
+// go value by value (4991 tokens x 20 bf16 heads, 40 of 80 turned: 44 -> 12 us).
+constexpr int rope_unit(bool interleaved, int half) { return !interleaved && half % 8 == 4 ? 4 : 8; }
+// Tokens of a thread in flight, and the next ones behind them: 64 bytes of 16-bit values any way.
+constexpr int rope_batch(bool interleaved, int unit) { return interleaved || unit == 4 ? 4 : 2; }
 constexpr int kMaxTokens = 16;            // tokens of one block (its cos and sin rows in shared memory)
 
 struct RopeHeads {
@@ -51,14 +54,14 @@ struct RopeParams {
 };
 
 // A block turns block_tokens tokens x its heads.  A thread owns one unit of a
-// head (8 values of the first half and their 8 partners, 8 interleaved values,
-// or 8 values behind the rotated part) and one row of blockDim.y: head h0 + y %
+// head (kUnit values of the first half and their partners, 8 interleaved values,
+// or kUnit values behind the rotated part) and one row of blockDim.y: head h0 + y %
 // row_heads, token y / row_heads; it walks down the tokens and then the heads.
 // The block's cos and sin lie in shared memory as [token][pair of pairs][unit],
 // so that neighbouring units read neighbouring 16 bytes.
-template <typename T, bool kInterleaved>
+template <typename T, bool kInterleaved, int kUnit>
 __global__ void __launch_bounds__(kThreads) rope_kernel(const RopeParams p) {
-    constexpr int kPairs = kInterleaved ? kUnit / 2 : kUnit, kBatch = rope_batch(kInterleaved);
+    constexpr int kPairs = kInterleaved ? kUnit / 2 : kUnit, kBatch = rope_batch(kInterleaved, kUnit);
     extern __shared__ float4 turn[];
     pdl_trigger();
     pdl_wait();
@@ -81,7 +84,7 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const RopeParams p) {
     };
     // kBatch tokens of a head at a time, the next ones' loads in flight.
     struct Batch {
-        Raw8<T> a[kBatch], b[kInterleaved ? 1 : kBatch];
+        Raw<T, kUnit> a[kBatch], b[kInterleaved ? 1 : kBatch];
     };
     auto load = [&](Batch &x, int h, int t1) {
 #pragma unroll
@@ -151,7 +154,7 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const RopeParams p) {
                     const float c2[4] = {cs.x, cs.y, cs.z, cs.w};
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        float &v = kInterleaved ? a[(2 * (j + i)) & 7] : a[j + i], &w = kInterleaved ? a[(2 * (j + i) + 1) & 7] : b[j + i];
+                        float &v = kInterleaved ? a[(2 * (j + i)) & (kUnit - 1)] : a[j + i], &w = kInterleaved ? a[(2 * (j + i) + 1) & (kUnit - 1)] : b[j + i];
                         const float v0 = v, v1 = w;
                         v = v0 * c2[2 * i] - v1 * c2[2 * i + 1];
                         w = v0 * c2[2 * i + 1] + v1 * c2[2 * i];
@@ -219,9 +222,10 @@ const char *rope_config_error(const sapphire_rope_config_t &c) {
 }
 
 template <typename T>
-cudaError_t launch_rope(const RopeParams &p, bool interleaved, dim3 grid, dim3 block, size_t smem, cudaStream_t st) {
-    if (interleaved) return launch_pdl(rope_kernel<T, true>, grid, block, smem, st, p);
-    return launch_pdl(rope_kernel<T, false>, grid, block, smem, st, p);
+cudaError_t launch_rope(const RopeParams &p, bool interleaved, int unit, dim3 grid, dim3 block, size_t smem, cudaStream_t st) {
+    if (interleaved) return launch_pdl(rope_kernel<T, true, 8>, grid, block, smem, st, p);
+    if (unit == 4) return launch_pdl(rope_kernel<T, false, 4>, grid, block, smem, st, p);
+    return launch_pdl(rope_kernel<T, false, 8>, grid, block, smem, st, p);
 }
 
 }  // namespace
@@ -322,6 +326,8 @@ extern "C" SAPPHIRE_API int sapphire_rope_device(sapphire_rope_t *rope, const sa
     p.k = heads(a->k, a->k_out, a->k_heads, a->k_token_stride, a->k_head_stride, a->k_out_token_stride,
                 a->k_out_head_stride);
     if (!on_device(ctx, who, "positions", a->positions)) return -1;
+    const bool inter = c.layout == SAPPHIRE_ROPE_INTERLEAVED;
+    const int unit = rope_unit(inter, p.half), align = std::min(16, unit * (int)size);
     p.wide = true;
     p.copy_tail = false;
     const RopeHeads *sides[2] = {a->q_heads ? &p.q : nullptr, a->k_heads ? &p.k : nullptr};
@@ -334,13 +340,13 @@ extern "C" SAPPHIRE_API int sapphire_rope_device(sapphire_rope_t *rope, const sa
             return -1;
         }
         p.copy_tail = p.copy_tail || h->out != h->in;
-        p.wide = p.wide && rows_aligned(h->in, h->in_ts, h->in_hs, size) && rows_aligned(h->out, h->out_ts, h->out_hs, size);
+        p.wide = p.wide && rows_aligned(h->in, h->in_ts, h->in_hs, size, align) &&
+                 rows_aligned(h->out, h->out_ts, h->out_hs, size, align);
     }
-    const bool inter = c.layout == SAPPHIRE_ROPE_INTERLEAVED;
-    // The partner half and the tail start on 16 bytes too.
-    p.wide = p.wide && (c.rot_dim * (int)size) % 16 == 0 && (inter || (p.half * (int)size) % 16 == 0);
-    p.pair_units = inter ? (p.half + kUnit / 2 - 1) / (kUnit / 2) : (p.half + kUnit - 1) / kUnit;
-    const int tail = p.copy_tail ? (c.head_dim - c.rot_dim + kUnit - 1) / kUnit : 0;
+    // The partner half and the tail start there too.
+    p.wide = p.wide && (c.rot_dim * (int)size) % align == 0 && (inter || (p.half * (int)size) % align == 0);
+    p.pair_units = inter ? (p.half + unit / 2 - 1) / (unit / 2) : (p.half + unit - 1) / unit;
+    const int tail = p.copy_tail ? (c.head_dim - c.rot_dim + unit - 1) / unit : 0;
     const int units = p.pair_units + tail;      // threads of one head
     const int rows = std::max(1, kThreads / units);
     // A block's rows are heads of one token, evenly divided where there are
@@ -350,7 +356,7 @@ extern "C" SAPPHIRE_API int sapphire_rope_device(sapphire_rope_t *rope, const sa
     // fewer tokens, then a block fewer heads, computing its own turns (1507
     // tokens x 96 heads of 256: 47 us with whole blocks, 31 us so).
     AttnDevice g(ctx->device);
-    const int batch = rope_batch(inter);
+    const int batch = rope_batch(inter, unit);
     auto cut = [](int n, int most) { return (n + (n + most - 1) / most - 1) / ((n + most - 1) / most); };
     p.block_heads = p.heads;
     p.row_heads = cut(p.heads, rows);
@@ -369,10 +375,10 @@ extern "C" SAPPHIRE_API int sapphire_rope_device(sapphire_rope_t *rope, const sa
     p.row_heads = cut(p.block_heads, p.row_heads);
     const dim3 grid((p.tokens + p.block_tokens - 1) / p.block_tokens, (p.heads + p.block_heads - 1) / p.block_heads);
     const dim3 block(units, p.row_heads * std::min(token_rows, p.block_tokens));
-    const size_t smem = (size_t)p.block_tokens * p.pair_units * (inter ? kUnit / 2 : kUnit) * sizeof(float2);
-    cudaError_t e = a->dtype == DTYPE_F32    ? launch_rope<float>(p, inter, grid, block, smem, ctx->stream)
-                    : a->dtype == DTYPE_BF16 ? launch_rope<__nv_bfloat16>(p, inter, grid, block, smem, ctx->stream)
-                                             : launch_rope<__half>(p, inter, grid, block, smem, ctx->stream);
+    const size_t smem = (size_t)p.block_tokens * p.pair_units * (inter ? unit / 2 : unit) * sizeof(float2);
+    cudaError_t e = a->dtype == DTYPE_F32    ? launch_rope<float>(p, inter, unit, grid, block, smem, ctx->stream)
+                    : a->dtype == DTYPE_BF16 ? launch_rope<__nv_bfloat16>(p, inter, unit, grid, block, smem, ctx->stream)
+                                             : launch_rope<__half>(p, inter, unit, grid, block, smem, ctx->stream);
     if (e != cudaSuccess) {
         cudaGetLastError();
         ctx_fail(ctx, who, "launch failed: %s", cudaGetErrorString(e));

@@ -130,6 +130,14 @@ def test_rope(dev_ctx, tokens, heads, kv_heads, dim, rot, layout, kind, scaling)
     r.close()
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("tokens,heads,kv_heads,dim,rot", [(300, 16, 4, 80, 40), (9, 3, 1, 90, 88), (65, 2, 2, 512, 8),
+                                                          (4991, 1, 1, 24, 24), (1, 5, 0, 510, 504)])
+def test_rope_halves_of_four(dev_ctx, kind, tokens, heads, kv_heads, dim, rot):
+    """Halves of a multiple of 4 values that is none of 8."""
+    test_rope(dev_ctx, tokens, heads, kv_heads, dim, rot, "half", kind, "banded")
+
+
 def test_rope_far_positions(dev_ctx):
     """Every 32-bit position, behind zero too."""
     from sapphire_b200.attention import Rope
