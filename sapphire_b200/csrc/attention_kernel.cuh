@@ -44,12 +44,17 @@
 // lanes read consecutive bytes.  V's codes become fp16 exactly (1024 + code - 1152,
 // or - 1032), and V's scale multiplies the probability, the product brought into
 // fp16's range by a power of two per warp that follows the largest seen.  K's codes become
-// fp16 the same way under fp32 and fp16 outputs; under a bf16 output they are
-// multiplied as the integers they are by the query as 15-bit integers (two
-// signed bytes), the sums exact, and one conversion and product with K's scale
-// brings a block's sum to fp32.  Q8_0's sums start at what the codes' offset
-// adds; a Q4_0 code in the high half of a byte, its top bit turned, is 16 (code -
-// 8) as it is.
+// fp16 the same way, except in narrow tiles under a bf16 query: there they are
+// multiplied as the integers they are by the query as 23-bit integers (three
+// signed bytes in two MMAs), the sums exact, and a product with K's scale brings
+// a block's sum to fp32.  A byte with its top bit turned is Q8_0's code, or 16
+// times a Q4_0 code of the byte's high half, without its offset.  Query values
+// down to 2^-14 of their head's largest keep all 8 of their bits, smaller ones
+// are off by at most 2^-22 of it.  (Two bytes leave 2^-15 of it, which a few large
+// channels of a query turn into errors above the output's rounding; they were 2
+// to 4 % faster.)  A wide tile would need three MMAs; one fp16 part of the query
+// is exact down to 2^-31 of the head's largest and faster (64 x 8192, 8 heads to
+// a KV head of 128: Q8_0 239 -> 230 us, Q4_0 198 -> 187).
 //
 // Split.  The tiles (64 tokens of one KV head and up to 8 query heads) of all
 // sequences are numbered in a row and cut into as many equal ranges as the GPU
@@ -122,9 +127,9 @@ constexpr int attn_blocks_per_sm(int cache, int hd, bool wide) {
 
 #ifdef __CUDACC__
 
-// K's codes are multiplied as integers where the output's rounding allows.
-template <int kCache, bool kExact>
-constexpr bool kAttnInt = (kCache == DTYPE_Q8_0 || kCache == DTYPE_Q4_0) && !kExact;
+// K's codes are multiplied as integers under a bf16 query in narrow tiles.
+template <int kCache, bool kWide, bool kExact>
+constexpr bool kAttnInt = (kCache == DTYPE_Q8_0 || kCache == DTYPE_Q4_0) && !kWide && !kExact;
 // 2^(p + kBias): probabilities use the upper end of fp16 over fp16 caches.
 template <int kCache>
 constexpr float kAttnBias = kCache == DTYPE_F16 ? 14.0f : 0.0f;
@@ -161,18 +166,12 @@ __device__ __forceinline__ float take_tf32(float &x) {
     x -= hi;
     return hi;
 }
-// d = a b + c on 32 bytes of a (signed or not) and signed bytes of b.
-template <bool kSigned>
+// d = a b on 32 signed bytes of each.
 __device__ __forceinline__ void mma8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                     uint32_t b1, int c0, int c1) {
-    if (kSigned)
-        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
-                     : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c0), "r"(c1));
-    else
-        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
-                     : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c0), "r"(c1));
+                                     uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
@@ -308,8 +307,6 @@ struct AttnShape {
     static constexpr int kQElem = kF32 ? 4 : 2;
     static constexpr int kQStride = (HD * kQElem) % 128 == 0 ? HD * kQElem + 64 : HD * kQElem;
     static constexpr int kDigitStride = HD % 128 == 96 ? HD : HD + 32;        // of a row of query bytes
-    static constexpr int kMaxSets = (kWide ? 2 : 1) + (kBf16 ? 1 : 0);
-    static_assert(kMaxSets * 8 * kQStride + 2 * kAttnWarps * kSlot + 2048 <= attn_smem(kBlocks), "the rows do not fit");
 };
 
 #ifdef __CUDACC__
@@ -341,10 +338,19 @@ template <int kCache, bool kWide, bool kExact>
 struct AttnParts {
     static constexpr int kQS = !kWide ? (kCache == DTYPE_BF16 && kExact ? 2 : 1)
                                : kCache == DTYPE_F32 ? 2 : kCache == DTYPE_BF16 ? (kExact ? 3 : 1) : kExact ? 2 : 1;
-    static constexpr bool kInt = kAttnInt<kCache, kExact>;        // wide: two signed bytes, an MMA each
-    static constexpr int kSets = kInt ? (kWide ? 2 : 1) : kQS;    // rows of 8 columns of the query
+    // Three signed bytes: the low and the middle one in one MMA, the high one in another.
+    static constexpr bool kInt = kAttnInt<kCache, kWide, kExact>;
+    static constexpr int kSets = kInt ? 2 : kQS;                  // rows of 8 columns of the query
     static constexpr int kPS = !kWide ? kQS : kCache == DTYPE_F32 ? 2 : kCache == DTYPE_BF16 ? (kExact ? 3 : 2) : kExact ? 2 : 1;
 };
+
+// Shared memory of the query's parts.
+template <int kCache, int HD, bool kWide, bool kExact>
+constexpr int attn_query_bytes() {
+    using Pt = AttnParts<kCache, kWide, kExact>;
+    using Sh = AttnShape<kCache, HD, kWide>;
+    return Pt::kSets * 8 * (Pt::kInt ? Sh::kDigitStride : Sh::kQStride);
+}
 
 // Adds holders i0, i0 + step, ... below n of head h's item to M, L and o,
 // kBatch of them in flight.  part: the first one's partial; the others' follow
@@ -401,12 +407,12 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
     constexpr int GH = kWide ? 8 : 4, HL = kWide ? 2 : 1;         // heads of a tile, and of a lane
     constexpr int NB = Sh::NB, MT = Sh::MT, kTok = Sh::kTok, kTile = kTok * kAttnWarps, kMTiles = HD / 16;
     constexpr int kQS = Pt::kQS, kPS = Pt::kPS;
-    constexpr bool kInt = kAttnInt<kCache, kExact>, kOff = kInt && kCache == DTYPE_Q8_0;
+    constexpr bool kInt = kAttnInt<kCache, kWide, kExact>;
     constexpr bool kBf16 = Sh::kBf16, kF32 = Sh::kF32;
     constexpr float kBias = kAttnBias<kCache>;
     extern __shared__ __align__(16) uint8_t shared[];
     uint8_t *const sq = shared;                                   // the query's parts
-    uint8_t *const slots = shared + Pt::kSets * 8 * Sh::kQStride;  // [warp][2]; at the end of an item the warps'
+    uint8_t *const slots = shared + attn_query_bytes<kCache, HD, kWide, kExact>();  // [warp][2]; at the end of an item the warps'
     float *const sacc = reinterpret_cast<float *>(slots);         // outputs [warp][head][dim]
     static_assert(2 * Sh::kSlot >= GH * HD * 4, "the warps' outputs do not fit the slots");
     __shared__ float sm_m[kAttnWarps][GH], sm_l[kAttnWarps][GH];
@@ -414,7 +420,6 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
     __shared__ unsigned warp_sum[kAttnWarps];
     __shared__ int found_seq;
     __shared__ unsigned found_base;
-    __shared__ int qoff[kOff ? GH : 1][NB];                       // what the codes' offsets add to a block's integer score
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     pdl_trigger();
     pdl_wait();
@@ -653,30 +658,28 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
 #pragma unroll
                 for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                 if (top > 0.0f && top < INFINITY) {
-                    const int e = min(141 - (int)(__float_as_uint(top) >> 23), 126);
+                    const int e = min(141 - (int)(__float_as_uint(top) >> 23), kInt ? 119 : 126);
                     up *= __uint_as_float((uint32_t)(127 + e) << 23);
                     mul = fmaxf(mul * __uint_as_float((uint32_t)(127 - e) << 23), 1.2e-38f);
                 }
             }
             const int col = kWide ? j : 2 * j;
             if constexpr (kInt) {
-                // 15-bit integers: the head's largest value goes to [2^13, 2^14);
+                // 23-bit integers: the head's largest value goes to [2^21, 2^22);
                 // a head with an infinity or a NaN has no score.
                 if (!(top < INFINITY)) mul = __uint_as_float(0x7fc00000u);
-                up *= 0.5f;
-                mul *= kOff ? 2.0f : 0.125f;                      // (Q4_0's codes come times 16)
+                up *= 128.0f;
+                mul *= kCache == DTYPE_Q8_0 ? 0x1p-7f : 0x1p-11f; // (Q4_0's codes come times 16)
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    const int y = top < INFINITY ? __float2int_rn(x[k][b] * up) : 0;
-                    if constexpr (kOff) {
-                        const int sum = __reduce_add_sync(0xffffffffu, y);
-                        if (lane == 0) qoff[j][b] = -128 * sum;
-                    }
+                    const int y = top < INFINITY ? __float2int_rn(x[k][b] * up) : 0, y1 = (y + 128) >> 8;
                     int d = 32 * b + lane;
                     if (kCache == DTYPE_Q4_0) d = (d & ~7) | ((d & 1) << 2) | ((d >> 1) & 3);   // evens, odds
                     uint8_t *to = sq + col * Sh::kDigitStride + d;
                     to[0] = (uint8_t)y;
-                    to[(kWide ? 8 : 1) * Sh::kDigitStride] = (uint8_t)((y + 128) >> 8);
+                    to[Sh::kDigitStride] = (uint8_t)y1;
+                    to[8 * Sh::kDigitStride] = (uint8_t)((y1 + 128) >> 8);
+                    to[9 * Sh::kDigitStride] = 0;
                 }
                 if (lane == 0) qmul[j] = mul;
                 continue;
@@ -719,12 +722,6 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
         for (int i = 0; i < kMTiles; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
-        int qo[HL][NB];
-        if constexpr (kOff)
-#pragma unroll
-            for (int j = 0; j < HL; ++j)
-#pragma unroll
-                for (int b = 0; b < NB; ++b) qo[j][b] = qoff[HL * t + j][b];
         float vlim = 0.0f, vinv = 0.0f;                           // p times V's scale: largest that fits, and the power of two
         // Adds what an accumulator of its own holds: an MMA truncates its
         // sums, so where that shows (kExact) only a tile's products share one.
@@ -772,8 +769,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
 #pragma unroll
                             for (int r = 0; r < 2; ++r) {
                                 if constexpr (kCache == DTYPE_Q8_0) {
-                                    a[r] = kr[i][r][b];
-                                    a[2 + r] = kr[i][r][NB + b];
+                                    a[r] = kr[i][r][b] ^ 0x80808080u;
+                                    a[2 + r] = kr[i][r][NB + b] ^ 0x80808080u;
                                 } else {
                                     const uint32_t u = kr[i][r][b / 2], v = kr[i][r][(NB + b) / 2];
                                     const uint32_t w = __byte_perm(u, v, (b & 1 ? 0x32 : 0x10) | ((NB + b) & 1 ? 0x7600 : 0x5400));
@@ -781,20 +778,15 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                                     a[2 + r] = (w & 0xf0f0f0f0u) ^ 0x80808080u;
                                 }
                             }
-                            // Q8_0: the sums start at what the codes' offset adds.
                             int c[Pt::kSets][4];
 #pragma unroll
-                            for (int set = 0; set < Pt::kSets; ++set) {
-                                if constexpr (kOff) mma8<false>(c[set], a[0], a[1], a[2], a[3], q[set].x, q[set].y, set ? 0 : qo[0][b], kWide && !set ? qo[HL - 1][b] : 0);
-                                else mma8<true>(c[set], a[0], a[1], a[2], a[3], q[set].x, q[set].y, 0, 0);
+                            for (int set = 0; set < Pt::kSets; ++set) mma8(c[set], a[0], a[1], a[2], a[3], q[set].x, q[set].y);
+                            // (low and middle bytes together stay below 2^27)
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) {
+                                const float low = (float)(c[0][2 * r] + c[0][2 * r + 1] * 256);
+                                s[0][2 * i + r] = fmaf(ks[i][r][b], fmaf((float)c[1][2 * r], 65536.0f, low), s[0][2 * i + r]);
                             }
-#pragma unroll
-                            for (int r = 0; r < 2; ++r)
-#pragma unroll
-                                for (int j = 0; j < HL; ++j) {
-                                    const int v = kWide ? c[0][2 * r + j] + c[Pt::kSets - 1][2 * r + j] * 256 : c[0][2 * r] + c[0][2 * r + 1] * 256;
-                                    s[j][2 * i + r] = fmaf(ks[i][r][b], (float)v, s[j][2 * i + r]);
-                                }
                         }
                     }
                 } else {
@@ -958,7 +950,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
 #pragma unroll
                     for (int set = 0; set < kPS; ++set) {
                         uint32_t u;
-                        if constexpr (kInt && !kWide) {
+                        if constexpr (kInt) {
                             u = pack16<kBf16>(y[0], 0.0f);        // one part
                         } else if constexpr (kWide) {
                             u = pack16<kBf16>(y[0], y[HL - 1]);
@@ -1354,7 +1346,8 @@ cudaError_t attn_allow(K *kernel, size_t bytes, int device, std::atomic<unsigned
 template <int kCache, int HD, bool kWide, bool kExact>
 cudaError_t attn_launch(const AttnParams &p, cudaStream_t st) {
     using Sh = AttnShape<kCache, HD, kWide>;
-    constexpr size_t kBytes = AttnParts<kCache, kWide, kExact>::kSets * 8 * Sh::kQStride + 2 * kAttnWarps * Sh::kSlot;
+    constexpr size_t kBytes = attn_query_bytes<kCache, HD, kWide, kExact>() + 2 * kAttnWarps * Sh::kSlot;
+    static_assert(kBytes + 2048 <= attn_smem(Sh::kBlocks), "the rows do not fit");
     static std::atomic<unsigned long long> done{0};
     cudaError_t e = attn_allow(attend_kernel<kCache, HD, kWide, kExact>, kBytes, p.device, done);
     if (e != cudaSuccess) return e;

@@ -847,3 +847,35 @@ def test_attend_values_beside_infinities(dev_ctx, dtype, kind):
     keep = torch.ones(dim, dtype=torch.bool, device="cuda")
     keep[hurt] = False
     assert_within(out[..., keep], want[..., keep], bound[..., keep])
+
+
+@pytest.mark.parametrize("dtype", ["q8_0", "q4_0"])
+@pytest.mark.parametrize("dim,group", [(64, 1), (128, 4), (128, 8), (192, 3), (256, 7)])
+@pytest.mark.parametrize("loud", [128.0, 8192.0])
+def test_attend_query_with_a_loud_channel(dev_ctx, dtype, dim, group, loud):
+    """One channel of a bf16 query 2^15 times the others; its keys are the same in every position, so the others
+    decide.  Those are whole multiples of 2^-21 of the loud one, which the query's integers hold exactly; a
+    block's sum and the score round fewer than 16 times, 2^-24 each of sum|q k|."""
+    g = gen(int(loud) + dim + group)
+    lengths, heads, page = [40, 9, 300], 2, 16
+    kv = make_cache(dev_ctx, dtype, page, heads, dim, 30, fill=0xFF)
+    table = make_table(lengths, page, 30, g)
+
+    def signs(*shape):
+        return torch.randint(0, 2, shape, device="cuda", generator=g).float() * 2 - 1
+
+    k = signs(sum(lengths), heads, dim)
+    k[..., 0] = 1.0                                       # the first of each block's largest: one scale for all
+    v = torch.randn(sum(lengths), heads, dim, device="cuda", generator=g)
+    kv.write(k, v, table, cu_tokens=ragged(lengths))
+    q = signs(3, heads * group, dim) * loud * 2.0 ** -15
+    q[..., 0] = loud * signs(3, heads * group)
+    q = q.bfloat16()
+    scale = 2.0 ** 11 / loud                              # the others' sum is then about 2^-4 sqrt(dim)
+    out, lse = torch.empty_like(q), torch.empty(3, heads * group, device="cuda")
+    kv.attend(q, table, torch.tensor(lengths, dtype=torch.int32, device="cuda"), out, scale=scale, lse=lse)
+    dev_ctx.synchronize()
+    want, bound, want_lse, lse_bound = attend_plain(kv, q, table, lengths, page, heads, dim, dtype, scale=scale)
+    ds = (2 ** 11 + dim * 2.0 ** -4) * 2.0 ** -20
+    assert_within(out, want, v.abs().max().double() * (4 * ds + 2.0 ** -17 + 2.0 ** -12))
+    assert_within(lse, want_lse, torch.tensor(2 * ds + 2.0 ** -17, device="cuda", dtype=torch.float64), "lse")
