@@ -723,8 +723,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
         float vlim = 0.0f, vinv = 0.0f;                           // p times V's scale: largest that fits, and the power of two
-        // Adds what an accumulator of its own holds: an MMA truncates its
-        // sums, so where that shows (kExact) only a tile's products share one.
+        // Adds what an accumulator of its own holds.  An MMA truncates its sums
+        // (of one sign over 2^20 tokens that is 2^-10 of them), so only a tile's
+        // products share one; of a score, a few where that shows (kExact).
         auto add_up = [](float (&to)[4], const float (&c)[4]) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) to[j] += c[j];
@@ -1059,12 +1060,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                             for (int set = 0; set < kPS; ++set)
 #pragma unroll
                                 for (int h = 0; h < 2; ++h)
-                                    mma16<false>(kExact ? own[h] : acc[2 * b + h], a[h][0], a[h][1], a[h][2], a[h][3], b0[set], b1[set]);
+                                    mma16<false>(own[h], a[h][0], a[h][1], a[h][2], a[h][3], b0[set], b1[set]);
                         }
-                        if (kExact) {
-                            add_up(acc[2 * b], own[0]);
-                            add_up(acc[2 * b + 1], own[1]);
-                        }
+                        add_up(acc[2 * b], own[0]);
+                        add_up(acc[2 * b + 1], own[1]);
                     }
                 }
             } else if constexpr (kF32) {
@@ -1146,15 +1145,14 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                         for (int j = 0; j < 4; ++j) {
                             if (j >= pairs) continue;
                             float own[4] = {};
-                            float(&to)[4] = kExact ? own : acc[off / 32 + j];
 #pragma unroll
                             for (int i = 0; i < MT; ++i) {
                                 const uint32_t a0 = __byte_perm(x[i][0][j], x[i][1][j], 0x5410), a1 = __byte_perm(x[i][0][j], x[i][1][j], 0x7632);
                                 const uint32_t a2 = __byte_perm(x[i][2][j], x[i][3][j], 0x5410), a3 = __byte_perm(x[i][2][j], x[i][3][j], 0x7632);
 #pragma unroll
-                                for (int set = 0; set < kPS; ++set) mma16<kBf16>(to, a0, a1, a2, a3, b0[i][set], b1[i][set]);
+                                for (int set = 0; set < kPS; ++set) mma16<kBf16>(own, a0, a1, a2, a3, b0[i][set], b1[i][set]);
                             }
-                            if (kExact) add_up(acc[off / 32 + j], own);
+                            add_up(acc[off / 32 + j], own);
                         }
                     }
                 }

@@ -879,3 +879,25 @@ def test_attend_query_with_a_loud_channel(dev_ctx, dtype, dim, group, loud):
     ds = (2 ** 11 + dim * 2.0 ** -4) * 2.0 ** -20
     assert_within(out, want, v.abs().max().double() * (4 * ds + 2.0 ** -17 + 2.0 ** -12))
     assert_within(lse, want_lse, torch.tensor(2 * ds + 2.0 ** -17, device="cuda", dtype=torch.float64), "lse")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "q8_0", "q4_0"])
+def test_attend_values_of_one_sign_over_a_million_tokens(dev_ctx, dtype):
+    """bf16 queries, so many sequences of 2^20 tokens (on the same pages) that one block walks the whole of one, and
+    positive values: what every sum loses in the same direction adds up.  A lane adds to its sum of probabilities
+    2^15 times and to an output 2^14 times; to nearest, errors of either sign, so at most 4 sqrt(2^15) 2^-24 =
+    2^-14.5 and 2^-15 of it.  With scores off by 2^-18 and probabilities rounded to 2^-12 each, either sign: 2^-13."""
+    g = gen(70)
+    n, dim, page, sequences = 1 << 20, 64, 4096, 600
+    kv = make_cache(dev_ctx, dtype, page, 1, dim, n // page)
+    table = torch.randperm(n // page, device="cuda", generator=g).int().expand(sequences, -1).contiguous()
+    k = torch.randn(n, 1, dim, device="cuda", generator=g)
+    v = (torch.rand(dim, device="cuda", generator=g) + 1) * (1 + torch.rand(n, 1, dim, device="cuda", generator=g) / 8)
+    kv.write(k.bfloat16(), v.bfloat16(), table[:1], cu_tokens=ragged([n]))
+    q = (torch.randn(sequences, 2, dim, device="cuda", generator=g) / 2).bfloat16()
+    out = torch.empty_like(q)
+    kv.attend(q, table, torch.full((sequences,), n, dtype=torch.int32, device="cuda"), out)
+    dev_ctx.synchronize()
+    for s in (0, 299, 599):
+        want, _, _, _ = attend_plain(kv, q[s:s + 1], table[s:s + 1], [n], page, 1, dim, dtype)
+        assert_within(out[s:s + 1], want, want.abs() * 2.0 ** -13, dtype)
