@@ -106,7 +106,10 @@ SAPPHIRE_API int kernel_gemv_device_noalloc(kernel_context_t *ctx, float *y, con
 SAPPHIRE_API int kernel_ctx_synchronize(kernel_context_t *ctx);
 /** The context's cudaStream_t (as void*). */
 SAPPHIRE_API void* kernel_ctx_get_stream(kernel_context_t *ctx);
-/** Use an external stream (void* cudaStream_t, NULL = legacy default stream). */
+/** Use an external stream (void* cudaStream_t, NULL = legacy default stream).
+ *  Waits for the old one.  -1, and the old one stays, where that may run work of
+ *  the context's and cannot be waited for: a capture began on it after it was
+ *  set, or it is the default stream and a blocking stream is being captured. */
 SAPPHIRE_API int kernel_ctx_set_stream(kernel_context_t *ctx, void *stream);
 /** CUDA ordinal the context is bound to, -1 for NULL. */
 SAPPHIRE_API int kernel_ctx_get_device(kernel_context_t *ctx);

@@ -224,7 +224,8 @@ extern "C" SAPPHIRE_API void kernel_ctx_destroy(kernel_context_t *ctx) {
         std::lock_guard<std::recursive_mutex> lk(ctx->exec_mutex);
         if (ctx->initialized || !ctx->weights.empty()) {
             DeviceGuard g(ctx->device);
-            if (ctx->stream) cudaStreamSynchronize(ctx->stream);
+            // (the NULL stream too: kernels write the error word, which no cudaFree waits for)
+            if (ctx->stream || ctx->initialized) cudaStreamSynchronize(ctx->stream);
             for (auto &kv : ctx->weights) free_weight(kv.second);
             ctx->weights.clear();
             if (ctx->d_x) cudaFree(ctx->d_x);
@@ -590,23 +591,60 @@ extern "C" SAPPHIRE_API void *kernel_ctx_get_stream(kernel_context_t *ctx) {
     return ctx ? (void *)ctx->stream : nullptr;
 }
 
+namespace {
+
+// While one lives, this thread's waits do not count against captures of other threads and streams.
+struct CaptureRelaxed {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    CaptureRelaxed() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~CaptureRelaxed() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
+// The capture that is going on on a stream, if any (on the NULL stream
+// cudaErrorStreamCaptureImplicit beside one of a blocking stream).
+cudaError_t stream_capture(cudaStream_t st, StreamCapture *c) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    const cudaError_t e = cudaStreamGetCaptureInfo(st, &status, &id);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return e;
+    }
+    c->on = status != cudaStreamCaptureStatusNone;
+    c->id = id;
+    return cudaSuccess;
+}
+
+}  // namespace
+
 extern "C" SAPPHIRE_API int kernel_ctx_set_stream(kernel_context_t *ctx, void *stream) {
     if (!ctx) return -1;
     std::lock_guard<std::recursive_mutex> lk(ctx->exec_mutex);
     DeviceGuard g(ctx->device);
     // What the old stream still runs may use the context's buffers, so it is
-    // waited for, the NULL stream too - unless it is being captured: a wait
-    // would end the capture, and nothing of it runs yet.  (Relaxed, because the
-    // wait is harmless to a capture on another stream.)
+    // waited for, the NULL stream too.  A stream that is being captured cannot
+    // be; nothing of the context's runs on it if that capture was going on when
+    // it was set, otherwise work from before the capture may.
+    CaptureRelaxed relaxed;
     if (ctx->initialized) {
-        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-        cudaThreadExchangeStreamCaptureMode(&mode);
-        cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-        if (cudaStreamIsCapturing(ctx->stream, &capturing) == cudaSuccess && capturing == cudaStreamCaptureStatusNone)
-            cudaStreamSynchronize(ctx->stream);
-        cudaThreadExchangeStreamCaptureMode(&mode);
-        cudaGetLastError();
+        StreamCapture now;
+        const cudaError_t e = stream_capture(ctx->stream, &now);
+        if (e == cudaErrorStreamCaptureImplicit) {
+            ctx_fail(ctx, "kernel_ctx_set_stream",
+                     "the default stream cannot be waited for while a blocking stream is being captured");
+            return -1;
+        }
+        if (e == cudaSuccess && now.on && !(ctx->capture.on && ctx->capture.id == now.id)) {
+            ctx_fail(ctx, "kernel_ctx_set_stream",
+                     "a capture began on the context's stream after it was set: work from before cannot be waited for");
+            return -1;
+        }
+        // (A stream that the caller has destroyed has nothing to wait for.)
+        if (e == cudaSuccess && !now.on) cudaStreamSynchronize(ctx->stream);
     }
+    ctx->capture = StreamCapture();
+    stream_capture((cudaStream_t)stream, &ctx->capture);
+    cudaGetLastError();
     if (ctx->own_stream && ctx->stream) cudaStreamDestroy(ctx->stream);
     ctx->stream = (cudaStream_t)stream;
     ctx->own_stream = false;

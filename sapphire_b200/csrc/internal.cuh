@@ -87,6 +87,12 @@ struct HostPool {
     std::atomic<int> next{0};
 };
 
+// A capture of a stream into a graph.
+struct StreamCapture {
+    bool on = false;
+    unsigned long long id = 0;
+};
+
 struct sapphire_context {
     int num_threads = 0;
     int chunk_size = 16;
@@ -95,6 +101,7 @@ struct sapphire_context {
     int device = 0;
     cudaStream_t stream = nullptr;
     bool own_stream = false;
+    StreamCapture capture;             // of `stream`, when it was set
     std::recursive_mutex exec_mutex;
 
     std::unordered_map<uint64_t, DevWeight> weights;

@@ -23,6 +23,7 @@ so out is off by 2^-12 max|v| more.
 """
 from __future__ import annotations
 
+import ctypes
 import math
 
 import numpy as np
@@ -901,3 +902,58 @@ def test_attend_values_of_one_sign_over_a_million_tokens(dev_ctx, dtype):
     for s in (0, 299, 599):
         want, _, _, _ = attend_plain(kv, q[s:s + 1], table[s:s + 1], [n], page, 1, dim, dtype)
         assert_within(out[s:s + 1], want, want.abs() * 2.0 ** -13, dtype)
+
+
+def test_set_stream_refuses_what_it_cannot_wait_for(sp, dev_ctx):
+    """Work from before a capture began on the context's stream, and work on the default stream while a blocking
+    stream is captured, cannot be waited for: the stream stays.  A stream that was set while captured holds no such
+    work (test_changing_streams)."""
+    st = torch.cuda.Stream()
+    dev_ctx.set_stream(st.cuda_stream)
+    x = torch.zeros(4, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        x += 1
+        with pytest.raises(sp.SapphireError, match="captur"):
+            dev_ctx.set_stream(0)
+    assert dev_ctx.stream == st.cuda_stream
+    graph.replay()                                        # the capture was not ended by it
+    torch.cuda.synchronize()
+    assert (x == 1).all()
+    dev_ctx.set_stream(0)
+    assert dev_ctx.stream == 0
+    # a capture that was going on when its stream was set, and another behind it
+    second, third = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(second, stream=st):
+        dev_ctx.set_stream(st.cuda_stream)
+        x += 1
+    with torch.cuda.graph(third, stream=st):
+        x += 1
+        with pytest.raises(sp.SapphireError, match="captur"):
+            dev_ctx.set_stream(0)
+    dev_ctx.set_stream(0)
+
+
+def test_set_stream_beside_the_capture_of_a_blocking_stream(sp, dev_ctx):
+    """The default stream cannot be waited for while a stream that waits for it is captured."""
+    cudart = torch.cuda.cudart()
+    handle = ctypes.c_void_p()
+    assert int(cudart.cudaStreamCreate(ctypes.addressof(handle))) == 0
+    blocking, other = torch.cuda.ExternalStream(handle.value), torch.cuda.Stream()
+    dev_ctx.set_stream(0)
+    x = torch.zeros(4, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=blocking):
+        x += 1
+        with pytest.raises(sp.SapphireError, match="captur"):
+            dev_ctx.set_stream(other.cuda_stream)
+        assert dev_ctx.stream == 0
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (x == 1).all()
+    dev_ctx.set_stream(other.cuda_stream)
+    dev_ctx.set_stream(0)
+    del graph
+    assert int(cudart.cudaStreamDestroy(handle.value)) == 0
