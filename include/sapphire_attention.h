@@ -20,7 +20,7 @@
  * by the next kernel_ctx_synchronize.  Strides are in elements; a stride of 0
  * means contiguous ([tokens, heads, head_dim], the last dimension always
  * contiguous).  No call allocates device memory except the first attention on
- * a context without a workspace of the caller's.
+ * a context without a workspace of the caller's (once, for calls of any shape).
  */
 #ifndef SAPPHIRE_ATTENTION_H
 #define SAPPHIRE_ATTENTION_H
@@ -178,7 +178,7 @@ typedef struct {
     float scale;             /* 0: 1 / sqrt(head_dim) */
     /* sapphire_attention_workspace_bytes of device memory, 16-byte aligned,
      * that no other call uses at the same time; its contents do not matter.
-     * NULL: the context's own (grown by the first call that needs it).  A call
+     * NULL: the context's own (allocated by the first call that needs it).  A call
      * captured into a graph keeps its workspace, so it has to bring one. */
     void *workspace;
     size_t workspace_bytes;

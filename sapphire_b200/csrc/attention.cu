@@ -20,6 +20,21 @@ size_t attn_workspace(kernel_context_t *ctx, const sapphire_kv_cache_t *c, int g
     return blocks * (sizeof(int4) + 2 * heads * (c->head_dim + 2) * sizeof(float));
 }
 
+// The largest of any call (under 5 MB), so that the context's never grows:
+// growing waits for the stream.
+size_t attn_workspace_most(kernel_context_t *ctx) {
+    size_t most = 0;
+    for (tensor_dtype_t type : {DTYPE_F32, DTYPE_BF16, DTYPE_F16, DTYPE_Q8_0, DTYPE_Q4_0})
+        for (int dim : {64, 96, 128, 192, 256})
+            for (int group : {1, 8}) {
+                sapphire_kv_cache_t c{};
+                c.dtype = type;
+                c.head_dim = dim;
+                most = std::max(most, attn_workspace(ctx, &c, group));
+            }
+    return most;
+}
+
 }  // namespace
 
 extern "C" SAPPHIRE_API size_t sapphire_attention_workspace_bytes(kernel_context_t *ctx,
@@ -130,7 +145,7 @@ extern "C" SAPPHIRE_API int sapphire_attention_device(kernel_context_t *ctx, con
         // The context's own begins with zeroed counters: with few blocks to an item
         // the last of them joins their pieces, which saves a launch.
         const size_t counts = ((size_t)sm_count(ctx->device) * kAttnMaxBlocks * sizeof(int) + 15) & ~(size_t)15;
-        if (ensure_scratch(ctx, &ctx->d_attn, &ctx->d_attn_cap, counts + need)) return -1;
+        if (!ctx->d_attn && ensure_scratch(ctx, &ctx->d_attn, &ctx->d_attn_cap, counts + attn_workspace_most(ctx))) return -1;
         ws = reinterpret_cast<char *>(ctx->d_attn) + counts;
         if (p.few_holders) p.count = reinterpret_cast<int *>(ctx->d_attn);
     }

@@ -957,3 +957,29 @@ def test_set_stream_beside_the_capture_of_a_blocking_stream(sp, dev_ctx):
     dev_ctx.set_stream(0)
     del graph
     assert int(cudart.cudaStreamDestroy(handle.value)) == 0
+
+
+def test_attend_context_workspace_does_not_grow(dev_ctx):
+    """The first call without a workspace allocates; a later one of a larger shape neither allocates nor waits for
+    what the stream still runs."""
+    sets = []
+    for dtype, dim, group in (("f32", 256, 1), ("f32", 64, 8), ("q8_0", 256, 8), ("q4_0", 128, 4), ("bf16", 128, 8)):
+        kv, table, q = attend_case(dev_ctx, dtype, "f32", [400, 30], 1, group, dim, 16, seed=dim)
+        n, out = torch.tensor([400, 30], dtype=torch.int32, device="cuda"), torch.empty_like(q)
+        # (once with a workspace, so that the kernels are loaded)
+        kv.attend(q, table, n, out, workspace=torch.empty(kv.workspace_bytes(2, group), dtype=torch.uint8, device="cuda"))
+        sets.append((kv, table, q, n, out, dtype, dim))
+    kv, table, q, n, out, _, _ = sets[0]
+    kv.attend(q, table, n, out)
+    dev_ctx.synchronize()
+    for kv, table, q, n, out, _, _ in sets:
+        torch.cuda._sleep(200_000_000)                    # cycles: about 0.1 s
+        slept = torch.cuda.Event()
+        slept.record()
+        kv.attend(q, table, n, out)
+        assert not slept.query()
+        torch.cuda.synchronize()
+    dev_ctx.synchronize()
+    for kv, table, q, n, out, dtype, dim in sets:
+        want, bound, _, _ = attend_plain(kv, q, table, [400, 30], 16, 1, dim, dtype)
+        assert_within(out, want, bound)
