@@ -211,6 +211,8 @@ class KVCache:
         op, os, oh = _heads(out, "out", n, heads, dim, dt)
         if lse is not None and (tuple(lse.shape) != (n, heads) or _io(lse, "lse") != DTYPE_F32 or not lse.is_contiguous()):
             raise SapphireError(f"lse must be contiguous float32 [{n}, {heads}]")
+        if workspace is not None and not workspace.is_contiguous():
+            raise SapphireError("workspace must be contiguous")
         table, stride = _table(page_table, n)
         args = AttentionArgs(dt, n, heads, qp, op, qs, qh, os, oh,
                              0 if lse is None else lse.data_ptr(), table, stride, _ints(lengths, "lengths", n),

@@ -107,3 +107,18 @@ def test_rope_configs_refused(sp, change, message):
     assert not sp.lib.sapphire_rope_create(ctx.handle, C.byref(cfg))
     assert message in ctx.last_error
     ctx.close()
+
+
+@pytest.mark.parametrize("bytes_", ["expanded", "strided"])
+def test_workspaces_whose_bytes_do_not_lie_together_are_refused(sp, bytes_):
+    """Its size is counted from its elements, so they have to be the bytes behind its address."""
+    torch = pytest.importorskip("torch")
+    from sapphire_b200.attention import KVCache, kv_page_bytes
+    ctx = sp.Context(num_threads=1, init=False)
+    kv = KVCache(ctx, "bf16", 16, 1, 64, torch.zeros(2, kv_page_bytes("bf16", 16, 1, 64), dtype=torch.uint8))
+    q = torch.zeros(1, 2, 64, dtype=torch.bfloat16)
+    one = torch.zeros(1, dtype=torch.uint8)
+    ws = one.expand(1 << 24) if bytes_ == "expanded" else torch.zeros(1 << 12, 2, dtype=torch.uint8)[:, 0]
+    with pytest.raises(sp.SapphireError, match="contiguous"):
+        kv.attend(q, torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, dtype=torch.int32), torch.empty_like(q), workspace=ws)
+    ctx.close()
