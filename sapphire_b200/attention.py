@@ -115,6 +115,8 @@ class Rope:
         x = q if q is not None else k
         if x is None:
             return
+        if not self.handle or not self.ctx.handle:
+            raise SapphireError("the rotation plan or its context is closed")
         n, dim = x.shape[0], self.head_dim
         dt = _io_seen.get(x.dtype)
         if dt is None:

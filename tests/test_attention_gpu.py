@@ -983,3 +983,21 @@ def test_attend_context_workspace_does_not_grow(dev_ctx):
     for kv, table, q, n, out, dtype, dim in sets:
         want, bound, _, _ = attend_plain(kv, q, table, [400, 30], 16, 1, dim, dtype)
         assert_within(out, want, bound)
+
+
+def test_rope_of_a_closed_plan_or_context(sp):
+    """The plan holds memory of its context: neither is used behind the other's end."""
+    from sapphire_b200.attention import Rope
+    ctx = sp.Context(num_threads=1)
+    ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+    a, b = Rope(ctx, 64), Rope(ctx, 64)
+    q, pos = torch.zeros(1, 1, 64, device="cuda"), torch.zeros(1, device="cuda", dtype=torch.int32)
+    a.apply(pos, q)
+    a.close()
+    with pytest.raises(sp.SapphireError, match="closed"):
+        a.apply(pos, q)
+    b.apply(pos, q)
+    ctx.close()
+    with pytest.raises(sp.SapphireError, match="closed"):
+        b.apply(pos, q)
+    b.close()
