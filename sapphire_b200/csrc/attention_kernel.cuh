@@ -75,6 +75,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 // the joining of the warps), in tiles: the ranges of blocks are cut in these
 // units, so one that meets many short sequences takes fewer tiles.
 constexpr int kAttnItemUnits = 2;
+// Positions of a sequence: tokens are numbered in 31 bits, and look-ups run up to
+// three times 2048 tokens ahead of a sequence's end.
+constexpr long long kAttnMaxTokens = 0x7fffc000;
 constexpr int kAttnMaxBlocks = 4;         // on an SM, of any variant
 
 struct AttnParams {
@@ -318,7 +321,7 @@ struct AttnSpan {
 template <int kTile>
 __device__ __forceinline__ AttnSpan attn_span(const AttnParams &p, int s, bool report) {
     long long n = (long long)__ldg(p.lengths + s) + p.length_offset;
-    const long long room = min((long long)p.table_stride * p.l.page_size, 0x7fffffc0ll);
+    const long long room = min((long long)p.table_stride * p.l.page_size, kAttnMaxTokens);
     if (n < 0 || n > room) {
         if (report) atomicOr(p.err, kErrCache);
         n = n < 0 ? 0 : room;

@@ -1001,3 +1001,27 @@ def test_rope_of_a_closed_plan_or_context(sp):
     with pytest.raises(sp.SapphireError, match="closed"):
         b.apply(pos, q)
     b.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "q8_0", "q4_0"])
+def test_attend_lengths_near_2_to_the_31(sp, dev_ctx, dtype):
+    """A window at the end of the longest sequence that positions of 31 bits allow, and lengths beyond it."""
+    g = gen(31)
+    page, dim, longest, window = 4096, 64, 2 ** 31 - 16384, 5000
+    kv = make_cache(dev_ctx, dtype, page, 1, dim, 3)
+    table = (torch.arange(2 ** 31 // page, device="cuda", dtype=torch.int32) % 3).expand(3, -1).contiguous()
+    k, v = (torch.randn(3 * page, 1, dim, device="cuda", generator=g) for _ in range(2))
+    kv.write(k, v, table[:1], cu_tokens=ragged([3 * page]))
+    q = torch.randn(3, 2, dim, device="cuda", generator=g)
+    out = torch.empty_like(q)
+    lengths = [longest - 5, 100, longest]
+    kv.attend(q, table, torch.tensor(lengths, dtype=torch.int32, device="cuda"), out, window=window)
+    dev_ctx.synchronize()
+    want, bound, _, _ = attend_plain(kv, q, table, lengths, page, 1, dim, dtype, window)
+    assert_within(out, want, bound)
+    again = torch.empty_like(q)
+    for beyond in (longest + 1, 2 ** 31 - 64, 2 ** 31 - 1):
+        kv.attend(q, table, torch.tensor([longest - 5, 100, beyond], dtype=torch.int32, device="cuda"), again, window=window)
+        with pytest.raises(sp.SapphireError, match="paged key-value cache"):
+            dev_ctx.synchronize()
+        assert torch.equal(again, out)
