@@ -46,7 +46,7 @@ extern "C" {
  *           lo = max(floor c(turns_fast), 0), hi = min(ceil c(turns_slow),
  *           rot_dim - 1), g = clamp((i - lo) / max(hi - lo, 0.001), 0, 1):
  *           (1 - g) f + g f / factor; cos and sin times attention_factor
- * Angles are exact to 2^-32 of a turn at any 32-bit position.
+ * Angles are within 2^-25 of a turn (that of fp32 half turns) at any 32-bit position.
  * ------------------------------------------------------------------------- */
 typedef enum {
     SAPPHIRE_ROPE_HALF = 0,         /* pairs (i, i + rot_dim / 2) */

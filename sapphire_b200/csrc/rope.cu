@@ -6,8 +6,8 @@
 // (src/transformer/rope.c:19-37).  Here a frequency is kept as a 64-bit
 // fixed-point fraction of a turn, F_i = round(f_i / 2pi * 2^64): position *
 // F_i mod 2^64 is the phase, reduced exactly by the overflow of an integer
-// product, good to 2^-32 of a turn at any 32-bit position, and sincospi takes
-// the reduced half turns.  No table is read, so a call moves its heads once in
+// product and good to 2^-32 of a turn at any 32-bit position; as the fp32 half
+// turns that sincospi takes it is good to 2^-26 of one.  No table is read, so a call moves its heads once in
 // and once out, and is bound by that: 16381 tokens x 40 bf16 heads of 128 take
 // 58 us, 5.8 TB/s.  Single tokens cost a launch.
 #include <cmath>
@@ -174,31 +174,33 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const RopeParams p) {
     }
 }
 
-// Frequencies in radians a position (include/sapphire_attention.h).
-double rope_frequency(const sapphire_rope_config_t &c, int i) {
-    const double pi = 3.14159265358979323846;
-    const double f = pow(c.theta, -2.0 * i / c.rot_dim);
+// Frequencies in radians a position (include/sapphire_attention.h), in the
+// host's 64-bit significands: a double's 2^-53 of one would be 2^-25 of a turn at
+// position 2^31.
+constexpr long double kPi = 3.14159265358979323846264338327950288L;
+long double rope_frequency(const sapphire_rope_config_t &c, int i) {
+    const long double f = powl(c.theta, -2.0L * i / c.rot_dim);
     if (c.scaling == SAPPHIRE_ROPE_LINEAR) return f / c.factor;
     if (c.scaling == SAPPHIRE_ROPE_BANDED) {
-        const double r = c.original_context * f / (2 * pi);
-        const double s = fmin(fmax((r - c.turns_slow) / (c.turns_fast - c.turns_slow), 0.0), 1.0);
+        const long double r = c.original_context * f / (2 * kPi);
+        const long double s = fminl(fmaxl((r - c.turns_slow) / ((long double)c.turns_fast - c.turns_slow), 0.0L), 1.0L);
         return (1 - s) * (f / c.factor) + s * f;
     }
     if (c.scaling == SAPPHIRE_ROPE_YARN) {
-        auto pair = [&](double turns) {
-            return c.rot_dim * log(c.original_context / (2 * pi * turns)) / (2 * log(c.theta));
+        auto pair = [&](long double turns) {
+            return c.rot_dim * logl(c.original_context / (2 * kPi * turns)) / (2 * logl(c.theta));
         };
-        const double lo = fmax(floor(pair(c.turns_fast)), 0.0);
-        const double hi = fmin(ceil(pair(c.turns_slow)), c.rot_dim - 1.0);
-        const double g = fmin(fmax((i - lo) / fmax(hi - lo, 1e-3), 0.0), 1.0);
+        const long double lo = fmaxl(floorl(pair(c.turns_fast)), 0.0L);
+        const long double hi = fminl(ceill(pair(c.turns_slow)), c.rot_dim - 1.0L);
+        const long double g = fminl(fmaxl((i - lo) / fmaxl(hi - lo, 1e-3L), 0.0L), 1.0L);
         return (1 - g) * f + g * (f / c.factor);
     }
     return f;
 }
 
 // Radians a position as a fraction of a turn in units of 2^-64.
-unsigned long long turn_fraction(double f) {
-    const long double turns = (long double)f / (2 * 3.14159265358979323846264338327950288L);
+unsigned long long turn_fraction(long double f) {
+    const long double turns = f / (2 * kPi);
     const long double frac = turns - floorl(turns);
     const long double x = frac * 18446744073709551616.0L;
     return x >= 18446744073709551615.0L ? 0ull : (unsigned long long)(x + 0.5L);

@@ -1025,3 +1025,25 @@ def test_attend_lengths_near_2_to_the_31(sp, dev_ctx, dtype):
         with pytest.raises(sp.SapphireError, match="paged key-value cache"):
             dev_ctx.synchronize()
         assert torch.equal(again, out)
+
+
+def test_rope_angles_at_the_farthest_positions(dev_ctx):
+    """cos and sin against decimals of 50 digits, without slack for the oracle: the phase is good to 2^-32 of a turn
+    and its fp32 half turns to 2^-26, so an angle is off by at most 2 pi 2^-25.9 < 2^-23.2, sincospi by one step
+    (2^-24) more."""
+    from decimal import Decimal, getcontext
+    from sapphire_b200.attention import Rope
+    getcontext().prec = 50
+    turn = 2 * Decimal("3.14159265358979323846264338327950288419716939937510")
+    pos = [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 77777, 1234567891, 2 ** 30 + 1, 3]
+    q = torch.zeros(len(pos), 1, 64, device="cuda")
+    q[..., :32] = 1.0
+    for theta, factor in ((1e4, 1), (5e5, 1), (1e6, 3)):
+        out = torch.empty_like(q)
+        Rope(dev_ctx, 64, theta=theta, scaling="linear", factor=factor).apply(
+            torch.tensor(pos, device="cuda", dtype=torch.int32), q, q_out=out)
+        dev_ctx.synchronize()
+        f = [(Decimal(theta).ln() * (Decimal(-2 * i) / 64)).exp() / factor for i in range(32)]
+        a = torch.tensor([[float(p * x / turn % 1 * turn) for x in f] for p in pos], dtype=torch.float64, device="cuda")
+        want = torch.cat((a.cos(), a.sin()), -1)[:, None]
+        assert (out.double() - want).abs().max().item() <= 2.0 ** -23.2 + 2.0 ** -24
