@@ -1047,3 +1047,73 @@ def test_rope_angles_at_the_farthest_positions(dev_ctx):
         a = torch.tensor([[float(p * x / turn % 1 * turn) for x in f] for p in pos], dtype=torch.float64, device="cuda")
         want = torch.cat((a.cos(), a.sin()), -1)[:, None]
         assert (out.double() - want).abs().max().item() <= 2.0 ** -23.2 + 2.0 ** -24
+
+
+# Sizes at which (on 148 SMs) a thread of the rotation walks down tokens (t) or heads (h), and its ends value by
+# value do (s).
+@pytest.mark.parametrize("kind,tokens,heads,kv_heads,dim,rot,layout,scaling", [
+    ("bf16", 9601, 8, 2, 128, 128, "half", "banded"),                # t
+    ("f32", 5003, 40, 8, 128, 128, "half", "none"),                  # t, h
+    ("f16", 5003, 40, 8, 128, 96, "interleaved", "linear"),          # h
+    ("bf16", 9601, 32, 8, 128, 128, "interleaved", "yarn"),          # t, h
+    ("f16", 9601, 2, 1, 512, 504, "half", "none"),                   # t, units of 4
+    ("f32", 20011, 4, 1, 96, 64, "half", "yarn"),                    # t
+    ("bf16", 4001, 64, 32, 256, 256, "half", "banded"),              # h
+    ("f32", 9601, 40, 8, 96, 22, "half", "none"),                    # t, h, s
+    ("bf16", 9601, 40, 8, 90, 42, "interleaved", "linear"),          # t, h, s
+])
+def test_rope_threads_that_walk(dev_ctx, kind, tokens, heads, kv_heads, dim, rot, layout, scaling):
+    test_rope(dev_ctx, tokens, heads, kv_heads, dim, rot, layout, kind, scaling)
+
+
+def test_rope_in_place_by_threads_that_walk(dev_ctx):
+    from sapphire_b200.attention import Rope
+    g = gen(9)
+    qkv = torch.randn(9601, 48, 128, device="cuda", generator=g).bfloat16()
+    before = qkv.clone()
+    pos = torch.randint(0, 131072, (9601,), device="cuda", generator=g, dtype=torch.int32)
+    Rope(dev_ctx, 128, rot_dim=96).apply(pos, qkv[:, :32], qkv[:, 32:40])
+    dev_ctx.synchronize()
+    want, e = rope_plain(before[:, :40], pos, 96, "half")
+    assert_within(qkv[:, :40], want, e)
+    assert torch.equal(qkv[:, 40:], before[:, 40:]) and torch.equal(qkv[..., 96:], before[..., 96:])
+
+
+# Sizes at which (on 148 SMs) a thread of the cache kernels walks down four batches of tokens (or two: 96 dims) and
+# down the heads, where a block has fewer rows than there are heads of K and V (256 x 5, 128 x 9, 192 x 12).
+@pytest.mark.parametrize("dtype", CACHES)
+@pytest.mark.parametrize("kind,rows,dim,heads,page", [
+    ("bf16", 4801, 128, 8, 16), ("f32", 6001, 256, 5, 7), ("f16", 6001, 128, 9, 64), ("bf16", 4801, 192, 12, 24),
+    ("f32", 9001, 96, 3, 16), ("f16", 12001, 64, 2, 100),
+])
+def test_write_and_read_by_threads_that_walk(sp, dev_ctx, ctx, dtype, kind, rows, dim, heads, page):
+    g = gen(dim + heads)
+    new = [rows // 3, 0, 1, rows - rows // 3 - 1 - 70]                # 70 rows belong to no sequence
+    before = [0, 3, 2 * page, 5]
+    total = [a + b for a, b in zip(before, new)]
+    pages = sum(-(-n // page) for n in total) + 2
+    kv = make_cache(dev_ctx, dtype, page, heads, dim, pages, fill=0xA5)
+    table = make_table(total, page, pages, g)
+    k, v = (torch.randn(rows, heads, dim, device="cuda", generator=g).to(IO[kind]) for _ in range(2))
+    old = kv.pages.clone()
+    start = torch.tensor(before, dtype=torch.int32, device="cuda")
+    kv.write(k, v, table, start=start, cu_tokens=ragged(new))
+    ko, vo = torch.full_like(k, 7.0), torch.full_like(v, 7.0)
+    kv.read(ko, vo, table, start=start, cu_tokens=ragged(new))
+    dev_ctx.synchronize()
+    n = sum(new)
+    t = torch.cat([torch.arange(b, b + m, device="cuda") for b, m in zip(before, new)])
+    seq = torch.repeat_interleave(torch.arange(4, device="cuda"), torch.tensor(new, device="cuda"))
+    pg, slot = table[seq, t // page].long(), t % page
+    for j, x, out in ((0, k, ko), (1, v, vo)):
+        got = cache_values(kv.pages, dtype, page, heads, dim, j)[pg, :, slot]
+        assert torch.equal(got, expected_store(sp, ctx, x, dtype)[:n])
+        assert torch.equal(out[:n], got.float().to(IO[kind])) and (out[n:] == 7.0).all()
+    # slots that no row went to keep their bytes
+    free = torch.ones(pages, page, dtype=torch.bool, device="cuda")
+    free[pg, slot] = False
+    rb, ns, at, chunk = layout(dtype, dim, page)
+    a, b = (x.reshape(pages, heads, chunk) for x in (kv.pages, old))
+    for o, size in ((at[0], rb), (at[1], rb), (at[2], 4 * ns), (at[3], 4 * ns)):
+        u, w = (x[..., o:o + page * size].reshape(pages, heads, page, size).transpose(1, 2)[free] for x in (a, b))
+        assert torch.equal(u, w)
