@@ -276,3 +276,76 @@ def test_paged_decoder_refusals(sp, ctx):
     for kv, page in (("tq2_0", 16), ("f32", 0), ("q8_0", 5000)):
         with pytest.raises(sp.SapphireError, match="no cache of this type"):
             Decoder(ctx, cfg, model, kv_dtype=kv, kv_page_size=page)
+
+
+def rounded_store(sp, ctx, kv):
+    """What a cache of type kv holds of x [positions, heads, dim], quantised by the library's quantisers."""
+    import torch
+
+    def store(x):
+        if kv in ("f32", "bf16", "f16"):
+            return x.to({"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[kv]).double()
+        size = 36 if kv == "q8_0" else 20
+        flat = np.ascontiguousarray(x.float().cpu().numpy().reshape(-1, x.shape[-1]))
+        b = sp.quantize(ctx, sp.DTYPE_Q8_0 if kv == "q8_0" else Q4_0, flat).reshape(-1, size)
+        scale = b[:, :4].copy().view(np.float32).astype(np.float64)
+        codes = b[:, 4:].view(np.int8) if kv == "q8_0" else \
+            np.stack((b[:, 4:] & 15, b[:, 4:] >> 4), -1).reshape(len(b), 32).astype(np.float64) - 8
+        return torch.from_numpy((codes * scale).reshape(x.shape)).to(x.device)
+    return store
+
+
+# Each of six layers adds four products to what its logits depend on, and the head one: 25 times the parity bar of
+# a product (1e-4) bounds the relative error of the logits.  (A code at the border of two may fall to either side:
+# one in 10^5 of them by fp32 rounding.)
+LOGITS_RTOL = 25e-4
+
+
+@pytest.mark.parametrize("kv,page", [("f32", 16), ("bf16", 24), ("f16", 50), ("q8_0", 16), ("q8_0", 7), ("q4_0", 32),
+                                     ("q4_0", 5)])
+def test_paged_decoder_against_a_plain_decode_of_the_same_cache(sp, ctx, kv, page):
+    """Logits at the first positions, inside the window and behind it, against the 64-bit decode whose keys and
+    values are rounded as the cache's type rounds them; a decode with others is further away than the tolerance."""
+    from decode_plain import plain_logits
+    from sapphire_b200 import workloads
+    from sapphire_b200.decode import Decoder
+    cfg = workloads.GQA_TINY
+    model = workloads.make_decode_model(cfg, lambda a: sp.quantize(ctx, Q4_0, a), seed=3)
+    tokens = np.random.default_rng(11).integers(0, cfg.vocab, size=120).astype(np.int32)
+    lengths = [1, 2, 5, 16, 33, 90, 120]
+    want = plain_logits(cfg, model, tokens, [n - 1 for n in lengths], rounded_store(sp, ctx, kv), "cuda").cpu().numpy()
+    other = plain_logits(cfg, model, tokens, [n - 1 for n in lengths], rounded_store(sp, ctx, "q4_0" if kv != "q4_0" else "q8_0"),
+                         "cuda").cpu().numpy()
+    dec = Decoder(ctx, cfg, model, kv_dtype=kv, kv_page_size=page)
+    try:
+        for n, w, o in zip(lengths, want, other):
+            dec.generate(tokens[:n], 1)
+            error = np.linalg.norm(dec.last_logits() - w) / np.linalg.norm(w)
+            assert error <= LOGITS_RTOL, (n, error)
+            assert np.linalg.norm(o - w) > 4 * LOGITS_RTOL * np.linalg.norm(w)
+    finally:
+        dec.close()
+
+
+@pytest.mark.parametrize("kv", ["f32", "q8_0", "q4_0"])
+def test_paged_decoder_past_the_dense_context(sp, ctx, kv):
+    """Logits behind 4096 positions against the 64-bit decode: windows, angles and offsets there."""
+    from decode_plain import plain_logits
+    from sapphire_b200 import workloads
+    from sapphire_b200.decode import Decoder
+    cfg = dataclasses.replace(workloads.GQA_TINY, context=6000)
+    model = workloads.make_decode_model(cfg, lambda a: sp.quantize(ctx, Q4_0, a), seed=3)
+    tokens = np.random.default_rng(12).integers(0, cfg.vocab, size=4500).astype(np.int32)
+    lengths = [4097, 4500]
+    want = plain_logits(cfg, model, tokens, [n - 1 for n in lengths], rounded_store(sp, ctx, kv), "cuda").cpu().numpy()
+    # the same with every token but the last 3000 left out: positions and the global layer's reach count
+    near = plain_logits(cfg, model, tokens[-3000:], [2999], rounded_store(sp, ctx, kv), "cuda").cpu().numpy()[0]
+    dec = Decoder(ctx, cfg, model, kv_dtype=kv, kv_page_size=64)
+    try:
+        for n, w in zip(lengths, want):
+            dec.generate(tokens[:n], 1)
+            error = np.linalg.norm(dec.last_logits() - w) / np.linalg.norm(w)
+            assert error <= LOGITS_RTOL, (n, error)
+        assert np.linalg.norm(near - want[-1]) > 2 * LOGITS_RTOL * np.linalg.norm(want[-1])
+    finally:
+        dec.close()
