@@ -17,7 +17,8 @@
  * kernel_gemv_device.  Return convention: 0 on success, -1 on error (details
  * via kernel_ctx_last_error).  What only the device can see - a page number, a
  * position or a length outside the cache - is skipped there and returned as -1
- * by the next kernel_ctx_synchronize.  Strides are in elements; a stride of 0
+ * by the next kernel_ctx_synchronize, or by a call before it that waits for its
+ * own result (kernel_gemv, a decoder).  Strides are in elements; a stride of 0
  * means contiguous ([tokens, heads, head_dim], the last dimension always
  * contiguous).  No call allocates device memory except the first attention on
  * a context without a workspace of the caller's (once, for calls of any shape).

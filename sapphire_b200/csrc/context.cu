@@ -392,16 +392,17 @@ int check_kernel_error(kernel_context_t *ctx, const char *who) {
     // A GEMV warp that gave up left the arrival counts of the tiles it had
     // joined behind; later launches sharing the counters would miscount.
     if (ctx->d_cnt && ctx->d_cnt_cap) cudaMemsetAsync(ctx->d_cnt, 0, ctx->d_cnt_cap, ctx->stream);
-    if (bits & 32)
-        ctx_fail(ctx, who, "a page number, position or length was outside the paged key-value cache");
-    else if (bits & 8)
+    const int cache = bits & 32;          // named only where nothing else went wrong
+    if (bits & 8)
         ctx_fail(ctx, who, "a peer-memory gather gave up waiting for another rank's rows (bounded wait expired)");
     else if (bits & 16)
         ctx_fail(ctx, who, "a persistent decode step gave up waiting for another block's output (bounded wait expired)");
-    else if (bits == 4)
+    else if ((bits & ~cache) == 4)
         ctx_fail(ctx, who, "a token id outside the vocabulary reached the embedding");
-    else
+    else if (bits & ~cache)
         ctx_fail(ctx, who, "a kernel gave up waiting for its asynchronous copies (bounded wait expired)");
+    else
+        ctx_fail(ctx, who, "a page number, position or length was outside the paged key-value cache");
     return -1;
 }
 

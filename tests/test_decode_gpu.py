@@ -349,3 +349,25 @@ def test_paged_decoder_past_the_dense_context(sp, ctx, kv):
         assert np.linalg.norm(near - want[-1]) > 2 * LOGITS_RTOL * np.linalg.norm(want[-1])
     finally:
         dec.close()
+
+
+def test_an_expired_wait_is_named_before_a_bad_page(sp, ctx, decoder):
+    """Both at the same synchronisation: the message names the wait."""
+    import torch
+    from sapphire_b200.attention import KVCache, kv_page_bytes
+    from sapphire_b200.decode import Decoder
+    cfg, model, _ = decoder
+    kv = KVCache(ctx, "bf16", 16, 1, 64, torch.zeros(1, kv_page_bytes("bf16", 16, 1, 64), dtype=torch.uint8, device="cuda"))
+    x = torch.zeros(1, 1, 64, dtype=torch.bfloat16, device="cuda")
+    torch.cuda.synchronize()
+    kv.write(x, x, torch.full((1, 1), 7, dtype=torch.int32, device="cuda"))
+    prev = sp.lib.sapphire_test_decode_stall(1)
+    try:
+        with pytest.raises(sp.SapphireError, match="gave up waiting"):
+            Decoder(ctx, cfg, model)
+    finally:
+        sp.lib.sapphire_test_decode_stall(prev)
+    ctx.synchronize()
+    kv.write(x, x, torch.full((1, 1), 7, dtype=torch.int32, device="cuda"))
+    with pytest.raises(sp.SapphireError, match="paged key-value cache"):
+        ctx.synchronize()
