@@ -107,7 +107,7 @@ SAPPHIRE_API int kernel_ctx_synchronize(kernel_context_t *ctx);
 /** The context's cudaStream_t (as void*). */
 SAPPHIRE_API void* kernel_ctx_get_stream(kernel_context_t *ctx);
 /** Use an external stream (void* cudaStream_t, NULL = legacy default stream).
- *  Waits for the old one.  -1, and the old one stays, where that may run work of
+ *  Waits for the old one; the context's first one may be set again.  -1, and the old one stays, where that may run work of
  *  the context's and cannot be waited for: a capture began on it after it was
  *  set, or it is the default stream and a blocking stream is being captured. */
 SAPPHIRE_API int kernel_ctx_set_stream(kernel_context_t *ctx, void *stream);

@@ -185,7 +185,7 @@ extern "C" SAPPHIRE_API int kernel_ctx_init(kernel_context_t *ctx) {
     DeviceGuard g(ctx->device);
     if (!ctx->stream) {
         CUDA_TRY(ctx, cudaStreamCreateWithFlags(&ctx->stream, cudaStreamNonBlocking));
-        ctx->own_stream = true;
+        ctx->own_stream = ctx->stream;
     }
     if (ensure_err_word(ctx)) return -1;
     if (!ctx->pool) {
@@ -238,7 +238,7 @@ extern "C" SAPPHIRE_API void kernel_ctx_destroy(kernel_context_t *ctx) {
             if (ctx->d_attn) cudaFree(ctx->d_attn);
             if (ctx->h_err) cudaFreeHost(ctx->h_err);
             shard_destroy(ctx);
-            if (ctx->own_stream && ctx->stream) cudaStreamDestroy(ctx->stream);
+            if (ctx->own_stream) cudaStreamDestroy(ctx->own_stream);
         }
         if (ctx->pool) {
             HostPool *p = ctx->pool;
@@ -646,9 +646,7 @@ extern "C" SAPPHIRE_API int kernel_ctx_set_stream(kernel_context_t *ctx, void *s
     ctx->capture = StreamCapture();
     stream_capture((cudaStream_t)stream, &ctx->capture);
     cudaGetLastError();
-    if (ctx->own_stream && ctx->stream) cudaStreamDestroy(ctx->stream);
     ctx->stream = (cudaStream_t)stream;
-    ctx->own_stream = false;
     return 0;
 }
 

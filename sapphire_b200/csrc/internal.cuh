@@ -100,7 +100,7 @@ struct sapphire_context {
     bool fp32_products = false;    // batched Q4_0 products keep fp32 activations (kernel_ctx_set_fp32_products)
     int device = 0;
     cudaStream_t stream = nullptr;
-    bool own_stream = false;
+    cudaStream_t own_stream = nullptr; // made by kernel_ctx_init, the context's for as long as it lives
     StreamCapture capture;             // of `stream`, when it was set
     std::recursive_mutex exec_mutex;
 

@@ -1117,3 +1117,24 @@ def test_write_and_read_by_threads_that_walk(sp, dev_ctx, ctx, dtype, kind, rows
     for o, size in ((at[0], rb), (at[1], rb), (at[2], 4 * ns), (at[3], 4 * ns)):
         u, w = (x[..., o:o + page * size].reshape(pages, heads, page, size).transpose(1, 2)[free] for x in (a, b))
         assert torch.equal(u, w)
+
+
+def test_the_first_stream_may_be_set_again(sp):
+    """kernel_ctx_get_stream, another stream, and back."""
+    ctx = sp.Context(num_threads=1)
+    first = ctx.stream
+    ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+    kv, table, q = attend_case(ctx, "bf16", "bf16", [40, 3], 1, 2, 64, 16)
+    n = torch.tensor([40, 3], dtype=torch.int32, device="cuda")
+    outs = [torch.empty_like(q) for _ in range(3)]
+    torch.cuda.synchronize()
+    kv.attend(q, table, n, outs[0])
+    for out in outs[1:]:
+        ctx.set_stream(first)
+        ctx.set_stream(ctx.stream)
+        assert ctx.stream == first
+        kv.attend(q, table, n, out)
+        ctx.synchronize()
+        ctx.set_stream(0)
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+    ctx.close()
