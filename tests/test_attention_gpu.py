@@ -1138,3 +1138,39 @@ def test_the_first_stream_may_be_set_again(sp):
         ctx.set_stream(0)
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
     ctx.close()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "q8_0", "q4_0"])
+@pytest.mark.parametrize("page", [16, 24])
+def test_attend_pages_before_the_window_may_be_gone(dev_ctx, dtype, page):
+    """Table entries of positions before the window are not looked at: freed ones (-1, or of another sequence)
+    change nothing and are no error."""
+    lengths, window = [1000, 333, 40], 100
+    kv, table, q = attend_case(dev_ctx, dtype, "bf16", lengths, 2, 4, 128, page, seed=page)
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    a, b = torch.empty_like(q), torch.empty_like(q)
+    kv.attend(q, table, n, a, window=window)
+    gone = table.clone()
+    for s, m in enumerate(lengths):
+        first = max(0, m - window) // page
+        gone[s, :first] = torch.tensor([-1, 2 ** 31 - 1], device="cuda", dtype=torch.int32).repeat(first)[:first]
+    kv.attend(q, gone, n, b, window=window)
+    dev_ctx.synchronize()
+    assert torch.equal(a, b)
+
+
+def test_attend_most_sequences_and_heads(dev_ctx):
+    """65535 sequences of few tokens on shared pages, and 1024 KV heads."""
+    g = gen(50)
+    kv, held, _ = attend_case(dev_ctx, "q8_0", "bf16", [200], 1, 1, 64, 16, seed=51)
+    n = torch.randint(0, 40, (65535,), device="cuda", generator=g, dtype=torch.int32)
+    table = held[0, torch.randint(0, 12, (65535, 3), device="cuda", generator=g)]     # full pages of the sequence
+    q = torch.randn(65535, 2, 64, device="cuda", generator=g).bfloat16()
+    out = torch.full_like(q, 3.0)
+    kv.attend(q, table, n, out)
+    dev_ctx.synchronize()
+    some = torch.cat((torch.arange(40), torch.arange(30000, 30040), torch.arange(65495, 65535))).cuda()
+    want, bound, _, _ = attend_plain(kv, q[some], table[some], n[some].tolist(), 16, 1, 64, "q8_0")
+    assert_within(out[some], want, bound)
+    assert (out[n == 0] == 0).all()
+    check_attend(dev_ctx, "f16", "f32", [70, 0, 5], 1024, 1, 64, 16, seed=52)
