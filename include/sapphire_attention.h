@@ -177,7 +177,7 @@ typedef struct {
     const int *lengths;      /* [sequences] */
     int length_offset;
     int window;
-    float scale;             /* 0: 1 / sqrt(head_dim) */
+    float scale;             /* 0: 1 / sqrt(head_dim); finite, times log2 e too */
     /* sapphire_attention_workspace_bytes of device memory, 16-byte aligned,
      * that no other call uses at the same time; its contents do not matter.
      * NULL: the context's own (allocated by the first call that needs it).  A call

@@ -71,8 +71,8 @@ extern "C" SAPPHIRE_API int sapphire_attention_device(kernel_context_t *ctx, con
         return -1;
     }
     if (a->sequences == 0) return 0;
-    if (a->table_stride <= 0 || a->window < 0 || !std::isfinite(a->scale)) {
-        ctx_fail(ctx, who, "table_stride must be positive, window not negative and scale finite");
+    if (a->table_stride <= 0 || a->window < 0 || !std::isfinite(a->scale * kLog2e)) {
+        ctx_fail(ctx, who, "table_stride must be positive, window not negative and scale finite (times log2 e too)");
         return -1;
     }
     if (!on_device(ctx, who, "pages", cache->pages) || !on_device(ctx, who, "q", a->q) ||

@@ -1174,3 +1174,14 @@ def test_attend_most_sequences_and_heads(dev_ctx):
     assert_within(out[some], want, bound)
     assert (out[n == 0] == 0).all()
     check_attend(dev_ctx, "f16", "f32", [70, 0, 5], 1024, 1, 64, 16, seed=52)
+
+
+def test_attend_scales_beyond_fp32_are_refused(sp, dev_ctx):
+    """Scores are kept times log2(e), so a scale is refused where that is not finite."""
+    kv, table, q = attend_case(dev_ctx, "bf16", "f32", [4], 1, 1, 64, 16)
+    n, out = torch.tensor([4], dtype=torch.int32, device="cuda"), torch.empty_like(q)
+    for scale in (3e38, -3e38):
+        with pytest.raises(sp.SapphireError, match="scale"):
+            kv.attend(q, table, n, out, scale=scale)
+    kv.attend(q, table, n, out, scale=2e38)
+    dev_ctx.synchronize()
