@@ -158,7 +158,9 @@ SAPPHIRE_API int sapphire_kv_read_device(kernel_context_t *ctx, const sapphire_k
  * with no position to attend to gets zeros, and -inf in lse.  What lies in
  * slots that are not attended to (NaN included) has no effect.  A NaN or an
  * infinity that is attended to makes the outputs it enters NaN or infinite
- * (an infinity may come out as NaN) and no others.  A length below 0 counts as
+ * (an infinity may come out as NaN) and no others; a head whose every score is
+ * -inf gets zeros.  A finite fp32 value from 2^128 (1 - 2^-9) on may count as
+ * infinite.  A length below 0 counts as
  * 0, one beyond the table (or 2^31 - 16384) as that end, and a token on a page
  * outside the cache does not count; each is an error at the next
  * kernel_ctx_synchronize.

@@ -75,7 +75,9 @@ SAPPHIRE_API sapphire_decoder_t *sapphire_decoder_create(kernel_context_t *ctx, 
  *  of page_size positions of type kv_dtype: F32, BF16, F16, or Q8_0 / Q4_0, which
  *  hold 3.6 / 6.4 times the context of F32 in the same memory.  The context may
  *  reach 2^20 positions (4096 otherwise).  Every stage is its own kernel (9 per
- *  layer): QK-norm, rotation, cache write and attention are the operators of
+ *  layer), so where the persistent step of sapphire_decoder_create fits a model
+ *  it is the faster one (Gemma-3-270M, context 2048: 0.43 ms a token against 0.74
+ *  to 0.81): QK-norm, rotation, cache write and attention are the operators of
  *  sapphire_attention.h, angles exact at far positions instead of the
  *  reference's fp32 tables. */
 SAPPHIRE_API sapphire_decoder_t *sapphire_decoder_create_paged(kernel_context_t *ctx,

@@ -8,14 +8,16 @@
 //
 // What bounds it: every visible K and V row is read once from HBM, so the work
 // is laid out to stream rows and to keep everything else off that path.  64
-// sequences of 8192, 8 KV heads of 128, 4 query heads each (of 6554 GB/s): bf16
-// 348 us, 0.94; Q8_0 204 us, 0.90; F32 364 us at 32 sequences, 0.90.  Q4_0
-// 147 us, 0.70, and 2 x 131071 with 5 query heads 87 us, 0.59, are bound by
-// instructions: schedulers issue in 0.6 of the cycles, a third of them ALU, and
-// unpacking is the most.  Short calls are latency: one fp32 sequence of 577
-// takes 11 us, a block's chain of lengths, page table, rows and joining (20 k
-// cycles: 2.5 k to its first item, 5 k to its first rows, 4 k for a tile, 8 k for
-// the joins of its warps and of the blocks).
+// sequences of 8192, 8 KV heads of 128, 4 query heads each (of 6554 GB/s; two
+// GPUs): bf16 350 - 358 us, 0.92 - 0.94; Q8_0 207 - 225 us, 0.82 - 0.89; F32 404 -
+// 437 us at 32 sequences, 0.75 - 0.81; Q4_0 166 - 176 us, 0.58 - 0.62.  2 x 131071
+// over Q4_0 with 5 query heads take 91 - 95 us, 0.54 - 0.56: DRAM is at 0.44 of
+// its peak, a scheduler issues in 0.60 of the cycles and no pipe is near full (ALU
+// 0.47), so it is the chain of each of a scheduler's 2.8 warps (copies, scores,
+// softmax, unpacking, values) that holds it up.  Short calls are latency: one
+// fp32 sequence of 577 takes 11 us, a block's chain of lengths, page table, rows and
+// joining (20 k cycles: 2.5 k to its first item, 5 k to its first rows, 4 k for a
+// tile, 8 k for the joins of its warps and of the blocks).
 //
 // Layout.  A warp takes 16 tokens at a time, or 32 where rows are short.  Scores are S^T = K Q^T and
 // outputs O^T = V^T P^T with warp MMAs whose M side is the tile (16 tokens, or
@@ -28,8 +30,10 @@
 //   wide: 8 heads are the columns and each part is an MMA of its own, one part
 //     where it is exact (a bf16 query) or its rounding is far below the
 //     output's (an fp16 probability under a bf16 output: 2^-12 against 2^-9).
-// A tcgen05 tile would leave 120 of its 128 rows empty here; the MMAs below are
-// a few percent of the pass.  Rows come by asynchronous copies into two slots of
+// The MMAs are a few percent of the pass (a fifth over Q4_0).  tcgen05 tiles of
+// 128 tokens or dims by 8 or 16 heads were not tried: their operands come from
+// shared memory, so quantised rows would be written back unpacked, and K's scales
+// need an accumulator for each 32 dims.  Rows come by asynchronous copies into two slots of
 // a warp, K's and V's, while the other's is used, and a lane reads its fragments
 // as vectors: the order of dims inside an MMA is free as long as both operands
 // share it, so a lane's consecutive bytes of a row are its fragment.
@@ -43,7 +47,10 @@
 // Quantised rows are kept as words of 4 codes in the order [8][nb], so the same
 // lanes read consecutive bytes.  V's codes become fp16 exactly (1024 + code - 1152,
 // or - 1032), and V's scale multiplies the probability, the product brought into
-// fp16's range by a power of two per warp that follows the largest seen.  K's codes become
+// fp16's range by a power of two per warp that follows the largest seen (products
+// below 2^-27 of that lose bits).  Under a bf16 output it is rounded to fp16 once,
+// 2^-12 of it against the output's 2^-9; so is the probability of wide tiles over
+// fp16 rows.  K's codes become
 // fp16 the same way, except in narrow tiles under a bf16 query: there they are
 // multiplied as the integers they are by the query as 23-bit integers (three
 // signed bytes in two MMAs), the sums exact, and a product with K's scale brings
@@ -433,7 +440,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
     const int s0 = min(tid * per_thread, p.sequences), s1 = min(s0 + per_thread, p.sequences);
     // The sides' blocks of one rank walk the same tokens for head tiles of their
     // own, so a row comes from HBM once and from L2 for the others (64 x 8192, 16
-    // query heads to a KV head of 128: bf16 687 -> 454 us, Q8_0 402 -> 350 us
+    // query heads to a KV head of 128: bf16 704 -> 576 us, Q8_0 454 -> 425 us
     // against one tile behind another).  An item: a KV head and one of this
     // side's head tiles.
     const int side = blockIdx.y, side_tiles = p.side_tiles, side_blocks = gridDim.x;
@@ -797,16 +804,16 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
 #pragma unroll
                     for (int b = 0; b < NB; ++b) {
                         uint4 q[kQS];
-    #pragma unroll
+#pragma unroll
                         for (int set = 0; set < kQS; ++set)
                             q[set] = *reinterpret_cast<const uint4 *>(sq + (set * 8 + g) * Sh::kQStride + 64 * b + 16 * t);
-    #pragma unroll
+#pragma unroll
                         for (int i = 0; i < MT; ++i) {
                             uint32_t a[2][4];
-    #pragma unroll
+#pragma unroll
                             for (int r = 0; r < 2; ++r) {
                                 if constexpr (kCache == DTYPE_Q8_0) {
-    #pragma unroll
+#pragma unroll
                                     for (int h = 0; h < 2; ++h) {
                                         const uint32_t w = kr[i][r][h * NB + b];
                                         a[h][r] = bytes_to_half2<0x5150>(w, codes);
@@ -823,12 +830,12 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                                 }
                             }
                             float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    #pragma unroll
+#pragma unroll
                             for (int set = 0; set < kQS; ++set) {
                                 mma16<false>(c, a[0][0], a[0][1], a[0][2], a[0][3], q[set].x, q[set].y);
                                 mma16<false>(c, a[1][0], a[1][1], a[1][2], a[1][3], q[set].z, q[set].w);
                             }
-    #pragma unroll
+#pragma unroll
                             for (int r = 0; r < 2; ++r) {
                                 if constexpr (kWide) {
                                     s[0][2 * i + r] = fmaf(ks[i][r][b], c[2 * r], s[0][2 * i + r]);

@@ -8,7 +8,7 @@
 //
 // Both directions move each value once in and once out and are bound by that:
 // 8192 fp16 tokens of 8 KV heads of 128 into Q8_0 pages and 65193 back out take
-// 92 us, 5.1 TB/s, in two launches.  A step of one token a sequence costs its
+// 94 us, 5.0 TB/s, in two launches.  A step of one token a sequence costs its
 // launch.
 #include <cstring>
 

@@ -9,7 +9,7 @@
 // product and good to 2^-32 of a turn at any 32-bit position; as the fp32 half
 // turns that sincospi takes it is good to 2^-26 of one.  No table is read, so a call moves its heads once in
 // and once out, and is bound by that: 16381 tokens x 40 bf16 heads of 128 take
-// 58 us, 5.8 TB/s.  Single tokens cost a launch.
+// 59 us, 5.7 TB/s.  Single tokens cost a launch.
 #include <cmath>
 #include <cstring>
 
