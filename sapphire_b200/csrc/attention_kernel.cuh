@@ -48,9 +48,10 @@
 // lanes read consecutive bytes.  V's codes become fp16 exactly (1024 + code - 1152,
 // or - 1032), and V's scale multiplies the probability, the product brought into
 // fp16's range by a power of two per warp that follows the largest seen (products
-// below 2^-27 of that lose bits).  Under a bf16 output it is rounded to fp16 once,
-// 2^-12 of it against the output's 2^-9; so is the probability of wide tiles over
-// fp16 rows.  K's codes become
+// below 2^-27 of that lose bits).  Wide tiles under a bf16 output round it to fp16
+// once, 2^-12 of it against the output's 2^-9, and the probability over fp16 rows
+// too; a second part would cost 9 to 12 % there (2 x 131071 over Q4_0, 5 heads: 96
+// -> 107 us), 0.5 to 3 % in narrow tiles, which have it.  K's codes become
 // fp16 the same way, except in narrow tiles under a bf16 query: there they are
 // multiplied as the integers they are by the query as 23-bit integers (three
 // signed bytes in two MMAs), the sums exact, and a product with K's scale brings
@@ -961,9 +962,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
 #pragma unroll
                     for (int set = 0; set < kPS; ++set) {
                         uint32_t u;
-                        if constexpr (kInt) {
-                            u = pack16<kBf16>(y[0], 0.0f);        // one part
-                        } else if constexpr (kWide) {
+                        if constexpr (kWide) {
                             u = pack16<kBf16>(y[0], y[HL - 1]);
                             if (set + 1 < kPS) {
                                 take16<kBf16>(y[0]);

@@ -1185,3 +1185,21 @@ def test_attend_scales_beyond_fp32_are_refused(sp, dev_ctx):
             kv.attend(q, table, n, out, scale=scale)
     kv.attend(q, table, n, out, scale=2e38)
     dev_ctx.synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "q8_0", "q4_0"])
+@pytest.mark.parametrize("dim,group", [(64, 1), (128, 4), (256, 3)])
+def test_attend_probabilities_of_small_groups_are_not_rounded_to_fp16(dev_ctx, dtype, dim, group):
+    """Groups of at most 4 heads under bf16 outputs: with queries so small that the scores' own error vanishes, a
+    value is off by the output's rounding and fp32's."""
+    lengths, heads, page = [3, 40, 1, 7, 500], 8, 16
+    kv, table, q = attend_case(dev_ctx, dtype, "bf16", lengths, heads, group, dim, page, seed=dim)
+    q, out = q * 2.0 ** -10, torch.empty_like(q)
+    kv.attend(q, table, torch.tensor(lengths, dtype=torch.int32, device="cuda"), out)
+    dev_ctx.synchronize()
+    want, _, _, _ = attend_plain(kv, q, table, lengths, page, heads, dim, dtype)
+    used = torch.cat([table[s, :-(-n // page)] for s, n in enumerate(lengths)]).long()
+    k, v = (cache_values(kv.pages, dtype, page, heads, dim, j)[used].nan_to_num(0.0, 0.0, 0.0) for j in (0, 1))
+    ds = dim ** -0.5 * q.abs().max().item() * k.abs().sum(-1).max().item() * 2.0 ** -19
+    assert ds < 2.0 ** -18
+    assert_within(out, want, v.abs().max() * (4 * ds + 2.0 ** -17))
