@@ -123,14 +123,14 @@ inline bool attn_wide(int group) { return group > 4; }
 inline int attn_tile_heads(int group) { return attn_wide(group) ? 8 : 4; }
 // MMA tiles (16 tokens) of a warp's tile, and resident blocks per SM.
 // (MMA tiles: two of short rows share a tile's overhead.  Blocks: as many as
-// registers and shared memory allow, but rows of 512 bytes and more are served
-// faster to one block: 32 x 8192 over F32 at 128 dims 391 us with two, 364 with
-// one.)
+// registers and shared memory allow; two for 512-byte rows of F32, 32 x 8192 over
+// 128 dims 421 us with one, 396 with two, 8 query heads to a KV head 414 and 350,
+// though one short sequence of 577 8.6 and 9.0.)
 constexpr int attn_m_tiles(int cache, int hd) {
     return cache == DTYPE_Q4_0 || cache == DTYPE_Q8_0 || (hd <= 64 && cache != DTYPE_F32) ? 2 : 1;
 }
 constexpr int attn_blocks_per_sm(int cache, int hd, bool wide) {
-    if (cache == DTYPE_F32) return hd <= 64 ? 3 : 1;
+    if (cache == DTYPE_F32) return hd <= 64 ? 3 : hd <= 128 ? 2 : 1;
     if (cache == DTYPE_Q4_0) return hd <= 64 ? 4 : hd <= 128 ? (wide ? 3 : 4) : 2;
     if (cache == DTYPE_Q8_0) return hd <= 64 ? 4 : hd <= 128 ? 3 : 2;
     return hd <= 128 ? 3 : 2;
