@@ -9,8 +9,8 @@
 // What bounds it: every visible K and V row is read once from HBM, so the work
 // is laid out to stream rows and to keep everything else off that path.  64
 // sequences of 8192, 8 KV heads of 128, 4 query heads each (of 6554 GB/s; two
-// GPUs): bf16 350 - 358 us, 0.92 - 0.94; Q8_0 205 - 228 us, 0.81 - 0.90; F32 403 -
-// 441 us at 32 sequences, 0.74 - 0.81; Q4_0 169 - 183 us, 0.56 - 0.61.  2 x 131071
+// GPUs): bf16 350 - 358 us, 0.92 - 0.94; Q8_0 205 - 228 us, 0.81 - 0.90; F32 397
+// us at 32 sequences, 0.83 (one GPU); Q4_0 169 - 183 us, 0.56 - 0.61.  2 x 131071
 // over Q4_0 with 5 query heads take 91 - 97 us, 0.53 - 0.56: DRAM is at 0.44 of
 // its peak, a scheduler issues in 0.60 of the cycles and no pipe is near full (ALU
 // 0.47), so it is the chain of each of a scheduler's 2.8 warps (copies, scores,
