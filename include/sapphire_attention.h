@@ -194,6 +194,69 @@ SAPPHIRE_API size_t sapphire_attention_workspace_bytes(kernel_context_t *ctx, co
 SAPPHIRE_API int sapphire_attention_device(kernel_context_t *ctx, const sapphire_kv_cache_t *cache,
                                            const sapphire_attention_args_t *args);
 
+/** The same where each KV head has pages of its own: page_table is
+ *  [sequences, kv_heads, table_stride], lengths are the sequences'. */
+SAPPHIRE_API int sapphire_attention_per_head_device(kernel_context_t *ctx, const sapphire_kv_cache_t *cache,
+                                                    const sapphire_attention_args_t *args);
+
+/* ------------------------------------------------------------------------- *
+ * Attention to selected pages.  A long sequence's new token gets most of its
+ * weight from a few pages; bounds of each page's keys tell which these may be
+ * without reading it.  A step writes its keys (sapphire_kv_write_device), brings
+ * the bounds of the pages it wrote up to date (sapphire_kv_summarise_device),
+ * selects a budget of pages for each KV head (sapphire_kv_select_device) and
+ * attends to them (sapphire_attention_per_head_device).
+ *
+ * A summary is the caller's memory: num_pages times sapphire_kv_summary_bytes.
+ * A page's summary is, for each KV head, head_dim signed bytes of upper bounds
+ * and head_dim of lower bounds, and behind the heads their scales, one fp32 number
+ * each, padded to 16 bytes.  With lo and hi the least and the largest key of a dim
+ * (as the cache holds them), s = max(|lo|, |hi| over dims) / 127 and r = 1 / s
+ * (both 0 where s is below 2^-126), the bytes are ceil(hi r) and floor(lo r), within
+ * -127 .. 127; each step rounds to fp32.  A page of keys that are not all finite has
+ * the scale inf and bytes 0.
+ * ------------------------------------------------------------------------- */
+
+/** Bytes of one page's summary, 0 when the cache's shape is not supported. */
+SAPPHIRE_API size_t sapphire_kv_summary_bytes(const sapphire_kv_cache_t *cache);
+/** Bounds of the pages that hold positions start[s] .. of the `tokens` new rows
+ *  of ragged sequences (the arguments of the write; dtype, k and v are not used), of
+ *  all of a page's tokens up to the newest.  summary: 16-byte aligned. */
+SAPPHIRE_API int sapphire_kv_summarise_device(kernel_context_t *ctx, const sapphire_kv_cache_t *cache, void *summary,
+                                              const sapphire_kv_args_t *args);
+
+/* Sequence s has n = lengths[s] + length_offset tokens on P = ceil(n / page_size)
+ * pages.  Up to `budget` pages: all are selected.  Else the first `first` and the
+ * last `last` are, and of the others those of the largest scores, the earlier one
+ * of two alike.  A page's score for a KV head: query head j of the KV head has codes
+ * c = q r_j rounded to whole numbers, half away from zero, t_j = max |q| / 127 and r_j
+ * = 1 / t_j as above (codes and t_j 0 where a value of the head is not finite); n_j =
+ * sum over dims of the larger of c hi and c lo, exact; the score is max_j (n_j t_j),
+ * times the page's scale s; 0 where s is 0 and inf where s is inf; each step rounds to
+ * fp32.  A page whose number is outside the cache has -inf (and is an error at the
+ * next kernel_ctx_synchronize, like a length outside the table).  Every page but the
+ * last is taken to be full, and every page's summary to be up to date. */
+typedef struct {
+    tensor_dtype_t dtype;    /* F32, BF16 or F16, of q */
+    int sequences;
+    int heads;               /* a multiple of kv_heads, at most 128 times as many */
+    const void *q;           /* [sequences, heads, head_dim] */
+    long long q_seq_stride, q_head_stride;
+    const void *summary;
+    const int *page_table;   /* [sequences, table_stride] */
+    int table_stride;        /* at most 2^18 */
+    const int *lengths;      /* [sequences] */
+    int length_offset;
+    int budget, first, last; /* pages; first + last at most budget, last at least 1 */
+    int *selected;           /* [sequences, kv_heads, budget]: page numbers of the cache in the sequence's order, then -1 */
+    int *selected_lengths;   /* [sequences]: tokens on the selected pages */
+} sapphire_kv_select_args_t;
+
+/** selected and selected_lengths are the page_table and lengths of
+ *  sapphire_attention_per_head_device (table_stride: budget, length_offset: 0). */
+SAPPHIRE_API int sapphire_kv_select_device(kernel_context_t *ctx, const sapphire_kv_cache_t *cache,
+                                           const sapphire_kv_select_args_t *args);
+
 #ifdef __cplusplus
 }
 #endif

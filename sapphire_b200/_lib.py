@@ -130,6 +130,10 @@ _SIGNATURES = {
     "sapphire_kv_read_device": (i32, [vp, vp, vp]),
     "sapphire_attention_workspace_bytes": (sz, [vp, vp, i32, i32]),
     "sapphire_attention_device": (i32, [vp, vp, vp]),
+    "sapphire_attention_per_head_device": (i32, [vp, vp, vp]),
+    "sapphire_kv_summary_bytes": (sz, [vp]),
+    "sapphire_kv_summarise_device": (i32, [vp, vp, vp, vp]),
+    "sapphire_kv_select_device": (i32, [vp, vp, vp]),
 }
 
 
@@ -185,6 +189,14 @@ class AttentionArgs(C.Structure):
                 ("q_head_stride", i64), ("out_seq_stride", i64), ("out_head_stride", i64), ("lse", vp),
                 ("page_table", vp), ("table_stride", i32), ("lengths", vp), ("length_offset", i32), ("window", i32),
                 ("scale", f32), ("workspace", vp), ("workspace_bytes", sz)]
+
+
+class KvSelectArgs(C.Structure):
+    """sapphire_kv_select_args_t."""
+    _fields_ = [("dtype", i32), ("sequences", i32), ("heads", i32), ("q", vp), ("q_seq_stride", i64),
+                ("q_head_stride", i64), ("summary", vp), ("page_table", vp), ("table_stride", i32), ("lengths", vp),
+                ("length_offset", i32), ("budget", i32), ("first", i32), ("last", i32), ("selected", vp),
+                ("selected_lengths", vp)]
 
 
 def load(path: str = LIB_PATH) -> C.CDLL:

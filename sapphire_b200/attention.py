@@ -1,5 +1,5 @@
 """Rotary positions, the paged key-value cache and the attention of one new
-token (include/sapphire_attention.h) from Python.
+token, to all pages or to selected ones (include/sapphire_attention.h) from Python.
 
 Buffers are CUDA tensors of the context's GPU (torch tensors, or anything with
 data_ptr(), shape, stride() and dtype); work is enqueued on the context's stream
@@ -11,8 +11,8 @@ from __future__ import annotations
 import ctypes as C
 
 from . import SapphireError, _lib, addr, lib
-from ._lib import (DTYPE_BF16, DTYPE_F16, DTYPE_F32, DTYPE_NAMES, AttentionArgs, KvArgs, KvCacheStruct, RopeArgs,
-                   RopeConfig)
+from ._lib import (DTYPE_BF16, DTYPE_F16, DTYPE_F32, DTYPE_NAMES, AttentionArgs, KvArgs, KvCacheStruct, KvSelectArgs,
+                   RopeArgs, RopeConfig)
 
 _BY_NAME = {name.lower(): dt for dt, name in DTYPE_NAMES.items()}
 _IO = {"float32": DTYPE_F32, "bfloat16": DTYPE_BF16, "float16": DTYPE_F16}
@@ -86,6 +86,16 @@ def _table(x, sequences: int):
     if not x.is_contiguous():
         raise SapphireError("page_table must be contiguous")
     return x.data_ptr(), x.shape[1]
+
+
+def _head_table(x, sequences: int, kv_heads: int, what: str = "page_table"):
+    """(address, pages) of an int32 page table [sequences, kv_heads, pages]."""
+    _int32(x, what)
+    if len(x.shape) != 3 or x.shape[0] != sequences or x.shape[1] != kv_heads:
+        raise SapphireError(f"{what} has shape {tuple(x.shape)}, not [{sequences}, {kv_heads}, pages]")
+    if not x.is_contiguous():
+        raise SapphireError(f"{what} must be contiguous")
+    return x.data_ptr(), x.shape[2]
 
 
 class Rope:
@@ -202,7 +212,9 @@ class KVCache:
                lse=None, workspace=None) -> None:
         """out = attention of q [sequences, heads, head_dim] over the first
         lengths[s] + length_offset positions of each sequence (the last
-        `window` of them, if set).  lse: float32 [sequences, heads] or None.
+        `window` of them, if set).  page_table: [sequences, pages], or
+        [sequences, kv_heads, pages] where each KV head has pages of its own.
+        lse: float32 [sequences, heads] or None.
         workspace: a byte tensor of workspace_bytes(...) (required when the
         call is captured into a graph)."""
         n, heads, dim = q.shape[0], q.shape[1], self.head_dim
@@ -215,10 +227,59 @@ class KVCache:
             raise SapphireError(f"lse must be contiguous float32 [{n}, {heads}]")
         if workspace is not None and not workspace.is_contiguous():
             raise SapphireError("workspace must be contiguous")
-        table, stride = _table(page_table, n)
+        per_head = len(page_table.shape) == 3
+        table, stride = _head_table(page_table, n, self.kv_heads) if per_head else _table(page_table, n)
         args = AttentionArgs(dt, n, heads, qp, op, qs, qh, os, oh,
                              0 if lse is None else lse.data_ptr(), table, stride, _ints(lengths, "lengths", n),
                              length_offset, window, scale, addr(workspace),
                              0 if workspace is None else workspace.numel() * workspace.element_size())
-        if lib.sapphire_attention_device(self.ctx.handle, self._ref, C.byref(args)) != 0:
-            raise SapphireError(f"sapphire_attention_device failed: {self.ctx.last_error}")
+        fn = lib.sapphire_attention_per_head_device if per_head else lib.sapphire_attention_device
+        if fn(self.ctx.handle, self._ref, C.byref(args)) != 0:
+            raise SapphireError(f"{fn.__name__} failed: {self.ctx.last_error}")
+
+    @property
+    def summary_bytes(self) -> int:
+        """Bytes of one page's summary."""
+        return int(lib.sapphire_kv_summary_bytes(self._ref))
+
+    def _summary(self, summary) -> int:
+        """The address of a byte tensor [num_pages, summary_bytes]."""
+        if tuple(summary.shape) != (self._struct.num_pages, self.summary_bytes) or summary.element_size() != 1 or \
+                not summary.is_contiguous():
+            raise SapphireError(f"summary must be a contiguous byte tensor [{self._struct.num_pages}, {self.summary_bytes}]")
+        return summary.data_ptr()
+
+    def summarise(self, summary, page_table, tokens: int | None = None, start=None, cu_tokens=None) -> None:
+        """Bring the bounds in `summary`, a uint8 tensor [num_pages, summary_bytes],
+        of the pages that a write of `tokens` rows went to up to date (its
+        page_table, start and cu_tokens; without cu_tokens one token each)."""
+        seqs = page_table.shape[0]
+        if tokens is None:
+            if cu_tokens is not None:
+                raise SapphireError("with cu_tokens, tokens must say how many rows there are")
+            tokens = seqs
+        table, stride = _table(page_table, seqs)
+        args = KvArgs(DTYPE_F32, tokens, seqs, None if cu_tokens is None else _ints(cu_tokens, "cu_tokens", seqs + 1),
+                      None if start is None else _ints(start, "start", seqs), table, stride, None, None, 0, 0, 0, 0)
+        if lib.sapphire_kv_summarise_device(self.ctx.handle, self._ref, self._summary(summary), C.byref(args)) != 0:
+            raise SapphireError(f"sapphire_kv_summarise_device failed: {self.ctx.last_error}")
+
+    def select(self, q, summary, page_table, lengths, selected, selected_lengths, first: int = 1, last: int = 1,
+               length_offset: int = 0) -> None:
+        """Select up to selected.shape[2] pages of each sequence for each KV head:
+        the first `first`, the last `last`, and those whose bounds promise q
+        [sequences, heads, head_dim] the largest scores.  selected (int32
+        [sequences, kv_heads, budget]) and selected_lengths (int32 [sequences]) are
+        the page_table and lengths of attend."""
+        n, dim = q.shape[0], self.head_dim
+        dt = _io_seen.get(q.dtype)
+        if dt is None:
+            dt = _io(q, "q")
+        qp, qs, qh = _heads(q, "q", n, None, dim, dt)
+        table, stride = _table(page_table, n)
+        out, budget = _head_table(selected, n, self.kv_heads, "selected")
+        args = KvSelectArgs(dt, n, q.shape[1], qp, qs, qh, self._summary(summary), table, stride,
+                            _ints(lengths, "lengths", n), length_offset, budget, first, last, out,
+                            _ints(selected_lengths, "selected_lengths", n))
+        if lib.sapphire_kv_select_device(self.ctx.handle, self._ref, C.byref(args)) != 0:
+            raise SapphireError(f"sapphire_kv_select_device failed: {self.ctx.last_error}")

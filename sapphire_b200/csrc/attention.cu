@@ -44,9 +44,8 @@ extern "C" SAPPHIRE_API size_t sapphire_attention_workspace_bytes(kernel_context
     return attn_workspace(ctx, cache, heads / cache->kv_heads);
 }
 
-extern "C" SAPPHIRE_API int sapphire_attention_device(kernel_context_t *ctx, const sapphire_kv_cache_t *cache,
-                                                      const sapphire_attention_args_t *a) {
-    const char *who = "sapphire_attention_device";
+static int attend(kernel_context_t *ctx, const sapphire_kv_cache_t *cache, const sapphire_attention_args_t *a,
+                  bool per_head, const char *who) {
     if (!ctx || !cache || !a) {
         LOG_ERROR("%s: NULL argument", who);
         return -1;
@@ -98,6 +97,8 @@ extern "C" SAPPHIRE_API int sapphire_attention_device(kernel_context_t *ctx, con
     p.sequences = a->sequences;
     p.heads = a->heads;
     p.table_stride = a->table_stride;
+    p.table_hs = per_head ? a->table_stride : 0;
+    p.table_ss = (long long)a->table_stride * (per_head ? cache->kv_heads : 1);
     p.length_offset = a->length_offset;
     p.window = a->window;
     p.scale = (a->scale != 0.0f ? a->scale : 1.0f / sqrtf((float)cache->head_dim)) * kLog2e;
@@ -167,4 +168,14 @@ extern "C" SAPPHIRE_API int sapphire_attention_device(kernel_context_t *ctx, con
         return -1;
     }
     return 0;
+}
+
+extern "C" SAPPHIRE_API int sapphire_attention_device(kernel_context_t *ctx, const sapphire_kv_cache_t *cache,
+                                                      const sapphire_attention_args_t *args) {
+    return attend(ctx, cache, args, false, "sapphire_attention_device");
+}
+
+extern "C" SAPPHIRE_API int sapphire_attention_per_head_device(kernel_context_t *ctx, const sapphire_kv_cache_t *cache,
+                                                               const sapphire_attention_args_t *args) {
+    return attend(ctx, cache, args, true, "sapphire_attention_per_head_device");
 }

@@ -100,6 +100,8 @@ struct AttnParams {
     int head_tiles;                // tiles of 4 or 8 query heads of a group
     int sides, side_tiles;         // head tiles that blocks work on side by side, and one behind another
     int table_stride, length_offset, window;
+    long long table_ss;            // entries from a sequence's table to the next one's
+    int table_hs;                  // and from a KV head's (0: one table for all)
     float scale;                   // scores times log2 e
     unsigned long long page_mul;   // floor(2^32 / page_size) + 1
     bool aligned;                  // pages of a multiple of 16 tokens
@@ -507,7 +509,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
         const int nh = min(GH, p.group - ht * GH);                // heads of this tile
         const int head0 = kh * p.group + ht * GH;
         const uint8_t *head = p.l.pages + (unsigned long long)kh * p.l.chunk_bytes;
-        const int *table = p.page_table + (long long)seq * p.table_stride;
+        const int *table = p.page_table + (long long)seq * p.table_ss + (long long)kh * p.table_hs;
         const unsigned page16 = (unsigned)(p.l.page_bytes >> 4);
         const int tile_first = sp.tile0 + piece0, tile_end = sp.tile0 + piece1;
 
