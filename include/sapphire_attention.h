@@ -21,7 +21,8 @@
  * own result (kernel_gemv, a decoder).  Strides are in elements; a stride of 0
  * means contiguous ([tokens, heads, head_dim], the last dimension always
  * contiguous).  No call allocates device memory except the first attention on
- * a context without a workspace of the caller's (once, for calls of any shape).
+ * a context without a workspace of the caller's (once, for calls of any shape),
+ * and attention with a shared prefix without one.
  */
 #ifndef SAPPHIRE_ATTENTION_H
 #define SAPPHIRE_ATTENTION_H
@@ -256,6 +257,48 @@ typedef struct {
  *  sapphire_attention_per_head_device (table_stride: budget, length_offset: 0). */
 SAPPHIRE_API int sapphire_kv_select_device(kernel_context_t *ctx, const sapphire_kv_cache_t *cache,
                                            const sapphire_kv_select_args_t *args);
+
+/* ------------------------------------------------------------------------- *
+ * Attention of a batch whose sequences begin with the same tokens (one system
+ * prompt, many answers to one question).  Sequence s attends to the prefix's first
+ * prefix_length[0] positions, on the pages of prefix_table, and to the n =
+ * lengths[s] + length_offset tokens that it has behind them (its new one among
+ * them), position p of which is slot p % page_size of page_table[s][p / page_size].
+ * The prefix is read once for the batch.  What else holds is as for
+ * sapphire_attention_device, but that 16-bit queries round probabilities and the
+ * values of caches of another type to 16 bits once: to bf16 over BF16 under bf16
+ * queries, else to fp16, values below 2^-29 of the largest of 16 or 32 neighbouring
+ * tokens less exactly.  The same call gives the same bits.
+ * ------------------------------------------------------------------------- */
+typedef struct {
+    tensor_dtype_t dtype;    /* F32, BF16 or F16, of q and out */
+    int sequences;
+    int heads;               /* a multiple of kv_heads; sequences * heads at most 2^24 */
+    const void *q;           /* [sequences, heads, head_dim] */
+    void *out;               /* the same, not overlapping q */
+    long long q_seq_stride, q_head_stride, out_seq_stride, out_head_stride;
+    float *lse;              /* [sequences, heads] log of the softmax's sum, or NULL */
+    const int *prefix_table; /* [prefix_pages] */
+    int prefix_pages;
+    const int *prefix_length;/* [1] */
+    const int *page_table;   /* [sequences, table_stride] */
+    int table_stride;
+    const int *lengths;      /* [sequences] */
+    int length_offset;
+    float scale;             /* 0: 1 / sqrt(head_dim); finite, times log2 e too */
+    /* sapphire_attention_shared_workspace_bytes of device memory, 16-byte aligned,
+     * that no other call uses at the same time; its contents do not matter.
+     * NULL: the context's own, which grows (and waits for the stream) where a call
+     * needs more than any before.  A call captured into a graph has to bring one. */
+    void *workspace;
+    size_t workspace_bytes;
+} sapphire_attention_shared_args_t;
+
+/** Workspace of one call, whatever the lengths; 0 when the shape is not supported. */
+SAPPHIRE_API size_t sapphire_attention_shared_workspace_bytes(kernel_context_t *ctx, const sapphire_kv_cache_t *cache,
+                                                              tensor_dtype_t dtype, int sequences, int heads);
+SAPPHIRE_API int sapphire_attention_shared_device(kernel_context_t *ctx, const sapphire_kv_cache_t *cache,
+                                                  const sapphire_attention_shared_args_t *args);
 
 #ifdef __cplusplus
 }

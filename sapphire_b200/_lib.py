@@ -134,6 +134,8 @@ _SIGNATURES = {
     "sapphire_kv_summary_bytes": (sz, [vp]),
     "sapphire_kv_summarise_device": (i32, [vp, vp, vp, vp]),
     "sapphire_kv_select_device": (i32, [vp, vp, vp]),
+    "sapphire_attention_shared_workspace_bytes": (sz, [vp, vp, i32, i32, i32]),
+    "sapphire_attention_shared_device": (i32, [vp, vp, vp]),
 }
 
 
@@ -197,6 +199,15 @@ class KvSelectArgs(C.Structure):
                 ("q_head_stride", i64), ("summary", vp), ("page_table", vp), ("table_stride", i32), ("lengths", vp),
                 ("length_offset", i32), ("budget", i32), ("first", i32), ("last", i32), ("selected", vp),
                 ("selected_lengths", vp)]
+
+
+class AttentionSharedArgs(C.Structure):
+    """sapphire_attention_shared_args_t."""
+    _fields_ = [("dtype", i32), ("sequences", i32), ("heads", i32), ("q", vp), ("out", vp), ("q_seq_stride", i64),
+                ("q_head_stride", i64), ("out_seq_stride", i64), ("out_head_stride", i64), ("lse", vp),
+                ("prefix_table", vp), ("prefix_pages", i32), ("prefix_length", vp), ("page_table", vp),
+                ("table_stride", i32), ("lengths", vp), ("length_offset", i32), ("scale", f32), ("workspace", vp),
+                ("workspace_bytes", sz)]
 
 
 def load(path: str = LIB_PATH) -> C.CDLL:

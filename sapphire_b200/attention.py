@@ -1,5 +1,5 @@
 """Rotary positions, the paged key-value cache and the attention of one new
-token, to all pages or to selected ones (include/sapphire_attention.h) from Python.
+token, to all pages, to selected ones or behind a shared prefix (include/sapphire_attention.h) from Python.
 
 Buffers are CUDA tensors of the context's GPU (torch tensors, or anything with
 data_ptr(), shape, stride() and dtype); work is enqueued on the context's stream
@@ -11,8 +11,8 @@ from __future__ import annotations
 import ctypes as C
 
 from . import SapphireError, _lib, addr, lib
-from ._lib import (DTYPE_BF16, DTYPE_F16, DTYPE_F32, DTYPE_NAMES, AttentionArgs, KvArgs, KvCacheStruct, KvSelectArgs,
-                   RopeArgs, RopeConfig)
+from ._lib import (DTYPE_BF16, DTYPE_F16, DTYPE_F32, DTYPE_NAMES, AttentionArgs, AttentionSharedArgs, KvArgs,
+                   KvCacheStruct, KvSelectArgs, RopeArgs, RopeConfig)
 
 _BY_NAME = {name.lower(): dt for dt, name in DTYPE_NAMES.items()}
 _IO = {"float32": DTYPE_F32, "bfloat16": DTYPE_BF16, "float16": DTYPE_F16}
@@ -283,3 +283,40 @@ class KVCache:
                             _ints(selected_lengths, "selected_lengths", n))
         if lib.sapphire_kv_select_device(self.ctx.handle, self._ref, C.byref(args)) != 0:
             raise SapphireError(f"sapphire_kv_select_device failed: {self.ctx.last_error}")
+
+    def shared_workspace_bytes(self, dtype, sequences: int, heads: int) -> int:
+        """Workspace of attend_shared for queries of this type (a DTYPE_* number or its name)."""
+        n = lib.sapphire_attention_shared_workspace_bytes(self.ctx.handle, self._ref, _dtype(dtype), sequences, heads)
+        if not n:
+            raise SapphireError(f"no attention of {heads} query heads over {self.kv_heads} KV heads, {sequences} sequences")
+        return int(n)
+
+    def attend_shared(self, q, prefix_table, prefix_length, page_table, lengths, out, scale: float = 0.0,
+                      length_offset: int = 0, lse=None, workspace=None) -> None:
+        """out = attention of q [sequences, heads, head_dim] over the positions
+        0 .. prefix_length[0] - 1 that all sequences begin with, on the pages of
+        prefix_table (int32 [pages]), and the first lengths[s] + length_offset
+        positions of each sequence's own page_table [sequences, pages] behind
+        them.  lse: float32 [sequences, heads] or None.  workspace: a byte tensor
+        of shared_workspace_bytes(...) (required when the call is captured into a
+        graph)."""
+        n, heads, dim = q.shape[0], q.shape[1], self.head_dim
+        dt = _io_seen.get(q.dtype)
+        if dt is None:
+            dt = _io(q, "q")
+        qp, qs, qh = _heads(q, "q", n, None, dim, dt)
+        op, os, oh = _heads(out, "out", n, heads, dim, dt)
+        if lse is not None and (tuple(lse.shape) != (n, heads) or _io(lse, "lse") != DTYPE_F32 or not lse.is_contiguous()):
+            raise SapphireError(f"lse must be contiguous float32 [{n}, {heads}]")
+        if workspace is not None and not workspace.is_contiguous():
+            raise SapphireError("workspace must be contiguous")
+        if len(prefix_table.shape) != 1:
+            raise SapphireError(f"prefix_table has shape {tuple(prefix_table.shape)}, not [pages]")
+        table, stride = _table(page_table, n)
+        args = AttentionSharedArgs(dt, n, heads, qp, op, qs, qh, os, oh, 0 if lse is None else lse.data_ptr(),
+                                   _ints(prefix_table, "prefix_table", None), prefix_table.shape[0],
+                                   _ints(prefix_length, "prefix_length", 1), table, stride, _ints(lengths, "lengths", n),
+                                   length_offset, scale, addr(workspace),
+                                   0 if workspace is None else workspace.numel() * workspace.element_size())
+        if lib.sapphire_attention_shared_device(self.ctx.handle, self._ref, C.byref(args)) != 0:
+            raise SapphireError(f"sapphire_attention_shared_device failed: {self.ctx.last_error}")

@@ -10,38 +10,81 @@
 namespace {
 
 // Blocks of one launch: all that the GPU holds at a time.
-int attn_blocks(kernel_context_t *ctx, const sapphire_kv_cache_t *c, int group) {
-    return sm_count(ctx->device) * attn_blocks_per_sm(c->dtype, c->head_dim, attn_wide(group));
-}
-
-// Workspace: the pieces' descriptions, then two partial results a block.
-size_t attn_workspace(kernel_context_t *ctx, const sapphire_kv_cache_t *c, int group) {
-    const size_t blocks = attn_blocks(ctx, c, group), heads = attn_tile_heads(group);
-    return blocks * (sizeof(int4) + 2 * heads * (c->head_dim + 2) * sizeof(float));
+int attn_blocks(kernel_context_t *ctx, int dtype, int head_dim, int group) {
+    return sm_count(ctx->device) * attn_blocks_per_sm(dtype, head_dim, attn_wide(group));
 }
 
 // The largest of any call (under 5 MB), so that the context's never grows:
 // growing waits for the stream.
 size_t attn_workspace_most(kernel_context_t *ctx) {
     size_t most = 0;
-    for (tensor_dtype_t type : {DTYPE_F32, DTYPE_BF16, DTYPE_F16, DTYPE_Q8_0, DTYPE_Q4_0})
+    for (int type : {DTYPE_F32, DTYPE_BF16, DTYPE_F16, DTYPE_Q8_0, DTYPE_Q4_0})
         for (int dim : {64, 96, 128, 192, 256})
-            for (int group : {1, 8}) {
-                sapphire_kv_cache_t c{};
-                c.dtype = type;
-                c.head_dim = dim;
-                most = std::max(most, attn_workspace(ctx, &c, group));
-            }
+            for (int group : {1, 8}) most = std::max(most, attn_workspace(ctx, type, dim, group));
     return most;
 }
 
 }  // namespace
 
+// The pieces' descriptions, then two partial results a block.
+size_t attn_workspace(kernel_context_t *ctx, int dtype, int head_dim, int group) {
+    const size_t blocks = attn_blocks(ctx, dtype, head_dim, group), heads = attn_tile_heads(group);
+    return blocks * (sizeof(int4) + 2 * heads * (head_dim + 2) * sizeof(float));
+}
+
+// The kernels number tiles (of 64 tokens or more, and what an item costs besides) in 31 bits.
+bool attn_numbered(long long sequences, long long heads, long long tokens) {
+    return (double)sequences * heads * ((double)tokens / 64 + 1 + kAttnItemUnits) < 2147483648.0;
+}
+
+void attn_plan(kernel_context_t *ctx, int dtype, AttnParams *p, char *workspace, int *count) {
+    p->err = ctx->d_err;
+    p->group = p->heads / p->l.kv_heads;
+    p->head_tiles = (p->group + attn_tile_heads(p->group) - 1) / attn_tile_heads(p->group);
+    p->page_mul = (1ull << 32) / p->l.page_size + 1;
+    // Side by side: as many head tiles as divide their number evenly, up to 8.
+    p->blocks = attn_blocks(ctx, dtype, p->l.head_dim, p->group);
+    p->sides = std::min(std::min(p->head_tiles, 8), p->blocks);
+    while (p->head_tiles % p->sides) --p->sides;
+    p->blocks -= p->blocks % p->sides;
+    p->side_tiles = p->head_tiles / p->sides;
+    p->code[0] = 0x64006400u;
+    p->code[1] = dtype == DTYPE_Q8_0 ? 0x64806480u : 0x64086408u;
+    p->code[2] = 0x2c002c00u;
+    p->code[3] = 0xd480d480u;
+    p->aligned = p->l.page_size % 16 == 0;
+    p->device = ctx->device;
+    const long long items = (long long)p->sequences * p->l.kv_heads * p->head_tiles;
+    p->by_item = items <= p->blocks;
+    p->joins = (int)std::min<long long>(items, p->blocks);
+    // Blocks to an item: on average, and at most one for each tile that the table
+    // or the window leaves it.  (The average says nothing of one sequence far longer
+    // than the others: 131072 tokens of Q8_0 beside 31 of 500, one KV head, 45 us
+    // where the last block joins, 27 where the other kernel does.)
+    const int tile = 16 * kAttnWarps * attn_m_tiles(dtype, p->l.head_dim);
+    const long long room = std::min((long long)p->table_stride * p->l.page_size, p->window ? (long long)p->window + tile : INT_MAX);
+    p->few_holders = p->blocks <= 16 * items || (room + tile - 1) / tile <= 16;
+    // With few blocks to an item the last of them joins their pieces, which saves a launch.
+    p->count = p->few_holders ? count : nullptr;
+    p->piece = reinterpret_cast<int4 *>(workspace);
+    p->part = reinterpret_cast<float *>(workspace + (size_t)p->blocks * sizeof(int4));
+}
+
+cudaError_t attn_run(int dtype, const AttnParams &p, cudaStream_t st) {
+    switch (dtype) {
+        case DTYPE_F32: return attn_run_f32(p, st);
+        case DTYPE_BF16: return attn_run_bf16(p, st);
+        case DTYPE_F16: return attn_run_f16(p, st);
+        case DTYPE_Q8_0: return attn_run_q8_0(p, st);
+        default: return attn_run_q4_0(p, st);
+    }
+}
+
 extern "C" SAPPHIRE_API size_t sapphire_attention_workspace_bytes(kernel_context_t *ctx,
                                                                   const sapphire_kv_cache_t *cache, int sequences,
                                                                   int heads) {
     if (!ctx || !cache || sequences < 0 || heads <= 0 || !sapphire_kv_page_bytes(cache) || heads % cache->kv_heads) return 0;
-    return attn_workspace(ctx, cache, heads / cache->kv_heads);
+    return attn_workspace(ctx, cache->dtype, cache->head_dim, heads / cache->kv_heads);
 }
 
 static int attend(kernel_context_t *ctx, const sapphire_kv_cache_t *cache, const sapphire_attention_args_t *a,
@@ -78,9 +121,7 @@ static int attend(kernel_context_t *ctx, const sapphire_kv_cache_t *cache, const
         !on_device(ctx, who, "out", a->out) || !on_device(ctx, who, "page_table", a->page_table) ||
         !on_device(ctx, who, "lengths", a->lengths) || (a->lse && !on_device(ctx, who, "lse", a->lse)))
         return -1;
-    // The kernels number tiles (of 64 tokens or more, and what an item costs besides) in 31 bits.
-    if ((double)a->sequences * a->heads * ((double)a->table_stride * cache->page_size / 64 + 1 + kAttnItemUnits) >=
-        2147483648.0) {
+    if (!attn_numbered(a->sequences, a->heads, (long long)a->table_stride * cache->page_size)) {
         ctx_fail(ctx, who, "%d sequences of up to %d pages are more tiles than 2^31", a->sequences, a->table_stride);
         return -1;
     }
@@ -102,35 +143,10 @@ static int attend(kernel_context_t *ctx, const sapphire_kv_cache_t *cache, const
     p.length_offset = a->length_offset;
     p.window = a->window;
     p.scale = (a->scale != 0.0f ? a->scale : 1.0f / sqrtf((float)cache->head_dim)) * kLog2e;
-    p.err = ctx->d_err;
-    p.io = a->dtype;
-    p.group = a->heads / cache->kv_heads;
-    p.head_tiles = (p.group + attn_tile_heads(p.group) - 1) / attn_tile_heads(p.group);
-    p.page_mul = (1ull << 32) / cache->page_size + 1;
-    // Side by side: as many head tiles as divide their number evenly, up to 8.
-    p.blocks = attn_blocks(ctx, cache, p.group);
-    p.sides = std::min(std::min(p.head_tiles, 8), p.blocks);
-    while (p.head_tiles % p.sides) --p.sides;
-    p.blocks -= p.blocks % p.sides;
-    p.side_tiles = p.head_tiles / p.sides;
-    p.code[0] = 0x64006400u;
-    p.code[1] = cache->dtype == DTYPE_Q8_0 ? 0x64806480u : 0x64086408u;
-    p.code[2] = 0x2c002c00u;
-    p.code[3] = 0xd480d480u;
-    p.aligned = cache->page_size % 16 == 0;
-    p.device = ctx->device;
-    const long long items = (long long)a->sequences * cache->kv_heads * p.head_tiles;
-    p.by_item = items <= p.blocks;
-    p.joins = (int)std::min<long long>(items, p.blocks);
-    // Blocks to an item: on average, and at most one for each tile that the table
-    // or the window leaves it.  (The average says nothing of one sequence far longer
-    // than the others: 131072 tokens of Q8_0 beside 31 of 500, one KV head, 45 us
-    // where the last block joins, 27 where the other kernel does.)
-    const int tile = 16 * kAttnWarps * attn_m_tiles(cache->dtype, cache->head_dim);
-    const long long room = std::min((long long)a->table_stride * cache->page_size, a->window ? (long long)a->window + tile : INT_MAX);
-    p.few_holders = p.blocks <= 16 * items || (room + tile - 1) / tile <= 16;
+    p.io = p.out_io = a->dtype;
     AttnDevice g(ctx->device);
-    const size_t need = attn_workspace(ctx, cache, p.group);
+    const size_t need = attn_workspace(ctx, cache->dtype, cache->head_dim, a->heads / cache->kv_heads);
+    int *count = nullptr;
     char *ws = static_cast<char *>(a->workspace);
     if (ws) {
         if (a->workspace_bytes < need || ((uintptr_t)ws & 15)) {
@@ -145,23 +161,14 @@ static int attend(kernel_context_t *ctx, const sapphire_kv_cache_t *cache, const
             ctx_fail(ctx, who, "a captured call needs a workspace of its own");
             return -1;
         }
-        // The context's own begins with zeroed counters: with few blocks to an item
-        // the last of them joins their pieces, which saves a launch.
+        // The context's own begins with zeroed counters.
         const size_t counts = ((size_t)sm_count(ctx->device) * kAttnMaxBlocks * sizeof(int) + 15) & ~(size_t)15;
         if (!ctx->d_attn && ensure_scratch(ctx, &ctx->d_attn, &ctx->d_attn_cap, counts + attn_workspace_most(ctx))) return -1;
         ws = reinterpret_cast<char *>(ctx->d_attn) + counts;
-        if (p.few_holders) p.count = reinterpret_cast<int *>(ctx->d_attn);
+        count = reinterpret_cast<int *>(ctx->d_attn);
     }
-    p.piece = reinterpret_cast<int4 *>(ws);
-    p.part = reinterpret_cast<float *>(ws + (size_t)p.blocks * sizeof(int4));
-    cudaError_t e;
-    switch (cache->dtype) {
-        case DTYPE_F32: e = attn_run_f32(p, ctx->stream); break;
-        case DTYPE_BF16: e = attn_run_bf16(p, ctx->stream); break;
-        case DTYPE_F16: e = attn_run_f16(p, ctx->stream); break;
-        case DTYPE_Q8_0: e = attn_run_q8_0(p, ctx->stream); break;
-        default: e = attn_run_q4_0(p, ctx->stream); break;
-    }
+    attn_plan(ctx, cache->dtype, &p, ws, count);
+    const cudaError_t e = attn_run(cache->dtype, p, ctx->stream);
     if (e != cudaSuccess) {
         cudaGetLastError();
         ctx_fail(ctx, who, "launch failed: %s", cudaGetErrorString(e));

@@ -93,9 +93,11 @@ struct AttnParams {
     const void *q;
     void *out;
     float *lse;
+    float2 *ml;                    // or, where another pass joins: maximum (in units of log2 e) and sum of what out is the mean of
     long long q_ss, q_hs, out_ss, out_hs;
     const int *page_table, *lengths;
-    int io;                        // tensor_dtype_t of q and out
+    int io, out_io;                // tensor_dtype_t of q and out
+    int row_group;                 // 0, or the heads are row_group heads of many sequences, of each KV head in turn
     int sequences, heads, group;   // group: query heads of a KV head
     int head_tiles;                // tiles of 4 or 8 query heads of a group
     int sides, side_tiles;         // head tiles that blocks work on side by side, and one behind another
@@ -408,9 +410,14 @@ __device__ __forceinline__ void attn_add_holders(const float *part, size_t strid
     }
 }
 __device__ __forceinline__ void attn_store(const AttnParams &p, long long at, float y) {
-    if (p.io == DTYPE_F32) static_cast<float *>(p.out)[at] = y;
-    else if (p.io == DTYPE_BF16) static_cast<__nv_bfloat16 *>(p.out)[at] = __float2bfloat16_rn(y);
+    if (p.out_io == DTYPE_F32) static_cast<float *>(p.out)[at] = y;
+    else if (p.out_io == DTYPE_BF16) static_cast<__nv_bfloat16 *>(p.out)[at] = __float2bfloat16_rn(y);
     else static_cast<__half *>(p.out)[at] = __float2half_rn(y);
+}
+
+__device__ __forceinline__ void attn_store_lse(const AttnParams &p, long long at, float M, float L) {
+    if (p.ml) p.ml[at] = make_float2(M, L);
+    else if (p.lse) p.lse[at] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
 }
 
 template <int kCache, int HD, bool kWide, bool kExact>
@@ -647,7 +654,11 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
 #pragma unroll
         for (int k = 0; k < kPerWarp; ++k) {
             const int j = warp + k * kAttnWarps;
-            const long long off = seq * p.q_ss + (long long)(head0 + j) * p.q_hs + lane;
+            long long off = seq * p.q_ss + (long long)(head0 + j) * p.q_hs + lane;
+            if (p.row_group) {
+                const int row = ht * GH + j, s = row / p.row_group;
+                off = s * p.q_ss + (long long)(kh * p.row_group + row - s * p.row_group) * p.q_hs + lane;
+            }
 #pragma unroll
             for (int b = 0; b < NB; ++b)
                 x[k][b] = j >= nh ? 0.0f
@@ -1223,9 +1234,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                     part[GH + h] = L[j];
                 } else {
                     qmul[h] = L[j] == 0.0f ? 0.0f : 1.0f / L[j];
-                    if (p.lse && h < nh)
-                        p.lse[(long long)seq * p.heads + head0 + h] =
-                            L[j] == 0.0f ? -INFINITY : (M[j] - kBias + log2f(L[j])) * 0.6931471805599453f;
+                    if (h < nh) attn_store_lse(p, (long long)seq * p.heads + head0 + h, M[j] - kBias, L[j]);
                 }
             }
         }
@@ -1268,8 +1277,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_blocks_per_sm(kCache, HD
                         for (int b = 0; b < NB; ++b) o1[b] = 0.0f;
                         attn_add_holders<HD, 8>(parts, (size_t)GH * (HD + 2), GH, h, 0, 1, (int)holders, M1, L1, o1);
                         const float inv = L1 == 0.0f ? 0.0f : 1.0f / L1;
-                        if (p.lse && lane == 0)
-                            p.lse[(long long)seq * p.heads + head0 + h] = L1 == 0.0f ? -INFINITY : (M1 - kBias + log2f(L1)) * 0.6931471805599453f;
+                        if (lane == 0) attn_store_lse(p, (long long)seq * p.heads + head0 + h, M1 - kBias, L1);
 #pragma unroll
                         for (int b = 0; b < NB; ++b)
                             attn_store(p, seq * p.out_ss + (long long)(head0 + h) * p.out_hs + 32 * b + lane, o1[b] * inv);
@@ -1331,8 +1339,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Attn
     }
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     const int head = kh * p.group + ht * tile_heads + h;
-    if (p.lse && threadIdx.x == 0)
-        p.lse[(long long)piece.x * p.heads + head] = L == 0.0f ? -INFINITY : (M - bias + log2f(L)) * 0.6931471805599453f;
+    if (threadIdx.x == 0) attn_store_lse(p, (long long)piece.x * p.heads + head, M - bias, L);
     const long long off = piece.x * p.out_ss + (long long)head * p.out_hs;
     for (int d = threadIdx.x; d < HD; d += kJoinWarps * 32) {
         float y = 0.0f;
@@ -1393,6 +1400,14 @@ cudaError_t attn_launch(const AttnParams &p, cudaStream_t st) {
     return attn_wide(p.group) ? attn_launch<kCache, true, true>(p, st) : attn_launch<kCache, false, true>(p, st);
 }
 #endif
+
+// Workspace of a call of this shape; how it is laid out and its tiles are shared,
+// from the fields that describe the call; its launches.  (attention.cu)
+size_t attn_workspace(kernel_context_t *ctx, int dtype, int head_dim, int group);
+void attn_plan(kernel_context_t *ctx, int dtype, AttnParams *p, char *workspace, int *count);
+cudaError_t attn_run(int dtype, const AttnParams &p, cudaStream_t st);
+// Whether the tiles of a call can be numbered.
+bool attn_numbered(long long sequences, long long heads, long long tokens);
 
 // One cache type each (attention_<type>.cu).
 cudaError_t attn_run_f32(const AttnParams &p, cudaStream_t st);

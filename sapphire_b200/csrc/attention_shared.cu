@@ -1,0 +1,314 @@
+// attention_shared.cu - attention of one new token of every sequence of a batch
+// whose sequences begin with the same tokens (include/sapphire_attention.h):
+// arguments, workspace, the choice of the prefix's kernel, and the joining of its
+// pieces with what each sequence has behind it.
+//
+// Reading the prefix once for the batch leaves each of its pages' bytes to 2 flops
+// for every row, so its kernel is a matrix product (prefix_kernel.cuh).  Under fp32
+// queries it is the one-token kernel (attention_kernel.cuh) with every sequence's
+// heads as query heads of one sequence: its tf32 parts hold what a 16-bit operand
+// would not.
+#include <algorithm>
+#include <climits>
+#include <cmath>
+
+#include "prefix_kernel.cuh"
+
+namespace {
+
+constexpr int kJoinWarps = 8;
+
+struct JoinParams {
+    PrefixParams prefix;          // of the tensor core kernel
+    bool tc;
+    int heads, kv_heads;
+    long long entries;            // sequences * heads
+    const float *own;             // [sequences][heads][head_dim]
+    const float2 *own_ml;         // [sequences][heads]
+    void *out;
+    float *lse;
+    long long out_ss, out_hs;
+    int io;
+};
+
+// A warp per sequence and query head adds up means, each with its maximum and sum:
+// the weight of one is l 2^(m - M).  Bound by the pieces' bytes: 64 sequences of 32
+// heads of 128 with nine pieces each read 11 MB.
+template <int HD>
+__global__ void __launch_bounds__(kJoinWarps * 32) shared_join_kernel(const JoinParams p) {
+    constexpr int NB = HD / 32;
+    const int lane = threadIdx.x & 31;
+    const long long entry = (long long)blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
+    pdl_wait();
+    if (entry >= p.entries) return;
+    const PrefixParams &f = p.prefix;
+    const int s = (int)(entry / p.heads), h = (int)(entry - (long long)s * p.heads), kh = h / f.group;
+    const int row = s * f.group + h - kh * f.group;
+    // The pieces: of consecutive slots, `stride` means apart.
+    int n = 1;
+    long long first = (long long)kh * f.rows + row, stride = 0;
+    if (p.tc) {
+        const int set_rows = f.streams * kPrefixRows, set = row / set_rows, item = kh * f.row_sets + set;
+        const PrefixRanges r = prefix_ranges(f.items, prefix_length(f, false), prefix_tile(HD), f.blocks);
+        n = 0;
+        if (r.tiles > 0) {
+            const unsigned unit = (unsigned)item * r.tiles, b0 = prefix_block_of(r, unit), b1 = prefix_block_of(r, unit + r.tiles - 1);
+            n = (int)(b1 - b0) + 1;
+            first = (long long)(b0 + item) * set_rows + row - set * set_rows;
+            stride = set_rows;
+        }
+    }
+    const float2 own = p.own_ml[entry];
+    float M = own.y == 0.0f ? -INFINITY : own.x;
+    for (int i = lane; i < n; i += 32) {
+        const float2 x = __ldcg(f.part_ml + first + i * stride);
+        if (x.y != 0.0f) M = fmaxf(M, x.x);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float ref = M == -INFINITY ? 0.0f : M;
+    auto weight = [&](float2 x) { return x.y == 0.0f ? 0.0f : x.y != x.y ? x.y : x.y * attn_exp2(x.x - ref); };
+    float L = weight(own), y[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) y[j] = own.y == 0.0f ? 0.0f : L * p.own[entry * HD + 32 * j + lane];
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        float mine = 0.0f;
+        if (i0 + lane < n) mine = weight(__ldcg(f.part_ml + first + (i0 + lane) * stride));
+        const int end = min(32, n - i0);
+#pragma unroll 4
+        for (int i = 0; i < end; ++i) {
+            const float w = __shfl_sync(0xffffffffu, mine, i);
+            const float *x = f.part + (first + (i0 + i) * stride) * HD + lane;
+            L += w;
+#pragma unroll
+            for (int j = 0; j < NB; ++j) y[j] = fmaf(w, w == 0.0f ? 0.0f : __ldcg(x + 32 * j), y[j]);
+        }
+    }
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    if (p.lse && lane == 0) p.lse[entry] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+    const long long at = s * p.out_ss + (long long)h * p.out_hs + lane;
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+        if (p.io == DTYPE_F32) static_cast<float *>(p.out)[at + 32 * j] = y[j] * inv;
+        else if (p.io == DTYPE_BF16) static_cast<__nv_bfloat16 *>(p.out)[at + 32 * j] = __float2bfloat16_rn(y[j] * inv);
+        else static_cast<__half *>(p.out)[at + 32 * j] = __float2half_rn(y[j] * inv);
+    }
+}
+
+cudaError_t run_join(const JoinParams &p, int head_dim, cudaStream_t st) {
+    const dim3 grid((unsigned)((p.entries + kJoinWarps - 1) / kJoinWarps)), block(kJoinWarps * 32);
+    switch (head_dim) {
+        case 64: return launch_pdl(shared_join_kernel<64>, grid, block, 0, st, p);
+        case 96: return launch_pdl(shared_join_kernel<96>, grid, block, 0, st, p);
+        case 128: return launch_pdl(shared_join_kernel<128>, grid, block, 0, st, p);
+        case 192: return launch_pdl(shared_join_kernel<192>, grid, block, 0, st, p);
+        default: return launch_pdl(shared_join_kernel<256>, grid, block, 0, st, p);
+    }
+}
+
+cudaError_t run_prefix(int dtype, const PrefixParams &p, cudaStream_t st) {
+    return dtype == DTYPE_BF16 ? prefix_run_bf16(p, st) : prefix_run_f16(p, st);
+}
+
+// Whether the prefix is a product on the tensor cores: where its rows are operands as they are.
+bool on_tensor_cores(int io, int cache) { return io != DTYPE_F32 && (cache == DTYPE_F16 || (cache == DTYPE_BF16 && io == DTYPE_BF16)); }
+
+// The workspace of a call, in bytes from its start.
+struct SharedLayout {
+    size_t own, own_ml, part, part_ml, attend, count, total;
+    int streams, row_sets, items, blocks;
+};
+SharedLayout shared_layout(kernel_context_t *ctx, const sapphire_kv_cache_t *c, int io, int sequences, int heads) {
+    SharedLayout w{};
+    const int group = heads / c->kv_heads;
+    const long long rows = (long long)sequences * group, entries = (long long)sequences * heads;
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t from = at;
+        at += (bytes + 255) & ~(size_t)255;
+        return from;
+    };
+    w.blocks = sm_count(ctx->device);
+    w.own = take(entries * c->head_dim * sizeof(float));
+    w.own_ml = take(entries * sizeof(float2));
+    size_t means = entries, attend = attn_workspace(ctx, c->dtype, c->head_dim, group);
+    if (on_tensor_cores(io, c->dtype)) {
+        // Two tiles of rows share a pass over the prefix where there are that many.
+        w.streams = rows > kPrefixRows ? prefix_streams(c->head_dim) : 1;
+        w.row_sets = (int)((rows + w.streams * kPrefixRows - 1) / (w.streams * kPrefixRows));
+        w.items = w.row_sets * c->kv_heads;
+        means = (size_t)(w.blocks + w.items) * w.streams * kPrefixRows;
+    } else {
+        attend = std::max(attend, attn_workspace(ctx, c->dtype, c->head_dim, (int)rows));
+    }
+    w.part = take(means * c->head_dim * sizeof(float));
+    w.part_ml = take(means * sizeof(float2));
+    w.attend = take(attend);
+    w.count = take((size_t)sm_count(ctx->device) * kAttnMaxBlocks * sizeof(int));
+    w.total = at;
+    return w;
+}
+
+// nullptr, or why this many sequences and heads are not supported.
+const char *shared_shape(const sapphire_kv_cache_t *c, int sequences, int heads) {
+    if (heads <= 0 || heads % c->kv_heads || heads > 65535) return "query heads must be a multiple of the KV heads, at most 65535";
+    if (sequences < 0 || sequences > 65535) return "sequences must be 0 to 65535";
+    if ((long long)sequences * heads > 1 << 24) return "sequences times heads must be at most 2^24";
+    return nullptr;
+}
+
+}  // namespace
+
+extern "C" SAPPHIRE_API size_t sapphire_attention_shared_workspace_bytes(kernel_context_t *ctx,
+                                                                         const sapphire_kv_cache_t *cache,
+                                                                         tensor_dtype_t dtype, int sequences, int heads) {
+    if (!ctx || !cache || !sapphire_kv_page_bytes(cache) || !io_size(dtype) || shared_shape(cache, sequences, heads)) return 0;
+    return shared_layout(ctx, cache, dtype, std::max(sequences, 1), heads).total;
+}
+
+extern "C" SAPPHIRE_API int sapphire_attention_shared_device(kernel_context_t *ctx, const sapphire_kv_cache_t *cache,
+                                                             const sapphire_attention_shared_args_t *a) {
+    const char *who = "sapphire_attention_shared_device";
+    if (!ctx || !cache || !a) {
+        LOG_ERROR("%s: NULL argument", who);
+        return -1;
+    }
+    std::lock_guard<std::recursive_mutex> lk(ctx->exec_mutex);
+    if (!ctx->initialized) {
+        ctx_fail(ctx, who, "context not initialized");
+        return -1;
+    }
+    KvLayout l{};
+    if (!kv_layout(ctx, who, cache, &l)) return -1;
+    const size_t size = io_size(a->dtype);
+    if (!size) {
+        ctx_fail(ctx, who, "q and out must be F32, BF16 or F16");
+        return -1;
+    }
+    if (const char *why = shared_shape(cache, a->sequences, a->heads)) {
+        ctx_fail(ctx, who, "%s (%d sequences, %d query heads over %d KV heads)", why, a->sequences, a->heads, cache->kv_heads);
+        return -1;
+    }
+    if (a->sequences == 0) return 0;
+    if (a->table_stride <= 0 || a->prefix_pages <= 0 || !std::isfinite(a->scale * kLog2e)) {
+        ctx_fail(ctx, who, "table_stride and prefix_pages must be positive and scale finite (times log2 e too)");
+        return -1;
+    }
+    if (!on_device(ctx, who, "pages", cache->pages) || !on_device(ctx, who, "q", a->q) ||
+        !on_device(ctx, who, "out", a->out) || !on_device(ctx, who, "prefix_table", a->prefix_table) ||
+        !on_device(ctx, who, "prefix_length", a->prefix_length) || !on_device(ctx, who, "page_table", a->page_table) ||
+        !on_device(ctx, who, "lengths", a->lengths) || (a->lse && !on_device(ctx, who, "lse", a->lse)))
+        return -1;
+    const long long prefix_room = (long long)a->prefix_pages * cache->page_size;
+    if (!attn_numbered(a->sequences, a->heads, (long long)a->table_stride * cache->page_size) ||
+        !attn_numbered(1, (long long)a->sequences * a->heads, prefix_room)) {
+        ctx_fail(ctx, who, "%d sequences of up to %d pages behind %d are more tiles than 2^31", a->sequences, a->table_stride, a->prefix_pages);
+        return -1;
+    }
+    AttnDevice g(ctx->device);
+    const SharedLayout w = shared_layout(ctx, cache, a->dtype, a->sequences, a->heads);
+    char *ws = static_cast<char *>(a->workspace);
+    if (ws) {
+        if (a->workspace_bytes < w.total || ((uintptr_t)ws & 15)) {
+            ctx_fail(ctx, who, "the workspace needs %zu bytes, 16-byte aligned", w.total);
+            return -1;
+        }
+        if (!on_device(ctx, who, "workspace", ws)) return -1;
+    } else {
+        cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(ctx->stream, &capturing) != cudaSuccess || capturing != cudaStreamCaptureStatusNone) {
+            cudaGetLastError();
+            ctx_fail(ctx, who, "a captured call needs a workspace of its own");
+            return -1;
+        }
+        if (ensure_scratch(ctx, &ctx->d_shared, &ctx->d_shared_cap, w.total)) return -1;
+        ws = reinterpret_cast<char *>(ctx->d_shared);
+    }
+
+    const int group = a->heads / cache->kv_heads, rows = a->sequences * group;
+    const float scale = (a->scale != 0.0f ? a->scale : 1.0f / sqrtf((float)cache->head_dim)) * kLog2e;
+    AttnParams own{};
+    own.l = l;
+    own.q = a->q;
+    own.out = ws + w.own;
+    own.ml = reinterpret_cast<float2 *>(ws + w.own_ml);
+    own.q_ss = a->q_seq_stride ? a->q_seq_stride : (long long)a->heads * cache->head_dim;
+    own.q_hs = a->q_head_stride ? a->q_head_stride : cache->head_dim;
+    own.out_ss = (long long)a->heads * cache->head_dim;
+    own.out_hs = cache->head_dim;
+    own.page_table = a->page_table;
+    own.lengths = a->lengths;
+    own.sequences = a->sequences;
+    own.heads = a->heads;
+    own.table_stride = a->table_stride;
+    own.table_ss = a->table_stride;
+    own.length_offset = a->length_offset;
+    own.scale = scale;
+    own.io = a->dtype;
+    own.out_io = DTYPE_F32;
+
+    JoinParams j{};
+    PrefixParams &f = j.prefix;
+    f.l = l;
+    f.q = a->q;
+    f.q_ss = own.q_ss;
+    f.q_hs = own.q_hs;
+    f.table = a->prefix_table;
+    f.length = a->prefix_length;
+    f.table_pages = a->prefix_pages;
+    f.io = a->dtype;
+    f.rows = rows;
+    f.group = group;
+    f.scale = scale;
+    f.part = reinterpret_cast<float *>(ws + w.part);
+    f.part_ml = reinterpret_cast<float2 *>(ws + w.part_ml);
+    f.err = ctx->d_err;
+    f.device = ctx->device;
+    j.tc = on_tensor_cores(a->dtype, cache->dtype);
+    j.heads = a->heads;
+    j.kv_heads = cache->kv_heads;
+    j.entries = (long long)a->sequences * a->heads;
+    j.own = reinterpret_cast<const float *>(ws + w.own);
+    j.own_ml = own.ml;
+    j.out = a->out;
+    j.lse = a->lse;
+    j.out_ss = a->out_seq_stride ? a->out_seq_stride : (long long)a->heads * cache->head_dim;
+    j.out_hs = a->out_head_stride ? a->out_head_stride : cache->head_dim;
+    j.io = a->dtype;
+    cudaError_t e;
+    if (j.tc) {
+        f.streams = w.streams;
+        f.row_sets = w.row_sets;
+        f.items = w.items;
+        f.blocks = w.blocks;
+        f.page_mul = (1ull << 32) / cache->page_size + 1;
+        f.q_wide = rows_aligned(a->q, f.q_ss, f.q_hs, size);
+        f.count = reinterpret_cast<int *>(ws + w.count);
+        f.counts = sm_count(ctx->device) * kAttnMaxBlocks;
+        e = run_prefix(cache->dtype, f, ctx->stream);
+        attn_plan(ctx, cache->dtype, &own, ws + w.attend, f.count);
+    } else {
+        AttnParams front = own;
+        front.out = f.part;
+        front.ml = f.part_ml;
+        front.out_ss = 0;
+        front.page_table = a->prefix_table;
+        front.lengths = a->prefix_length;
+        front.sequences = 1;
+        front.heads = cache->kv_heads * rows;
+        front.row_group = group;
+        front.table_stride = a->prefix_pages;
+        front.length_offset = 0;
+        attn_plan(ctx, cache->dtype, &front, ws + w.attend, nullptr);
+        e = attn_run(cache->dtype, front, ctx->stream);
+        attn_plan(ctx, cache->dtype, &own, ws + w.attend, nullptr);
+    }
+    if (e == cudaSuccess) e = attn_run(cache->dtype, own, ctx->stream);
+    if (e == cudaSuccess) e = run_join(j, cache->head_dim, ctx->stream);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        ctx_fail(ctx, who, "launch failed: %s", cudaGetErrorString(e));
+        return -1;
+    }
+    return 0;
+}

@@ -236,6 +236,7 @@ extern "C" SAPPHIRE_API void kernel_ctx_destroy(kernel_context_t *ctx) {
             if (ctx->d_cnt) cudaFree(ctx->d_cnt);
             if (ctx->d_xb) cudaFree(ctx->d_xb);
             if (ctx->d_attn) cudaFree(ctx->d_attn);
+            if (ctx->d_shared) cudaFree(ctx->d_shared);
             if (ctx->h_err) cudaFreeHost(ctx->h_err);
             shard_destroy(ctx);
             if (ctx->own_stream) cudaStreamDestroy(ctx->own_stream);

@@ -121,6 +121,8 @@ struct sapphire_context {
     float *d_xb = nullptr;   size_t d_xb_cap = 0;
     // Partial results of split sequences (attention.cu).
     float *d_attn = nullptr; size_t d_attn_cap = 0;
+    // Workspace of attention with a shared prefix (attention_shared.cu).
+    float *d_shared = nullptr; size_t d_shared_cap = 0;
 
     HostPool *pool = nullptr;
 
