@@ -280,6 +280,8 @@ def run_reference_arm(args, cfg):
     threads = os.cpu_count() or 1
     bytes_per = algorithmic_bytes(cfg.dtype, cfg.rows, cfg.cols)
     ref_kernel = cfg.dtype in (WL.DTYPE_Q4_0, WL.DTYPE_Q8_0)
+    # (Where the reference's kernels were not built, the oracle's port of them, named as such.)
+    ref_kernel = ref_kernel and cpu_reference_time(cfg, packed, X, 0.0, threads) is not None
     fn = cpu_reference_time if ref_kernel else cpu_port_time
     kind = "reference" if ref_kernel else "port"
     for _ in range(args.warmup):
