@@ -16,7 +16,7 @@
 
 namespace {
 
-constexpr int kJoinWarps = 8;
+constexpr int kJoinWarps = 8, kEntryWarps = 4;    // of a block, and of a sequence and query head
 
 struct JoinParams {
     PrefixParams prefix;          // of the tensor core kernel
@@ -31,16 +31,21 @@ struct JoinParams {
     int io;
 };
 
-// A warp per sequence and query head adds up means, each with its maximum and sum:
-// the weight of one is l 2^(m - M).  Bound by the pieces' bytes: 64 sequences of 32
-// heads of 128 with nine pieces each read 11 MB.
+// Adds up means, each with its maximum and sum: the weight of one is l 2^(m - M).
+// kWarps warps take a sequence and query head, each every kWarps-th piece with all its
+// loads in flight, and are joined in shared memory: bound by latency, the fewer steps
+// behind one another the better (64 sequences of 32 heads of 128, 18 pieces of 0.5 KB
+// each: 10.4 us with one warp, .. with four).
 template <int HD>
 __global__ void __launch_bounds__(kJoinWarps * 32) shared_join_kernel(const JoinParams p) {
-    constexpr int NB = HD / 32;
-    const int lane = threadIdx.x & 31;
-    const long long entry = (long long)blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
+    // A lane has four dims, or eight of 192 and 256.
+    constexpr int kLanes = HD <= 128 ? HD / 4 : HD / 8, NB = HD / kLanes / 4, kBatch = 8 / NB;
+    __shared__ float4 means[kJoinWarps][NB][32];
+    __shared__ float sums[kJoinWarps], tops[kJoinWarps];
+    const int warp = threadIdx.x >> 5, part = warp % kEntryWarps, lane = threadIdx.x & 31, at = 4 * min(lane, kLanes - 1);
+    const long long entry = (long long)blockIdx.x * (kJoinWarps / kEntryWarps) + warp / kEntryWarps;
+    const bool there = entry < p.entries;
     pdl_wait();
-    if (entry >= p.entries) return;
     const PrefixParams &f = p.prefix;
     const int s = (int)(entry / p.heads), h = (int)(entry - (long long)s * p.heads), kh = h / f.group;
     const int row = s * f.group + h - kh * f.group;
@@ -58,45 +63,93 @@ __global__ void __launch_bounds__(kJoinWarps * 32) shared_join_kernel(const Join
             stride = set_rows;
         }
     }
-    const float2 own = p.own_ml[entry];
-    float M = own.y == 0.0f ? -INFINITY : own.x;
-    for (int i = lane; i < n; i += 32) {
-        const float2 x = __ldcg(f.part_ml + first + i * stride);
-        if (x.y != 0.0f) M = fmaxf(M, x.x);
-    }
+    // This warp's: what lies behind the prefix (-1) for the first, and every
+    // kEntryWarps-th piece.  M: their maximum, L: the sum of their weights.
+    float M = -INFINITY, L = 0.0f, y[NB][4] = {};
+    for (int i0 = part - 1; there && i0 < n; i0 += kBatch * kEntryWarps) {
+        float4 z[kBatch][NB];
+        float2 ml[kBatch];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    const float ref = M == -INFINITY ? 0.0f : M;
-    auto weight = [&](float2 x) { return x.y == 0.0f ? 0.0f : x.y != x.y ? x.y : x.y * attn_exp2(x.x - ref); };
-    float L = weight(own), y[NB];
+        for (int k = 0; k < kBatch; ++k) {
+            const int i = min(i0 + k * kEntryWarps, n - 1);
+            const float *from = i < 0 ? p.own + entry * HD : f.part + (first + i * stride) * HD;
+            ml[k] = __ldcg(i < 0 ? p.own_ml + entry : f.part_ml + first + i * stride);
+            if (i0 + k * kEntryWarps >= n) ml[k].y = 0.0f;
 #pragma unroll
-    for (int j = 0; j < NB; ++j) y[j] = own.y == 0.0f ? 0.0f : L * p.own[entry * HD + 32 * j + lane];
-    for (int i0 = 0; i0 < n; i0 += 32) {
-        float mine = 0.0f;
-        if (i0 + lane < n) mine = weight(__ldcg(f.part_ml + first + (i0 + lane) * stride));
-        const int end = min(32, n - i0);
-#pragma unroll 4
-        for (int i = 0; i < end; ++i) {
-            const float w = __shfl_sync(0xffffffffu, mine, i);
-            const float *x = f.part + (first + (i0 + i) * stride) * HD + lane;
+            for (int b = 0; b < NB; ++b) z[k][b] = __ldcg(reinterpret_cast<const float4 *>(from + b * (HD / NB) + at));
+        }
+        float top = M;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) top = ml[k].y != 0.0f ? fmaxf(top, ml[k].x) : top;
+        const float ref = top == -INFINITY ? 0.0f : top, keep = attn_exp2(M - ref);
+        M = top;
+        L *= keep;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[b][j] *= keep;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            // (What has no weight may be anything.)
+            const float w = ml[k].y == 0.0f ? 0.0f : ml[k].y != ml[k].y ? ml[k].y : ml[k].y * attn_exp2(ml[k].x - ref);
             L += w;
 #pragma unroll
-            for (int j = 0; j < NB; ++j) y[j] = fmaf(w, w == 0.0f ? 0.0f : __ldcg(x + 32 * j), y[j]);
+            for (int b = 0; b < NB; ++b) {
+                const float x[4] = {z[k][b].x, z[k][b].y, z[k][b].z, z[k][b].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[b][j] = fmaf(w, w == 0.0f ? 0.0f : x[j], y[b][j]);
+            }
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) means[warp][b][lane] = make_float4(y[b][0], y[b][1], y[b][2], y[b][3]);
+    if (lane == 0) {
+        tops[warp] = M;
+        sums[warp] = L;
+    }
+    __syncthreads();
+    if (part || !there) return;
+    float all = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kEntryWarps; ++k) all = fmaxf(all, tops[warp + k]);
+    const float ref = all == -INFINITY ? 0.0f : all;
+    L = 0.0f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[b][j] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kEntryWarps; ++k) {
+        const float sum = sums[warp + k], w = sum != sum ? sum : attn_exp2(tops[warp + k] - ref);
+        L = fmaf(w, sum, L);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const float4 x = means[warp + k][b][lane];
+            y[b][0] = fmaf(w, x.x, y[b][0]);
+            y[b][1] = fmaf(w, x.y, y[b][1]);
+            y[b][2] = fmaf(w, x.z, y[b][2]);
+            y[b][3] = fmaf(w, x.w, y[b][3]);
         }
     }
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    if (p.lse && lane == 0) p.lse[entry] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
-    const long long at = s * p.out_ss + (long long)h * p.out_hs + lane;
+    if (p.lse && lane == 0) p.lse[entry] = L == 0.0f ? -INFINITY : (all + log2f(L)) * 0.6931471805599453f;
+    if (lane >= kLanes) return;
+    const long long to = s * p.out_ss + (long long)h * p.out_hs + at;
 #pragma unroll
-    for (int j = 0; j < NB; ++j) {
-        if (p.io == DTYPE_F32) static_cast<float *>(p.out)[at + 32 * j] = y[j] * inv;
-        else if (p.io == DTYPE_BF16) static_cast<__nv_bfloat16 *>(p.out)[at + 32 * j] = __float2bfloat16_rn(y[j] * inv);
-        else static_cast<__half *>(p.out)[at + 32 * j] = __float2half_rn(y[j] * inv);
-    }
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const long long o = to + b * (HD / NB) + j;
+            const float v = y[b][j] * inv;
+            if (p.io == DTYPE_F32) static_cast<float *>(p.out)[o] = v;
+            else if (p.io == DTYPE_BF16) static_cast<__nv_bfloat16 *>(p.out)[o] = __float2bfloat16_rn(v);
+            else static_cast<__half *>(p.out)[o] = __float2half_rn(v);
+        }
 }
 
 cudaError_t run_join(const JoinParams &p, int head_dim, cudaStream_t st) {
-    const dim3 grid((unsigned)((p.entries + kJoinWarps - 1) / kJoinWarps)), block(kJoinWarps * 32);
+    constexpr int kEntries = kJoinWarps / kEntryWarps;
+    const dim3 grid((unsigned)((p.entries + kEntries - 1) / kEntries)), block(kJoinWarps * 32);
     switch (head_dim) {
         case 64: return launch_pdl(shared_join_kernel<64>, grid, block, 0, st, p);
         case 96: return launch_pdl(shared_join_kernel<96>, grid, block, 0, st, p);
@@ -107,11 +160,17 @@ cudaError_t run_join(const JoinParams &p, int head_dim, cudaStream_t st) {
 }
 
 cudaError_t run_prefix(int dtype, const PrefixParams &p, cudaStream_t st) {
-    return dtype == DTYPE_BF16 ? prefix_run_bf16(p, st) : prefix_run_f16(p, st);
+    switch (dtype) {
+        case DTYPE_F32: return prefix_run_f32(p, st);
+        case DTYPE_BF16: return prefix_run_bf16(p, st);
+        case DTYPE_F16: return prefix_run_f16(p, st);
+        case DTYPE_Q8_0: return prefix_run_q8_0(p, st);
+        default: return prefix_run_q4_0(p, st);
+    }
 }
 
-// Whether the prefix is a product on the tensor cores: where its rows are operands as they are.
-bool on_tensor_cores(int io, int cache) { return io != DTYPE_F32 && (cache == DTYPE_F16 || (cache == DTYPE_BF16 && io == DTYPE_BF16)); }
+// Whether the prefix is a product on the tensor cores.
+bool on_tensor_cores(int io) { return io != DTYPE_F32; }
 
 // The workspace of a call, in bytes from its start.
 struct SharedLayout {
@@ -132,7 +191,7 @@ SharedLayout shared_layout(kernel_context_t *ctx, const sapphire_kv_cache_t *c, 
     w.own = take(entries * c->head_dim * sizeof(float));
     w.own_ml = take(entries * sizeof(float2));
     size_t means = entries, attend = attn_workspace(ctx, c->dtype, c->head_dim, group);
-    if (on_tensor_cores(io, c->dtype)) {
+    if (on_tensor_cores(io)) {
         // Two tiles of rows share a pass over the prefix where there are that many.
         w.streams = rows > kPrefixRows ? prefix_streams(c->head_dim) : 1;
         w.row_sets = (int)((rows + w.streams * kPrefixRows - 1) / (w.streams * kPrefixRows));
@@ -264,7 +323,7 @@ extern "C" SAPPHIRE_API int sapphire_attention_shared_device(kernel_context_t *c
     f.part_ml = reinterpret_cast<float2 *>(ws + w.part_ml);
     f.err = ctx->d_err;
     f.device = ctx->device;
-    j.tc = on_tensor_cores(a->dtype, cache->dtype);
+    j.tc = on_tensor_cores(a->dtype);
     j.heads = a->heads;
     j.kv_heads = cache->kv_heads;
     j.entries = (long long)a->sequences * a->heads;
@@ -282,7 +341,9 @@ extern "C" SAPPHIRE_API int sapphire_attention_shared_device(kernel_context_t *c
         f.items = w.items;
         f.blocks = w.blocks;
         f.page_mul = (1ull << 32) / cache->page_size + 1;
-        f.q_wide = rows_aligned(a->q, f.q_ss, f.q_hs, size);
+        // (Copies of 16 bytes count their offsets in 32 bits.)
+        f.q_wide = rows_aligned(a->q, f.q_ss, f.q_hs, size) && f.q_ss >= 0 && f.q_hs >= 0 &&
+                   ((double)f.q_ss * a->sequences + (double)f.q_hs * a->heads) * size < 6.8e10;
         f.count = reinterpret_cast<int *>(ws + w.count);
         f.counts = sm_count(ctx->device) * kAttnMaxBlocks;
         e = run_prefix(cache->dtype, f, ctx->stream);

@@ -17,10 +17,13 @@
 // Layout.  A block per SM, whose roles are warps:
 //   0 - 3, 4 - 7  softmax of the first and the second tile of rows: a thread has a
 //                 row, as tensor memory does
-//   8             issues the MMAs
-//   9 - 12        bring rows into shared memory: K and V tiles in a ring of slots,
+//   8, 9          issue the MMAs of the first and the second tile of rows
+//   10            hands copied rows over to them (11 only lends its registers)
+//   12 - 15       bring rows into shared memory: K and V tiles in a ring of slots,
 //                 [64 dims][tokens][128 bytes] with the 128-byte swizzle, which is
 //                 K-major for S and N-major for O, so V needs no transposing
+// Launched with 128 registers a thread; the softmax takes 176 (a row's scores are in
+// registers), the others leave 80: 256 * 176 + 256 * 80 = 512 * 128.
 // Tensor memory holds, for each tile of rows, S (one column a token; P takes the
 // place of its first half as 16-bit pairs, the A operand of O's MMAs) and O.
 // While one tile of rows is in its softmax the other's MMAs run.  Its pages are of
@@ -44,7 +47,8 @@
 #include "tc.cuh"
 
 constexpr int kPrefixRows = 128;                  // of a tile
-constexpr int kPrefixThreads = 13 * 32;
+constexpr int kPrefixThreads = 16 * 32;
+constexpr int kPrefixMma = 8, kPrefixCopy = 12;    // first warps of these roles
 constexpr int kRunTokens = 8192;
 
 struct PrefixParams {
@@ -70,20 +74,26 @@ struct PrefixParams {
     int device;
 };
 
-// Tokens of a tile: S and O of two tiles of rows fit tensor memory's 512 columns
-// up to 192 dims.
-constexpr int prefix_tile(int hd) { return hd <= 128 ? 128 : 64; }
-constexpr int prefix_streams(int hd) { return hd <= 192 ? 2 : 1; }
+// Tiles of rows side by side, and tokens of a tile: S, P (half as many columns) and
+// O of each tile of rows share tensor memory's 512 columns, and K and V tiles what
+// shared memory the queries leave (four slots or more).
+constexpr int prefix_streams(int hd) { return hd <= 128 ? 2 : 1; }
+constexpr int prefix_tile(int hd) { return hd <= 64 ? 128 : hd <= 96 ? 96 : hd <= 128 ? 80 : hd <= 192 ? 96 : 64; }
 constexpr int prefix_chunks(int hd) { return (hd + 63) / 64; }
 constexpr int prefix_query_bytes(int hd) { return prefix_chunks(hd) * kPrefixRows * 128; }
 constexpr int prefix_slot_bytes(int hd) { return prefix_chunks(hd) * prefix_tile(hd) * 128; }
 constexpr int prefix_slots(int hd) {
-    const int n = (222 * 1024 - prefix_streams(hd) * prefix_query_bytes(hd)) / prefix_slot_bytes(hd);
+    const int n = (217 * 1024 - prefix_streams(hd) * prefix_query_bytes(hd)) / prefix_slot_bytes(hd);
     return n < 8 ? n : 8;
 }
-// How the blocks share the units (a tile of tokens of one item), item by item.
+// How the blocks share the units (a tile of tokens of one item): each item cut into
+// `parts` equal pieces, a block each; or, where that would leave blocks without work for
+// longer than a block's second item costs it (its queries, and results of its own: about
+// kItemUnits units), all units in a row into equal ranges, item by item.
+constexpr int kItemUnits = 5;
 struct PrefixRanges {
     int tiles;                     // of an item
+    int parts;                     // of an item, or 0: ranges
     unsigned total, blocks, each, longer;
 };
 __host__ __device__ inline PrefixRanges prefix_ranges(int items, long long length, int tile, int blocks) {
@@ -93,9 +103,27 @@ __host__ __device__ inline PrefixRanges prefix_ranges(int items, long long lengt
     r.blocks = r.total < (unsigned)blocks ? r.total : (unsigned)blocks;
     r.each = r.blocks ? r.total / r.blocks : 0;
     r.longer = r.total - r.each * r.blocks;
+    r.parts = 0;
+    if (r.blocks && items <= blocks) {
+        const int parts = blocks / items < r.tiles ? blocks / items : r.tiles;
+        if ((unsigned)((r.tiles + parts - 1) / parts) <= r.each + kItemUnits) {
+            r.parts = parts;
+            r.blocks = (unsigned)(items * parts);
+        }
+    }
     return r;
 }
+// The first unit of a block, and the block of a unit.
+__host__ __device__ inline unsigned prefix_first(const PrefixRanges &r, unsigned block) {
+    if (!r.parts) return block * r.each + (block < r.longer ? block : r.longer);
+    const unsigned item = block / r.parts, part = block - item * r.parts;
+    return item * r.tiles + (unsigned)((unsigned long long)part * r.tiles / r.parts);
+}
 __host__ __device__ inline unsigned prefix_block_of(const PrefixRanges &r, unsigned unit) {
+    if (r.parts) {
+        const unsigned item = unit / r.tiles, tile = unit - item * r.tiles;
+        return item * r.parts + (unsigned)((((unsigned long long)tile + 1) * r.parts - 1) / r.tiles);
+    }
     const unsigned split = r.longer * (r.each + 1);
     return unit < split ? unit / (r.each + 1) : r.longer + (unit - split) / r.each;
 }
@@ -112,64 +140,232 @@ __device__ __forceinline__ long long prefix_length(const PrefixParams &p, bool r
     return n;
 }
 
+// Two sums or products of fp32 in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n"
+        " fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n add.rn.f32x2 d, a, b;\n"
+        " mov.b64 {%0, %1}, d;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+// The larger, or NaN where one is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
 __device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<const uint32_t *>(&h); }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }      // e in -126 .. 127
 
+// 16 bytes from global to shared memory, or zeros.
+__device__ __forceinline__ void copy16_zfill(uint32_t dst, const uint8_t *src, bool ok) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+// Magnitudes, ordered like their bits, of those that are finite.
+__device__ __forceinline__ uint32_t finite_bits(uint32_t x) {
+    x &= 0x7fffffffu;
+    return x < 0x7f800000u ? x : 0u;
+}
+// The powers of two by which a warp's keys and values are divided before they become
+// fp16: the largest value (127 or 8 scales, quantised) goes to [2^14, 2^15).
+template <int kCache, int HD, int GT>
+__device__ __forceinline__ void prefix_exponents(const PrefixParams &p, const uint8_t *head, unsigned row16, unsigned page16, int slot, uint32_t valid,
+                                                 int lane, int (&e)[2]) {
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+        uint32_t top = 0;
+        if constexpr (kCache == DTYPE_Q8_0 || kCache == DTYPE_Q4_0) {
+            if ((valid >> lane) & 1) {
+                const uint8_t *at = head + (half ? p.l.vs_off : p.l.ks_off) + (unsigned long long)page16 * 16 + slot * p.l.scale_stride * 4;
+#pragma unroll
+                for (int b = 0; b < HD / 32; ++b) top = max(top, finite_bits(__ldg(reinterpret_cast<const uint32_t *>(at) + b)));
+            }
+        } else {
+            constexpr int PR = kCache == DTYPE_F32 ? HD / 4 : HD / 8;
+            const uint8_t *from = head + (half ? p.l.v_off : 0);
+#pragma unroll 4
+            for (int k = lane; k < (GT * PR + 31) / 32 * 32; k += 32) {
+                const int t = k / PR, c = k - t * PR;
+                const unsigned at = __shfl_sync(0xffffffffu, row16, t & 31) + c;
+                if (!((valid >> (t & 31)) & 1) || t >= GT) continue;
+                const uint4 x = __ldg(reinterpret_cast<const uint4 *>(from + ((unsigned long long)at << 4)));
+                const uint32_t v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (kCache == DTYPE_F32) top = max(top, finite_bits(v[j]));
+                    else top = max(top, max(finite_bits(v[j] << 16), finite_bits(v[j] & 0xffff0000u)));
+                }
+            }
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        constexpr int kTo = kCache == DTYPE_Q8_0 ? 7 : kCache == DTYPE_Q4_0 ? 11 : 14;
+        const int x = top == 0 ? -100 : min(max((int)(top >> 23) - 127 - kTo, -100), 120);
+        if (half) e[1] = x;
+        else e[0] = x;
+    }
+}
+
+// A warp's rows of K or V as fp16 into a slot, zeros where a token does not count.
+template <int kCache, int HD, int TN>
+__device__ __forceinline__ void prefix_convert(const PrefixParams &p, const uint8_t *head, int half, unsigned row16, unsigned page16, int slot,
+                                               uint32_t valid, int w, int lane, int e, uint8_t *to, uint32_t *scales) {
+    constexpr int GT = TN / 4, NB = HD / 32;
+    const uint8_t *from = head + (half ? p.l.v_off : 0);
+    const float down = pow2(-e);
+    // 16 bytes (8 bytes) of row t, dims d ..
+    auto place = [&](int t, int d) {
+        const int row = w * GT + t;
+        return to + (d >> 6) * (TN * 128) + row * 128 + ((((d >> 3) & 7) ^ (row & 7)) << 4) + (d & 7) * 2;
+    };
+    if constexpr (kCache == DTYPE_Q8_0 || kCache == DTYPE_Q4_0) {
+        constexpr int PR = kCache == DTYPE_Q8_0 ? HD / 16 : HD / 32, kN = (GT * PR + 31) / 32;
+        uint4 x[kN];
+#pragma unroll
+        for (int j = 0; j < kN; ++j) {
+            const int k = 32 * j + lane, t = k / PR, c = k - t * PR;
+            const unsigned at = __shfl_sync(0xffffffffu, row16, t & 31) + c;
+            if (t < GT) x[j] = __ldg(reinterpret_cast<const uint4 *>(from + ((unsigned long long)at << 4)));
+        }
+        // A scale in two fp16 parts, so that a value is rounded once.
+        if (lane < GT) {
+            const float *at = reinterpret_cast<const float *>(head + (half ? p.l.vs_off : p.l.ks_off) + (unsigned long long)page16 * 16 + slot * p.l.scale_stride * 4);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const float f = (valid >> lane) & 1 ? __ldg(at + b) * down : 0.0f;
+                const __half high = __float2half_rn(f);
+                scales[lane * NB + b] = half2_bits(__halves2half2(high, __float2half_rn(f - __half2float(high))));
+            }
+        }
+        __syncwarp();
+        const CodeConst codes = {0x64006400u, kCache == DTYPE_Q8_0 ? 0x64806480u : 0x64086408u, 0x2c002c00u, 0xd480d480u};
+        // Four dims of word `word`: code pairs times the scale of their block.
+        auto put = [&](int t, int word, uint32_t a, uint32_t b, bool there) {
+            const int i = word / NB, block = word - i * NB;
+            const uint32_t u = scales[t * NB + block];
+            const __half2 high = __low2half2(*reinterpret_cast<const __half2 *>(&u)), low = __high2half2(*reinterpret_cast<const __half2 *>(&u));
+            uint2 y;
+            y.x = half2_bits(__hfma2(*reinterpret_cast<const __half2 *>(&a), high, __hmul2(*reinterpret_cast<const __half2 *>(&a), low)));
+            y.y = half2_bits(__hfma2(*reinterpret_cast<const __half2 *>(&b), high, __hmul2(*reinterpret_cast<const __half2 *>(&b), low)));
+            *reinterpret_cast<uint2 *>(place(t, 32 * block + 4 * i)) = there ? y : make_uint2(0, 0);
+        };
+#pragma unroll
+        for (int j = 0; j < kN; ++j) {
+            const int k = 32 * j + lane, t = k / PR, c = k - t * PR;
+            if (t >= GT) continue;
+            const bool there = (valid >> t) & 1;
+            const uint32_t v[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (kCache == DTYPE_Q8_0) {
+                    put(t, 4 * c + i, bytes_to_half2<0x5150>(v[i], codes), bytes_to_half2<0x5352>(v[i], codes), there);
+                } else {
+                    // Two words: codes 0 .. 3 of each, code by code.
+                    const uint32_t c0 = nibbles_to_half2<0>(v[i], codes), c1 = nibbles_to_half2<4>(v[i], codes);
+                    const uint32_t c2 = nibbles_to_half2<0>(v[i] >> 8, codes), c3 = nibbles_to_half2<4>(v[i] >> 8, codes);
+                    put(t, 8 * c + 2 * i, __byte_perm(c0, c1, 0x5410), __byte_perm(c2, c3, 0x5410), there);
+                    put(t, 8 * c + 2 * i + 1, __byte_perm(c0, c1, 0x7632), __byte_perm(c2, c3, 0x7632), there);
+                }
+            }
+        }
+        __syncwarp();                                             // (the scales' readers)
+    } else {
+        constexpr int PR = HD / 8, kWords = kCache == DTYPE_F32 ? 2 : 1;       // of 16 bytes in 8 values
+#pragma unroll 4
+        for (int k = lane; k < GT * PR; k += 32) {
+            const int t = k / PR, c = k - t * PR;
+            const unsigned at = __shfl_sync(0xffffffffu, row16, t) + c * kWords;
+            uint32_t y[4] = {0, 0, 0, 0};
+            if ((valid >> t) & 1) {
+                float f[8];
+                if constexpr (kCache == DTYPE_F32) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float4 x = __ldg(reinterpret_cast<const float4 *>(from + ((unsigned long long)(at + i) << 4)));
+                        f[4 * i] = x.x, f[4 * i + 1] = x.y, f[4 * i + 2] = x.z, f[4 * i + 3] = x.w;
+                    }
+                } else {
+                    const uint4 x = __ldg(reinterpret_cast<const uint4 *>(from + ((unsigned long long)at << 4)));
+                    const uint32_t v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(v[i] << 16), f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] = half2_bits(__floats2half2_rn(f[2 * i] * down, f[2 * i + 1] * down));
+            }
+            *reinterpret_cast<uint4 *>(place(t, 8 * c)) = make_uint4(y[0], y[1], y[2], y[3]);
+        }
+    }
+}
+
 template <int kCache, int HD, bool kBf16>
 __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixParams p) {
-    constexpr int TN = prefix_tile(HD), GT = TN / 4, kChunks = prefix_chunks(HD), kSlots = prefix_slots(HD);
+    constexpr int TN = prefix_tile(HD), GT = TN / 4, kSlots = prefix_slots(HD), NB = HD / 32;
     constexpr int kQueryBytes = prefix_query_bytes(HD), kSlotBytes = prefix_slot_bytes(HD), kMaxStreams = prefix_streams(HD);
     constexpr int kRunTiles = kRunTokens / TN, kTileRing = 8;
     constexpr bool kRaw = (kCache == DTYPE_BF16 && kBf16) || kCache == DTYPE_F16;      // rows are copied as they are
     constexpr bool kQuant = kCache == DTYPE_Q8_0 || kCache == DTYPE_Q4_0;
     constexpr float kBias = kBf16 ? 0.0f : 7.0f, kLag = 8.0f;
+    // Columns: the tiles' O, then their S, then their P.
+    constexpr int kSCol = kMaxStreams * HD, kPCol = kSCol + kMaxStreams * TN, kPStep = (TN / 2 + 15) / 16 * 16;
+    static_assert(kPCol + kMaxStreams * kPStep <= 512 && kSlots >= 4 && HD % 32 == 0 && TN % 16 == 0, "");
     // fp32 += A B, both K-major for S; B's rows are the product's K for O
     constexpr uint32_t kFormat = (1u << 4) | (kBf16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(kPrefixRows >> 4) << 24);
     constexpr uint32_t kIdescS = kFormat | ((uint32_t)(TN >> 3) << 17), kIdescO = kFormat | (1u << 16) | ((uint32_t)(HD >> 3) << 17);
     extern __shared__ uint8_t smem_raw[];
     uint8_t *const smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    __shared__ uint64_t full[kSlots], empty[kSlots], q_full, s_full[2], p_ready[2], o_full[2], done;
+    __shared__ uint64_t landed[kRaw ? kSlots : 1], full[kSlots], empty[kSlots], q_full, s_full[2], s_free[2], p_ready[2], p_done[2], done[2];
     __shared__ uint32_t tmem_slot;
     __shared__ int s_abort;
     __shared__ float qmul[2][2][kPrefixRows];                     // [item's parity][tile of rows]
     __shared__ uint32_t counts[kTileRing][4];                     // tokens of a group that count
     __shared__ float k_up[kTileRing][4];                          // a group's keys are the operand's times this
     __shared__ int v_up[kTileRing][4];                            // and its values times 2 to this
+    __shared__ uint32_t block_scales[kQuant ? 4 : 1][kQuant ? GT * NB : 1];      // of the producers
     volatile int *const abort_flag = &s_abort;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     pdl_trigger();
     pdl_wait();
     const long long length = prefix_length(p, blockIdx.x == 0 && threadIdx.x == 0);
     for (int i = blockIdx.x * kPrefixThreads + threadIdx.x; i < p.counts; i += gridDim.x * kPrefixThreads) p.count[i] = 0;
     const PrefixRanges r = prefix_ranges(p.items, length, TN, p.blocks);
     if (blockIdx.x >= r.blocks) return;
-    const unsigned lo = blockIdx.x * r.each + min(blockIdx.x, r.longer), hi = lo + r.each + (blockIdx.x < r.longer ? 1 : 0);
-    const int item0 = (int)(lo / (unsigned)r.tiles), tile0 = (int)(lo - (unsigned)item0 * r.tiles), units = (int)(hi - lo);
+    const unsigned lo = prefix_first(r, blockIdx.x), hi = blockIdx.x + 1 < r.blocks ? prefix_first(r, blockIdx.x + 1) : r.total;
+    const int item0 = __shfl_sync(0xffffffffu, (int)(lo / (unsigned)r.tiles), 0);
+    const int tile0 = __shfl_sync(0xffffffffu, (int)(lo - (unsigned)item0 * r.tiles), 0), units = __shfl_sync(0xffffffffu, (int)(hi - lo), 0);
     auto fail = [&]() {
         *abort_flag = 1;
         atomicOr(p.err, 2);
     };
     // Tiles of rows of an item.
     auto streams_of = [&](int item) { return min(p.streams, (p.rows - (item % p.row_sets) * p.streams * kPrefixRows + kPrefixRows - 1) / kPrefixRows); };
-    // Whether a unit is the last of its item in this block, or the last of a run.
-    auto last_of_item = [&](int n, int tile) { return n + 1 == units || tile + 1 == r.tiles; };
 
     if (threadIdx.x == 0) {
         s_abort = 0;
         for (int s = 0; s < kSlots; ++s) {
-            mbar_init(full + s, 4);
-            mbar_init(empty + s, 1);
+            if (kRaw) mbar_init(landed + s, 4 + 4 * 32);          // a lane of each copying warp, and all lanes' copies
+            mbar_init(full + s, kRaw ? 1 : 4);
+            mbar_init(empty + s, p.streams);                      // of the issuing warps
         }
         mbar_init(&q_full, 4);
         for (int i = 0; i < 2; ++i) {
             mbar_init(s_full + i, 1);
+            mbar_init(s_free + i, 4);
             mbar_init(p_ready + i, 4);
-            mbar_init(o_full + i, 1);
+            mbar_init(p_done + i, 1);
+            mbar_init(done + i, 1);
         }
-        mbar_init(&done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) {
+    if (warp == kPrefixMma) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&tmem_slot)), "r"(512)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -178,75 +374,85 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
-    const uint32_t s_col[2] = {tmem, tmem + TN}, o_col[2] = {tmem + kMaxStreams * TN, tmem + kMaxStreams * TN + HD};
+    // (Arithmetic, not arrays: an index that the compiler does not know would put them
+    // into local memory, whose cache is what shared memory leaves.)
+    auto s_col = [&](int i) { return tmem + (uint32_t)(kSCol + i * TN); };
+    auto p_col = [&](int i) { return tmem + (uint32_t)(kPCol + i * kPStep); };
+    auto o_col = [&](int i) { return tmem + (uint32_t)(i * HD); };
     uint8_t *const slots = smem + kMaxStreams * kQueryBytes;
 
-    if (warp < 8) {
+    if (warp < kPrefixMma) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
         // ------------------------------------------------------- softmax --
         const int i = warp >> 2, row = (warp & 3) * 32 + lane;
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = s_col[i] + lanes, o_at = o_col[i] + lanes;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = s_col(i) + lanes, p_at = p_col(i) + lanes, o_at = o_col(i) + lanes;
         float m = -INFINITY, l = 0.0f, qm = 0.0f;                 // of the run
         float m_item = -INFINITY, l_item = 0.0f;                  // of the item's runs before it
         int e_run = -1000, item = item0, tile = tile0, run = 0;
-        uint32_t turn = 0, o_turn = 0;                            // tiles and runs of this tile of rows
+        uint32_t turn = 0;                                        // tiles of this tile of rows
         bool first_run = true;
+        int now = i < kMaxStreams ? streams_of(item) : 0;
         for (int n = 0; n < units; ++n) {
-            const bool last = last_of_item(n, tile);
-            if (i < streams_of(item)) {
+            const bool last = n + 1 == units || tile + 1 == r.tiles;
+            if (i < now) {
                 if (!wait_bounded(s_full + i, turn & 1, abort_flag)) {
                     if (lane == 0) fail();
                     break;
                 }
-                ++turn;
                 tc_fence_after();
-                const int ring = n % kTileRing;
+                const int ring = n & (kTileRing - 1);
                 if (run == 0 && first_run) qm = qmul[(item - item0) & 1][i][row];
                 uint32_t word[4];
+                float qg[4];
+                int eg[4], e_tile = -1000;
                 bool whole = true;
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     word[g] = counts[ring][g];
-                    whole = whole && word[g] == (GT == 32 ? 0xffffffffu : 0xffffu);
-                }
-                float qg[4];
-                int eg[4], e_tile = -1000;
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
+                    whole = whole && word[g] == 0xffffffffu >> (32 - GT);
                     qg[g] = kRaw ? qm : fmaxf(qm * k_up[ring][g], 1.2e-38f);
                     eg[g] = kRaw ? 0 : v_up[ring][g];
                     e_tile = max(e_tile, eg[g]);
                 }
-                // Scores of groups a and b, -inf where a token does not count.
-                float s[2][GT];
-                auto load = [&](int a) {
+                // The row's scores, -inf where a token does not count.
+                float s[TN];
+                uint32_t *const raw = reinterpret_cast<uint32_t *>(s);
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) tmem_load<GT>(s_at + (a + k) * GT, reinterpret_cast<uint32_t *>(s[k]));
-                    tmem_ld_wait();
-                    if (!whole) {
+                for (int c = 0; c < TN; c += 32) {
+                    if (c + 32 <= TN) tmem_load<32>(s_at + c, raw + c);
+                    else tmem_load<16>(s_at + c, raw + c);
+                }
+                tmem_ld_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_free + i);
+                if (!whole) {
 #pragma unroll
-                        for (int k = 0; k < 2; ++k)
-#pragma unroll
-                            for (int j = 0; j < GT; ++j)
-                                if (!((word[a + k] >> j) & 1)) s[k][j] = -INFINITY;
-                    }
-                };
+                    for (int j = 0; j < TN; ++j)
+                        if (!((word[j / GT] >> (j % GT)) & 1)) s[j] = -INFINITY;
+                }
+                // (A NaN among them makes every one of the row's probabilities NaN.)
                 float top = -INFINITY;
-                auto maximum = [&](int a) {
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        float t0 = s[k][0], t1 = s[k][1];
+                for (int g = 0; g < 4; ++g) {
+                    float t0 = s[g * GT], t1 = s[g * GT + 1];
 #pragma unroll
-                        for (int j = 2; j < GT; j += 2) {
-                            t0 = fmaxf(t0, s[k][j]);
-                            t1 = fmaxf(t1, s[k][j + 1]);
-                        }
-                        top = fmaxf(top, fmaxf(t0, t1) * qg[a + k]);
+                    for (int j = 2; j < GT; j += 2) {
+                        t0 = max_nan(t0, s[g * GT + j]);
+                        t1 = max_nan(t1, s[g * GT + j + 1]);
                     }
-                };
-                load(2);
-                maximum(2);
-                load(0);
-                maximum(0);
+                    const float t2 = max_nan(t0, t1) * qg[g];
+                    if (t2 != t2) qm = t2;
+                    top = fmaxf(top, t2);
+                }
+                // ---- the tile before has left P and O ----
+                if (turn > 0) {
+                    if (!wait_bounded(p_done + i, (turn - 1) & 1, abort_flag)) {
+                        if (lane == 0) fail();
+                        break;
+                    }
+                    tc_fence_after();
+                }
                 // ---- the reference, and O in its units ----
                 const bool grew = top > m + kLag || (m == -INFINITY && top > m), up = !kRaw && e_tile > e_run;
                 if (__any_sync(0xffffffffu, grew) || up) {
@@ -259,79 +465,76 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
                         e_run = e_tile;
                     }
                     if (run > 0) {
-                        // (S is behind the product of the tile before: O is at rest)
 #pragma unroll 1
-                        for (int c = 0; c < HD; c += 32) {
-                            float o[32];
-                            tmem_load<32>(o_at + c, reinterpret_cast<uint32_t *>(o));
+                        for (int c = 0; c < HD; c += 16) {
+                            float o[16];
+                            tmem_load<16>(o_at + c, reinterpret_cast<uint32_t *>(o));
                             tmem_ld_wait();
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) o[j] *= f;
-                            tmem_store<32>(o_at + c, reinterpret_cast<uint32_t *>(o));
+                            for (int j = 0; j < 16; ++j) o[j] *= f;
+                            tmem_store<16>(o_at + c, reinterpret_cast<uint32_t *>(o));
                         }
                     }
                 }
                 const float ref = m == -INFINITY ? 0.0f : kBias - m;
-                auto probabilities = [&](int a) {
+                float2 sum[4] = {};
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const int d = kRaw ? 0 : max(eg[a + k] - e_run, -100);
-                        const float at = kRaw ? ref : ref + (float)d;
-                        uint32_t w[GT / 2];
-                        float sum[2] = {0.0f, 0.0f};
+                for (int c = 0; c < TN; c += 16) {
+                    uint32_t w[8];
 #pragma unroll
-                        for (int j = 0; j < GT; j += 2) {
-                            const float x = attn_exp2(fmaf(s[k][j], qg[a + k], at)), y = attn_exp2(fmaf(s[k][j + 1], qg[a + k], at));
-                            sum[0] += x;
-                            sum[1] += y;
-                            w[j / 2] = pack16<kBf16>(x, y);
-                        }
-                        l += kRaw ? sum[0] + sum[1] : (sum[0] + sum[1]) * pow2(-d);
-                        tmem_store<GT / 2>(s_at + (a + k) * (GT / 2), w);
+                    for (int k = 0; k < 16; k += 2) {
+                        const int j = c + k, g = j / GT;
+                        const float mul = qm != qm ? qm : qg[g], at = kRaw ? ref : ref + (float)max(eg[g] - e_run, -100);
+                        const float2 x = fma2(make_float2(s[j], s[j + 1]), make_float2(mul, mul), make_float2(at, at));
+                        const float2 y = make_float2(attn_exp2(x.x), attn_exp2(x.y));
+                        sum[g] = add2(sum[g], y);
+                        w[k / 2] = pack16<kBf16>(y.x, y.y);
                     }
-                };
-                probabilities(0);
-                load(2);
-                probabilities(2);
+                    tmem_store<8>(p_at + c / 2, w);
+                }
+#pragma unroll
+                for (int g = 0; g < 4; ++g) l += kRaw ? sum[g].x + sum[g].y : (sum[g].x + sum[g].y) * pow2(min(e_run - eg[g], 100));
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_ready + i);
+                ++turn;
                 if (++run == kRunTiles || last) {
                     // ---- the run's O, added to the item's ----
-                    if (!wait_bounded(o_full + i, o_turn & 1, abort_flag)) {
+                    if (!wait_bounded(p_done + i, (turn - 1) & 1, abort_flag)) {
                         if (lane == 0) fail();
                         break;
                     }
-                    ++o_turn;
                     tc_fence_after();
                     m -= kBias;
                     const size_t at = ((size_t)(blockIdx.x + item) * p.streams + i) * kPrefixRows + row;
                     float *to = p.part + at * HD;
                     const float top_ml = fmaxf(m, m_item), ref_ml = top_ml == -INFINITY ? 0.0f : top_ml;
                     const float w0 = first_run || l_item == 0.0f ? 0.0f : l_item * attn_exp2(m_item - ref_ml);
-                    const float w1 = l == 0.0f ? 0.0f : l * attn_exp2(m - ref_ml), sum = w0 + w1;
-                    const float f0 = sum == 0.0f ? 0.0f : w0 / sum;
-                    const float f1 = l == 0.0f ? 0.0f : (w1 / sum) / l * (kRaw ? 1.0f : pow2(min(max(e_run, -126), 127)));
+                    const float w1 = l == 0.0f ? 0.0f : l * attn_exp2(m - ref_ml), all = w0 + w1;
+                    const float f0 = all == 0.0f ? 0.0f : w0 / all;
+                    const float f1 = l == 0.0f ? 0.0f : (w1 / all) / l * (kRaw ? 1.0f : pow2(min(max(e_run, -126), 127)));
 #pragma unroll 1
                     for (int c = 0; c < HD; c += 32) {
                         float o[32];
                         tmem_load<32>(o_at + c, reinterpret_cast<uint32_t *>(o));
                         tmem_ld_wait();
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                            if (l != 0.0f) y = make_float4(o[j] * f1, o[j + 1] * f1, o[j + 2] * f1, o[j + 3] * f1);
-                            if (!first_run) {
-                                const float4 x = *reinterpret_cast<const float4 *>(to + c + j);
-                                y = make_float4(fmaf(x.x, f0, y.x), fmaf(x.y, f0, y.y), fmaf(x.z, f0, y.z), fmaf(x.w, f0, y.w));
+                        for (int j = 0; j < 32; j += 8) {
+                            float y[8];
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) {
+                                y[k] = l == 0.0f ? 0.0f : o[j + k] * f1;
+                                if (!first_run) y[k] = fmaf(to[c + j + k], f0, y[k]);
                             }
-                            *reinterpret_cast<float4 *>(to + c + j) = y;
+                            asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + c + j), "f"(y[0]), "f"(y[1]),
+                                         "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7])
+                                         : "memory");
                         }
                     }
                     tc_fence_before();
                     m_item = top_ml;
-                    l_item = sum;
+                    l_item = all;
                     if (last) p.part_ml[at] = make_float2(m_item, l_item);
                     first_run = last;
                     m = -INFINITY;
@@ -343,93 +546,113 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
             if (++tile == r.tiles) {
                 tile = 0;
                 ++item;
+                if (n + 1 < units && i < kMaxStreams) now = streams_of(item);
             }
         }
-    } else if (warp == 8) {
-        // ---------------------------------------------------------- MMAs --
-        if (lane == 0) {
-            uint32_t p_turn[2] = {0, 0};
-            int item = item0, tile = tile0, run = 0;
-            auto scores = [&](int i, int slot) {
-                const uint32_t q = saddr(smem) + i * kQueryBytes, k = saddr(slots) + slot * kSlotBytes;
-#pragma unroll
-                for (int j = 0; j < HD / 16; ++j)
-                    umma_bf16(s_col[i], sw128_desc(q + (j / 4) * (kPrefixRows * 128) + (j % 4) * 32),
-                              sw128_desc(k + (j / 4) * (TN * 128) + (j % 4) * 32), kIdescS, j > 0);
-                umma_commit(s_full + i);
+    } else if (warp < kPrefixCopy) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        const int i = warp - kPrefixMma;                          // tile of rows
+        if (i < p.streams) {
+            // ------------------------------------------------------ MMAs --
+            // A warp for each tile of rows, so that neither waits for the other's softmax.
+            // The next tile's scores come before this one's outputs: the softmax has them
+            // when it is done with this one.
+            constexpr uint32_t kHigh = (1024u >> 4) | 1u << 14 | 2u << 29;  // stride, version, 128-byte swizzle
+            const uint32_t q_low = ((saddr(smem) + i * kQueryBytes) >> 4) | 1u << 16, k_low = (saddr(slots) >> 4) | 1u << 16;
+            const uint32_t v_low = (saddr(slots) >> 4) | (uint32_t)(TN * 128 >> 4) << 16;
+            const uint32_t s_at = s_col(i), p_at = p_col(i), o_at = o_col(i);
+            int item = item0, tile = tile0, run = 0, k_slot = 0, v_slot = 1;
+            uint32_t k_phase = 0, v_phase = 0, q_phase = 0, s_turn = 0, p_turn = 0;
+            auto step = [&](int &slot, uint32_t &phase) {         // two slots on
+                slot += 2;
+                if (slot >= kSlots) {
+                    slot -= kSlots;
+                    phase ^= 1;
+                }
             };
-            auto wait_full = [&](int index) { return wait_bounded(full + index % kSlots, (index / kSlots) & 1, abort_flag); };
-            bool ok = wait_bounded(&q_full, 0, abort_flag) && wait_full(0);
-            if (ok) {
-                tc_fence_after();
-                for (int i = 0; i < streams_of(item); ++i) scores(i, 0);
-                umma_commit(empty);
-            }
-            for (int n = 0; ok && n < units; ++n) {
-                const bool last = last_of_item(n, tile), flush = run + 1 == kRunTiles || last;
-                const int now = streams_of(item), next_item = tile + 1 == r.tiles ? item + 1 : item;
-                const int next = n + 1 < units ? streams_of(next_item) : 0;
-                const int vs = (2 * n + 1) % kSlots, ks = (2 * n + 2) % kSlots;
-                bool ready = false;
-                for (int i = 0; ok && i < max(now, next); ++i) {
-                    if (i < now) {
-                        ok = wait_bounded(p_ready + i, p_turn[i]++ & 1, abort_flag) && (i > 0 || wait_full(2 * n + 1));
-                        if (!ok) break;
-                        tc_fence_after();
-                        const uint32_t v = saddr(slots) + vs * kSlotBytes;
+            // (A tile of rows that an item does not have still gives its slots back.)
+            auto scores = [&](bool active, bool new_item) {
+                if (new_item && !wait_bounded(&q_full, q_phase++ & 1, abort_flag)) return false;
+                if (!wait_bounded(full + k_slot, k_phase, abort_flag)) return false;
+                if (active) {
+                    if (s_turn > 0 && !wait_bounded(s_free + i, (s_turn - 1) & 1, abort_flag)) return false;
+                    ++s_turn;
+                    tc_fence_after();
 #pragma unroll
-                        for (int j = 0; j < TN / 16; ++j)
-                            umma_ts(o_col[i], s_col[i] + 8 * j, sw128_desc_mn(v + j * 2048, TN * 128), kIdescO, run > 0 || j > 0);
-                        if (flush) umma_commit(o_full + i);
-                        if (i + 1 == now) umma_commit(empty + vs);
-                    }
-                    if (i < next) {
-                        if (!ready) {
-                            if (next_item != item) ok = wait_bounded(&q_full, (next_item - item0) & 1, abort_flag);
-                            ok = ok && wait_full(2 * n + 2);
-                            if (!ok) break;
-                            tc_fence_after();
-                            ready = true;
-                        }
-                        scores(i, ks);
-                        if (i + 1 == next) umma_commit(empty + ks);
-                    }
+                    for (int j = 0; j < HD / 16; ++j)
+                        umma_ss(s_at, q_low + (j / 4) * (kPrefixRows * 128 >> 4) + (j % 4) * 2,
+                                k_low + k_slot * (kSlotBytes >> 4) + (j / 4) * (TN * 128 >> 4) + (j % 4) * 2, kHigh, kIdescS, j > 0);
+                    umma_commit_warp(s_full + i);
+                    umma_commit_warp(empty + k_slot);
+                } else if (lane == 0) {
+                    mbar_arrive(empty + k_slot);
                 }
-                run = flush ? 0 : run + 1;
-                if (++tile == r.tiles) {
-                    tile = 0;
-                    ++item;
+                step(k_slot, k_phase);
+                return true;
+            };
+            auto outputs = [&](bool active) {
+                if (!wait_bounded(full + v_slot, v_phase, abort_flag)) return false;
+                if (active) {
+                    if (!wait_bounded(p_ready + i, p_turn++ & 1, abort_flag)) return false;
+                    tc_fence_after();
+#pragma unroll
+                    for (int j = 0; j < TN / 16; ++j)
+                        umma_ts(o_at, p_at + 8 * j, v_low + v_slot * (kSlotBytes >> 4) + j * (2048 >> 4), kHigh, kIdescO, run > 0 || j > 0);
+                    umma_commit_warp(p_done + i);
+                    umma_commit_warp(empty + v_slot);
+                } else if (lane == 0) {
+                    mbar_arrive(empty + v_slot);
+                }
+                step(v_slot, v_phase);
+                return true;
+            };
+            bool now = i < streams_of(item), ok = scores(now, true);
+            for (int n = 0; ok && n < units; ++n) {
+                const bool ends = tile + 1 == r.tiles, more = n + 1 < units;
+                const bool next = ends && more ? i < streams_of(item + 1) : now;
+                // (An item's first scores wait for its queries, which wait for the last one's
+                // scores, so outputs go first there.)
+                if (more && !ends) ok = scores(next, false);
+                ok = ok && outputs(now);
+                if (more && ends) ok = ok && scores(next, true);
+                run = run + 1 == kRunTiles || ends ? 0 : run + 1;
+                now = next;
+                if (ends) ++item;
+                tile = ends ? 0 : tile + 1;
+            }
+            if (!ok && lane == 0) fail();
+            __syncwarp();
+            umma_commit_warp(done + i);
+            (void)wait_bounded(done + i, 0, nullptr);
+        } else if (kRaw && i == 2) {
+            // What has landed is handed to the tensor cores' proxy by a warp that nobody
+            // waits for (by the issuing one: 500 cycles of every tile).
+            int s = 0;
+            uint32_t phase = 0;
+            for (int index = 0; index < 2 * units; ++index) {
+                if (!wait_bounded(landed + s, phase, abort_flag)) {
+                    if (lane == 0) fail();
+                    break;
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full + s);
+                if (++s == kSlots) {
+                    s = 0;
+                    phase ^= 1;
                 }
             }
-            if (!ok) fail();
-            umma_commit(&done);
-            (void)wait_bounded(&done, 0, nullptr);
         }
-        __syncwarp();
     } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         // ----------------------------------------------------- producers --
-        const int w = warp - 9;                                   // its tokens: GT w .. of a tile, and rows 32 w .. of the query
-        constexpr int kAhead = kRaw ? kSlots - 2 : 0;             // slots whose copies are on their way
-        const int total = 2 * units;
-        int signalled = 0;                                        // slots that this warp has filled
+        const int w = warp - kPrefixCopy;                         // its tokens: GT w .. of a tile, and rows 32 w .. of the query
         bool ok = true;
-        auto signal = [&](int index) {
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(full + index % kSlots);
-        };
-        auto drain = [&](int issued) {
-            if constexpr (kRaw) copies_wait<0>();
-            for (; signalled < issued; ++signalled) signal(signalled);
-        };
-        int item = item0, tile = tile0;
-        unsigned row16 = 0, page16 = 0;                           // of token `lane` of the tile: its row, and its page
-        int page_slot = 0;
-        uint32_t valid = 0;
-        int entry = -1, slot = 0;
-        auto fetch = [&](int t) {                                 // looks the tokens of a tile up
+        // Token `lane` of a tile: its page (-1: none) and slot.
+        auto fetch = [&](int t, int &entry, int &slot) {
             const long long tok = (long long)t * TN + w * GT + lane;
             entry = -1;
+            slot = 0;
             if (lane < GT && tok < length) {
                 int pg = (int)(((unsigned long long)(unsigned)tok * p.page_mul) >> 32);
                 slot = (int)tok - pg * p.l.page_size;
@@ -440,50 +663,140 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
                 entry = __ldg(p.table + pg);
             }
         };
-        fetch(tile);
+        // Copies of a lane (of rows as they are): piece 32 j + lane of the warp's rows, where
+        // it goes in a slot, and whose it is.
+        constexpr int PR = HD / 8, kCopies = kRaw ? GT * PR / 32 : 1;
+        static_assert(GT * PR % 32 == 0, "");
+        uint32_t to[kCopies];
+        if constexpr (kRaw) {
+#pragma unroll
+            for (int j = 0; j < kCopies; ++j) {
+                const int k = 32 * j + lane, t = k / PR, c = k - t * PR, row = w * GT + t;
+                to[j] = saddr(slots) + (c >> 3) * (TN * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+            }
+        }
+        int item = item0, tile = tile0, entry, slot, ring = 0, next_slot = 0, kh = item / p.row_sets;
+        uint32_t next_phase = 1;
+        fetch(tile, entry, slot);
         for (int n = 0; ok && n < units; ++n) {
-            const int kh = item / p.row_sets;
-            if (n == 0 || tile == 0) {
+            // ---- where the tile's tokens are ----
+            const bool wanted = lane < GT && (long long)tile * TN + w * GT + lane < length, found = (unsigned)entry < (unsigned)p.l.num_pages;
+            const unsigned page16 = (found ? (unsigned)entry : 0u) * (unsigned)(p.l.page_bytes >> 4);
+            const unsigned row16 = page16 + (unsigned)(slot * (p.l.row_bytes >> 4));
+            const uint32_t valid = __ballot_sync(0xffffffffu, found && wanted);
+            const int page_slot = slot;
+            if (wanted && !found) atomicOr(p.err, kErrCache);
+            if (n + 1 < units) fetch(tile + 1 == r.tiles ? 0 : tile + 1, entry, slot);
+            const uint8_t *const head = p.l.pages + (unsigned long long)kh * p.l.chunk_bytes;
+            if (lane == 0) counts[ring][w] = valid;
+            int e_half[2] = {0, 0};                               // powers of two of the group's keys and values
+            unsigned from[kCopies];
+            if constexpr (kRaw) {
+#pragma unroll
+                for (int j = 0; j < kCopies; ++j) {
+                    const int k = 32 * j + lane, t = k / PR;
+                    from[j] = __shfl_sync(0xffffffffu, row16, t) + (k - t * PR);
+                }
+            } else {
+                prefix_exponents<kCache, HD, GT>(p, head, row16, page16, page_slot, valid, lane, e_half);
+                if (lane == 0) {
+                    k_up[ring][w] = pow2(e_half[0]);
+                    v_up[ring][w] = e_half[1];
+                }
+            }
+            // ---- K, then V ----
+#pragma unroll 1
+            for (int half = 0; half < 2; ++half) {
+                if (!wait_bounded(empty + next_slot, next_phase, abort_flag)) {
+                    if (lane == 0) fail();
+                    ok = false;
+                    break;
+                }
+                const uint32_t at = next_slot * kSlotBytes;
+                if constexpr (kRaw) {
+                    const uint8_t *const rows = head + (half ? p.l.v_off : 0);
+                    if (valid == 0xffffffffu >> (32 - GT)) {
+#pragma unroll
+                        for (int j = 0; j < kCopies; ++j) copy_bytes<16>(to[j] + at, rows + ((unsigned long long)from[j] << 4));
+                    } else {
+#pragma unroll 1
+                        for (int j = 0; j < kCopies; ++j) {
+                            const int k = 32 * j + lane, t = k / PR, c = k - t * PR, row = w * GT + t;
+                            const unsigned src = __shfl_sync(0xffffffffu, row16, t) + c;
+                            copy16_zfill(saddr(slots) + at + (c >> 3) * (TN * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4),
+                                         rows + ((unsigned long long)src << 4), (valid >> t) & 1);
+                        }
+                    }
+                    // (They arrive when they land, whatever this warp does meanwhile.)
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(saddr(landed + next_slot)) : "memory");
+                    if (lane == 0) mbar_arrive(landed + next_slot);
+                } else {
+                    prefix_convert<kCache, HD, TN>(p, head, half, row16, page16, page_slot, valid, w, lane, half ? e_half[1] : e_half[0], slots + at,
+                                                   block_scales[kQuant ? w : 0]);
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(full + next_slot);
+                }
+                if (++next_slot == kSlots) {
+                    next_slot = 0;
+                    next_phase ^= 1;
+                }
+            }
+            ring = (ring + 1) % kTileRing;
+            if (ok && (n == 0 || tile == 0)) {
                 // ---- the item's queries ----
                 if (n > 0) {
-                    drain(2 * n);
                     const int index = 2 * n - 2;                  // the last scores of the item before
                     if (!wait_bounded(empty + index % kSlots, (index / kSlots) & 1, abort_flag)) {
                         if (lane == 0) fail();
                         break;
                     }
                 }
-                const int row = w * 32 + lane, swz = row & 7;
-                for (int i = 0; i < streams_of(item); ++i) {
+                // Rows by 16-byte copies, or by values where they lie anywhere; then, where
+                // they are converted or turned, each thread its row in place.
+                const int row = w * 32 + lane, streams = streams_of(item);
+                for (int i = 0; i < streams; ++i) {
                     const int at = ((item % p.row_sets) * p.streams + i) * kPrefixRows + row;
-                    const bool there = at < p.rows;
-                    const int seq = there ? at / p.group : 0;
-                    const long long from = seq * p.q_ss + (long long)(kh * p.group + (there ? at - seq * p.group : 0)) * p.q_hs;
-                    uint8_t *to = smem + i * kQueryBytes + row * 128;
-                    const bool convert = !kBf16 && p.io == DTYPE_BF16;
-                    const uint16_t *src = static_cast<const uint16_t *>(p.q) + from;
-                    auto piece = [&](int c, uint32_t (&x)[4]) {
-                        uint4 u = make_uint4(0, 0, 0, 0);
-                        if (there && p.q_wide) {
-                            u = __ldg(reinterpret_cast<const uint4 *>(src) + c);
-                        } else if (there) {
-                            uint16_t h[8];
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) h[j] = __ldg(src + 8 * c + j);
-                            memcpy(&u, h, sizeof u);
+                    const int seq = at < p.rows ? at / p.group : -1;
+                    const long long from = seq * p.q_ss + (long long)(kh * p.group + at - seq * p.group) * p.q_hs;
+                    const uint32_t rows_there = __ballot_sync(0xffffffffu, seq >= 0);
+                    if (p.q_wide) {
+                        const uint32_t from16 = (uint32_t)(from >> 3);        // (within 64 GB, checked on the host)
+#pragma unroll 4
+                        for (int j = 0; j < PR; ++j) {
+                            const int k = 32 * j + lane, t = k / PR, c = k - t * PR, q_row = w * 32 + t;
+                            const bool there = (rows_there >> t) & 1;
+                            const uint32_t at16 = __shfl_sync(0xffffffffu, from16, t), src = there ? at16 + c : 0u;
+                            copy16_zfill(saddr(smem) + i * kQueryBytes + (c >> 3) * (kPrefixRows * 128) + q_row * 128 + (((c & 7) ^ (q_row & 7)) << 4),
+                                         static_cast<const uint8_t *>(p.q) + ((unsigned long long)src << 4), there);
                         }
-                        const uint32_t sign = p.scale < 0.0f ? 0x80008000u : 0u;
-                        x[0] = u.x ^ sign, x[1] = u.y ^ sign, x[2] = u.z ^ sign, x[3] = u.w ^ sign;
-                    };
+                    } else {
+#pragma unroll 1
+                        for (int c = 0; c < PR; ++c) {
+                            uint16_t v[8] = {};
+                            if (seq >= 0) {
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) v[e] = __ldg(static_cast<const uint16_t *>(p.q) + from + 8 * c + e);
+                            }
+                            memcpy(smem + i * kQueryBytes + (c >> 3) * (kPrefixRows * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4), v, sizeof v);
+                        }
+                    }
+                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                __syncwarp();
+                const bool convert = !kBf16 && p.io == DTYPE_BF16;
+                const uint32_t sign = p.scale < 0.0f ? 0x80008000u : 0u;
+                for (int i = 0; i < streams; ++i) {
                     float up = 1.0f, mul = fmaxf(fabsf(p.scale), 1.2e-38f);
+                    auto piece = [&](int c) { return reinterpret_cast<uint4 *>(smem + i * kQueryBytes + (c >> 3) * (kPrefixRows * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)); };
                     if (convert) {
                         uint32_t top = 0;                         // magnitudes are ordered like their bits
 #pragma unroll 4
-                        for (int c = 0; c < HD / 8; ++c) {
-                            uint32_t x[4];
-                            piece(c, x);
+                        for (int c = 0; c < PR; ++c) {
+                            const uint4 x = *piece(c);
+                            const uint32_t v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) top = max(top, max(x[j] & 0x7fffu, (x[j] >> 16) & 0x7fffu));
+                            for (int j = 0; j < 4; ++j) top = max(top, max(v[j] & 0x7fffu, (v[j] >> 16) & 0x7fffu));
                         }
                         if (top > 0 && top < 0x7f80u) {
                             const int e = min(141 - (int)(top >> 7), 126);        // the largest goes to [2^14, 2^15)
@@ -491,16 +804,18 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
                             mul = fmaxf(mul * pow2(-e), 1.2e-38f);
                         }
                     }
+                    if (convert || sign) {
 #pragma unroll 4
-                    for (int c = 0; c < HD / 8; ++c) {
-                        uint32_t x[4];
-                        piece(c, x);
-                        if (convert) {
+                        for (int c = 0; c < PR; ++c) {
+                            const uint4 x = *piece(c);
+                            uint32_t v[4] = {x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign};
+                            if (convert) {
 #pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                x[j] = half2_bits(__floats2half2_rn(__uint_as_float(x[j] << 16) * up, __uint_as_float(x[j] & 0xffff0000u) * up));
+                                for (int j = 0; j < 4; ++j)
+                                    v[j] = half2_bits(__floats2half2_rn(__uint_as_float(v[j] << 16) * up, __uint_as_float(v[j] & 0xffff0000u) * up));
+                            }
+                            *piece(c) = make_uint4(v[0], v[1], v[2], v[3]);
                         }
-                        *reinterpret_cast<uint4 *>(to + (c / 8) * (kPrefixRows * 128) + (((c & 7) ^ swz) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
                     }
                     qmul[(item - item0) & 1][i][row] = mul;
                 }
@@ -508,61 +823,16 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_full);
             }
-            // ---- where the tile's tokens are ----
-            const bool found = (unsigned)entry < (unsigned)p.l.num_pages, wanted = lane < GT && (long long)tile * TN + w * GT + lane < length;
-            page16 = (found ? (unsigned)entry : 0u) * (unsigned)(p.l.page_bytes >> 4);
-            page_slot = slot;
-            row16 = page16 + (unsigned)(slot * (p.l.row_bytes >> 4));
-            valid = __ballot_sync(0xffffffffu, found && wanted);
-            if (wanted && !found) atomicOr(p.err, kErrCache);
-            if (n + 1 < units) fetch(tile + 1 == r.tiles ? 0 : tile + 1);
-            const uint8_t *head = p.l.pages + (unsigned long long)kh * p.l.chunk_bytes;
-            const int ring = n % kTileRing;
-
-            // ---- K, then V ----
-#pragma unroll 1
-            for (int half = 0; ok && half < 2; ++half) {
-                const int index = 2 * n + half;
-                if (!wait_bounded(empty + index % kSlots, ((index / kSlots) & 1) ^ 1, abort_flag)) {
-                    if (lane == 0) fail();
-                    ok = false;
-                    break;
-                }
-                uint8_t *const to = slots + (index % kSlots) * kSlotBytes;
-                if constexpr (kRaw) {
-                    constexpr int PR = HD / 8;                    // 16-byte pieces of a row
-                    const uint8_t *from = head + (half ? p.l.v_off : 0);
-                    const uint32_t dst = saddr(to);
-#pragma unroll 8
-                    for (int j = 0; j < GT * PR / 32; ++j) {
-                        const int k = 32 * j + lane, t = k / PR, c = k - t * PR, row = w * GT + t;
-                        const unsigned at = __shfl_sync(0xffffffffu, row16, t) + c;
-                        copy_or_zero<16>(dst + (c >> 3) * (TN * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4),
-                                         from + ((unsigned long long)at << 4), (valid >> t) & 1);
-                    }
-                    if (half == 0 && lane == 0) counts[ring][w] = valid;
-                    copies_commit();
-                    if (signalled + kAhead <= index) {
-                        copies_wait<kAhead>();
-                        signal(signalled++);
-                    }
-                }
-                (void)kQuant;
-                (void)page_slot;
-                (void)k_up;
-                (void)v_up;
-            }
             if (++tile == r.tiles) {
                 tile = 0;
-                ++item;
+                kh = ++item / p.row_sets;
             }
         }
-        if (ok) drain(total);
-        else if constexpr (kRaw) copies_wait<0>();
+        asm volatile("cp.async.wait_all;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == kPrefixMma) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
@@ -589,5 +859,8 @@ cudaError_t prefix_launch(const PrefixParams &p, cudaStream_t st) {
 #endif
 
 // One cache type each (prefix_<type>.cu).
+cudaError_t prefix_run_f32(const PrefixParams &p, cudaStream_t st);
 cudaError_t prefix_run_bf16(const PrefixParams &p, cudaStream_t st);
 cudaError_t prefix_run_f16(const PrefixParams &p, cudaStream_t st);
+cudaError_t prefix_run_q8_0(const PrefixParams &p, cudaStream_t st);
+cudaError_t prefix_run_q4_0(const PrefixParams &p, cudaStream_t st);

@@ -38,15 +38,16 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
     return ok != 0;
 }
 // Waits for the phase of `bar` with the given parity; false after kWaitNs or,
-// when abort_flag is given, once another role has set it.
+// when abort_flag is given, once another role has set it.  (Reading the timer
+// takes longer than a tile's softmax, so it is read between many tries.)
 __device__ __forceinline__ bool wait_bounded(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
-    for (int i = 0; i < 64; ++i)
-        if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = globaltimer();
+    uint64_t t0 = 0;
     for (;;) {
-        if (mbar_try_wait(bar, parity)) return true;
+        for (int i = 0; i < 4096; ++i)
+            if (mbar_try_wait(bar, parity)) return true;
         if (abort_flag && *abort_flag) return false;
-        if (globaltimer() - t0 > kWaitNs) return false;
+        if (t0 == 0) t0 = globaltimer();
+        else if (globaltimer() - t0 > kWaitNs) return false;
     }
 }
 __device__ __forceinline__ void fence_proxy_async() {
@@ -103,23 +104,35 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
-// The same of an operand whose rows are the product's K and hold N (64 bf16 of
-// it, 128 B), swizzled: 8-row groups 1024 B apart, the next 64 of N `next` bytes on.
-__device__ __forceinline__ uint64_t sw128_desc_mn(uint32_t addr, uint32_t next) {
-    uint64_t d = (uint64_t)((addr >> 4) & 0x3FFFu);
-    d |= (uint64_t)(next >> 4) << 16;       // leading byte offset
-    d |= (uint64_t)(1024 >> 4) << 32;       // stride byte offset
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)2 << 61;
-    return d;
-}
-// A from tensor memory.
-__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
+// An operand whose rows are the product's K and hold N (64 bf16 of it, 128 B) has the
+// same descriptor, but that the leading byte offset is the distance to the next 64 of N.
+// For a warp that runs together: one lane issues, elected within the instruction's
+// block, so what descriptors are made of stays in uniform registers (issued from a
+// branch of one lane an MMA takes 70 to 115 cycles, whatever its size; 33 to 64 so).
+// Operands by their descriptors' low words, whose high words are alike; A from shared
+// or from tensor memory.
+__device__ __forceinline__ void umma_ss(uint32_t tmem_d, uint32_t a_low, uint32_t b_low, uint32_t high, uint32_t idesc,
                                         uint32_t accumulate) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
-        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "{\n .reg .pred p, q;\n .reg .b64 a, b;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %5, 0;\n"
+        " mov.b64 a, {%1, %3};\n mov.b64 b, {%2, %3};\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n}\n" ::"r"(tmem_d),
+        "r"(a_low), "r"(b_low), "r"(high), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_low, uint32_t high, uint32_t idesc,
+                                        uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p, q;\n .reg .b64 b;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %5, 0;\n"
+        " mov.b64 b, {%2, %3};\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}\n" ::"r"(tmem_d),
+        "r"(tmem_a), "r"(b_low), "r"(high), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void umma_commit_warp(uint64_t *bar) {
+    asm volatile(
+        "{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n"
+        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(saddr(bar))
         : "memory");
 }
 // N (32 or 16) columns of a warp's 32 lanes, on their way until tmem_ld_wait.
