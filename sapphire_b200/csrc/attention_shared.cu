@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) shared_join_kernel(const Join
     long long first = (long long)kh * f.rows + row, stride = 0;
     if (p.tc) {
         const int set_rows = f.streams * kPrefixRows, set = row / set_rows, item = kh * f.row_sets + set;
-        const PrefixRanges r = prefix_ranges(f.items, prefix_length(f, false), prefix_tile(HD), f.blocks);
+        const PrefixRanges r = prefix_ranges(f.items, prefix_length(f, false), f.tile, f.blocks);
         n = 0;
         if (r.tiles > 0) {
             const unsigned unit = (unsigned)item * r.tiles, b0 = prefix_block_of(r, unit), b1 = prefix_block_of(r, unit + r.tiles - 1);
@@ -340,6 +340,7 @@ extern "C" SAPPHIRE_API int sapphire_attention_shared_device(kernel_context_t *c
         f.row_sets = w.row_sets;
         f.items = w.items;
         f.blocks = w.blocks;
+        f.tile = prefix_tile(cache->head_dim, cache->dtype);
         f.page_mul = (1ull << 32) / cache->page_size + 1;
         // (Copies of 16 bytes count their offsets in 32 bits.)
         f.q_wide = rows_aligned(a->q, f.q_ss, f.q_hs, size) && f.q_ss >= 0 && f.q_hs >= 0 &&

@@ -19,11 +19,12 @@
 //                 row, as tensor memory does
 //   8, 9          issue the MMAs of the first and the second tile of rows
 //   10            hands copied rows over to them (11 only lends its registers)
-//   12 - 15       bring rows into shared memory: K and V tiles in a ring of slots,
+//   12 - 15 (19)  bring rows into shared memory: K and V tiles in a ring of slots,
 //                 [64 dims][tokens][128 bytes] with the 128-byte swizzle, which is
 //                 K-major for S and N-major for O, so V needs no transposing
-// Launched with 128 registers a thread; the softmax takes 176 (a row's scores are in
-// registers), the others leave 80: 256 * 176 + 256 * 80 = 512 * 128.
+// Launched with 96 registers a thread (128 of 16 warps); the softmax takes 152 (168: a
+// row's scores are in registers), the MMAs' warps leave 48 (88) and the others 64 (88):
+// 256 * 152 + 128 * 48 + 256 * 64 = 640 * 96 (256 * 168 + 256 * 88 = 512 * 128).
 // Tensor memory holds, for each tile of rows, S (one column a token; P takes the
 // place of its first half as 16-bit pairs, the A operand of O's MMAs) and O.
 // While one tile of rows is in its softmax the other's MMAs run.  Its pages are of
@@ -32,9 +33,9 @@
 // Rounding.  Operands are bf16 over bf16 caches under bf16 queries, else fp16:
 //   a query of bf16 is brought to [2^14, 2^15) by a power of two a row, exact down to
 //   2^-29 of its largest value;
-//   Q8_0 and Q4_0 values are rounded to fp16 once, and F32 and BF16 ones too, each
-//   group of tokens (a warp's 32 or 16) times a power of two that brings its largest
-//   value below 2^15.  K's power multiplies the group's scores, V's is added to their
+//   Q8_0 and Q4_0 values are products of fp16 (their scale is rounded to it, and the
+//   product), F32 and BF16 values are rounded to it once; each group of tokens (a warp's, 6
+//   to 16) times a power of two that brings its largest scale or value to [2^14, 2^15).  K's power multiplies the group's scores, V's is added to their
 //   exponent, relative to the largest so far, and O carries that one;
 //   probabilities are rounded to the operand type once, as the outputs are.  m may lag
 //   behind the maximum by 2^8 before O is brought up to date, so fp16 probabilities
@@ -47,8 +48,12 @@
 #include "tc.cuh"
 
 constexpr int kPrefixRows = 128;                  // of a tile
-constexpr int kPrefixThreads = 16 * 32;
 constexpr int kPrefixMma = 8, kPrefixCopy = 12;    // first warps of these roles
+constexpr int kConverters = 8;                    // warps that bring rows and convert them
+// Rows that are operands as they are take four (eight: 53 -> 58 us, 64 sequences behind
+// 32768 tokens in bf16).
+constexpr bool prefix_raw(int cache, bool bf16) { return cache == DTYPE_F16 || (cache == DTYPE_BF16 && bf16); }
+constexpr int prefix_copiers(int cache, bool bf16) { return prefix_raw(cache, bf16) ? 4 : kConverters; }
 constexpr int kRunTokens = 8192;
 
 struct PrefixParams {
@@ -63,6 +68,7 @@ struct PrefixParams {
     int row_sets;                  // sets of `streams` tiles of a KV head
     int items;                     // kv_heads * row_sets
     int blocks;                    // of the launch
+    int tile;                      // tokens of a tile
     float scale;                   // scores times log2 e
     unsigned long long page_mul;
     bool q_wide;                   // rows of q on 16 bytes
@@ -76,15 +82,27 @@ struct PrefixParams {
 
 // Tiles of rows side by side, and tokens of a tile: S, P (half as many columns) and
 // O of each tile of rows share tensor memory's 512 columns, and K and V tiles what
-// shared memory the queries leave (four slots or more).
+// shared memory the queries leave.
 constexpr int prefix_streams(int hd) { return hd <= 128 ? 2 : 1; }
-constexpr int prefix_tile(int hd) { return hd <= 64 ? 128 : hd <= 96 ? 96 : hd <= 128 ? 80 : hd <= 192 ? 96 : 64; }
+constexpr bool prefix_quant(int cache) { return cache == DTYPE_Q8_0 || cache == DTYPE_Q4_0; }
+constexpr int prefix_tile(int hd, int cache) { return hd <= 64 ? 128 : hd <= 96 ? 96 : hd <= 192 ? 80 : prefix_quant(cache) ? 48 : 64; }
 constexpr int prefix_chunks(int hd) { return (hd + 63) / 64; }
 constexpr int prefix_query_bytes(int hd) { return prefix_chunks(hd) * kPrefixRows * 128; }
-constexpr int prefix_slot_bytes(int hd) { return prefix_chunks(hd) * prefix_tile(hd) * 128; }
-constexpr int prefix_slots(int hd) {
-    const int n = (217 * 1024 - prefix_streams(hd) * prefix_query_bytes(hd)) / prefix_slot_bytes(hd);
-    return n < 8 ? n : 8;
+constexpr int prefix_slot_bytes(int hd, int cache) { return prefix_chunks(hd) * prefix_tile(hd, cache) * 128; }
+constexpr int kPrefixShared = 217 * 1024;
+constexpr int prefix_slots(int hd, int cache) {
+    const int most = prefix_quant(cache) ? (hd <= 128 ? 4 : 3) : 8;
+    const int n = (kPrefixShared - prefix_streams(hd) * prefix_query_bytes(hd)) / prefix_slot_bytes(hd, cache);
+    return n < most ? n : most;
+}
+// Quantised rows wait in a ring of two tiles before they become fp16: bytes of a token's
+// row there (off the banks of its neighbours'), and of a warp's tile: K rows, V rows, eight
+// scales of each.
+constexpr int prefix_raw_row(int hd, int cache) { return (cache == DTYPE_Q8_0 ? hd : hd / 2) + 16; }
+constexpr int prefix_raw_tile(int hd, int cache) { return prefix_quant(cache) ? prefix_tile(hd, cache) / kConverters * 2 * (prefix_raw_row(hd, cache) + 32) : 0; }
+constexpr size_t prefix_shared_bytes(int hd, int cache) {
+    return 1024 + (size_t)prefix_streams(hd) * prefix_query_bytes(hd) + (size_t)prefix_slots(hd, cache) * prefix_slot_bytes(hd, cache) +
+           2 * kConverters * prefix_raw_tile(hd, cache);
 }
 // How the blocks share the units (a tile of tokens of one item): each item cut into
 // `parts` equal pieces, a block each; or, where that would leave blocks without work for
@@ -175,148 +193,122 @@ __device__ __forceinline__ uint32_t finite_bits(uint32_t x) {
     x &= 0x7fffffffu;
     return x < 0x7f800000u ? x : 0u;
 }
-// The powers of two by which a warp's keys and values are divided before they become
-// fp16: the largest value (127 or 8 scales, quantised) goes to [2^14, 2^15).
-template <int kCache, int HD, int GT>
-__device__ __forceinline__ void prefix_exponents(const PrefixParams &p, const uint8_t *head, unsigned row16, unsigned page16, int slot, uint32_t valid,
-                                                 int lane, int (&e)[2]) {
+// The power of two that a group's largest magnitude (its bits: of a value, or of a scale)
+// is divided by, to go to [2^14, 2^15).
+__device__ __forceinline__ int prefix_exponent(uint32_t top) {
+    top = __reduce_max_sync(0xffffffffu, top);
+    return top == 0 ? -100 : min(max((int)(top >> 23) - 127 - 14, -100), 96);
+}
+
+// A warp's quantised rows of a tile, which wait in shared memory (K rows, V rows, their
+// scales), as fp16 into the slots of K and V, zeros where a token does not count.  A lane
+// takes one block of 32 codes a round, which lie in 8 words nb apart, and writes them as 64
+// neighbouring bytes.
+template <int kCache, int HD>
+__device__ __forceinline__ void prefix_unpack(const uint8_t *raw, uint32_t valid, int first_row, int lane, float k_down, float v_down, uint8_t *k_to, uint8_t *v_to) {
+    constexpr int TN = prefix_tile(HD, kCache), GT = TN / kConverters, NB = HD / 32, kRow = prefix_raw_row(HD, kCache);
+    const float *const scales = reinterpret_cast<const float *>(raw + 2 * GT * kRow);
+    // A code's bits are an fp16 subnormal, 2^-24 times it (a nibble four bits up: 2^-20),
+    // so one product and sum, rounded once, with the scale and its offset make it a value
+    // (2^-24, 2^-20 of it, which the group's power of two makes up for).
 #pragma unroll 1
-    for (int half = 0; half < 2; ++half) {
-        uint32_t top = 0;
-        if constexpr (kCache == DTYPE_Q8_0 || kCache == DTYPE_Q4_0) {
-            if ((valid >> lane) & 1) {
-                const uint8_t *at = head + (half ? p.l.vs_off : p.l.ks_off) + (unsigned long long)page16 * 16 + slot * p.l.scale_stride * 4;
+    for (int k = lane; k < 2 * GT * NB; k += 32) {
+        const int t2 = k / NB, b = k - t2 * NB, t = t2 < GT ? t2 : t2 - GT, row = first_row + t;
+        uint32_t w[8];
 #pragma unroll
-                for (int b = 0; b < HD / 32; ++b) top = max(top, finite_bits(__ldg(reinterpret_cast<const uint32_t *>(at) + b)));
-            }
-        } else {
-            constexpr int PR = kCache == DTYPE_F32 ? HD / 4 : HD / 8;
-            const uint8_t *from = head + (half ? p.l.v_off : 0);
-#pragma unroll 4
-            for (int k = lane; k < (GT * PR + 31) / 32 * 32; k += 32) {
-                const int t = k / PR, c = k - t * PR;
-                const unsigned at = __shfl_sync(0xffffffffu, row16, t & 31) + c;
-                if (!((valid >> (t & 31)) & 1) || t >= GT) continue;
-                const uint4 x = __ldg(reinterpret_cast<const uint4 *>(from + ((unsigned long long)at << 4)));
-                const uint32_t v[4] = {x.x, x.y, x.z, x.w};
+        for (int i = 0; i < 8; ++i)
+            w[i] = kCache == DTYPE_Q8_0 ? reinterpret_cast<const uint32_t *>(raw + t2 * kRow)[i * NB + b] : reinterpret_cast<const uint16_t *>(raw + t2 * kRow)[i * NB + b];
+        const __half f = __float2half_rn((valid >> t) & 1 ? scales[t2 * 8 + b] * (t2 < GT ? k_down : v_down) : 0.0f);
+        const __half2 mul = __half2half2(f), add = __half2half2(__float2half_rn(__half2float(f) * -0x1p-17f));      // 128 2^-24 and 8 2^-20
+        uint8_t *at = (t2 < GT ? k_to : v_to) + (b >> 1) * (TN * 128) + row * 128;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (kCache == DTYPE_F32) top = max(top, finite_bits(v[j]));
-                    else top = max(top, max(finite_bits(v[j] << 16), finite_bits(v[j] & 0xffff0000u)));
+        for (int u = 0; u < 4; ++u) {
+            uint32_t c[4];
+            if constexpr (kCache == DTYPE_Q8_0) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    c[2 * i] = __byte_perm(w[2 * u + i], 0u, 0x4140);
+                    c[2 * i + 1] = __byte_perm(w[2 * u + i], 0u, 0x4342);
                 }
+            } else {
+                // Code by code of two words, then word by word.
+                const uint32_t x = w[2 * u] | w[2 * u + 1] << 16;
+                const uint32_t c0 = (x << 4) & 0x00f000f0u, c1 = x & 0x00f000f0u, c2 = (x >> 4) & 0x00f000f0u, c3 = (x >> 8) & 0x00f000f0u;
+                c[0] = __byte_perm(c0, c1, 0x5410);
+                c[1] = __byte_perm(c2, c3, 0x5410);
+                c[2] = __byte_perm(c0, c1, 0x7632);
+                c[3] = __byte_perm(c2, c3, 0x7632);
             }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[i] = half2_bits(__hfma2(*reinterpret_cast<const __half2 *>(&c[i]), mul, add));
+            *reinterpret_cast<uint4 *>(at + ((((b & 1) * 4 + u) ^ (row & 7)) << 4)) = make_uint4(c[0], c[1], c[2], c[3]);
         }
-        top = __reduce_max_sync(0xffffffffu, top);
-        constexpr int kTo = kCache == DTYPE_Q8_0 ? 7 : kCache == DTYPE_Q4_0 ? 11 : 14;
-        const int x = top == 0 ? -100 : min(max((int)(top >> 23) - 127 - kTo, -100), 120);
-        if (half) e[1] = x;
-        else e[0] = x;
     }
 }
 
-// A warp's rows of K or V as fp16 into a slot, zeros where a token does not count.
-template <int kCache, int HD, int TN>
-__device__ __forceinline__ void prefix_convert(const PrefixParams &p, const uint8_t *head, int half, unsigned row16, unsigned page16, int slot,
-                                               uint32_t valid, int w, int lane, int e, uint8_t *to, uint32_t *scales) {
-    constexpr int GT = TN / 4, NB = HD / 32;
-    const uint8_t *from = head + (half ? p.l.v_off : 0);
-    const float down = pow2(-e);
-    // 16 bytes (8 bytes) of row t, dims d ..
-    auto place = [&](int t, int d) {
-        const int row = w * GT + t;
-        return to + (d >> 6) * (TN * 128) + row * 128 + ((((d >> 3) & 7) ^ (row & 7)) << 4) + (d & 7) * 2;
-    };
-    if constexpr (kCache == DTYPE_Q8_0 || kCache == DTYPE_Q4_0) {
-        constexpr int PR = kCache == DTYPE_Q8_0 ? HD / 16 : HD / 32, kN = (GT * PR + 31) / 32;
-        uint4 x[kN];
-#pragma unroll
-        for (int j = 0; j < kN; ++j) {
-            const int k = 32 * j + lane, t = k / PR, c = k - t * PR;
-            const unsigned at = __shfl_sync(0xffffffffu, row16, t & 31) + c;
-            if (t < GT) x[j] = __ldg(reinterpret_cast<const uint4 *>(from + ((unsigned long long)at << 4)));
-        }
-        // A scale in two fp16 parts, so that a value is rounded once.
-        if (lane < GT) {
-            const float *at = reinterpret_cast<const float *>(head + (half ? p.l.vs_off : p.l.ks_off) + (unsigned long long)page16 * 16 + slot * p.l.scale_stride * 4);
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const float f = (valid >> lane) & 1 ? __ldg(at + b) * down : 0.0f;
-                const __half high = __float2half_rn(f);
-                scales[lane * NB + b] = half2_bits(__halves2half2(high, __float2half_rn(f - __half2float(high))));
-            }
-        }
-        __syncwarp();
-        const CodeConst codes = {0x64006400u, kCache == DTYPE_Q8_0 ? 0x64806480u : 0x64086408u, 0x2c002c00u, 0xd480d480u};
-        // Four dims of word `word`: code pairs times the scale of their block.
-        auto put = [&](int t, int word, uint32_t a, uint32_t b, bool there) {
-            const int i = word / NB, block = word - i * NB;
-            const uint32_t u = scales[t * NB + block];
-            const __half2 high = __low2half2(*reinterpret_cast<const __half2 *>(&u)), low = __high2half2(*reinterpret_cast<const __half2 *>(&u));
-            uint2 y;
-            y.x = half2_bits(__hfma2(*reinterpret_cast<const __half2 *>(&a), high, __hmul2(*reinterpret_cast<const __half2 *>(&a), low)));
-            y.y = half2_bits(__hfma2(*reinterpret_cast<const __half2 *>(&b), high, __hmul2(*reinterpret_cast<const __half2 *>(&b), low)));
-            *reinterpret_cast<uint2 *>(place(t, 32 * block + 4 * i)) = there ? y : make_uint2(0, 0);
-        };
-#pragma unroll
-        for (int j = 0; j < kN; ++j) {
-            const int k = 32 * j + lane, t = k / PR, c = k - t * PR;
-            if (t >= GT) continue;
-            const bool there = (valid >> t) & 1;
-            const uint32_t v[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (kCache == DTYPE_Q8_0) {
-                    put(t, 4 * c + i, bytes_to_half2<0x5150>(v[i], codes), bytes_to_half2<0x5352>(v[i], codes), there);
-                } else {
-                    // Two words: codes 0 .. 3 of each, code by code.
-                    const uint32_t c0 = nibbles_to_half2<0>(v[i], codes), c1 = nibbles_to_half2<4>(v[i], codes);
-                    const uint32_t c2 = nibbles_to_half2<0>(v[i] >> 8, codes), c3 = nibbles_to_half2<4>(v[i] >> 8, codes);
-                    put(t, 8 * c + 2 * i, __byte_perm(c0, c1, 0x5410), __byte_perm(c2, c3, 0x5410), there);
-                    put(t, 8 * c + 2 * i + 1, __byte_perm(c0, c1, 0x7632), __byte_perm(c2, c3, 0x7632), there);
-                }
-            }
-        }
-        __syncwarp();                                             // (the scales' readers)
-    } else {
-        constexpr int PR = HD / 8, kWords = kCache == DTYPE_F32 ? 2 : 1;       // of 16 bytes in 8 values
+// The largest finite magnitude of a warp's F32 or BF16 rows.
+template <int kCache, int HD, int GT>
+__device__ __forceinline__ uint32_t prefix_largest(const uint8_t *from, unsigned row16, uint32_t valid, int lane) {
+    constexpr int PR = kCache == DTYPE_F32 ? HD / 4 : HD / 8;
+    uint32_t top = 0;
 #pragma unroll 4
-        for (int k = lane; k < GT * PR; k += 32) {
-            const int t = k / PR, c = k - t * PR;
-            const unsigned at = __shfl_sync(0xffffffffu, row16, t) + c * kWords;
-            uint32_t y[4] = {0, 0, 0, 0};
-            if ((valid >> t) & 1) {
-                float f[8];
-                if constexpr (kCache == DTYPE_F32) {
+    for (int k = lane; k < (GT * PR + 31) / 32 * 32; k += 32) {
+        const int t = k / PR, c = k - t * PR;
+        const unsigned at = __shfl_sync(0xffffffffu, row16, t & 31) + c;
+        if (!((valid >> (t & 31)) & 1) || t >= GT) continue;
+        const uint4 x = __ldg(reinterpret_cast<const uint4 *>(from + ((unsigned long long)at << 4)));
+        const uint32_t v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const float4 x = __ldg(reinterpret_cast<const float4 *>(from + ((unsigned long long)(at + i) << 4)));
-                        f[4 * i] = x.x, f[4 * i + 1] = x.y, f[4 * i + 2] = x.z, f[4 * i + 3] = x.w;
-                    }
-                } else {
-                    const uint4 x = __ldg(reinterpret_cast<const uint4 *>(from + ((unsigned long long)at << 4)));
-                    const uint32_t v[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(v[i] << 16), f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] = half2_bits(__floats2half2_rn(f[2 * i] * down, f[2 * i + 1] * down));
-            }
-            *reinterpret_cast<uint4 *>(place(t, 8 * c)) = make_uint4(y[0], y[1], y[2], y[3]);
+        for (int j = 0; j < 4; ++j) {
+            if (kCache == DTYPE_F32) top = max(top, finite_bits(v[j]));
+            else top = max(top, max(finite_bits(v[j] << 16), finite_bits(v[j] & 0xffff0000u)));
         }
+    }
+    return top;
+}
+// They as fp16 into a slot, zeros where a token does not count.
+template <int kCache, int HD, int TN>
+__device__ __forceinline__ void prefix_convert(const uint8_t *from, unsigned row16, uint32_t valid, int first_row, int lane, float down, uint8_t *to) {
+    constexpr int GT = TN / kConverters, PR = HD / 8, kWords = kCache == DTYPE_F32 ? 2 : 1;       // of 16 bytes in 8 values
+#pragma unroll 4
+    for (int k = lane; k < (GT * PR + 31) / 32 * 32; k += 32) {
+        const int t = k / PR, c = k - t * PR, row = first_row + t;
+        const unsigned at = __shfl_sync(0xffffffffu, row16, t & 31) + c * kWords;
+        if (t >= GT) continue;
+        uint32_t y[4] = {0, 0, 0, 0};
+        if ((valid >> t) & 1) {
+            float f[8];
+            if constexpr (kCache == DTYPE_F32) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float4 x = __ldg(reinterpret_cast<const float4 *>(from + ((unsigned long long)(at + i) << 4)));
+                    f[4 * i] = x.x, f[4 * i + 1] = x.y, f[4 * i + 2] = x.z, f[4 * i + 3] = x.w;
+                }
+            } else {
+                const uint4 x = __ldg(reinterpret_cast<const uint4 *>(from + ((unsigned long long)at << 4)));
+                const uint32_t v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(v[i] << 16), f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = half2_bits(__floats2half2_rn(f[2 * i] * down, f[2 * i + 1] * down));
+        }
+        *reinterpret_cast<uint4 *>(to + (c >> 3) * (TN * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
     }
 }
 
 template <int kCache, int HD, bool kBf16>
-__global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixParams p) {
-    constexpr int TN = prefix_tile(HD), GT = TN / 4, kSlots = prefix_slots(HD), NB = HD / 32;
-    constexpr int kQueryBytes = prefix_query_bytes(HD), kSlotBytes = prefix_slot_bytes(HD), kMaxStreams = prefix_streams(HD);
+__global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) * 32, 1) prefix_kernel(const PrefixParams p) {
+    constexpr int TN = prefix_tile(HD, kCache), kGroups = prefix_copiers(kCache, kBf16), GT = TN / kGroups, kSlots = prefix_slots(HD, kCache), NB = HD / 32;
+    constexpr int kQueryBytes = prefix_query_bytes(HD), kSlotBytes = prefix_slot_bytes(HD, kCache), kMaxStreams = prefix_streams(HD);
     constexpr int kRunTiles = kRunTokens / TN, kTileRing = 8;
-    constexpr bool kRaw = (kCache == DTYPE_BF16 && kBf16) || kCache == DTYPE_F16;      // rows are copied as they are
-    constexpr bool kQuant = kCache == DTYPE_Q8_0 || kCache == DTYPE_Q4_0;
+    constexpr bool kRaw = prefix_raw(kCache, kBf16);              // rows are copied as they are
+    constexpr bool kQuant = prefix_quant(kCache);
     constexpr float kBias = kBf16 ? 0.0f : 7.0f, kLag = 8.0f;
     // Columns: the tiles' O, then their S, then their P.
     constexpr int kSCol = kMaxStreams * HD, kPCol = kSCol + kMaxStreams * TN, kPStep = (TN / 2 + 15) / 16 * 16;
-    static_assert(kPCol + kMaxStreams * kPStep <= 512 && kSlots >= 4 && HD % 32 == 0 && TN % 16 == 0, "");
+    static_assert(kPCol + kMaxStreams * kPStep <= 512 && kSlots >= 3 && HD % 32 == 0 && TN % 16 == 0 && GT % 2 == 0 && GT <= 32 &&
+                  prefix_shared_bytes(HD, kCache) <= kPrefixShared + 4096, "");
     // fp32 += A B, both K-major for S; B's rows are the product's K for O
     constexpr uint32_t kFormat = (1u << 4) | (kBf16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(kPrefixRows >> 4) << 24);
     constexpr uint32_t kIdescS = kFormat | ((uint32_t)(TN >> 3) << 17), kIdescO = kFormat | (1u << 16) | ((uint32_t)(HD >> 3) << 17);
@@ -326,17 +318,16 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
     __shared__ uint32_t tmem_slot;
     __shared__ int s_abort;
     __shared__ float qmul[2][2][kPrefixRows];                     // [item's parity][tile of rows]
-    __shared__ uint32_t counts[kTileRing][4];                     // tokens of a group that count
-    __shared__ float k_up[kTileRing][4];                          // a group's keys are the operand's times this
-    __shared__ int v_up[kTileRing][4];                            // and its values times 2 to this
-    __shared__ uint32_t block_scales[kQuant ? 4 : 1][kQuant ? GT * NB : 1];      // of the producers
+    __shared__ uint32_t counts[kTileRing][kGroups];                     // tokens of a group that count
+    __shared__ float k_up[kTileRing][kGroups];                          // a group's keys are the operand's times this
+    __shared__ int v_up[kTileRing][kGroups];                            // and its values times 2 to this
     volatile int *const abort_flag = &s_abort;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     pdl_trigger();
     pdl_wait();
     const long long length = prefix_length(p, blockIdx.x == 0 && threadIdx.x == 0);
-    for (int i = blockIdx.x * kPrefixThreads + threadIdx.x; i < p.counts; i += gridDim.x * kPrefixThreads) p.count[i] = 0;
-    const PrefixRanges r = prefix_ranges(p.items, length, TN, p.blocks);
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < p.counts; i += gridDim.x * blockDim.x) p.count[i] = 0;
+    const PrefixRanges r = prefix_ranges(p.items, length, TN, p.blocks);        // (TN: p.tile)
     if (blockIdx.x >= r.blocks) return;
     const unsigned lo = prefix_first(r, blockIdx.x), hi = blockIdx.x + 1 < r.blocks ? prefix_first(r, blockIdx.x + 1) : r.total;
     const int item0 = __shfl_sync(0xffffffffu, (int)(lo / (unsigned)r.tiles), 0);
@@ -351,11 +342,11 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
     if (threadIdx.x == 0) {
         s_abort = 0;
         for (int s = 0; s < kSlots; ++s) {
-            if (kRaw) mbar_init(landed + s, 4 + 4 * 32);          // a lane of each copying warp, and all lanes' copies
-            mbar_init(full + s, kRaw ? 1 : 4);
+            if (kRaw) mbar_init(landed + s, kGroups + kGroups * 32);      // a lane of each copying warp, and all lanes' copies
+            mbar_init(full + s, kRaw ? 1 : kGroups);
             mbar_init(empty + s, p.streams);                      // of the issuing warps
         }
-        mbar_init(&q_full, 4);
+        mbar_init(&q_full, kGroups);
         for (int i = 0; i < 2; ++i) {
             mbar_init(s_full + i, 1);
             mbar_init(s_free + i, 4);
@@ -382,7 +373,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
     uint8_t *const slots = smem + kMaxStreams * kQueryBytes;
 
     if (warp < kPrefixMma) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+        if constexpr (kRaw) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+        else asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
         // ------------------------------------------------------- softmax --
         const int i = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = s_col(i) + lanes, p_at = p_col(i) + lanes, o_at = o_col(i) + lanes;
@@ -402,12 +394,12 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
                 tc_fence_after();
                 const int ring = n & (kTileRing - 1);
                 if (run == 0 && first_run) qm = qmul[(item - item0) & 1][i][row];
-                uint32_t word[4];
-                float qg[4];
-                int eg[4], e_tile = -1000;
+                uint32_t word[kGroups];
+                float qg[kGroups];
+                int eg[kGroups], e_tile = -1000;
                 bool whole = true;
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
+                for (int g = 0; g < kGroups; ++g) {
                     word[g] = counts[ring][g];
                     whole = whole && word[g] == 0xffffffffu >> (32 - GT);
                     qg[g] = kRaw ? qm : fmaxf(qm * k_up[ring][g], 1.2e-38f);
@@ -434,7 +426,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
                 // (A NaN among them makes every one of the row's probabilities NaN.)
                 float top = -INFINITY;
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
+                for (int g = 0; g < kGroups; ++g) {
                     float t0 = s[g * GT], t1 = s[g * GT + 1];
 #pragma unroll
                     for (int j = 2; j < GT; j += 2) {
@@ -477,7 +469,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
                     }
                 }
                 const float ref = m == -INFINITY ? 0.0f : kBias - m;
-                float2 sum[4] = {};
+                float2 sum[kGroups] = {};
 #pragma unroll
                 for (int c = 0; c < TN; c += 16) {
                     uint32_t w[8];
@@ -493,7 +485,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
                     tmem_store<8>(p_at + c / 2, w);
                 }
 #pragma unroll
-                for (int g = 0; g < 4; ++g) l += kRaw ? sum[g].x + sum[g].y : (sum[g].x + sum[g].y) * pow2(min(e_run - eg[g], 100));
+                for (int g = 0; g < kGroups; ++g) l += kRaw ? sum[g].x + sum[g].y : (sum[g].x + sum[g].y) * pow2(min(e_run - eg[g], 100));
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
@@ -550,7 +542,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
             }
         }
     } else if (warp < kPrefixCopy) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if constexpr (kRaw) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
         const int i = warp - kPrefixMma;                          // tile of rows
         if (i < p.streams) {
             // ------------------------------------------------------ MMAs --
@@ -644,9 +637,10 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
             }
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if constexpr (kRaw) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         // ----------------------------------------------------- producers --
-        const int w = warp - kPrefixCopy;                         // its tokens: GT w .. of a tile, and rows 32 w .. of the query
+        const int w = warp - kPrefixCopy;                         // its tokens: GT w .. of a tile
         bool ok = true;
         // Token `lane` of a tile: its page (-1: none) and slot.
         auto fetch = [&](int t, int &entry, int &slot) {
@@ -665,8 +659,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
         };
         // Copies of a lane (of rows as they are): piece 32 j + lane of the warp's rows, where
         // it goes in a slot, and whose it is.
-        constexpr int PR = HD / 8, kCopies = kRaw ? GT * PR / 32 : 1;
-        static_assert(GT * PR % 32 == 0, "");
+        constexpr int PR = HD / 8, kCopies = kRaw ? (GT * PR + 31) / 32 : 1;
         uint32_t to[kCopies];
         if constexpr (kRaw) {
 #pragma unroll
@@ -675,71 +668,170 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
                 to[j] = saddr(slots) + (c >> 3) * (TN * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
             }
         }
-        int item = item0, tile = tile0, entry, slot, ring = 0, next_slot = 0, kh = item / p.row_sets;
+        // Where a tile's tokens are: of token `lane` its page's and its row's offset (in 16
+        // bytes) and its slot; which of them count.
+        struct Tokens {
+            unsigned page16, row16;
+            int slot;
+            uint32_t valid;
+        };
+        auto resolve = [&](int t, int entry, int slot) {
+            Tokens x;
+            const bool wanted = lane < GT && (long long)t * TN + w * GT + lane < length, found = (unsigned)entry < (unsigned)p.l.num_pages;
+            x.page16 = (found ? (unsigned)entry : 0u) * (unsigned)(p.l.page_bytes >> 4);
+            x.row16 = x.page16 + (unsigned)(slot * (p.l.row_bytes >> 4));
+            x.slot = slot;
+            x.valid = __ballot_sync(0xffffffffu, found && wanted);
+            if (wanted && !found) atomicOr(p.err, kErrCache);
+            return x;
+        };
+        auto head_of = [&](int item) { return p.l.pages + (unsigned long long)(item / p.row_sets) * p.l.chunk_bytes; };
+        auto after = [&](int t) { return t + 1 == r.tiles ? 0 : t + 1; };
+        int item = item0, tile = tile0, entry, slot, ring = 0, next_slot = 0;
         uint32_t next_phase = 1;
         fetch(tile, entry, slot);
-        for (int n = 0; ok && n < units; ++n) {
-            // ---- where the tile's tokens are ----
-            const bool wanted = lane < GT && (long long)tile * TN + w * GT + lane < length, found = (unsigned)entry < (unsigned)p.l.num_pages;
-            const unsigned page16 = (found ? (unsigned)entry : 0u) * (unsigned)(p.l.page_bytes >> 4);
-            const unsigned row16 = page16 + (unsigned)(slot * (p.l.row_bytes >> 4));
-            const uint32_t valid = __ballot_sync(0xffffffffu, found && wanted);
-            const int page_slot = slot;
-            if (wanted && !found) atomicOr(p.err, kErrCache);
-            if (n + 1 < units) fetch(tile + 1 == r.tiles ? 0 : tile + 1, entry, slot);
-            const uint8_t *const head = p.l.pages + (unsigned long long)kh * p.l.chunk_bytes;
-            if (lane == 0) counts[ring][w] = valid;
-            int e_half[2] = {0, 0};                               // powers of two of the group's keys and values
-            unsigned from[kCopies];
-            if constexpr (kRaw) {
+        // ---- quantised rows on their way, a tile ahead ----
+        constexpr int kRawTile = prefix_raw_tile(HD, kCache), kRawRow = prefix_raw_row(HD, kCache);
+        uint8_t *const raw = slots + kSlots * kSlotBytes + w * 2 * kRawTile;
+        int ahead_item = item0, ahead_tile = tile0;
+        const uint8_t *ahead_head = head_of(item0);
+        auto bring = [&](int n) {
+            if (n < units) {
+                const Tokens x = resolve(ahead_tile, entry, slot);
+                if (n + 1 < units) fetch(after(ahead_tile), entry, slot);
+                if (lane == 0) counts[n % kTileRing][w] = x.valid;
+                const uint32_t dst = saddr(raw) + (n & 1) * kRawTile;
+                if ((x.valid >> lane) & 1) {
+                    const uint8_t *from = ahead_head + p.l.ks_off + ((unsigned long long)x.page16 << 4) + x.slot * p.l.scale_stride * 4;
+                    const uint32_t at = dst + 2 * GT * kRawRow + lane * 32;
 #pragma unroll
-                for (int j = 0; j < kCopies; ++j) {
-                    const int k = 32 * j + lane, t = k / PR;
-                    from[j] = __shfl_sync(0xffffffffu, row16, t) + (k - t * PR);
+                    for (int h = 0; h < 2; ++h, from += p.l.vs_off - p.l.ks_off) {
+                        if constexpr (NB <= 2) copy_bytes<8>(at + h * GT * 32, from);
+                        else copy_bytes<16>(at + h * GT * 32, from);
+                        if constexpr (NB > 4) copy_bytes<16>(at + h * GT * 32 + 16, from + 16);
+                    }
                 }
-            } else {
-                prefix_exponents<kCache, HD, GT>(p, head, row16, page16, page_slot, valid, lane, e_half);
-                if (lane == 0) {
-                    k_up[ring][w] = pow2(e_half[0]);
-                    v_up[ring][w] = e_half[1];
+                constexpr int kPieces = kRawRow / 16 - 1;
+#pragma unroll
+                for (int j = 0; j < (GT * kPieces + 31) / 32; ++j) {
+                    const int k = 32 * j + lane, t = k / kPieces, c = k - t * kPieces;
+                    const unsigned src = __shfl_sync(0xffffffffu, x.row16, t & 31) + c;
+                    if (t < GT && (x.valid >> t) & 1) {
+                        const uint8_t *from = ahead_head + ((unsigned long long)src << 4);
+                        copy_bytes<16>(dst + t * kRawRow + c * 16, from);
+                        copy_bytes<16>(dst + (GT + t) * kRawRow + c * 16, from + p.l.v_off);
+                    }
+                }
+                if (++ahead_tile == r.tiles) {
+                    ahead_tile = 0;
+                    ahead_head = head_of(++ahead_item);
                 }
             }
-            // ---- K, then V ----
-#pragma unroll 1
-            for (int half = 0; half < 2; ++half) {
-                if (!wait_bounded(empty + next_slot, next_phase, abort_flag)) {
+            copies_commit();
+        };
+        if constexpr (kQuant) bring(0);
+        const uint8_t *head = head_of(item);
+        auto next_slots = [&]() {
+            if (++next_slot == kSlots) {
+                next_slot = 0;
+                next_phase ^= 1;
+            }
+        };
+        for (int n = 0; ok && n < units; ++n) {
+            if constexpr (kQuant) {
+                bring(n + 1);
+                copies_wait<1>();
+                __syncwarp();
+                const uint8_t *const these = raw + (n & 1) * kRawTile;
+                const uint32_t valid = counts[ring][w];
+                int e[2];                                         // powers of two of the group's keys and values
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t top = 0;
+                    if ((valid >> lane) & 1) {
+                        const uint32_t *at = reinterpret_cast<const uint32_t *>(these + 2 * GT * kRawRow) + (h * GT + lane) * 8;
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) top = max(top, finite_bits(at[b]));
+                    }
+                    e[h] = prefix_exponent(top);
+                }
+                if (lane == 0) {
+                    constexpr int kUp = kCache == DTYPE_Q8_0 ? 24 : 20;
+                    k_up[ring][w] = pow2(e[0] + kUp);
+                    v_up[ring][w] = e[1] + kUp;
+                }
+                const int k_slot = next_slot;
+                ok = wait_bounded(empty + next_slot, next_phase, abort_flag);
+                next_slots();
+                ok = ok && wait_bounded(empty + next_slot, next_phase, abort_flag);
+                if (!ok) {
                     if (lane == 0) fail();
-                    ok = false;
                     break;
                 }
-                const uint32_t at = next_slot * kSlotBytes;
-                if constexpr (kRaw) {
-                    const uint8_t *const rows = head + (half ? p.l.v_off : 0);
-                    if (valid == 0xffffffffu >> (32 - GT)) {
-#pragma unroll
-                        for (int j = 0; j < kCopies; ++j) copy_bytes<16>(to[j] + at, rows + ((unsigned long long)from[j] << 4));
-                    } else {
-#pragma unroll 1
-                        for (int j = 0; j < kCopies; ++j) {
-                            const int k = 32 * j + lane, t = k / PR, c = k - t * PR, row = w * GT + t;
-                            const unsigned src = __shfl_sync(0xffffffffu, row16, t) + c;
-                            copy16_zfill(saddr(slots) + at + (c >> 3) * (TN * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4),
-                                         rows + ((unsigned long long)src << 4), (valid >> t) & 1);
-                        }
-                    }
-                    // (They arrive when they land, whatever this warp does meanwhile.)
-                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(saddr(landed + next_slot)) : "memory");
-                    if (lane == 0) mbar_arrive(landed + next_slot);
-                } else {
-                    prefix_convert<kCache, HD, TN>(p, head, half, row16, page16, page_slot, valid, w, lane, half ? e_half[1] : e_half[0], slots + at,
-                                                   block_scales[kQuant ? w : 0]);
-                    fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(full + next_slot);
+                prefix_unpack<kCache, HD>(these, valid, w * GT, lane, pow2(-e[0]), pow2(-e[1]), slots + k_slot * kSlotBytes, slots + next_slot * kSlotBytes);
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(full + k_slot);
+                    mbar_arrive(full + next_slot);
                 }
-                if (++next_slot == kSlots) {
-                    next_slot = 0;
-                    next_phase ^= 1;
+                next_slots();
+            } else {
+                const Tokens now = resolve(tile, entry, slot);
+                if (n + 1 < units) fetch(after(tile), entry, slot);
+                if (lane == 0) counts[ring][w] = now.valid;
+                int e[2] = {0, 0};
+                unsigned from[kCopies];
+                if constexpr (kRaw) {
+#pragma unroll
+                    for (int j = 0; j < kCopies; ++j) {
+                        const int k = 32 * j + lane, t = k / PR;
+                        from[j] = __shfl_sync(0xffffffffu, now.row16, t & 31) + (k - t * PR);
+                    }
+                } else {
+#pragma unroll
+                    for (int half = 0; half < 2; ++half)
+                        e[half] = prefix_exponent(prefix_largest<kCache, HD, GT>(head + (half ? p.l.v_off : 0), now.row16, now.valid, lane));
+                    if (lane == 0) {
+                        k_up[ring][w] = pow2(e[0]);
+                        v_up[ring][w] = e[1];
+                    }
+                }
+                // ---- K, then V ----
+#pragma unroll 1
+                for (int half = 0; half < 2; ++half) {
+                    if (!wait_bounded(empty + next_slot, next_phase, abort_flag)) {
+                        if (lane == 0) fail();
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t at = next_slot * kSlotBytes;
+                    const uint8_t *const rows = head + (half ? p.l.v_off : 0);
+                    if constexpr (kRaw) {
+                        if (now.valid == 0xffffffffu >> (32 - GT)) {
+#pragma unroll
+                            for (int j = 0; j < kCopies; ++j)
+                                if (32 * (j + 1) <= GT * PR || 32 * j + lane < GT * PR) copy_bytes<16>(to[j] + at, rows + ((unsigned long long)from[j] << 4));
+                        } else {
+#pragma unroll 1
+                            for (int j = 0; j < kCopies; ++j) {
+                                const int k = 32 * j + lane, t = k / PR, c = k - t * PR, row = w * GT + t;
+                                const unsigned src = __shfl_sync(0xffffffffu, now.row16, t & 31) + c;
+                                if (t < GT)
+                                    copy16_zfill(saddr(slots) + at + (c >> 3) * (TN * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4),
+                                                 rows + ((unsigned long long)src << 4), (now.valid >> t) & 1);
+                            }
+                        }
+                        // (They arrive when they land, whatever this warp does meanwhile.)
+                        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(saddr(landed + next_slot)) : "memory");
+                        if (lane == 0) mbar_arrive(landed + next_slot);
+                    } else {
+                        prefix_convert<kCache, HD, TN>(rows, now.row16, now.valid, w * GT, lane, pow2(half ? -e[1] : -e[0]), slots + at);
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(full + next_slot);
+                    }
+                    next_slots();
                 }
             }
             ring = (ring + 1) % kTileRing;
@@ -754,17 +846,18 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
                 }
                 // Rows by 16-byte copies, or by values where they lie anywhere; then, where
                 // they are converted or turned, each thread its row in place.
-                const int row = w * 32 + lane, streams = streams_of(item);
+                constexpr int kRows = kPrefixRows / kGroups;
+                const int row = w * kRows + min(lane, kRows - 1), streams = streams_of(item);
                 for (int i = 0; i < streams; ++i) {
                     const int at = ((item % p.row_sets) * p.streams + i) * kPrefixRows + row;
                     const int seq = at < p.rows ? at / p.group : -1;
-                    const long long from = seq * p.q_ss + (long long)(kh * p.group + at - seq * p.group) * p.q_hs;
+                    const long long from = seq * p.q_ss + (long long)(item / p.row_sets * p.group + at - seq * p.group) * p.q_hs;
                     const uint32_t rows_there = __ballot_sync(0xffffffffu, seq >= 0);
                     if (p.q_wide) {
                         const uint32_t from16 = (uint32_t)(from >> 3);        // (within 64 GB, checked on the host)
 #pragma unroll 4
-                        for (int j = 0; j < PR; ++j) {
-                            const int k = 32 * j + lane, t = k / PR, c = k - t * PR, q_row = w * 32 + t;
+                        for (int j = 0; j < kRows * PR / 32; ++j) {
+                            const int k = 32 * j + lane, t = k / PR, c = k - t * PR, q_row = w * kRows + t;
                             const bool there = (rows_there >> t) & 1;
                             const uint32_t at16 = __shfl_sync(0xffffffffu, from16, t), src = there ? at16 + c : 0u;
                             copy16_zfill(saddr(smem) + i * kQueryBytes + (c >> 3) * (kPrefixRows * 128) + q_row * 128 + (((c & 7) ^ (q_row & 7)) << 4),
@@ -772,7 +865,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
                         }
                     } else {
 #pragma unroll 1
-                        for (int c = 0; c < PR; ++c) {
+                        for (int c = 0; c < PR && lane < kRows; ++c) {
                             uint16_t v[8] = {};
                             if (seq >= 0) {
 #pragma unroll
@@ -786,7 +879,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
                 __syncwarp();
                 const bool convert = !kBf16 && p.io == DTYPE_BF16;
                 const uint32_t sign = p.scale < 0.0f ? 0x80008000u : 0u;
-                for (int i = 0; i < streams; ++i) {
+                for (int i = 0; i < streams && lane < kRows; ++i) {
                     float up = 1.0f, mul = fmaxf(fabsf(p.scale), 1.2e-38f);
                     auto piece = [&](int c) { return reinterpret_cast<uint4 *>(smem + i * kQueryBytes + (c >> 3) * (kPrefixRows * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)); };
                     if (convert) {
@@ -825,7 +918,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
             }
             if (++tile == r.tiles) {
                 tile = 0;
-                kh = ++item / p.row_sets;
+                head = head_of(++item);
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
@@ -840,11 +933,11 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
 
 template <int kCache, int HD, bool kBf16>
 cudaError_t prefix_launch(const PrefixParams &p, cudaStream_t st) {
-    constexpr size_t kBytes = 1024 + (size_t)prefix_streams(HD) * prefix_query_bytes(HD) + (size_t)prefix_slots(HD) * prefix_slot_bytes(HD);
+    constexpr size_t kBytes = prefix_shared_bytes(HD, kCache);
     static std::atomic<unsigned long long> done{0};
     cudaError_t e = attn_allow(prefix_kernel<kCache, HD, kBf16>, kBytes, p.device, done);
     if (e != cudaSuccess) return e;
-    return launch_pdl(prefix_kernel<kCache, HD, kBf16>, dim3(p.blocks), dim3(kPrefixThreads), kBytes, st, p);
+    return launch_pdl(prefix_kernel<kCache, HD, kBf16>, dim3(p.blocks), dim3((kPrefixCopy + prefix_copiers(kCache, kBf16)) * 32), kBytes, st, p);
 }
 template <int kCache, bool kBf16>
 cudaError_t prefix_launch(const PrefixParams &p, cudaStream_t st) {
