@@ -222,7 +222,8 @@ SAPPHIRE_API int sapphire_attention_per_head_device(kernel_context_t *ctx, const
 SAPPHIRE_API size_t sapphire_kv_summary_bytes(const sapphire_kv_cache_t *cache);
 /** Bounds of the pages that hold positions start[s] .. of the `tokens` new rows
  *  of ragged sequences (the arguments of the write; dtype, k and v are not used), of
- *  all of a page's tokens up to the newest.  summary: 16-byte aligned. */
+ *  all of a page's tokens up to the newest.  A page that several sequences of a call
+ *  hold has the same tokens of each.  summary: 16-byte aligned. */
 SAPPHIRE_API int sapphire_kv_summarise_device(kernel_context_t *ctx, const sapphire_kv_cache_t *cache, void *summary,
                                               const sapphire_kv_args_t *args);
 
@@ -265,10 +266,12 @@ SAPPHIRE_API int sapphire_kv_select_device(kernel_context_t *ctx, const sapphire
  * lengths[s] + length_offset tokens that it has behind them (its new one among
  * them), position p of which is slot p % page_size of page_table[s][p / page_size].
  * The prefix is read once for the batch.  What else holds is as for
- * sapphire_attention_device, but that 16-bit queries round probabilities and the
- * values of caches of another type to 16 bits once: to bf16 over BF16 under bf16
- * queries, else to fp16, values below 2^-29 of the largest of 16 or 32 neighbouring
- * tokens less exactly.  The same call gives the same bits.
+ * sapphire_attention_device, but that 16-bit queries use 16-bit operands over the
+ * prefix: over BF16 under bf16 queries probabilities are rounded to bf16; else
+ * probabilities and F32 and BF16 values are rounded to fp16, Q8_0 and Q4_0 scales and
+ * their products with codes too; values below 2^-20 of the largest of neighbouring
+ * tokens are less exact, and scales from 2^112 on may count as infinite.  The same
+ * call gives the same bits.
  * ------------------------------------------------------------------------- */
 typedef struct {
     tensor_dtype_t dtype;    /* F32, BF16 or F16, of q and out */

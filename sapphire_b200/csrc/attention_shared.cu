@@ -16,7 +16,7 @@
 
 namespace {
 
-constexpr int kJoinWarps = 8, kEntryWarps = 4;    // of a block, and of a sequence and query head
+constexpr int kJoinWarps = 8;     // of a block
 
 struct JoinParams {
     PrefixParams prefix;          // of the tensor core kernel
@@ -32,11 +32,12 @@ struct JoinParams {
 };
 
 // Adds up means, each with its maximum and sum: the weight of one is l 2^(m - M).
-// kWarps warps take a sequence and query head, each every kWarps-th piece with all its
-// loads in flight, and are joined in shared memory: bound by latency, the fewer steps
-// behind one another the better (64 sequences of 32 heads of 128, 18 pieces of 0.5 KB
-// each: 10.4 us with one warp, .. with four).
-template <int HD>
+// kEntryWarps warps take a sequence and query head, each every kEntryWarps-th piece with
+// its loads in flight, and are joined in shared memory: few entries are bound by latency,
+// the fewer steps behind one another the better (16 sequences of 32 heads of 128, 18 pieces
+// each: 8.2 us with one warp, 6.0 with four), many by what a warp costs (64 sequences: 10.5
+// and 14 us).
+template <int HD, int kEntryWarps>
 __global__ void __launch_bounds__(kJoinWarps * 32) shared_join_kernel(const JoinParams p) {
     // A lane has four dims, or eight of 192 and 256.
     constexpr int kLanes = HD <= 128 ? HD / 4 : HD / 8, NB = HD / kLanes / 4, kBatch = 8 / NB;
@@ -147,15 +148,22 @@ __global__ void __launch_bounds__(kJoinWarps * 32) shared_join_kernel(const Join
         }
 }
 
-cudaError_t run_join(const JoinParams &p, int head_dim, cudaStream_t st) {
-    constexpr int kEntries = kJoinWarps / kEntryWarps;
-    const dim3 grid((unsigned)((p.entries + kEntries - 1) / kEntries)), block(kJoinWarps * 32);
+template <int HD>
+cudaError_t run_join(const JoinParams &p, int sms, cudaStream_t st) {
+    // One warp to an entry where that fills the GPU.
+    const dim3 block(kJoinWarps * 32);
+    if (p.entries >= 8ll * sms)
+        return launch_pdl(shared_join_kernel<HD, 1>, dim3((unsigned)((p.entries + kJoinWarps - 1) / kJoinWarps)), block, 0, st, p);
+    constexpr int kEntries = kJoinWarps / 4;
+    return launch_pdl(shared_join_kernel<HD, 4>, dim3((unsigned)((p.entries + kEntries - 1) / kEntries)), block, 0, st, p);
+}
+cudaError_t run_join(const JoinParams &p, int head_dim, int sms, cudaStream_t st) {
     switch (head_dim) {
-        case 64: return launch_pdl(shared_join_kernel<64>, grid, block, 0, st, p);
-        case 96: return launch_pdl(shared_join_kernel<96>, grid, block, 0, st, p);
-        case 128: return launch_pdl(shared_join_kernel<128>, grid, block, 0, st, p);
-        case 192: return launch_pdl(shared_join_kernel<192>, grid, block, 0, st, p);
-        default: return launch_pdl(shared_join_kernel<256>, grid, block, 0, st, p);
+        case 64: return run_join<64>(p, sms, st);
+        case 96: return run_join<96>(p, sms, st);
+        case 128: return run_join<128>(p, sms, st);
+        case 192: return run_join<192>(p, sms, st);
+        default: return run_join<256>(p, sms, st);
     }
 }
 
@@ -188,6 +196,8 @@ SharedLayout shared_layout(kernel_context_t *ctx, const sapphire_kv_cache_t *c, 
         return from;
     };
     w.blocks = sm_count(ctx->device);
+    // (First, and of one size: the context's own workspace keeps them at zero from call to call.)
+    w.count = take((size_t)sm_count(ctx->device) * kAttnMaxBlocks * sizeof(int));
     w.own = take(entries * c->head_dim * sizeof(float));
     w.own_ml = take(entries * sizeof(float2));
     size_t means = entries, attend = attn_workspace(ctx, c->dtype, c->head_dim, group);
@@ -203,8 +213,7 @@ SharedLayout shared_layout(kernel_context_t *ctx, const sapphire_kv_cache_t *c, 
     w.part = take(means * c->head_dim * sizeof(float));
     w.part_ml = take(means * sizeof(float2));
     w.attend = take(attend);
-    w.count = take((size_t)sm_count(ctx->device) * kAttnMaxBlocks * sizeof(int));
-    w.total = at;
+    w.total = at + 256;                           // (the caller's starts on 16 bytes, results on 32)
     return w;
 }
 
@@ -284,6 +293,8 @@ extern "C" SAPPHIRE_API int sapphire_attention_shared_device(kernel_context_t *c
         ws = reinterpret_cast<char *>(ctx->d_shared);
     }
 
+    ws = reinterpret_cast<char *>(((uintptr_t)ws + 255) & ~(uintptr_t)255);
+
     const int group = a->heads / cache->kv_heads, rows = a->sequences * group;
     const float scale = (a->scale != 0.0f ? a->scale : 1.0f / sqrtf((float)cache->head_dim)) * kLog2e;
     AttnParams own{};
@@ -361,12 +372,24 @@ extern "C" SAPPHIRE_API int sapphire_attention_shared_device(kernel_context_t *c
         front.row_group = group;
         front.table_stride = a->prefix_pages;
         front.length_offset = 0;
-        attn_plan(ctx, cache->dtype, &front, ws + w.attend, nullptr);
+        // (The last block of an item joins it, by counters that are zero between calls on
+        // the context's workspace: two launches fewer, 4 sequences of one KV head of 256 behind
+        // 1531 tokens .. us against 26.)
+        int *const count = reinterpret_cast<int *>(ws + w.count);
+        if (a->workspace) {
+            e = cudaMemsetAsync(count, 0, (size_t)sm_count(ctx->device) * kAttnMaxBlocks * sizeof(int), ctx->stream);
+            if (e != cudaSuccess) {
+                cudaGetLastError();
+                ctx_fail(ctx, who, "cudaMemsetAsync failed: %s", cudaGetErrorString(e));
+                return -1;
+            }
+        }
+        attn_plan(ctx, cache->dtype, &front, ws + w.attend, count);
         e = attn_run(cache->dtype, front, ctx->stream);
-        attn_plan(ctx, cache->dtype, &own, ws + w.attend, nullptr);
+        attn_plan(ctx, cache->dtype, &own, ws + w.attend, count);
     }
     if (e == cudaSuccess) e = attn_run(cache->dtype, own, ctx->stream);
-    if (e == cudaSuccess) e = run_join(j, cache->head_dim, ctx->stream);
+    if (e == cudaSuccess) e = run_join(j, cache->head_dim, sm_count(ctx->device), ctx->stream);
     if (e != cudaSuccess) {
         cudaGetLastError();
         ctx_fail(ctx, who, "launch failed: %s", cudaGetErrorString(e));

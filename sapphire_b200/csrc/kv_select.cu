@@ -103,11 +103,14 @@ __global__ void __launch_bounds__(kMaxWarps * 32) kv_summary_kernel(const Summar
     //      many as its new tokens touch pages: floor(cu[s] / page_size) + 2 s on ----
     int s = blockIdx.x, j = 0, n = 1;
     if (p.r.cu_tokens) {
-        int lo = 0, hi = p.r.sequences - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) / 2;
-            if ((long long)(__ldg(p.r.cu_tokens + mid) / page_size) + 2ll * mid <= (long long)blockIdx.x) lo = mid;
-            else hi = mid - 1;
+        // (Lanes look at 32 places between at a time: a load for each factor of 33.)
+        int lo = 0, hi = p.r.sequences;                           // the sequence is in [lo, hi)
+        while (hi - lo > 1) {
+            const int gap = (hi - lo + 32) / 33, at = lo + ((int)threadIdx.x % 32 + 1) * gap;
+            const bool before = at < hi && (long long)(__ldg(p.r.cu_tokens + at) / page_size) + 2ll * at <= (long long)blockIdx.x;
+            const int steps = __popc(__ballot_sync(0xffffffffu, before));
+            hi = min(hi, lo + (steps + 1) * gap);
+            lo += steps * gap;
         }
         s = lo;
         const int cu = __ldg(p.r.cu_tokens + s);
@@ -318,6 +321,35 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const SelectPara
     const int wanted = p.budget - p.first - p.last, middle = pages - p.first - p.last;      // of these pages
     if (wanted == 0) return;
 
+    // ---- this block's pages [begin, begin + mine) of the middle: page numbers are looked up
+    //      a turn ahead, and the first turn's rows are on their way while the query is
+    //      made codes ----
+    const int per = (middle + (int)blocks - 1) / (int)blocks, begin = min((int)rank * per, middle), mine = min(per, middle - begin);
+    const uint8_t *const codes = p.summary + (unsigned long long)h * 2 * HD;
+    const unsigned long long scale_at = (unsigned long long)p.kv_heads * 2 * HD + 4ull * h;
+    int ids[2];
+    auto look = [&](int i0) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) ids[k] = i0 + 8 * k + g < mine ? __ldg(table + p.first + begin + i0 + 8 * k + g) : -1;
+    };
+    // Lane (g, t) reads 16 bytes of each 64 of rows g and g + 8: as the order of dims is
+    // the query's too, they are the MMA's fragments.
+    uint4 a[2][kChunks];
+    float d[2];
+    bool ok[2];
+    auto rows = [&](int i0) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            ok[k] = (unsigned)ids[k] < (unsigned)p.num_pages;
+            if (i0 + 8 * k + g < mine && !ok[k]) atomicOr(p.err, kErrCache);
+            const uint8_t *row = codes + (unsigned long long)(ok[k] ? ids[k] : 0) * p.summary_bytes;
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) a[k][c] = __ldg(reinterpret_cast<const uint4 *>(row + 64 * c) + t);
+            d[k] = __ldg(reinterpret_cast<const float *>(p.summary + (unsigned long long)(ok[k] ? ids[k] : 0) * p.summary_bytes + scale_at));
+        }
+    };
+    look(warp * 16);
+    rows(warp * 16);
     // ---- the query's codes: columns of [max(c, 0) | min(c, 0)] ----
     const int columns = (p.group + 7) & ~7;
     for (int j = warp; j < columns; j += kSelWarps) {
@@ -347,28 +379,10 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const SelectPara
     __syncthreads();
 
     // ---- scores of this block's pages [begin, begin + mine) of the middle ----
-    const int per = (middle + (int)blocks - 1) / (int)blocks, begin = min((int)rank * per, middle), mine = min(per, middle - begin);
-    const uint8_t *const codes = p.summary + (unsigned long long)h * 2 * HD;
-    const unsigned long long scale_at = (unsigned long long)p.kv_heads * 2 * HD + 4ull * h;
     uint32_t least = 0xffffffffu, most = 0;
     for (int i0 = warp * 16; i0 < mine; i0 += kSelWarps * 16) {
-        const int page = p.first + begin + i0;
-        // Lane (g, t) reads 16 bytes of each 64 of rows g and g + 8: as the order of
-        // dims is the query's too, they are the MMA's fragments.
-        uint4 a[2][kChunks];
-        float d[2];
-        bool ok[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const bool inside = i0 + 8 * k + g < mine;
-            const int id = inside ? __ldg(table + page + 8 * k + g) : -1;
-            ok[k] = (unsigned)id < (unsigned)p.num_pages;
-            if (inside && !ok[k]) atomicOr(p.err, kErrCache);
-            const uint8_t *row = codes + (unsigned long long)(ok[k] ? id : 0) * p.summary_bytes;
-#pragma unroll
-            for (int c = 0; c < kChunks; ++c) a[k][c] = __ldg(reinterpret_cast<const uint4 *>(row + 64 * c) + t);
-            d[k] = __ldg(reinterpret_cast<const float *>(p.summary + (unsigned long long)(ok[k] ? id : 0) * p.summary_bytes + scale_at));
-        }
+        if (i0 >= kSelWarps * 16) rows(i0);
+        look(i0 + kSelWarps * 16);
         float best[2] = {-INFINITY, -INFINITY};
         for (int j0 = 0; j0 < p.group; j0 += 8) {
             int c[4] = {0, 0, 0, 0};

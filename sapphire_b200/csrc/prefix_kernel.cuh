@@ -195,9 +195,11 @@ __device__ __forceinline__ uint32_t finite_bits(uint32_t x) {
 }
 // The power of two that a group's largest magnitude (its bits: of a value, or of a scale)
 // is divided by, to go to [2^14, 2^15).
+// (Of scales at most 2^96: 24 more has to be a power of two in fp32.)
+template <int kCache>
 __device__ __forceinline__ int prefix_exponent(uint32_t top) {
     top = __reduce_max_sync(0xffffffffu, top);
-    return top == 0 ? -100 : min(max((int)(top >> 23) - 127 - 14, -100), 96);
+    return top == 0 ? -100 : min(max((int)(top >> 23) - 127 - 14, -100), prefix_quant(kCache) ? 96 : 113);
 }
 
 // A warp's quantised rows of a tile, which wait in shared memory (K rows, V rows, their
@@ -753,7 +755,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
 #pragma unroll
                         for (int b = 0; b < NB; ++b) top = max(top, finite_bits(at[b]));
                     }
-                    e[h] = prefix_exponent(top);
+                    e[h] = prefix_exponent<kCache>(top);
                 }
                 if (lane == 0) {
                     constexpr int kUp = kCache == DTYPE_Q8_0 ? 24 : 20;
@@ -791,7 +793,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                 } else {
 #pragma unroll
                     for (int half = 0; half < 2; ++half)
-                        e[half] = prefix_exponent(prefix_largest<kCache, HD, GT>(head + (half ? p.l.v_off : 0), now.row16, now.valid, lane));
+                        e[half] = prefix_exponent<kCache>(prefix_largest<kCache, HD, GT>(head + (half ? p.l.v_off : 0), now.row16, now.valid, lane));
                     if (lane == 0) {
                         k_up[ring][w] = pow2(e[0]);
                         v_up[ring][w] = e[1];

@@ -7,12 +7,15 @@ by at most 4 ds A.
 fp32 queries: ds = scale sum|q k| 2^-19 and 2^-17 A besides, as attention over one
 table (test_attention_gpu).
 16-bit queries: products of 16-bit operands are exact and sums fp32, so ds is that
-and, where the cache's values are rounded to fp16 (Q8_0, Q4_0, F32: 2^-11 of a key),
-scale sum|q k| 2^-11 more; a probability is rounded once, by 2^-8 (bf16 operands) or
-2^-11 of it (fp16), and a converted value by 2^-11; the largest values of a group of
-tokens are at least 2^13 and fp16 steps are at least 2^-24, so small ones are off by
-2^-38 of the largest, and probabilities below 2^-21 of the largest by 2^-32 of it;
-512 truncating steps of an MMA cost 2^-15 of A.  Together A (4 ds + 2^-14 + p + v).
+and, where the cache's values become fp16, r scale sum|q k| more: r = 2^-11 of F32, one
+rounding, and 2^-10 of Q8_0 and Q4_0, (1 + 2^-11)^2 - 1 to 2^-22, the scale's and the
+product's.  A probability is rounded once, by 2^-8 (bf16 operands) or 2^-11 of it (fp16),
+a converted value by r.  Small values: an fp16 step is at least 2^-24, and a group's
+largest value is at least 2^-4 (a code of 127 times a scale of 2^14, 2^-24 times; 8 times
+2^14, 2^-20 times: 2^-3), so half a step of a value or of its offset is 2^-21 of it, and
+probabilities below 2^-21 of the largest are off by 2^-32 of it: 2^-20 max|v| together, and
+scale sum|q| max|k| 2^-20 of a score.  512 truncating steps of an MMA cost 2^-15 of A.
+Together A (4 ds + 2^-14 + p + r) + max|v| 2^-20.
 What a sequence has behind the prefix is off as in attend_plain there, over bf16
 queries one fp16 rounding of p (2^-12) and of integer queries (max|q| sum|k| 2^-14)
 more.
@@ -68,7 +71,7 @@ def shared_plain(kv, q, prefix_table, prefix, table, lengths, page, heads, dim, 
     group, scale = q.shape[1] // heads, dim ** -0.5 if scale is None else scale
     small = q.dtype != torch.float32
     bf16 = dtype == "bf16" and q.dtype == torch.bfloat16
-    rounded = small and dtype in ("q8_0", "q4_0", "f32")
+    r = 0.0 if not small else 2.0 ** -10 if dtype in ("q8_0", "q4_0") else 2.0 ** -11 if dtype == "f32" else 0.0
     for s, n in enumerate(lengths):
         if prefix + n == 0:
             continue
@@ -80,15 +83,17 @@ def shared_plain(kv, q, prefix_table, prefix, table, lengths, page, heads, dim, 
             x = q[s, at].double()
             ks, vs = k[pg, h, slot], v[pg, h, slot]
             score = x @ ks.T * scale
-            ds = (x.abs() @ ks.abs().T * abs(scale)).amax(-1) * (2.0 ** -19 + rounded * 2.0 ** -11)
+            ds = (x.abs() @ ks.abs().T * abs(scale)).amax(-1) * (2.0 ** -19 + r)
+            if r:
+                ds = ds + abs(scale) * x.abs().sum(-1) * ks.abs().max() * 2.0 ** -20
             if n and dtype in ("q8_0", "q4_0") and q.dtype == torch.bfloat16:
                 ds = ds + abs(scale) * x.abs().amax(-1) * ks[prefix:].abs().sum(-1).amax() * 2.0 ** -14
             p = torch.softmax(score, -1)
             rel = 2.0 ** -17
             if small:
-                rel = 2.0 ** -14 + (2.0 ** -8 if bf16 else 2.0 ** -11) + rounded * 2.0 ** -11 + 2.0 ** -12
+                rel = 2.0 ** -14 + (2.0 ** -8 if bf16 else 2.0 ** -11) + r + 2.0 ** -12
             out[s, at] = p @ vs
-            bound[s, at] = (p @ vs.abs()) * (4 * ds[:, None] + rel) + vs.abs().max() * 2.0 ** -24
+            bound[s, at] = (p @ vs.abs()) * (4 * ds[:, None] + rel) + vs.abs().max() * 2.0 ** -20
             lse[s, at] = torch.logsumexp(score, -1)
             lse_bound[s, at] = 2 * ds + 2.0 ** -15
     return out, bound, lse, lse_bound
@@ -221,6 +226,82 @@ def test_shared_is_repeatable_on_either_workspace(dev_ctx):
             assert torch.equal(out, first)
 
 
+@pytest.mark.parametrize("kind,dtype", [("bf16", "bf16"), ("bf16", "q8_0"), ("f16", "bf16"), ("f32", "q4_0")])
+def test_shared_workspace_on_any_sixteen_bytes(dev_ctx, kind, dtype):
+    """A workspace that starts on 16 bytes and on no more, of no byte too many."""
+    kv, prefix_table, table, q = shared_case(dev_ctx, dtype, kind, 700, [90, 0, 33], 2, 4, 128, 16, seed=13)
+    n, m = torch.tensor([90, 0, 33], dtype=torch.int32, device="cuda"), torch.tensor([700], dtype=torch.int32, device="cuda")
+    size = kv.shared_workspace_bytes(kind, 3, 8)
+    outs = []
+    for shift in (0, 16, 240):
+        room = torch.full((size + 512,), 0xEE, dtype=torch.uint8, device="cuda")
+        ws, out = room[shift:shift + size], torch.full_like(q, 3.0)
+        kv.attend_shared(q, prefix_table, m, table, n, out, workspace=ws)
+        dev_ctx.synchronize()
+        assert (room[:shift] == 0xEE).all() and (room[shift + size:] == 0xEE).all()
+        outs.append(out)
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+    with pytest.raises(Exception, match="16-byte"):
+        kv.attend_shared(q, prefix_table, m, table, n, outs[0], workspace=room[8:8 + size])
+
+
+def test_shared_far_offsets(dev_ctx):
+    """Prefix pages and summaries behind 4 GB of cache give the bits of near ones."""
+    from sapphire_b200.attention import KVCache, kv_page_bytes
+    for dtype in ("bf16", "q8_0"):
+        per = kv_page_bytes(dtype, 64, 8, 128)
+        count = (5 << 30) // per
+        far = KVCache(dev_ctx, dtype, 64, 8, 128, torch.empty(count, per, dtype=torch.uint8, device="cuda"))
+        near = make_cache(dev_ctx, dtype, 64, 8, 128, 8)
+        g = gen(13)
+        k, v = (torch.randn(400, 8, 128, device="cuda", generator=g).bfloat16() for _ in range(2))
+        q = torch.randn(2, 32, 128, device="cuda", generator=g).bfloat16()
+        outs, bounds = [], []
+        for kv, pages in ((far, [count - 1, 0, count - 2, count - 5, count - 3, 1, count - 4]), (near, [3, 0, 2, 1, 4, 5, 6])):
+            table = torch.tensor([pages], dtype=torch.int32, device="cuda")
+            kv.write(k, v, table, cu_tokens=ragged([400]))
+            own, prefix = table[:, 5:].expand(2, -1).contiguous(), table[0, :5].contiguous()
+            out = torch.empty_like(q)
+            kv.attend_shared(q, prefix, torch.tensor([320], dtype=torch.int32, device="cuda"), own,
+                             torch.tensor([80, 5], dtype=torch.int32, device="cuda"), out)
+            summary = torch.zeros(kv.pages.shape[0], kv.summary_bytes, dtype=torch.uint8, device="cuda")
+            kv.summarise(summary, table, tokens=400, cu_tokens=ragged([400]))
+            dev_ctx.synchronize()
+            outs.append(out)
+            bounds.append(summary[table[0].long()])
+        assert torch.equal(outs[0], outs[1]) and torch.equal(bounds[0], bounds[1])
+
+
+def test_shared_two_contexts_at_once(sp):
+    """Two contexts on streams of their own, whose calls overlap, give what each gives alone."""
+    ctxs = [sp.Context(num_threads=1) for _ in range(2)]
+    sets = []
+    for i, ctx in enumerate(ctxs):
+        kv, prefix_table, table, q = shared_case(ctx, ("bf16", "q4_0")[i], "bf16", 4000, [60, 7], 2, 40, 128, 16, seed=50 + i)
+        sets.append((ctx, kv, prefix_table, table, q, torch.tensor([60, 7], dtype=torch.int32, device="cuda"), torch.tensor([4000], dtype=torch.int32, device="cuda")))
+        ctx.synchronize()
+    torch.cuda.synchronize()
+    alone = []
+    for ctx, kv, prefix_table, table, q, n, m in sets:
+        out = torch.empty_like(q)
+        torch.cuda.synchronize()
+        kv.attend_shared(q, prefix_table, m, table, n, out)
+        ctx.synchronize()
+        alone.append(out)
+    outs = [[torch.empty_like(s[4]) for _ in range(6)] for s in sets]
+    torch.cuda.synchronize()
+    for k in range(6):
+        for (ctx, kv, prefix_table, table, q, n, m), o in zip(sets, outs):
+            kv.attend_shared(q, prefix_table, m, table, n, o[k])
+    for ctx in ctxs:
+        ctx.synchronize()
+    for o, want in zip(outs, alone):
+        for x in o:
+            assert torch.equal(x, want)
+    for ctx in ctxs:
+        ctx.close()
+
+
 def test_shared_growing_and_shrinking_calls(dev_ctx):
     """Calls of many shapes behind one another on the context's workspace."""
     kinds = [("bf16", 40, 2, 1, 64), ("bf16", 900, 60, 8, 128), ("q8_0", 300, 5, 2, 256), ("f16", 2000, 130, 2, 64)]
@@ -244,10 +325,10 @@ def test_shared_captured_calls(sp, dev_ctx):
     st = torch.cuda.Stream()
     dev_ctx.set_stream(st.cuda_stream)
     sets = []
-    for i, dtype in enumerate(("bf16", "q8_0")):
-        kv, prefix_table, table, q = shared_case(dev_ctx, dtype, "bf16", 1500, [90, 9, 40], 2, 4, 128, 16, seed=40 + i)
+    for i, (dtype, kind) in enumerate((("bf16", "bf16"), ("q8_0", "bf16"), ("f32", "f32"))):
+        kv, prefix_table, table, q = shared_case(dev_ctx, dtype, kind, 1500, [90, 9, 40], 2, 4, 128, 16, seed=40 + i)
         n, m = torch.tensor([90, 9, 40], dtype=torch.int32, device="cuda"), torch.tensor([1500], dtype=torch.int32, device="cuda")
-        ws = torch.full((kv.shared_workspace_bytes("bf16", 3, 8),), 0xEE, dtype=torch.uint8, device="cuda")
+        ws = torch.full((kv.shared_workspace_bytes(kind, 3, 8),), 0xEE, dtype=torch.uint8, device="cuda")
         sets.append((dtype, kv, prefix_table, table, q, n, m, torch.empty_like(q), ws))
     dev_ctx.synchronize()
     graphs = []
