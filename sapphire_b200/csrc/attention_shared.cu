@@ -55,10 +55,11 @@ __global__ void __launch_bounds__(kJoinWarps * 32) shared_join_kernel(const Join
     long long first = (long long)kh * f.rows + row, stride = 0;
     if (p.tc) {
         const int set_rows = f.streams * kPrefixRows, set = row / set_rows, item = kh * f.row_sets + set;
-        const PrefixRanges r = prefix_ranges(f.items, prefix_length(f, false), f.tile, f.blocks);
+        const PrefixRanges r = prefix_ranges(f.items, (uint32_t)prefix_length(f, false), f.tile, f.blocks);
         n = 0;
         if (r.tiles > 0) {
-            const unsigned unit = (unsigned)item * r.tiles, b0 = prefix_block_of(r, unit), b1 = prefix_block_of(r, unit + r.tiles - 1);
+            unsigned b0, b1;
+            prefix_holders(r, item, &b0, &b1);
             n = (int)(b1 - b0) + 1;
             first = (long long)(b0 + item) * set_rows + row - set * set_rows;
             stride = set_rows;
@@ -196,7 +197,6 @@ SharedLayout shared_layout(kernel_context_t *ctx, const sapphire_kv_cache_t *c, 
         return from;
     };
     w.blocks = sm_count(ctx->device);
-    // (First, and of one size: the context's own workspace keeps them at zero from call to call.)
     w.count = take((size_t)sm_count(ctx->device) * kAttnMaxBlocks * sizeof(int));
     w.own = take(entries * c->head_dim * sizeof(float));
     w.own_ml = take(entries * sizeof(float2));
@@ -372,21 +372,9 @@ extern "C" SAPPHIRE_API int sapphire_attention_shared_device(kernel_context_t *c
         front.row_group = group;
         front.table_stride = a->prefix_pages;
         front.length_offset = 0;
-        // (The last block of an item joins it, by counters that are zero between calls on
-        // the context's workspace: two launches fewer, 4 sequences of one KV head of 256 behind
-        // 1531 tokens .. us against 26.)
-        int *const count = reinterpret_cast<int *>(ws + w.count);
-        if (a->workspace) {
-            e = cudaMemsetAsync(count, 0, (size_t)sm_count(ctx->device) * kAttnMaxBlocks * sizeof(int), ctx->stream);
-            if (e != cudaSuccess) {
-                cudaGetLastError();
-                ctx_fail(ctx, who, "cudaMemsetAsync failed: %s", cudaGetErrorString(e));
-                return -1;
-            }
-        }
-        attn_plan(ctx, cache->dtype, &front, ws + w.attend, count);
+        attn_plan(ctx, cache->dtype, &front, ws + w.attend, nullptr);
         e = attn_run(cache->dtype, front, ctx->stream);
-        attn_plan(ctx, cache->dtype, &own, ws + w.attend, count);
+        attn_plan(ctx, cache->dtype, &own, ws + w.attend, nullptr);
     }
     if (e == cudaSuccess) e = attn_run(cache->dtype, own, ctx->stream);
     if (e == cudaSuccess) e = run_join(j, cache->head_dim, sm_count(ctx->device), ctx->stream);

@@ -110,40 +110,52 @@ constexpr size_t prefix_shared_bytes(int hd, int cache) {
 // kItemUnits units), all units in a row into equal ranges, item by item.
 constexpr int kItemUnits = 5;
 struct PrefixRanges {
-    int tiles;                     // of an item
-    int parts;                     // of an item, or 0: ranges
-    unsigned total, blocks, each, longer;
+    unsigned tiles;                // of an item
+    unsigned parts;                // of an item, or 0: ranges
+    unsigned total, blocks, each, longer;      // of an item's tiles where it has parts, of all units else: `longer` pieces of each + 1, then pieces of each
 };
-__host__ __device__ inline PrefixRanges prefix_ranges(int items, long long length, int tile, int blocks) {
+__host__ __device__ inline PrefixRanges prefix_ranges(unsigned items, unsigned length, unsigned tile, unsigned blocks) {
     PrefixRanges r;
-    r.tiles = (int)((length + tile - 1) / tile);
-    r.total = (unsigned)items * (unsigned)r.tiles;
-    r.blocks = r.total < (unsigned)blocks ? r.total : (unsigned)blocks;
+    r.tiles = (length + tile - 1) / tile;
+    r.total = items * r.tiles;
+    r.blocks = r.total < blocks ? r.total : blocks;
+    r.parts = 0;
     r.each = r.blocks ? r.total / r.blocks : 0;
     r.longer = r.total - r.each * r.blocks;
-    r.parts = 0;
     if (r.blocks && items <= blocks) {
-        const int parts = blocks / items < r.tiles ? blocks / items : r.tiles;
-        if ((unsigned)((r.tiles + parts - 1) / parts) <= r.each + kItemUnits) {
+        const unsigned most = blocks / items, parts = most < r.tiles ? most : r.tiles, each = r.tiles / parts, longer = r.tiles - each * parts;
+        if (each + (longer ? 1 : 0) <= r.each + kItemUnits) {
             r.parts = parts;
-            r.blocks = (unsigned)(items * parts);
+            r.blocks = items * parts;
+            r.each = each;
+            r.longer = longer;
         }
     }
     return r;
 }
-// The first unit of a block, and the block of a unit.
-__host__ __device__ inline unsigned prefix_first(const PrefixRanges &r, unsigned block) {
-    if (!r.parts) return block * r.each + (block < r.longer ? block : r.longer);
-    const unsigned item = block / r.parts, part = block - item * r.parts;
-    return item * r.tiles + (unsigned)((unsigned long long)part * r.tiles / r.parts);
+// A block's item, and the first of its tiles there and its units.
+struct PrefixPiece {
+    unsigned item, tile, units;
+};
+__host__ __device__ inline PrefixPiece prefix_piece(const PrefixRanges &r, unsigned block) {
+    PrefixPiece x;
+    const unsigned item = r.parts ? block / r.parts : 0, piece = block - item * r.parts;       // (parts 0: the block)
+    const unsigned first = piece * r.each + (piece < r.longer ? piece : r.longer);
+    x.units = r.each + (piece < r.longer ? 1 : 0);
+    x.item = r.parts ? item : first / r.tiles;
+    x.tile = r.parts ? first : first - x.item * r.tiles;
+    return x;
 }
-__host__ __device__ inline unsigned prefix_block_of(const PrefixRanges &r, unsigned unit) {
+// The blocks that hold an item.
+__host__ __device__ inline void prefix_holders(const PrefixRanges &r, unsigned item, unsigned *first, unsigned *last) {
     if (r.parts) {
-        const unsigned item = unit / r.tiles, tile = unit - item * r.tiles;
-        return item * r.parts + (unsigned)((((unsigned long long)tile + 1) * r.parts - 1) / r.tiles);
+        *first = item * r.parts;
+        *last = *first + r.parts - 1;
+        return;
     }
-    const unsigned split = r.longer * (r.each + 1);
-    return unit < split ? unit / (r.each + 1) : r.longer + (unit - split) / r.each;
+    const unsigned split = r.longer * (r.each + 1), a = item * r.tiles, b = a + r.tiles - 1;
+    *first = a < split ? a / (r.each + 1) : r.longer + (a - split) / r.each;
+    *last = b < split ? b / (r.each + 1) : r.longer + (b - split) / r.each;
 }
 
 #ifdef __CUDACC__
@@ -325,22 +337,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
     __shared__ int v_up[kTileRing][kGroups];                            // and its values times 2 to this
     volatile int *const abort_flag = &s_abort;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    pdl_trigger();
-    pdl_wait();
-    const long long length = prefix_length(p, blockIdx.x == 0 && threadIdx.x == 0);
-    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < p.counts; i += gridDim.x * blockDim.x) p.count[i] = 0;
-    const PrefixRanges r = prefix_ranges(p.items, length, TN, p.blocks);        // (TN: p.tile)
-    if (blockIdx.x >= r.blocks) return;
-    const unsigned lo = prefix_first(r, blockIdx.x), hi = blockIdx.x + 1 < r.blocks ? prefix_first(r, blockIdx.x + 1) : r.total;
-    const int item0 = __shfl_sync(0xffffffffu, (int)(lo / (unsigned)r.tiles), 0);
-    const int tile0 = __shfl_sync(0xffffffffu, (int)(lo - (unsigned)item0 * r.tiles), 0), units = __shfl_sync(0xffffffffu, (int)(hi - lo), 0);
-    auto fail = [&]() {
-        *abort_flag = 1;
-        atomicOr(p.err, 2);
-    };
-    // Tiles of rows of an item.
-    auto streams_of = [&](int item) { return min(p.streams, (p.rows - (item % p.row_sets) * p.streams * kPrefixRows + kPrefixRows - 1) / kPrefixRows); };
-
+    // Barriers and tensor memory need nothing of an earlier kernel.
     if (threadIdx.x == 0) {
         s_abort = 0;
         for (int s = 0; s < kSlots; ++s) {
@@ -366,6 +363,22 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_trigger();
+    pdl_wait();
+    const uint32_t length = (uint32_t)prefix_length(p, blockIdx.x == 0 && threadIdx.x == 0);
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < p.counts; i += gridDim.x * blockDim.x) p.count[i] = 0;
+    const PrefixRanges r = prefix_ranges(p.items, length, TN, p.blocks);        // (TN: p.tile)
+    PrefixPiece mine{0, 0, 0};
+    if (blockIdx.x < r.blocks) mine = prefix_piece(r, blockIdx.x);
+    const int item0 = __shfl_sync(0xffffffffu, (int)mine.item, 0), tile0 = __shfl_sync(0xffffffffu, (int)mine.tile, 0);
+    const int units = __shfl_sync(0xffffffffu, (int)mine.units, 0), tiles = __shfl_sync(0xffffffffu, (int)r.tiles, 0);
+    auto fail = [&]() {
+        *abort_flag = 1;
+        atomicOr(p.err, 2);
+    };
+    // Tiles of rows of an item.
+    auto streams_of = [&](int item) { return min(p.streams, (p.rows - (item % p.row_sets) * p.streams * kPrefixRows + kPrefixRows - 1) / kPrefixRows); };
+
     const uint32_t tmem = tmem_slot;
     // (Arithmetic, not arrays: an index that the compiler does not know would put them
     // into local memory, whose cache is what shared memory leaves.)
@@ -385,9 +398,9 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
         int e_run = -1000, item = item0, tile = tile0, run = 0;
         uint32_t turn = 0;                                        // tiles of this tile of rows
         bool first_run = true;
-        int now = i < kMaxStreams ? streams_of(item) : 0;
+        int now = i < kMaxStreams && units > 0 ? streams_of(item) : 0;
         for (int n = 0; n < units; ++n) {
-            const bool last = n + 1 == units || tile + 1 == r.tiles;
+            const bool last = n + 1 == units || tile + 1 == tiles;
             if (i < now) {
                 if (!wait_bounded(s_full + i, turn & 1, abort_flag)) {
                     if (lane == 0) fail();
@@ -537,7 +550,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                     run = 0;
                 }
             }
-            if (++tile == r.tiles) {
+            if (++tile == tiles) {
                 tile = 0;
                 ++item;
                 if (n + 1 < units && i < kMaxStreams) now = streams_of(item);
@@ -601,9 +614,9 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                 step(v_slot, v_phase);
                 return true;
             };
-            bool now = i < streams_of(item), ok = scores(now, true);
+            bool now = i < streams_of(item), ok = units == 0 || scores(now, true);
             for (int n = 0; ok && n < units; ++n) {
-                const bool ends = tile + 1 == r.tiles, more = n + 1 < units;
+                const bool ends = tile + 1 == tiles, more = n + 1 < units;
                 const bool next = ends && more ? i < streams_of(item + 1) : now;
                 // (An item's first scores wait for its queries, which wait for the last one's
                 // scores, so outputs go first there.)
@@ -659,8 +672,8 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                 entry = __ldg(p.table + pg);
             }
         };
-        // Copies of a lane (of rows as they are): piece 32 j + lane of the warp's rows, where
-        // it goes in a slot, and whose it is.
+        // Copies of a lane (of rows as they are): 16-byte piece 32 j + lane of the warp's
+        // rows, and where it goes in a slot.
         constexpr int PR = HD / 8, kCopies = kRaw ? (GT * PR + 31) / 32 : 1;
         uint32_t to[kCopies];
         if constexpr (kRaw) {
@@ -688,10 +701,10 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
             return x;
         };
         auto head_of = [&](int item) { return p.l.pages + (unsigned long long)(item / p.row_sets) * p.l.chunk_bytes; };
-        auto after = [&](int t) { return t + 1 == r.tiles ? 0 : t + 1; };
+        auto after = [&](int t) { return t + 1 == tiles ? 0 : t + 1; };
         int item = item0, tile = tile0, entry, slot, ring = 0, next_slot = 0;
         uint32_t next_phase = 1;
-        fetch(tile, entry, slot);
+        if (units > 0) fetch(tile, entry, slot);
         // ---- quantised rows on their way, a tile ahead ----
         constexpr int kRawTile = prefix_raw_tile(HD, kCache), kRawRow = prefix_raw_row(HD, kCache);
         uint8_t *const raw = slots + kSlots * kSlotBytes + w * 2 * kRawTile;
@@ -724,7 +737,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                         copy_bytes<16>(dst + (GT + t) * kRawRow + c * 16, from + p.l.v_off);
                     }
                 }
-                if (++ahead_tile == r.tiles) {
+                if (++ahead_tile == tiles) {
                     ahead_tile = 0;
                     ahead_head = head_of(++ahead_item);
                 }
@@ -857,7 +870,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                     const uint32_t rows_there = __ballot_sync(0xffffffffu, seq >= 0);
                     if (p.q_wide) {
                         const uint32_t from16 = (uint32_t)(from >> 3);        // (within 64 GB, checked on the host)
-#pragma unroll 4
+#pragma unroll 1
                         for (int j = 0; j < kRows * PR / 32; ++j) {
                             const int k = 32 * j + lane, t = k / PR, c = k - t * PR, q_row = w * kRows + t;
                             const bool there = (rows_there >> t) & 1;
@@ -918,7 +931,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_full);
             }
-            if (++tile == r.tiles) {
+            if (++tile == tiles) {
                 tile = 0;
                 head = head_of(++item);
             }
