@@ -1,12 +1,15 @@
 /*
  * sapphire_attention.h - rotary positions, a paged key-value cache and the
- * attention of one new token over it.
+ * attention of one new token over it, over selected pages or behind a shared prefix.
  *
  * The operators a serving loop puts between the library's projections: the
  * query and key heads are rotated (sapphire_rope_device), the new keys and
  * values are stored in a paged cache, as they are or quantised
  * (sapphire_kv_write_device), and every sequence's new token attends to its
- * pages (sapphire_attention_device); whole sequences come back dense with
+ * pages (sapphire_attention_device), to those of its pages that a cheap score
+ * selects (sapphire_kv_summarise_device, sapphire_kv_select_device,
+ * sapphire_attention_per_head_device), or with a beginning that the whole batch
+ * shares (sapphire_attention_shared_device); whole sequences come back dense with
  * sapphire_kv_read_device.  The reference does these steps on the host for one
  * sequence and a contiguous fp32 cache (src/transformer/rope.c:65-80,
  * src/transformer/attention.c:93-163, 292-309); it has no paged or quantised

@@ -21,7 +21,7 @@ constexpr int kJoinWarps = 8;     // of a block
 struct JoinParams {
     PrefixParams prefix;          // of the tensor core kernel
     bool tc;
-    int heads, kv_heads;
+    int heads;
     long long entries;            // sequences * heads
     const float *own;             // [sequences][heads][head_dim]
     const float2 *own_ml;         // [sequences][heads]
@@ -336,7 +336,6 @@ extern "C" SAPPHIRE_API int sapphire_attention_shared_device(kernel_context_t *c
     f.device = ctx->device;
     j.tc = on_tensor_cores(a->dtype);
     j.heads = a->heads;
-    j.kv_heads = cache->kv_heads;
     j.entries = (long long)a->sequences * a->heads;
     j.own = reinterpret_cast<const float *>(ws + w.own);
     j.own_ml = own.ml;

@@ -5,14 +5,23 @@
 // Mathematics.  The rows of a KV head are the query heads it serves, of every
 // sequence: S = Q K^T over the prefix, P = 2^(S - m), O = P V, with a running
 // maximum m and sum l a row.  A piece of the prefix leaves O / l, m and l, which
-// attend_shared_join adds up with the other pieces and with what each sequence has
+// shared_join_kernel adds up with the other pieces and with what each sequence has
 // behind the prefix.
 //
 // What bounds it.  One pass over K and V serves up to 256 rows (two tiles of 128), so
-// up to about 250 rows a KV head it is HBM that does (4 bytes a token, dim and KV
+// up to about 250 rows a KV head it is HBM by the count (4 bytes a token, dim and KV
 // head in bf16 against 4 rows flops), and above that the tensor cores and the
 // exponentials: a tile of 128 rows by 128 tokens of 128 dims is 1024 cycles of MMA
-// and 1024 of ex2.
+// and 1024 of ex2.  Measured, 64 sequences of 32 query heads on 8 KV heads of 128
+// behind 32768 tokens in bf16: 54 us for 134 MB (20 at HBM's rate) and 34 GFLOP, tensor
+// pipe 36 %, ex2 37 %, issue 37 %.  A block takes 80 tokens of both tiles of rows in
+// about 2570 cycles: a softmax of 1500, of which 1280 are ex2's for the two tiles
+// together, then the chain of P's store, O's MMAs, S's of the next tile and their load,
+// which the two tiles of rows fill for each other in part only; and 15 to 19 thousand
+// cycles pass before the first tile, most of them instructions that come from memory for
+// the first time.  Quantised: 24 sequences of 40 heads on 8, 40000 tokens of Q4_0,
+// 110 us (tensor pipe 15 %, issue 48 %): the converting warps are what
+// the MMAs wait for.
 //
 // Layout.  A block per SM, whose roles are warps:
 //   0 - 3, 4 - 7  softmax of the first and the second tile of rows: a thread has a
@@ -25,18 +34,25 @@
 // Launched with 96 registers a thread (128 of 16 warps); the softmax takes 152 (168: a
 // row's scores are in registers), the MMAs' warps leave 48 (88) and the others 64 (88):
 // 256 * 152 + 128 * 48 + 256 * 64 = 640 * 96 (256 * 168 + 256 * 88 = 512 * 128).
-// Tensor memory holds, for each tile of rows, S (one column a token; P takes the
-// place of its first half as 16-bit pairs, the A operand of O's MMAs) and O.
-// While one tile of rows is in its softmax the other's MMAs run.  Its pages are of
-// any size, so rows come by 16-byte copies from wherever they lie.
+// Tensor memory holds, for each tile of rows, O, S (one column a token) and P (16-bit
+// pairs, the A operand of O's MMAs) in columns of their own, so S of the next tile runs
+// under O of this one.  Where there are two tiles of rows each has its softmax, its MMAs'
+// warp and its barriers, and they share only the slots of K and V.  Pages are of any
+// size, so rows come by 16-byte copies from wherever they lie.
+//
+// An MMA is issued by a whole warp with the lane elected inside the instruction's own
+// asm block: 33 to 64 cycles each, against 70 to 115 from a branch that one lane takes.
+// Dropped, as none gained: a polynomial for part of the exponentials, the two tiles
+// of rows started half a turn apart, a turn over nothing before the first tile.
 //
 // Rounding.  Operands are bf16 over bf16 caches under bf16 queries, else fp16:
 //   a query of bf16 is brought to [2^14, 2^15) by a power of two a row, exact down to
 //   2^-29 of its largest value;
 //   Q8_0 and Q4_0 values are products of fp16 (their scale is rounded to it, and the
-//   product), F32 and BF16 values are rounded to it once; each group of tokens (a warp's, 6
-//   to 16) times a power of two that brings its largest scale or value to [2^14, 2^15).  K's power multiplies the group's scores, V's is added to their
-//   exponent, relative to the largest so far, and O carries that one;
+//   product), F32 and BF16 values are rounded to it once; each group of tokens (a warp's,
+//   6 to 16) times a power of two that brings its largest scale or value to [2^14, 2^15).
+//   K's power multiplies the group's scores, V's is added to their exponent, relative to
+//   the largest so far, and O carries that one;
 //   probabilities are rounded to the operand type once, as the outputs are.  m may lag
 //   behind the maximum by 2^8 before O is brought up to date, so fp16 probabilities
 //   reach 2^15 and keep their bits down to 2^-21 of the largest.
