@@ -418,7 +418,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
         for (int n = 0; n < units; ++n) {
             const bool last = n + 1 == units || tile + 1 == tiles;
             if (i < now) {
-                if (!wait_bounded(s_full + i, turn & 1, abort_flag)) {
+                if (!wait_warp(s_full + i, turn & 1, abort_flag)) {
                     if (lane == 0) fail();
                     break;
                 }
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                 }
                 // ---- the tile before has left P and O ----
                 if (turn > 0) {
-                    if (!wait_bounded(p_done + i, (turn - 1) & 1, abort_flag)) {
+                    if (!wait_warp(p_done + i, (turn - 1) & 1, abort_flag)) {
                         if (lane == 0) fail();
                         break;
                     }
@@ -524,7 +524,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                 ++turn;
                 if (++run == kRunTiles || last) {
                     // ---- the run's O, added to the item's ----
-                    if (!wait_bounded(p_done + i, (turn - 1) & 1, abort_flag)) {
+                    if (!wait_warp(p_done + i, (turn - 1) & 1, abort_flag)) {
                         if (lane == 0) fail();
                         break;
                     }
@@ -596,10 +596,10 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
             };
             // (A tile of rows that an item does not have still gives its slots back.)
             auto scores = [&](bool active, bool new_item) {
-                if (new_item && !wait_bounded(&q_full, q_phase++ & 1, abort_flag)) return false;
-                if (!wait_bounded(full + k_slot, k_phase, abort_flag)) return false;
+                if (new_item && !wait_warp(&q_full, q_phase++ & 1, abort_flag)) return false;
+                if (!wait_warp(full + k_slot, k_phase, abort_flag)) return false;
                 if (active) {
-                    if (s_turn > 0 && !wait_bounded(s_free + i, (s_turn - 1) & 1, abort_flag)) return false;
+                    if (s_turn > 0 && !wait_warp(s_free + i, (s_turn - 1) & 1, abort_flag)) return false;
                     ++s_turn;
                     tc_fence_after();
 #pragma unroll
@@ -615,9 +615,9 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                 return true;
             };
             auto outputs = [&](bool active) {
-                if (!wait_bounded(full + v_slot, v_phase, abort_flag)) return false;
+                if (!wait_warp(full + v_slot, v_phase, abort_flag)) return false;
                 if (active) {
-                    if (!wait_bounded(p_ready + i, p_turn++ & 1, abort_flag)) return false;
+                    if (!wait_warp(p_ready + i, p_turn++ & 1, abort_flag)) return false;
                     tc_fence_after();
 #pragma unroll
                     for (int j = 0; j < TN / 16; ++j)
@@ -647,14 +647,14 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
             if (!ok && lane == 0) fail();
             __syncwarp();
             umma_commit_warp(done + i);
-            (void)wait_bounded(done + i, 0, nullptr);
+            (void)wait_warp(done + i, 0, nullptr);
         } else if (kRaw && i == 2) {
             // What has landed is handed to the tensor cores' proxy by a warp that nobody
             // waits for (by the issuing one: 500 cycles of every tile).
             int s = 0;
             uint32_t phase = 0;
             for (int index = 0; index < 2 * units; ++index) {
-                if (!wait_bounded(landed + s, phase, abort_flag)) {
+                if (!wait_warp(landed + s, phase, abort_flag)) {
                     if (lane == 0) fail();
                     break;
                 }
@@ -792,9 +792,9 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                     v_up[ring][w] = e[1] + kUp;
                 }
                 const int k_slot = next_slot;
-                ok = wait_bounded(empty + next_slot, next_phase, abort_flag);
+                ok = wait_warp(empty + next_slot, next_phase, abort_flag);
                 next_slots();
-                ok = ok && wait_bounded(empty + next_slot, next_phase, abort_flag);
+                ok = ok && wait_warp(empty + next_slot, next_phase, abort_flag);
                 if (!ok) {
                     if (lane == 0) fail();
                     break;
@@ -831,7 +831,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                 // ---- K, then V ----
 #pragma unroll 1
                 for (int half = 0; half < 2; ++half) {
-                    if (!wait_bounded(empty + next_slot, next_phase, abort_flag)) {
+                    if (!wait_warp(empty + next_slot, next_phase, abort_flag)) {
                         if (lane == 0) fail();
                         ok = false;
                         break;
@@ -870,7 +870,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                 // ---- the item's queries ----
                 if (n > 0) {
                     const int index = 2 * n - 2;                  // the last scores of the item before
-                    if (!wait_bounded(empty + index % kSlots, (index / kSlots) & 1, abort_flag)) {
+                    if (!wait_warp(empty + index % kSlots, (index / kSlots) & 1, abort_flag)) {
                         if (lane == 0) fail();
                         break;
                     }

@@ -50,6 +50,19 @@ __device__ __forceinline__ bool wait_bounded(uint64_t *bar, uint32_t parity, vol
         else if (globaltimer() - t0 > kWaitNs) return false;
     }
 }
+// The same for a whole warp, whose lanes get one answer: where some were to give up and
+// others not, the ones would wait for the others at the next instruction for all lanes.
+__device__ __forceinline__ bool wait_warp(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
+    uint64_t t0 = 0;
+    for (;;) {
+        for (int i = 0; i < 4096; ++i)
+            if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+        bool stop = abort_flag && *abort_flag;
+        if (t0 == 0) t0 = globaltimer();
+        else stop = stop || globaltimer() - t0 > kWaitNs;
+        if (__any_sync(0xffffffffu, stop)) return false;
+    }
+}
 __device__ __forceinline__ void fence_proxy_async() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
