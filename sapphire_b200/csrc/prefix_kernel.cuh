@@ -20,8 +20,7 @@
 // which the two tiles of rows fill for each other in part only; and 15 to 19 thousand
 // cycles pass before the first tile, most of them instructions that come from memory for
 // the first time.  Quantised: 24 sequences of 40 heads on 8, 40000 tokens of Q4_0,
-// 110 us (tensor pipe 15 %, issue 48 %): the converting warps are what
-// the MMAs wait for.
+// 98 us (tensor pipe 15 %, issue 48 %): the converting warps are what the MMAs wait for.
 //
 // Layout.  A block per SM, whose roles are warps:
 //   0 - 3, 4 - 7  softmax of the first and the second tile of rows: a thread has a
@@ -230,6 +229,11 @@ __device__ __forceinline__ int prefix_exponent(uint32_t top) {
     return top == 0 ? -100 : min(max((int)(top >> 23) - 127 - 14, -100), prefix_quant(kCache) ? 96 : 113);
 }
 
+// Where an operand's row has dim d of each eight: Q4_0's codes stay as two words side by
+// side give them (0 4 1 5 2 6 3 7), for queries and outputs are put in that order for less.
+template <int kCache>
+__host__ __device__ constexpr int prefix_place(int d) { return kCache == DTYPE_Q4_0 ? 2 * (d & 3) + (d >> 2) : d; }
+
 // A warp's quantised rows of a tile, which wait in shared memory (K rows, V rows, their
 // scales), as fp16 into the slots of K and V, zeros where a token does not count.  A lane
 // takes one block of 32 codes a round, which lie in 8 words nb apart, and writes them as 64
@@ -243,7 +247,9 @@ __device__ __forceinline__ void prefix_unpack(const uint8_t *raw, uint32_t valid
     // (2^-24, 2^-20 of it, which the group's power of two makes up for).
 #pragma unroll 1
     for (int k = lane; k < 2 * GT * NB; k += 32) {
-        const int t2 = k / NB, b = k - t2 * NB, t = t2 < GT ? t2 : t2 - GT, row = first_row + t;
+        // (Eight neighbouring lanes write 4 rows' 2 neighbouring blocks, which lie on all banks.)
+        const int pair = NB % 2 ? 0 : (k >> 3) % (NB / 2), t2 = NB % 2 ? k / NB : (k >> 3) / (NB / 2) * 4 + ((k >> 1) & 3), b = NB % 2 ? k - t2 * NB : 2 * pair + (k & 1);
+        const int t = t2 < GT ? t2 : t2 - GT, row = first_row + t;
         uint32_t w[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -251,6 +257,7 @@ __device__ __forceinline__ void prefix_unpack(const uint8_t *raw, uint32_t valid
         const __half f = __float2half_rn((valid >> t) & 1 ? scales[t2 * 8 + b] * (t2 < GT ? k_down : v_down) : 0.0f);
         const __half2 mul = __half2half2(f), add = __half2half2(__float2half_rn(__half2float(f) * -0x1p-17f));      // 128 2^-24 and 8 2^-20
         uint8_t *at = (t2 < GT ? k_to : v_to) + (b >> 1) * (TN * 128) + row * 128;
+        const int chunk = ((b & 1) * 4) ^ (row & 7);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             uint32_t c[4];
@@ -261,17 +268,16 @@ __device__ __forceinline__ void prefix_unpack(const uint8_t *raw, uint32_t valid
                     c[2 * i + 1] = __byte_perm(w[2 * u + i], 0u, 0x4342);
                 }
             } else {
-                // Code by code of two words, then word by word.
-                const uint32_t x = w[2 * u] | w[2 * u + 1] << 16;
-                const uint32_t c0 = (x << 4) & 0x00f000f0u, c1 = x & 0x00f000f0u, c2 = (x >> 4) & 0x00f000f0u, c3 = (x >> 8) & 0x00f000f0u;
-                c[0] = __byte_perm(c0, c1, 0x5410);
-                c[1] = __byte_perm(c2, c3, 0x5410);
-                c[2] = __byte_perm(c0, c1, 0x7632);
-                c[3] = __byte_perm(c2, c3, 0x7632);
+                // Code by code of two words, as prefix_place has them.
+                const uint32_t x = w[2 * u] + w[2 * u + 1] * 65536u, y = x >> 8;
+                c[0] = (x * 16u) & 0x00f000f0u;
+                c[1] = x & 0x00f000f0u;
+                c[2] = (y * 16u) & 0x00f000f0u;
+                c[3] = y & 0x00f000f0u;
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) c[i] = half2_bits(__hfma2(*reinterpret_cast<const __half2 *>(&c[i]), mul, add));
-            *reinterpret_cast<uint4 *>(at + ((((b & 1) * 4 + u) ^ (row & 7)) << 4)) = make_uint4(c[0], c[1], c[2], c[3]);
+            *reinterpret_cast<uint4 *>(at + ((chunk ^ u) << 4)) = make_uint4(c[0], c[1], c[2], c[3]);
         }
     }
 }
@@ -547,7 +553,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                             float y[8];
 #pragma unroll
                             for (int k = 0; k < 8; ++k) {
-                                y[k] = l == 0.0f ? 0.0f : o[j + k] * f1;
+                                y[k] = l == 0.0f ? 0.0f : o[j + prefix_place<kCache>(k)] * f1;
                                 if (!first_run) y[k] = fmaf(to[c + j + k], f0, y[k]);
                             }
                             asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + c + j), "f"(y[0]), "f"(y[1]),
@@ -675,11 +681,11 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
         bool ok = true;
         // Token `lane` of a tile: its page (-1: none) and slot.
         auto fetch = [&](int t, int &entry, int &slot) {
-            const long long tok = (long long)t * TN + w * GT + lane;
+            const uint32_t tok = (uint32_t)t * TN + w * GT + lane;         // (at most a tile behind the length)
             entry = -1;
             slot = 0;
             if (lane < GT && tok < length) {
-                int pg = (int)(((unsigned long long)(unsigned)tok * p.page_mul) >> 32);
+                int pg = (int)(((unsigned long long)tok * p.page_mul) >> 32);
                 slot = (int)tok - pg * p.l.page_size;
                 if (slot < 0) {
                     --pg;
@@ -708,7 +714,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
         };
         auto resolve = [&](int t, int entry, int slot) {
             Tokens x;
-            const bool wanted = lane < GT && (long long)t * TN + w * GT + lane < length, found = (unsigned)entry < (unsigned)p.l.num_pages;
+            const bool wanted = lane < GT && (uint32_t)t * TN + w * GT + lane < length, found = (unsigned)entry < (unsigned)p.l.num_pages;
             x.page16 = (found ? (unsigned)entry : 0u) * (unsigned)(p.l.page_bytes >> 4);
             x.row16 = x.page16 + (unsigned)(slot * (p.l.row_bytes >> 4));
             x.slot = slot;
@@ -928,7 +934,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                             mul = fmaxf(mul * pow2(-e), 1.2e-38f);
                         }
                     }
-                    if (convert || sign) {
+                    if (convert || sign || kCache == DTYPE_Q4_0) {
 #pragma unroll 4
                         for (int c = 0; c < PR; ++c) {
                             const uint4 x = *piece(c);
@@ -938,7 +944,9 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                                 for (int j = 0; j < 4; ++j)
                                     v[j] = half2_bits(__floats2half2_rn(__uint_as_float(v[j] << 16) * up, __uint_as_float(v[j] & 0xffff0000u) * up));
                             }
-                            *piece(c) = make_uint4(v[0], v[1], v[2], v[3]);
+                            if (kCache == DTYPE_Q4_0)             // (prefix_place)
+                                *piece(c) = make_uint4(__byte_perm(v[0], v[2], 0x5410), __byte_perm(v[0], v[2], 0x7632), __byte_perm(v[1], v[3], 0x5410), __byte_perm(v[1], v[3], 0x7632));
+                            else *piece(c) = make_uint4(v[0], v[1], v[2], v[3]);
                         }
                     }
                     qmul[(item - item0) & 1][i][row] = mul;
