@@ -60,6 +60,7 @@
 #pragma once
 
 #include "attention_kernel.cuh"
+#include "prefix_ranges.h"
 #include "tc.cuh"
 
 constexpr int kPrefixRows = 128;                  // of a tile
@@ -119,60 +120,6 @@ constexpr size_t prefix_shared_bytes(int hd, int cache) {
     return 1024 + (size_t)prefix_streams(hd) * prefix_query_bytes(hd) + (size_t)prefix_slots(hd, cache) * prefix_slot_bytes(hd, cache) +
            2 * kConverters * prefix_raw_tile(hd, cache);
 }
-// How the blocks share the units (a tile of tokens of one item): each item cut into
-// `parts` equal pieces, a block each; or, where that would leave blocks without work for
-// longer than a block's second item costs it (its queries, and results of its own: about
-// kItemUnits units), all units in a row into equal ranges, item by item.
-constexpr int kItemUnits = 5;
-struct PrefixRanges {
-    unsigned tiles;                // of an item
-    unsigned parts;                // of an item, or 0: ranges
-    unsigned total, blocks, each, longer;      // of an item's tiles where it has parts, of all units else: `longer` pieces of each + 1, then pieces of each
-};
-__host__ __device__ inline PrefixRanges prefix_ranges(unsigned items, unsigned length, unsigned tile, unsigned blocks) {
-    PrefixRanges r;
-    r.tiles = (length + tile - 1) / tile;
-    r.total = items * r.tiles;
-    r.blocks = r.total < blocks ? r.total : blocks;
-    r.parts = 0;
-    r.each = r.blocks ? r.total / r.blocks : 0;
-    r.longer = r.total - r.each * r.blocks;
-    if (r.blocks && items <= blocks) {
-        const unsigned most = blocks / items, parts = most < r.tiles ? most : r.tiles, each = r.tiles / parts, longer = r.tiles - each * parts;
-        if (each + (longer ? 1 : 0) <= r.each + kItemUnits) {
-            r.parts = parts;
-            r.blocks = items * parts;
-            r.each = each;
-            r.longer = longer;
-        }
-    }
-    return r;
-}
-// A block's item, and the first of its tiles there and its units.
-struct PrefixPiece {
-    unsigned item, tile, units;
-};
-__host__ __device__ inline PrefixPiece prefix_piece(const PrefixRanges &r, unsigned block) {
-    PrefixPiece x;
-    const unsigned item = r.parts ? block / r.parts : 0, piece = block - item * r.parts;       // (parts 0: the block)
-    const unsigned first = piece * r.each + (piece < r.longer ? piece : r.longer);
-    x.units = r.each + (piece < r.longer ? 1 : 0);
-    x.item = r.parts ? item : first / r.tiles;
-    x.tile = r.parts ? first : first - x.item * r.tiles;
-    return x;
-}
-// The blocks that hold an item.
-__host__ __device__ inline void prefix_holders(const PrefixRanges &r, unsigned item, unsigned *first, unsigned *last) {
-    if (r.parts) {
-        *first = item * r.parts;
-        *last = *first + r.parts - 1;
-        return;
-    }
-    const unsigned split = r.longer * (r.each + 1), a = item * r.tiles, b = a + r.tiles - 1;
-    *first = a < split ? a / (r.each + 1) : r.longer + (a - split) / r.each;
-    *last = b < split ? b / (r.each + 1) : r.longer + (b - split) / r.each;
-}
-
 #ifdef __CUDACC__
 // The prefix's tokens: its length, within its table.
 __device__ __forceinline__ long long prefix_length(const PrefixParams &p, bool report) {
@@ -539,7 +486,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                     const size_t at = ((size_t)(blockIdx.x + item) * p.streams + i) * kPrefixRows + row;
                     float *to = p.part + at * HD;
                     const float top_ml = fmaxf(m, m_item), ref_ml = top_ml == -INFINITY ? 0.0f : top_ml;
-                    const float w0 = first_run || l_item == 0.0f ? 0.0f : l_item * attn_exp2(m_item - ref_ml);
+                    const float w0 = l_item == 0.0f ? 0.0f : l_item * attn_exp2(m_item - ref_ml);
                     const float w1 = l == 0.0f ? 0.0f : l * attn_exp2(m - ref_ml), all = w0 + w1;
                     const float f0 = all == 0.0f ? 0.0f : w0 / all;
                     const float f1 = l == 0.0f ? 0.0f : (w1 / all) / l * (kRaw ? 1.0f : pow2(min(max(e_run, -126), 127)));
@@ -562,9 +509,10 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                         }
                     }
                     tc_fence_before();
-                    m_item = top_ml;
-                    l_item = all;
-                    if (last) p.part_ml[at] = make_float2(m_item, l_item);
+                    if (last) p.part_ml[at] = make_float2(top_ml, all);
+                    // (The next item's rows know nothing of this one's.)
+                    m_item = last ? -INFINITY : top_ml;
+                    l_item = last ? 0.0f : all;
                     first_run = last;
                     m = -INFINITY;
                     l = 0.0f;
