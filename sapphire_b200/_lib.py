@@ -103,6 +103,7 @@ _SIGNATURES = {
     "kernel_ctx_init_sharded": (i32, [vp, i32, i32, vp]),
     "kernel_ctx_shard_info": (i32, [vp, C.POINTER(i32), C.POINTER(i32)]),
     "sapphire_test_stream_unarmed": (i32, [i32]),
+    "sapphire_test_tc_unarmed": (i32, [i32]),
     "sapphire_test_pull_expiry": (i32, [vp, vp, C.c_longlong, C.c_ulonglong]),
     # include/sapphire_safetensors.h
     "sapphire_safetensors_open": (vp, [C.c_char_p]),

@@ -42,6 +42,7 @@
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 
+#include <atomic>
 #include <mutex>
 
 #include "internal.cuh"
@@ -82,6 +83,8 @@ struct GemmParams {
     // of full tiles full_tiles, full_tiles + 1, ... (the last wave, split so
     // that twice as many SMs share it).
     int full_tiles;
+    unsigned long long wait_ns;
+    bool unarmed;         // test hook: the first block's first stage gets no copies
 };
 
 struct TileGeom {
@@ -180,10 +183,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int ks = 0; ks < p.kstages; ++ks, ++kc) {
                     const int s = (int)(kc % kStages);
                     const uint32_t ph = (uint32_t)(kc / kStages) & 1u;
-                    if (!wait_bounded(empty + s, ph ^ 1u, abort_flag)) {
+                    if (!wait_bounded(empty + s, ph ^ 1u, abort_flag, p.wait_ns)) {
                         fail();
                         break;
                     }
+                    if (kc == 0 && p.unarmed && blockIdx.x == 0) continue;
                     // Blocks 2ks, 2ks+1 of each 32-row group: codes and scales
                     // of consecutive blocks are contiguous in the device layout.
                     const int nblk = min(2, p.nb - 2 * ks);
@@ -199,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             // Drain: the last copy issued into each stage has landed.
             for (long long q = kc - 1; q >= 0 && q >= kc - kStages; --q)
-                (void)wait_bounded(xfull + (int)(q % kStages), (uint32_t)(q / kStages) & 1u, nullptr);
+                (void)wait_bounded(xfull + (int)(q % kStages), (uint32_t)(q / kStages) & 1u, nullptr, p.wait_ns);
         }
         __syncwarp();
     } else if (warp == kWarpMma) {
@@ -210,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             bool ok = true;
             for (int tile = blockIdx.x; ok && tile < p.total_tiles; tile += gridDim.x, ++it) {
                 const int b = it & 1;
-                if (!wait_bounded(tempty + b, ((uint32_t)(it >> 1) & 1u) ^ 1u, abort_flag)) {
+                if (!wait_bounded(tempty + b, ((uint32_t)(it >> 1) & 1u) ^ 1u, abort_flag, p.wait_ns)) {
                     fail();
                     break;
                 }
@@ -220,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int ks = 0; ks < p.kstages; ++ks, ++kc) {
                     const int s = (int)(kc % kStages);
                     const uint32_t ph = (uint32_t)(kc / kStages) & 1u;
-                    if (!wait_bounded(xfull + s, ph, abort_flag) || !wait_bounded(afull + s, ph, abort_flag)) {
+                    if (!wait_bounded(xfull + s, ph, abort_flag, p.wait_ns) || !wait_bounded(afull + s, ph, abort_flag, p.wait_ns)) {
                         fail();
                         ok = false;
                         break;
@@ -239,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             // All MMAs issued by this thread have completed before TMEM is freed.
             umma_commit(mdone);
-            (void)wait_bounded(mdone, 0u, nullptr);
+            (void)wait_bounded(mdone, 0u, nullptr, p.wait_ns);
         }
         __syncwarp();
     } else if (warp >= kWarpDeq0) {
@@ -247,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int d = warp - kWarpDeq0;           // 32-row group of the 128-row tile
         const int g = lane >> 2, tig = lane & 3;
         long long kc = 0;
-        for (int tile = blockIdx.x; tile < p.total_tiles && !*abort_flag; tile += gridDim.x) {
+        for (int tile = blockIdx.x; tile < p.total_tiles; tile += gridDim.x) {
             const int t32 = tile_geom(p, tile).m * 4 + d;
             const bool tile_ok = t32 < p.ntiles32;
             bool ok = true;
@@ -256,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t ph = (uint32_t)(kc / kStages) & 1u;
                 // The stage's raw bytes have landed; its previous MMAs are done
                 // (the TMA warp waited for that before copying).
-                if (!wait_bounded(xfull + s, ph, abort_flag)) {
+                if (!wait_bounded_warp(xfull + s, ph, abort_flag, p.wait_ns)) {
                     if (lane == 0) fail();
                     ok = false;
                     break;
@@ -297,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         int it = 0;
         for (int tile = blockIdx.x; tile < p.total_tiles; tile += gridDim.x, ++it) {
             const int b = it & 1;
-            if (!wait_bounded(tfull + b, (uint32_t)(it >> 1) & 1u, abort_flag)) {
+            if (!wait_bounded_warp(tfull + b, (uint32_t)(it >> 1) & 1u, abort_flag, p.wait_ns)) {
                 if (lane == 0) fail();
                 break;
             }
@@ -379,7 +383,16 @@ int sm_count_of(int dev) {
     return n;
 }
 
+std::atomic<int> g_test_unarmed{0};     // sapphire_test_tc_unarmed
+
 }  // namespace
+
+int test_tc_unarmed() { return g_test_unarmed.load(); }
+
+extern "C" SAPPHIRE_API int sapphire_test_tc_unarmed(int on) {
+    g_test_unarmed.store(on);
+    return 0;
+}
 
 bool gemm_tc_supported(const DevWeight &w, int batch) {
     return w.dtype == DTYPE_Q4_0 && batch >= kGemmTcMinBatch && w.ntiles > 0;
@@ -457,6 +470,8 @@ int launch_gemm_tc_bf16(kernel_context_t *ctx, const DevWeight &w, const void *x
     p.full_tiles = split ? full - rest : full;
     p.total_tiles = split ? full + rest : full;
     p.kstages = kp / kBK;
+    p.unarmed = test_tc_unarmed() != 0;
+    p.wait_ns = p.unarmed ? kTestWaitNs : kWaitNs;
     const int grid = std::min(p.total_tiles, sm_count_of(ctx->device));
 
     // The shared-memory opt-in is a per-device function attribute.

@@ -294,6 +294,8 @@ int check_kernel_error(kernel_context_t *ctx, const char *who);
 // exactly (hi + lo bf16 halves), fp32 accumulation.  err: error word.
 constexpr int kGemmTcMinBatch = 16;
 bool gemm_tc_supported(const DevWeight &w, int batch);
+// sapphire_test_tc_unarmed's argument (gemm_tc.cu).
+int test_tc_unarmed();
 int launch_gemm_tc(kernel_context_t *ctx, const DevWeight &w, const float *x, int ldx, float *y, int ldy, int batch,
                    int *err, cudaStream_t stream);
 // Same product from bf16 activations already on the device: xb [batch][ldxb],

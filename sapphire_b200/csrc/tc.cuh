@@ -10,6 +10,7 @@
 namespace {
 
 constexpr unsigned long long kWaitNs = 2000000000ull;   // 2 s per wait
+constexpr unsigned long long kTestWaitNs = 1000000ull;  // where a test lets one run out
 
 __device__ __forceinline__ uint32_t saddr(const void *p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -40,18 +41,22 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
 // Waits for the phase of `bar` with the given parity; false after kWaitNs or,
 // when abort_flag is given, once another role has set it.  (Reading the timer
 // takes longer than a tile's softmax, so it is read between many tries.)
-__device__ __forceinline__ bool wait_bounded(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
+__device__ __forceinline__ bool wait_bounded(uint64_t *bar, uint32_t parity, volatile int *abort_flag, uint64_t limit = kWaitNs) {
     uint64_t t0 = 0;
     for (;;) {
         for (int i = 0; i < 4096; ++i)
             if (mbar_try_wait(bar, parity)) return true;
         if (abort_flag && *abort_flag) return false;
         if (t0 == 0) t0 = globaltimer();
-        else if (globaltimer() - t0 > kWaitNs) return false;
+        else if (globaltimer() - t0 > limit) return false;
     }
 }
 // The same for a whole warp, whose lanes get one answer: where some were to give up and
 // others not, the ones would wait for the others at the next instruction for all lanes.
+__device__ __forceinline__ bool wait_bounded_warp(uint64_t *bar, uint32_t parity, volatile int *abort_flag, uint64_t limit = kWaitNs) {
+    return __all_sync(0xffffffffu, wait_bounded(bar, parity, abort_flag, limit));
+}
+// Asked by a whole warp at a time.
 __device__ __forceinline__ bool wait_warp(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
     uint64_t t0 = 0;
     for (;;) {
