@@ -83,8 +83,6 @@ struct GemmParams {
     // of full tiles full_tiles, full_tiles + 1, ... (the last wave, split so
     // that twice as many SMs share it).
     int full_tiles;
-    unsigned long long wait_ns;
-    bool unarmed;         // test hook: the first block's first stage gets no copies
 };
 
 struct TileGeom {
@@ -123,6 +121,8 @@ __device__ __forceinline__ void dequant8(uint32_t word, float s, uint8_t *hi_dst
 }
 
 // ---------------------------------------------------------------- kernel --
+// kUnarmed: for sapphire_test_tc_unarmed (as a parameter: 172.6 -> 176 us).
+template <bool kUnarmed>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_q4_0_tc(const __grid_constant__ CUtensorMap xmap, const GemmParams p) {
     extern __shared__ uint8_t smem_raw[];
@@ -133,6 +133,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kBarriers);
     __shared__ int s_abort;
     volatile int *abort_flag = &s_abort;
+    constexpr unsigned long long kLimit = kUnarmed ? kTestWaitNs : kWaitNs;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     auto stage_x = [&](int s) { return smem + (size_t)s * kStageBytes; };
@@ -183,11 +184,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int ks = 0; ks < p.kstages; ++ks, ++kc) {
                     const int s = (int)(kc % kStages);
                     const uint32_t ph = (uint32_t)(kc / kStages) & 1u;
-                    if (!wait_bounded(empty + s, ph ^ 1u, abort_flag, p.wait_ns)) {
+                    if (!wait_bounded(empty + s, ph ^ 1u, abort_flag, kLimit)) {
                         fail();
                         break;
                     }
-                    if (kc == 0 && p.unarmed && blockIdx.x == 0) continue;
+                    if (kUnarmed && kc == 0 && blockIdx.x == 0) continue;
                     // Blocks 2ks, 2ks+1 of each 32-row group: codes and scales
                     // of consecutive blocks are contiguous in the device layout.
                     const int nblk = min(2, p.nb - 2 * ks);
@@ -203,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             // Drain: the last copy issued into each stage has landed.
             for (long long q = kc - 1; q >= 0 && q >= kc - kStages; --q)
-                (void)wait_bounded(xfull + (int)(q % kStages), (uint32_t)(q / kStages) & 1u, nullptr, p.wait_ns);
+                (void)wait_bounded(xfull + (int)(q % kStages), (uint32_t)(q / kStages) & 1u, nullptr, kLimit);
         }
         __syncwarp();
     } else if (warp == kWarpMma) {
@@ -214,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             bool ok = true;
             for (int tile = blockIdx.x; ok && tile < p.total_tiles; tile += gridDim.x, ++it) {
                 const int b = it & 1;
-                if (!wait_bounded(tempty + b, ((uint32_t)(it >> 1) & 1u) ^ 1u, abort_flag, p.wait_ns)) {
+                if (!wait_bounded(tempty + b, ((uint32_t)(it >> 1) & 1u) ^ 1u, abort_flag, kLimit)) {
                     fail();
                     break;
                 }
@@ -224,7 +225,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int ks = 0; ks < p.kstages; ++ks, ++kc) {
                     const int s = (int)(kc % kStages);
                     const uint32_t ph = (uint32_t)(kc / kStages) & 1u;
-                    if (!wait_bounded(xfull + s, ph, abort_flag, p.wait_ns) || !wait_bounded(afull + s, ph, abort_flag, p.wait_ns)) {
+                    if (!wait_bounded(xfull + s, ph, abort_flag, kLimit) || !wait_bounded(afull + s, ph, abort_flag, kLimit)) {
                         fail();
                         ok = false;
                         break;
@@ -243,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             // All MMAs issued by this thread have completed before TMEM is freed.
             umma_commit(mdone);
-            (void)wait_bounded(mdone, 0u, nullptr, p.wait_ns);
+            (void)wait_bounded(mdone, 0u, nullptr, kLimit);
         }
         __syncwarp();
     } else if (warp >= kWarpDeq0) {
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t ph = (uint32_t)(kc / kStages) & 1u;
                 // The stage's raw bytes have landed; its previous MMAs are done
                 // (the TMA warp waited for that before copying).
-                if (!wait_bounded_warp(xfull + s, ph, abort_flag, p.wait_ns)) {
+                if (!wait_bounded_warp(xfull + s, ph, abort_flag, kLimit)) {
                     if (lane == 0) fail();
                     ok = false;
                     break;
@@ -301,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         int it = 0;
         for (int tile = blockIdx.x; tile < p.total_tiles; tile += gridDim.x, ++it) {
             const int b = it & 1;
-            if (!wait_bounded_warp(tfull + b, (uint32_t)(it >> 1) & 1u, abort_flag, p.wait_ns)) {
+            if (!wait_bounded_warp(tfull + b, (uint32_t)(it >> 1) & 1u, abort_flag, kLimit)) {
                 if (lane == 0) fail();
                 break;
             }
@@ -470,8 +471,6 @@ int launch_gemm_tc_bf16(kernel_context_t *ctx, const DevWeight &w, const void *x
     p.full_tiles = split ? full - rest : full;
     p.total_tiles = split ? full + rest : full;
     p.kstages = kp / kBK;
-    p.unarmed = test_tc_unarmed() != 0;
-    p.wait_ns = p.unarmed ? kTestWaitNs : kWaitNs;
     const int grid = std::min(p.total_tiles, sm_count_of(ctx->device));
 
     // The shared-memory opt-in is a per-device function attribute.
@@ -481,7 +480,9 @@ int launch_gemm_tc_bf16(kernel_context_t *ctx, const DevWeight &w, const void *x
         std::lock_guard<std::mutex> lk(attr_mu);
         const int dev = ctx->device;
         if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-            e = cudaFuncSetAttribute(gemm_q4_0_tc, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
+            e = cudaFuncSetAttribute(gemm_q4_0_tc<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
+            if (e == cudaSuccess)
+                e = cudaFuncSetAttribute(gemm_q4_0_tc<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
             if (e != cudaSuccess) {
                 ctx_fail(ctx, "launch_gemm_tc", "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
                 return -1;
@@ -489,7 +490,7 @@ int launch_gemm_tc_bf16(kernel_context_t *ctx, const DevWeight &w, const void *x
             if (dev >= 0 && dev < 64) attr_set[dev] = true;
         }
     }
-    gemm_q4_0_tc<<<grid, kThreads, kSmemBytes, st>>>(xmap, p);
+    (test_tc_unarmed() ? gemm_q4_0_tc<true> : gemm_q4_0_tc<false>)<<<grid, kThreads, kSmemBytes, st>>>(xmap, p);
     e = cudaGetLastError();
     if (e != cudaSuccess) {
         ctx_fail(ctx, "launch_gemm_tc", "launch failed: %s", cudaGetErrorString(e));

@@ -42,3 +42,23 @@ def test_prefill_product_reports_and_recovers(sp, ctx, oracle, unarmed, rows, co
     assert sp.lib.kernel_ctx_synchronize(ctx.handle) == 0
     for _ in range(2):
         assert np.array_equal(sp.gemm(ctx, A, X, batch), want)
+
+
+def test_prefill_product_waits_little_longer_than_its_limit(sp, ctx, oracle, unarmed):
+    """Two waits of 1 ms behind one another: 2 ms, and 16 where the timer is read between thousands of tries."""
+    rng = np.random.default_rng(1)
+    A = sp.Tensor(Q4_0, (256, 640), oracle.quantize(Q4_0, (rng.standard_normal((256, 640)) * 0.02).astype(np.float32)))
+    x, y = torch.randn(16, 640, device="cuda"), torch.zeros(16, 256, device="cuda")
+
+    def run():
+        torch.cuda.synchronize()
+        t0 = time.perf_counter()
+        assert sp.lib.kernel_gemm_device(ctx.handle, y.data_ptr(), A.handle, x.data_ptr(), 16) == 0
+        return sp.lib.kernel_ctx_synchronize(ctx.handle), time.perf_counter() - t0
+
+    for _ in range(2):
+        assert run()[0] == 0
+    unarmed(1)
+    times = [run() for _ in range(5)]
+    assert all(rc == -1 for rc, _ in times)
+    assert min(t for _, t in times) < 8e-3, times
