@@ -181,12 +181,14 @@ SAPPHIRE_API int sapphire_shard_rows(int rows, int rank, int world_size, int *ro
  *  the next kernel_ctx_synchronize) returns -1.  on = 0 restores normal
  *  launches.  Process-wide. */
 SAPPHIRE_API int sapphire_test_stream_unarmed(int on);
-/** on != 0: in the following tensor-core products (kernel_gemm of a Q4_0 weight
+/** which != 0: in the following tensor-core products (kernel_gemm of a Q4_0 weight
  *  with batch_size >= 16) the first block's first shared-memory stage gets no
  *  copies, and waits have a limit of 1 ms; the call (or the next
- *  kernel_ctx_synchronize) returns -1.  on = 0 restores normal launches.
- *  Process-wide. */
-SAPPHIRE_API int sapphire_test_tc_unarmed(int on);
+ *  kernel_ctx_synchronize) returns -1.  In sapphire_attention_shared_device of
+ *  128 dims under 16-bit queries one warp of the first block withholds that its
+ *  first queries (1), probabilities (2) or rows (3) are there.  0 restores normal
+ *  launches.  Process-wide. */
+SAPPHIRE_API int sapphire_test_tc_unarmed(int which);
 /** Runs the peer-gather pull of a sharded product over a local buffer of
  *  `rows` words that nothing writes, with a wait limit of wait_ns
  *  nanoseconds: y (device, `rows` floats) receives NaN and the call returns -1

@@ -334,6 +334,7 @@ extern "C" SAPPHIRE_API int sapphire_attention_shared_device(kernel_context_t *c
     f.part_ml = reinterpret_cast<float2 *>(ws + w.part_ml);
     f.err = ctx->d_err;
     f.device = ctx->device;
+    f.unarmed = test_tc_unarmed();
     j.tc = on_tensor_cores(a->dtype);
     j.heads = a->heads;
     j.entries = (long long)a->sequences * a->heads;

@@ -94,6 +94,7 @@ struct PrefixParams {
     int counts;
     int *err;
     int device;
+    int unarmed;                   // test hook: which arrival the first block withholds
 };
 
 // Tiles of rows side by side, and tokens of a tile: S, P (half as many columns) and
@@ -280,7 +281,8 @@ __device__ __forceinline__ void prefix_convert(const uint8_t *from, unsigned row
     }
 }
 
-template <int kCache, int HD, bool kBf16>
+// kUnarmed: for sapphire_test_tc_unarmed.
+template <int kCache, int HD, bool kBf16, bool kUnarmed>
 __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) * 32, 1) prefix_kernel(const PrefixParams p) {
     constexpr int TN = prefix_tile(HD, kCache), kGroups = prefix_copiers(kCache, kBf16), GT = TN / kGroups, kSlots = prefix_slots(HD, kCache), NB = HD / 32;
     constexpr int kQueryBytes = prefix_query_bytes(HD), kSlotBytes = prefix_slot_bytes(HD, kCache), kMaxStreams = prefix_streams(HD);
@@ -305,6 +307,8 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
     __shared__ float k_up[kTileRing][kGroups];                          // a group's keys are the operand's times this
     __shared__ int v_up[kTileRing][kGroups];                            // and its values times 2 to this
     volatile int *const abort_flag = &s_abort;
+    constexpr uint64_t kLimit = kUnarmed ? kTestWaitNs : kWaitNs;
+    auto withheld = [&](int which, bool first) { return kUnarmed && first && p.unarmed == which && blockIdx.x == 0; };
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     // Barriers and tensor memory need nothing of an earlier kernel.
     if (threadIdx.x == 0) {
@@ -371,7 +375,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
         for (int n = 0; n < units; ++n) {
             const bool last = n + 1 == units || tile + 1 == tiles;
             if (i < now) {
-                if (!wait_warp(s_full + i, turn & 1, abort_flag)) {
+                if (!wait_warp(s_full + i, turn & 1, abort_flag, kLimit)) {
                     if (lane == 0) fail();
                     break;
                 }
@@ -423,7 +427,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                 }
                 // ---- the tile before has left P and O ----
                 if (turn > 0) {
-                    if (!wait_warp(p_done + i, (turn - 1) & 1, abort_flag)) {
+                    if (!wait_warp(p_done + i, (turn - 1) & 1, abort_flag, kLimit)) {
                         if (lane == 0) fail();
                         break;
                     }
@@ -473,11 +477,11 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(p_ready + i);
+                if (lane == 0 && !withheld(2, n == 0 && warp == 0)) mbar_arrive(p_ready + i);
                 ++turn;
                 if (++run == kRunTiles || last) {
                     // ---- the run's O, added to the item's ----
-                    if (!wait_warp(p_done + i, (turn - 1) & 1, abort_flag)) {
+                    if (!wait_warp(p_done + i, (turn - 1) & 1, abort_flag, kLimit)) {
                         if (lane == 0) fail();
                         break;
                     }
@@ -550,10 +554,10 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
             };
             // (A tile of rows that an item does not have still gives its slots back.)
             auto scores = [&](bool active, bool new_item) {
-                if (new_item && !wait_warp(&q_full, q_phase++ & 1, abort_flag)) return false;
-                if (!wait_warp(full + k_slot, k_phase, abort_flag)) return false;
+                if (new_item && !wait_warp(&q_full, q_phase++ & 1, abort_flag, kLimit)) return false;
+                if (!wait_warp(full + k_slot, k_phase, abort_flag, kLimit)) return false;
                 if (active) {
-                    if (s_turn > 0 && !wait_warp(s_free + i, (s_turn - 1) & 1, abort_flag)) return false;
+                    if (s_turn > 0 && !wait_warp(s_free + i, (s_turn - 1) & 1, abort_flag, kLimit)) return false;
                     ++s_turn;
                     tc_fence_after();
 #pragma unroll
@@ -569,9 +573,9 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                 return true;
             };
             auto outputs = [&](bool active) {
-                if (!wait_warp(full + v_slot, v_phase, abort_flag)) return false;
+                if (!wait_warp(full + v_slot, v_phase, abort_flag, kLimit)) return false;
                 if (active) {
-                    if (!wait_warp(p_ready + i, p_turn++ & 1, abort_flag)) return false;
+                    if (!wait_warp(p_ready + i, p_turn++ & 1, abort_flag, kLimit)) return false;
                     tc_fence_after();
 #pragma unroll
                     for (int j = 0; j < TN / 16; ++j)
@@ -601,14 +605,14 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
             if (!ok && lane == 0) fail();
             __syncwarp();
             umma_commit_warp(done + i);
-            (void)wait_warp(done + i, 0, nullptr);
+            (void)wait_warp(done + i, 0, nullptr, kLimit);
         } else if (kRaw && i == 2) {
             // What has landed is handed to the tensor cores' proxy by a warp that nobody
             // waits for (by the issuing one: 500 cycles of every tile).
             int s = 0;
             uint32_t phase = 0;
             for (int index = 0; index < 2 * units; ++index) {
-                if (!wait_warp(landed + s, phase, abort_flag)) {
+                if (!wait_warp(landed + s, phase, abort_flag, kLimit)) {
                     if (lane == 0) fail();
                     break;
                 }
@@ -746,9 +750,9 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                     v_up[ring][w] = e[1] + kUp;
                 }
                 const int k_slot = next_slot;
-                ok = wait_warp(empty + next_slot, next_phase, abort_flag);
+                ok = wait_warp(empty + next_slot, next_phase, abort_flag, kLimit);
                 next_slots();
-                ok = ok && wait_warp(empty + next_slot, next_phase, abort_flag);
+                ok = ok && wait_warp(empty + next_slot, next_phase, abort_flag, kLimit);
                 if (!ok) {
                     if (lane == 0) fail();
                     break;
@@ -757,7 +761,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) {
-                    mbar_arrive(full + k_slot);
+                    if (!withheld(3, n == 0 && w == 0)) mbar_arrive(full + k_slot);
                     mbar_arrive(full + next_slot);
                 }
                 next_slots();
@@ -785,7 +789,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                 // ---- K, then V ----
 #pragma unroll 1
                 for (int half = 0; half < 2; ++half) {
-                    if (!wait_warp(empty + next_slot, next_phase, abort_flag)) {
+                    if (!wait_warp(empty + next_slot, next_phase, abort_flag, kLimit)) {
                         if (lane == 0) fail();
                         ok = false;
                         break;
@@ -809,12 +813,12 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                         }
                         // (They arrive when they land, whatever this warp does meanwhile.)
                         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(saddr(landed + next_slot)) : "memory");
-                        if (lane == 0) mbar_arrive(landed + next_slot);
+                        if (lane == 0 && !withheld(3, n == 0 && half == 0 && w == 0)) mbar_arrive(landed + next_slot);
                     } else {
                         prefix_convert<kCache, HD, TN>(rows, now.row16, now.valid, w * GT, lane, pow2(half ? -e[1] : -e[0]), slots + at);
                         fence_proxy_async();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(full + next_slot);
+                        if (lane == 0 && !withheld(3, n == 0 && half == 0 && w == 0)) mbar_arrive(full + next_slot);
                     }
                     next_slots();
                 }
@@ -824,7 +828,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                 // ---- the item's queries ----
                 if (n > 0) {
                     const int index = 2 * n - 2;                  // the last scores of the item before
-                    if (!wait_warp(empty + index % kSlots, (index / kSlots) & 1, abort_flag)) {
+                    if (!wait_warp(empty + index % kSlots, (index / kSlots) & 1, abort_flag, kLimit)) {
                         if (lane == 0) fail();
                         break;
                     }
@@ -901,7 +905,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                 }
                 fence_proxy_async();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&q_full);
+                if (lane == 0 && !withheld(1, n == 0 && w == 0)) mbar_arrive(&q_full);
             }
             if (++tile == tiles) {
                 tile = 0;
@@ -918,13 +922,15 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
     }
 }
 
-template <int kCache, int HD, bool kBf16>
+template <int kCache, int HD, bool kBf16, bool kUnarmed = false>
 cudaError_t prefix_launch(const PrefixParams &p, cudaStream_t st) {
+    if constexpr (HD == 128 && !kUnarmed)
+        if (p.unarmed) return prefix_launch<kCache, HD, kBf16, true>(p, st);
     constexpr size_t kBytes = prefix_shared_bytes(HD, kCache);
     static std::atomic<unsigned long long> done{0};
-    cudaError_t e = attn_allow(prefix_kernel<kCache, HD, kBf16>, kBytes, p.device, done);
+    cudaError_t e = attn_allow(prefix_kernel<kCache, HD, kBf16, kUnarmed>, kBytes, p.device, done);
     if (e != cudaSuccess) return e;
-    return launch_pdl(prefix_kernel<kCache, HD, kBf16>, dim3(p.blocks), dim3((kPrefixCopy + prefix_copiers(kCache, kBf16)) * 32), kBytes, st, p);
+    return launch_pdl(prefix_kernel<kCache, HD, kBf16, kUnarmed>, dim3(p.blocks), dim3((kPrefixCopy + prefix_copiers(kCache, kBf16)) * 32), kBytes, st, p);
 }
 template <int kCache, bool kBf16>
 cudaError_t prefix_launch(const PrefixParams &p, cudaStream_t st) {

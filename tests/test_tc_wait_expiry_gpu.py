@@ -11,6 +11,9 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 
+from test_attention_gpu import dev_ctx  # noqa: E402,F401
+from test_shared_prefix_gpu import shared_case  # noqa: E402
+
 Q4_0 = 3
 
 
@@ -62,3 +65,36 @@ def test_prefill_product_waits_little_longer_than_its_limit(sp, ctx, oracle, una
     times = [run() for _ in range(5)]
     assert all(rc == -1 for rc, _ in times)
     assert min(t for _, t in times) < 8e-3, times
+
+
+@pytest.mark.parametrize("which", [1, 2, 3])
+@pytest.mark.parametrize("dtype,kind,seqs,prefix", [("bf16", "bf16", 2, 300), ("bf16", "bf16", 40, 20000), ("f16", "f16", 70, 5000), ("q8_0", "bf16", 40, 5000),
+                                                    ("q4_0", "f16", 2, 300), ("f32", "bf16", 40, 2000), ("bf16", "f16", 70, 700)])
+def test_shared_prefix_reports_and_recovers(sp, dev_ctx, unarmed, dtype, kind, seqs, prefix, which):
+    """A warp of the first block withholds its first queries, probabilities or rows: short pieces and long ones, one tile
+    of rows and two, rows that are copied and that are converted."""
+    kv, prefix_table, table, q = shared_case(dev_ctx, dtype, kind, prefix, [3] * seqs, 2, 4, 128, 16, seed=seqs)
+    n, m = torch.full((seqs,), 3, dtype=torch.int32, device="cuda"), torch.tensor([prefix], dtype=torch.int32, device="cuda")
+    ws = torch.zeros(kv.shared_workspace_bytes(kind, seqs, 8), dtype=torch.uint8, device="cuda")
+
+    def run():
+        out = torch.empty_like(q)
+        torch.cuda.synchronize()
+        t0 = time.perf_counter()
+        kv.attend_shared(q, prefix_table, m, table, n, out, workspace=ws)
+        try:
+            dev_ctx.synchronize()
+        finally:
+            run.elapsed = time.perf_counter() - t0
+        return out
+
+    want = run()
+    unarmed(which)
+    for _ in range(2):
+        with pytest.raises(sp.SapphireError, match="bounded wait expired"):
+            run()
+        assert run.elapsed < 0.05, run.elapsed      # 1 ms, and 4096 tries of about 1 us three times
+    unarmed(0)
+    dev_ctx.synchronize()
+    for _ in range(2):
+        assert torch.equal(run(), want)
