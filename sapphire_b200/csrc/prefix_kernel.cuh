@@ -51,7 +51,8 @@
 //   product), F32 and BF16 values are rounded to it once; each group of tokens (a warp's,
 //   6 to 16) times a power of two that brings its largest scale or value to [2^14, 2^15).
 //   K's power multiplies the group's scores, V's is added to their exponent, relative to
-//   the largest so far, and O carries that one;
+//   the row's largest sum of score and power so far, and O carries that one: a large value
+//   without weight takes no bits from what has weight;
 //   probabilities are rounded to the operand type once, as the outputs are.  m may lag
 //   behind the maximum by 2^8 before O is brought up to date, so fp16 probabilities
 //   reach 2^15 and keep their bits down to 2^-21 of the largest.
@@ -384,7 +385,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                 if (run == 0 && first_run) qm = qmul[(item - item0) & 1][i][row];
                 uint32_t word[kGroups];
                 float qg[kGroups];
-                int eg[kGroups], e_tile = -1000;
+                int eg[kGroups];
                 bool whole = true;
 #pragma unroll
                 for (int g = 0; g < kGroups; ++g) {
@@ -392,7 +393,6 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                     whole = whole && word[g] == 0xffffffffu >> (32 - GT);
                     qg[g] = kRaw ? qm : fmaxf(qm * k_up[ring][g], 1.2e-38f);
                     eg[g] = kRaw ? 0 : v_up[ring][g];
-                    e_tile = max(e_tile, eg[g]);
                 }
                 // The row's scores, -inf where a token does not count.
                 float s[TN];
@@ -412,7 +412,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                         if (!((word[j / GT] >> (j % GT)) & 1)) s[j] = -INFINITY;
                 }
                 // (A NaN among them makes every one of the row's probabilities NaN.)
-                float top = -INFINITY;
+                float top = -INFINITY, top_value = -INFINITY;     // (the largest score; probability times value)
 #pragma unroll
                 for (int g = 0; g < kGroups; ++g) {
                     float t0 = s[g * GT], t1 = s[g * GT + 1];
@@ -424,6 +424,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                     const float t2 = max_nan(t0, t1) * qg[g];
                     if (t2 != t2) qm = t2;
                     top = fmaxf(top, t2);
+                    if (!kRaw) top_value = fmaxf(top_value, t2 + (float)eg[g]);
                 }
                 // ---- the tile before has left P and O ----
                 if (turn > 0) {
@@ -434,16 +435,18 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                     tc_fence_after();
                 }
                 // ---- the reference, and O in its units ----
-                const bool grew = top > m + kLag || (m == -INFINITY && top > m), up = !kRaw && e_tile > e_run;
-                if (__any_sync(0xffffffffu, grew) || up) {
+                const bool grew = top > m + kLag || (m == -INFINITY && top > m) || (!kRaw && top_value - m > (float)e_run + kLag);
+                if (__any_sync(0xffffffffu, grew)) {
                     const float mn = fmaxf(m, top);
                     float f = mn == -INFINITY ? 1.0f : attn_exp2(m - mn);
                     l *= f;
-                    m = mn;
-                    if (up) {
-                        if (run > 0) f *= pow2(max(e_run - e_tile, -126));
-                        e_run = e_tile;
+                    if (!kRaw) {
+                        // (m + e_run never falls, so f is at most 1; -1000 is where there is no score.)
+                        const int e = (int)ceilf(fmaxf(fmaxf(top_value - mn, (float)e_run + (m - mn)), -1000.0f));
+                        if (mn != -INFINITY) f = attn_exp2((m - mn) + (float)(e_run - e));
+                        e_run = e;
                     }
+                    m = mn;
                     if (run > 0) {
 #pragma unroll 1
                         for (int c = 0; c < HD; c += 16) {
@@ -464,7 +467,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
 #pragma unroll
                     for (int k = 0; k < 16; k += 2) {
                         const int j = c + k, g = j / GT;
-                        const float mul = qm != qm ? qm : qg[g], at = kRaw ? ref : ref + (float)max(eg[g] - e_run, -100);
+                        const float mul = qm != qm ? qm : qg[g], at = kRaw ? ref : ref + (float)min(max(eg[g] - e_run, -100), 300);
                         const float2 x = fma2(make_float2(s[j], s[j + 1]), make_float2(mul, mul), make_float2(at, at));
                         const float2 y = make_float2(attn_exp2(x.x), attn_exp2(x.y));
                         sum[g] = add2(sum[g], y);
@@ -473,7 +476,7 @@ __global__ void __launch_bounds__((kPrefixCopy + prefix_copiers(kCache, kBf16)) 
                     tmem_store<8>(p_at + c / 2, w);
                 }
 #pragma unroll
-                for (int g = 0; g < kGroups; ++g) l += kRaw ? sum[g].x + sum[g].y : (sum[g].x + sum[g].y) * pow2(min(e_run - eg[g], 100));
+                for (int g = 0; g < kGroups; ++g) l += kRaw ? sum[g].x + sum[g].y : (sum[g].x + sum[g].y) * pow2(min(max(e_run - eg[g], -126), 100));
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
