@@ -10,9 +10,10 @@ bf16 queries) or 2^-11 (fp16) of a probability:
 * probabilities below 2^-21 of the largest times its group's value lose bits: 2^-20 M, M the
   largest of p_t |v_u| over tokens t and u less than 16 apart;
 * roundings of different tokens know nothing of each other, so the norm of out's error is
-  about u / sqrt(3) that of S = sqrt(sum (p v)^2).  4 u |S|, and 8 ds |S| for the scores,
+  about u / sqrt(3) that of S = sqrt(sum (p v)^2).  2 u |S|, and 8 ds |S| for the scores,
   2^-14 |out| for sums that truncate (512 steps of 2^-24, and their like in fp32), 2^-20 |M|
-  and the outputs' own half steps are the bound of the norm, whatever the length.
+  and the outputs' own half steps are the bound of the norm, whatever the length.  What the
+  fewest tokens that a warp brings at a time add to the outputs is more.
 """
 from __future__ import annotations
 
@@ -52,7 +53,7 @@ def exact_rows(g, dtype, tokens, heads, dim, exponents=None, one_sign=False):
     size = torch.ones(tokens, device="cuda") if exponents is None else torch.exp2(exponents.float())
     if dtype in IO:
         x = torch.randn(tokens, heads, dim, device="cuda", generator=g).bfloat16().float()
-        x = (x.abs() + 0.5).bfloat16().float() if one_sign else x
+        x = (x.abs() + 0.5).bfloat16().float() if one_sign else torch.where(x.abs() < 2.0 ** -7, 0.0, x)      # (fp16 holds 2^-14 in 8 bits)
         x = x * size[:, None, None]
         assert torch.equal(x.to(IO[dtype]).float(), x)
         return x.double(), x, None
@@ -61,6 +62,13 @@ def exact_rows(g, dtype, tokens, heads, dim, exponents=None, one_sign=False):
     scales = torch.exp2(torch.randint(-7, -4, (tokens, heads, dim // 32), device="cuda", generator=g).float() + (0 if dtype == "q8_0" else 4))
     scales = scales * size[:, None, None]
     return codes.double() * scales.double().repeat_interleave(32, -1), codes, scales
+
+
+def warp_tokens(dtype, kind, dim):
+    """Tokens that a warp of the product brings at a time: a quarter of a tile's where rows are copied as they are, else an eighth."""
+    quant = dtype not in IO
+    tile = 128 if dim <= 64 else 96 if dim <= 96 else 80 if dim <= 192 else 48 if quant else 64
+    return tile // (4 if dtype == "f16" or (dtype == "bf16" and kind == "bf16") else 8)
 
 
 class Exact:
@@ -123,7 +131,7 @@ class Exact:
                 rest = rest / rest.sum(-1, keepdim=True)
                 gone2 += (torch.einsum("shgt,thd->shgd", rest, self.v) - want).square().sum()
         root = lambda x: math.sqrt(float(x))                                   # noqa: E731
-        tol = 4 * self.u * root(tol_u) + 8 * root(tol_ds) + 2.0 ** -14 * root(want2) + 2.0 ** -20 * root(m2) + root(half2)
+        tol = 2 * self.u * root(tol_u) + 8 * root(tol_ds) + 2.0 ** -14 * root(want2) + 2.0 ** -20 * root(m2) + root(half2)
         assert root(err2) <= tol, (root(err2), tol)
         if lost is not None:
-            assert root(gone2) > 2 * tol, (root(gone2), tol)
+            assert root(gone2) > 1.25 * tol, (root(gone2), tol)
