@@ -268,13 +268,18 @@ SAPPHIRE_API int sapphire_kv_select_device(kernel_context_t *ctx, const sapphire
  * prefix_length[0] positions, on the pages of prefix_table, and to the n =
  * lengths[s] + length_offset tokens that it has behind them (its new one among
  * them), position p of which is slot p % page_size of page_table[s][p / page_size].
- * The prefix is read once for the batch.  What else holds is as for
- * sapphire_attention_device, but that 16-bit queries use 16-bit operands over the
+ * The prefix is read once for 256 rows of a KV head (its query heads of every
+ * sequence; 128 rows of 192 and 256 dims), on the tensor cores; F32 pages and, under f16
+ * queries, BF16 pages are read a second time to find their range.  Under fp32 queries it
+ * is read once for the rows of up to 8 tiles of 8 (4 where there are no more), as many
+ * tiles as divide their number: of a prime number of them, once for each.  What else
+ * holds is as for sapphire_attention_device, but that 16-bit queries use 16-bit operands over the
  * prefix: over BF16 under bf16 queries probabilities are rounded to bf16; else
  * probabilities and F32 and BF16 values are rounded to fp16, Q8_0 and Q4_0 scales and
  * their products with codes too; values below 2^-20 of the largest of neighbouring
- * tokens are less exact, and scales from 2^112 on may count as infinite.  The same
- * call gives the same bits.
+ * tokens are less exact, and scales from 2^112 on may count as infinite.  fp32 queries
+ * (and outputs) keep what sapphire_attention_device keeps.  The same call gives the
+ * same bits.
  * ------------------------------------------------------------------------- */
 typedef struct {
     tensor_dtype_t dtype;    /* F32, BF16 or F16, of q and out */

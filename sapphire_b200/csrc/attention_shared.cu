@@ -3,11 +3,12 @@
 // arguments, workspace, the choice of the prefix's kernel, and the joining of its
 // pieces with what each sequence has behind it.
 //
-// Reading the prefix once for the batch leaves each of its pages' bytes to 2 flops
-// for every row, so its kernel is a matrix product (prefix_kernel.cuh).  Under fp32
-// queries it is the one-token kernel (attention_kernel.cuh) with every sequence's
-// heads as query heads of one sequence: its tf32 parts hold what a 16-bit operand
-// would not.
+// Reading the prefix once for many rows (a KV head's query heads, of every sequence)
+// leaves each of its pages' bytes to 2 flops for each, so its kernel is a matrix
+// product (prefix_kernel.cuh).  Under fp32 queries it is the one-token kernel
+// (attention_kernel.cuh) with every sequence's heads as query heads of one sequence:
+// its tf32 parts hold what a 16-bit operand would not, and it reads the prefix again
+// for every few tiles of 8 rows (as many as divide their number, up to 8).
 #include <algorithm>
 #include <climits>
 #include <cmath>
