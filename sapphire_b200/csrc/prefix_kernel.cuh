@@ -19,8 +19,8 @@
 // together, then the chain of P's store, O's MMAs, S's of the next tile and their load,
 // which the two tiles of rows fill for each other in part only; and 15 to 19 thousand
 // cycles pass before the first tile, most of them instructions that come from memory for
-// the first time.  Quantised: 24 sequences of 40 heads on 8, 40000 tokens of Q4_0,
-// 98 us (tensor pipe 15 %, issue 48 %): the converting warps are what the MMAs wait for.
+// the first time.  Quantised: 24 sequences of 40 heads on 8, 60001 tokens of Q4_0,
+// 98 us (tensor pipe 14 %, issue 45 %): the converting warps are what the MMAs wait for.
 //
 // Layout.  A block per SM, whose roles are warps:
 //   0 - 3, 4 - 7  softmax of the first and the second tile of rows: a thread has a
