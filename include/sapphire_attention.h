@@ -273,13 +273,14 @@ SAPPHIRE_API int sapphire_kv_select_device(kernel_context_t *ctx, const sapphire
  * queries, BF16 pages are read a second time to find their range.  Under fp32 queries it
  * is read once for the rows of up to 8 tiles of 8 (4 where there are no more), as many
  * tiles as divide their number: of a prime number of them, once for each.  What else
- * holds is as for sapphire_attention_device, but that 16-bit queries use 16-bit operands over the
- * prefix: over BF16 under bf16 queries probabilities are rounded to bf16; else
- * probabilities and F32 and BF16 values are rounded to fp16, Q8_0 and Q4_0 scales and
- * their products with codes too; values below 2^-20 of the largest of neighbouring
- * tokens are less exact, and scales from 2^112 on may count as infinite.  fp32 queries
- * (and outputs) keep what sapphire_attention_device keeps.  The same call gives the
- * same bits.
+ * holds is as for sapphire_attention_device, but that 16-bit queries use 16-bit
+ * operands over the prefix: over BF16 under bf16 queries probabilities are rounded to
+ * bf16; else probabilities and F32 and BF16 values are rounded to fp16, Q8_0 and Q4_0
+ * scales and their products with codes too (a score is off by up to 2^-11 of scale
+ * sum |q k| over F32, 2^-10 over Q8_0 and Q4_0); values below 2^-20 of the largest of
+ * neighbouring tokens are less exact, and scales from 2^112 on may count as infinite.
+ * Queries and outputs in fp32 (a copy of 16-bit ones) keep what
+ * sapphire_attention_device keeps.  The same call gives the same bits.
  * ------------------------------------------------------------------------- */
 typedef struct {
     tensor_dtype_t dtype;    /* F32, BF16 or F16, of q and out */
