@@ -13,14 +13,14 @@
 // head in bf16 against 4 rows flops), and above that the tensor cores and the
 // exponentials: a tile of 128 rows by 128 tokens of 128 dims is 1024 cycles of MMA
 // and 1024 of ex2.  Measured, 64 sequences of 32 query heads on 8 KV heads of 128
-// behind 32768 tokens in bf16: 54 us for 134 MB (20 at HBM's rate) and 34 GFLOP, tensor
-// pipe 36 %, ex2 37 %, issue 37 %.  A block takes 80 tokens of both tiles of rows in
-// about 2570 cycles: a softmax of 1500, of which 1280 are ex2's for the two tiles
+// behind 32768 tokens in bf16: 49 us for 134 MB (20 at HBM's rate) and 34 GFLOP, tensor
+// pipe 33 %, ex2 34 %, issue 35 %.  A block takes 80 tokens of both tiles of rows in
+// about 2650 cycles: a softmax of 1500, of which 1280 are ex2's for the two tiles
 // together, then the chain of P's store, O's MMAs, S's of the next tile and their load,
-// which the two tiles of rows fill for each other in part only; and 15 to 19 thousand
+// which the two tiles of rows fill for each other in part only; and 8 to 9 thousand
 // cycles pass before the first tile, most of them instructions that come from memory for
 // the first time.  Quantised: 24 sequences of 40 heads on 8, 60001 tokens of Q4_0,
-// 98 us (tensor pipe 14 %, issue 45 %): the converting warps are what the MMAs wait for.
+// 88 us (tensor pipe 16 %, issue 51 %): the converting warps are what the MMAs wait for.
 //
 // Layout.  A block per SM, whose roles are warps:
 //   0 - 3, 4 - 7  softmax of the first and the second tile of rows: a thread has a

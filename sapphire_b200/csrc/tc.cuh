@@ -57,14 +57,16 @@ __device__ __forceinline__ bool wait_bounded(uint64_t *bar, uint32_t parity, vol
 __device__ __forceinline__ bool wait_bounded_warp(uint64_t *bar, uint32_t parity, volatile int *abort_flag, uint64_t limit = kWaitNs) {
     return __all_sync(0xffffffffu, wait_bounded(bar, parity, abort_flag, limit));
 }
-// The same answer, but with the timer and the abort flag read once in 4096 tries of about
-// 1 us each, so it gives up 4 ms after another role's failure and up to 8 ms behind the
-// limit.  (In the shared prefix reading them between all tries costs 1 to 3 %: 64 sequences
-// behind 32768 tokens in bf16 91 -> 92.6 us, 48 behind 6001 in f16 53.5 -> 56.)
+// The same answer, but with the timer and the abort flag read once in 64 tries of up to
+// 4 us each, so it gives up 0.3 ms after another role's failure and up to 0.6 ms behind
+// the limit.  (Not unrolled: the shared prefix has many waits, and its start is instructions
+// that come from memory for the first time.  24 sequences behind 60001 tokens of Q4_0
+// 122 -> 106 us, 64 behind 32768 in bf16 91 -> 87, 48 behind 6001 in f16 53.5 -> 48.2.)
 __device__ __forceinline__ bool wait_warp(uint64_t *bar, uint32_t parity, volatile int *abort_flag, uint64_t limit = kWaitNs) {
     uint64_t t0 = 0;
     for (;;) {
-        for (int i = 0; i < 4096; ++i)
+#pragma unroll 1
+        for (int i = 0; i < 64; ++i)
             if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
         bool stop = abort_flag && *abort_flag;
         if (t0 == 0) t0 = globaltimer();

@@ -90,10 +90,12 @@ def test_shared_prefix_reports_and_recovers(sp, dev_ctx, unarmed, dtype, kind, s
 
     want = run()
     unarmed(which)
+    times = []
     for _ in range(2):
         with pytest.raises(sp.SapphireError, match="bounded wait expired"):
             run()
-        assert run.elapsed < 0.05, run.elapsed      # 1 ms, and 4096 tries of about 1 us three times
+        times.append(run.elapsed)
+    assert min(times) < 0.01, times                 # 1.4 ms, and 32 where the timer is read once in 4096 tries
     unarmed(0)
     dev_ctx.synchronize()
     for _ in range(2):
